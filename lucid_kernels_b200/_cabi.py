@@ -259,7 +259,7 @@ def tma_delivery_rate(t: torch.Tensor, slots: int = 4, boxes_per_sm: int = 4000)
             ev0.record(stream)
         rc = lib.lucid_probe_tma_delivery(t.data_ptr(), strides3(t), B, N, H, dtype_code(t.dtype), slots,
                                           boxes_per_sm, clocks.data_ptr(), sms, stream.cuda_stream)
-        check_rc(rc, "lucid_probe_tma_delivery", "lucid_query_chain_group")
+        check_rc(rc, "lucid_probe_tma_delivery")
         if timed:
             ev1.record(stream)
     stream.synchronize()
