@@ -25,13 +25,23 @@ BWD_DV_ONLY = 0
 BWD_COMBINED = 1
 
 _I64x3 = ctypes.c_int64 * 3
+_I64x2 = ctypes.c_int64 * 2
 
 EXPORTS = ("lucid_workspace_bytes", "lucid_fwd_sub", "lucid_bwd_sub", "lucid_read_status",
            "lucid_status_string", "lucid_set_wait_limit_ns", "lucid_workspace_timestamps_offset",
            "lucid_profile_next_call", "lucid_set_head_steps", "lucid_set_group_overlap", "lucid_set_dk_split", "lucid_fwd_sub_static",
            "lucid_set_fused_backward", "lucid_fwd_sub_scaled", "lucid_bwd_sub_scaled",
            "lucid_set_pair_solve", "lucid_set_pair_limits", "lucid_fwd_workspace_bytes", "lucid_stream_capture_id", "lucid_query_pair_solve", "lucid_set_solve_variant", "lucid_set_upper_in_solve", "lucid_query_upper_in_solve",
-           "lucid_probe_tma_delivery", "lucid_query_chain_group")
+           "lucid_probe_tma_delivery", "lucid_query_chain_group",
+           "lucid_window_attn_fwd", "lucid_window_attn_bwd", "lucid_window_attn_bwd_workspace_bytes", "lucid_paged_append",
+           "lucid_paged_window_attn", "lucid_paged_lucid_attn", "lucid_paged_attn_workspace_bytes", "lucid_attn_status")
+
+
+class PagedCache(ctypes.Structure):
+    """``lucid_paged_cache``"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_strides", _I64x3), ("v_strides", _I64x3),
+                ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32),
+                ("pages", ctypes.c_int32), ("page_rows", ctypes.c_int32)]
 
 
 class LucidKernelError(RuntimeError):
@@ -137,6 +147,23 @@ def load() -> ctypes.CDLL:
         lib.lucid_profile_next_call.argtypes = [c.c_void_p, c.c_void_p, c.c_void_p, c.c_void_p]
         lib.lucid_set_wait_limit_ns.restype = None
         lib.lucid_set_wait_limit_ns.argtypes = [c.c_uint64]
+        p, i, f, cache = c.c_void_p, c.c_int, c.c_float, c.POINTER(PagedCache)
+        lib.lucid_window_attn_fwd.restype = i
+        lib.lucid_window_attn_fwd.argtypes = [p] * 5 + [_I64x3] * 4 + [i] * 9 + [f, p, p]
+        lib.lucid_window_attn_bwd_workspace_bytes.restype = c.c_size_t
+        lib.lucid_window_attn_bwd_workspace_bytes.argtypes = [i] * 7
+        lib.lucid_window_attn_bwd.restype = i
+        lib.lucid_window_attn_bwd.argtypes = [p] * 9 + [_I64x3] * 8 + [i] * 9 + [f, p, p, c.c_size_t, p]
+        lib.lucid_paged_append.restype = i
+        lib.lucid_paged_append.argtypes = [p] * 4 + [_I64x2] * 3 + [cache, p, p, p] + [i] * 8 + [p]
+        lib.lucid_paged_attn_workspace_bytes.restype = c.c_size_t
+        lib.lucid_paged_attn_workspace_bytes.argtypes = [i] * 8
+        lib.lucid_paged_window_attn.restype = i
+        lib.lucid_paged_window_attn.argtypes = [p, p, _I64x2, cache, p] + [i] * 7 + [f, p, c.c_size_t, p]
+        lib.lucid_paged_lucid_attn.restype = i
+        lib.lucid_paged_lucid_attn.argtypes = [p, p, p, _I64x2, _I64x2, cache, p] + [i] * 5 + [f, f, p, c.c_size_t, p]
+        lib.lucid_attn_status.restype = i
+        lib.lucid_attn_status.argtypes = [p, c.POINTER(c.c_int32)]
         _lib = lib
     return _lib
 
@@ -240,6 +267,16 @@ def raise_on_device_error(ws: torch.Tensor, stream_ptr: int, what: str) -> None:
         kern = {0: "diag-prep", 1: "solve", 2: "dK"}.get(st[1], "?")
         raise LucidKernelError(
             f"{what}: {msg} [kernel={kern} chain={st[2]} row_block={st[3]} detail={st[4]} barrier={st[5]}]")
+
+
+def raise_on_attention_error(stream_ptr: int, what: str) -> None:
+    """Synchronise the stream; raise if an attention or cache kernel on the current device reported an error."""
+    out = (ctypes.c_int32 * 8)()
+    check_rc(load().lucid_attn_status(stream_ptr, out), "lucid_attn_status")
+    if out[0] != 0:
+        msg = load().lucid_status_string(out[0]).decode()
+        kern = {0: "window forward", 1: "window backward", 2: "append", 3: "paged attention"}[out[1]]
+        raise LucidKernelError(f"{what}: {msg} [kernel={kern} {list(out)[2:7]}]")
 
 
 def tma_delivery_rate(t: torch.Tensor, slots: int = 4, boxes_per_sm: int = 4000) -> dict:

@@ -3,12 +3,13 @@
 #include <string.h>
 
 #include "../../include/lucid_b200.h"
+#include "host.h"
 #include "kernels.h"
-#include "tmap.h"
 
 namespace lucid {
 
 static unsigned long long g_wait_ns = 2000000000ull;
+unsigned long long wait_limit_ns() { return g_wait_ns; }
 // optional per-kernel timing: events recorded around the kernels of the NEXT call made by the same host
 // thread, then forgotten (thread-local, so one thread's request is never consumed by another thread's call)
 static thread_local cudaEvent_t g_events[4] = {nullptr, nullptr, nullptr, nullptr};
@@ -59,52 +60,11 @@ static Layout make_layout(int B, int N, int H) {
   return l;
 }
 
-static int sm_count() {
-  static int cached[64] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (dev < 0 || dev >= 64) dev = 0;
-  if (cached[dev] == 0) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    cached[dev] = n;
-  }
-  return cached[dev];
-}
-
-// st = element strides {batch, sequence, head}; ext = the extents of those dimensions.  A zero stride in a
-// dimension of extent > 1 is an expanded (broadcast) tensor: the tensor maps cannot express it, and writing
-// through one would alias.
-static int check_tensor(const void* p, const int64_t st[3], int B, int N, int H) {
-  if (!p || !st) return LUCID_E_NULL_POINTER;
-  if (reinterpret_cast<uintptr_t>(p) % 16) return LUCID_E_BAD_ALIGNMENT;
-  const int ext[3] = {B, N, H};
-  for (int i = 0; i < 3; ++i) {
-    if (st[i] % 8 || st[i] < 0) return LUCID_E_BAD_ALIGNMENT;
-    if (st[i] == 0 && ext[i] > 1) return LUCID_E_BAD_STRIDE;
-  }
-  return 0;
-}
-
 static int check_shape(int B, int N, int H, int D, int dtype) {
   if (B <= 0 || N <= 0 || H <= 0 || D != kBlock || N % kBlock) return LUCID_E_BAD_SHAPE;
   if ((long long)B * H * (N / kBlock) > (1ll << 30) / kBlock) return LUCID_E_BAD_SHAPE;
   if (dtype != LUCID_DTYPE_FP16 && dtype != LUCID_DTYPE_BF16) return LUCID_E_BAD_DTYPE;
   return 0;
-}
-
-// (B, N, H, 128) tensor -> 4-D map {d, n, h, b}
-static int bshd_map(CUtensorMap* m, bool bf16, const void* p, const int64_t st[3], int B, int N, int H,
-                    uint32_t box_rows) {
-  uint64_t dims[4] = {(uint64_t)kBlock, (uint64_t)N, (uint64_t)H, (uint64_t)B};
-  // size-1 dimensions may carry any stride; give them a harmless valid one.  (Zero strides of longer
-  // dimensions never get here: check_tensor refuses them.)
-  uint64_t sn = (uint64_t)st[1] * 2, sh = (uint64_t)st[2] * 2, sb = (uint64_t)st[0] * 2;
-  if (H == 1) sh = 256;
-  if (B == 1) sb = 256;
-  if (sn == 0 || sh == 0 || sb == 0) return LUCID_E_BAD_STRIDE;
-  uint64_t strides[3] = {sn, sh, sb};
-  return make_tmap_16bit(m, bf16, p, 4, dims, strides, box_rows) ? LUCID_E_TENSOR_MAP : 0;
 }
 
 static int auto_group(int C, int N, int requested, bool backward) {
@@ -580,6 +540,11 @@ const char* lucid_status_string(int code) {
     case LUCID_E_STATIC_SCRATCH_TOO_SMALL:
       return "problem too large for the library-owned scratch of lucid_fwd_sub_static "
              "(lucid_workspace_bytes(B, N, H) must not exceed LUCID_STATIC_SCRATCH_BYTES - 1023)";
+    case 4: return "a position lies outside the block table or its page outside the pool (skipped)";
+    case LUCID_E_BAD_HEADS: return "bad heads: the query heads must be a multiple of the key heads (LUCID step: at most 15 per key head)";
+    case LUCID_E_BAD_PAGE: return "bad cache: pages of a power of two up to 65536 rows, at least one page and one table column";
+    case LUCID_E_BAD_ROTATION: return "bad rotation: rotated elements must be a multiple of 16 up to 128";
+    case LUCID_E_BAD_SCALE: return "bad scale: must be positive and finite";
     default: return code > 0 ? "CUDA runtime error" : "unknown";
   }
 }

@@ -1,0 +1,373 @@
+// Sliding-window attention with visible first keys, forward, on sm_100a.
+//
+//   s_ij = scale q_i . k_j over the visible j (attn_geometry.h),  O_i = sum_j exp(s_ij - lse_i) v_j
+//
+// One pass over the keys with a running maximum m and sum l per row; O is kept in tensor memory relative to a
+// reference maximum that is only moved when the running one has outgrown it by 2^8 (exact in the end: O and l share
+// the reference, and 2^8 is far from the limits of fp32 sums and 16-bit weights).
+//
+// A CTA works on two tiles of 128 queries that read the same keys (two heads of a key head, or two neighbouring
+// blocks), so a key/value tile brought into shared memory feeds four products.  Per tile of queries: S (fp32, 128
+// columns of TMEM; the 16-bit weights P overwrite it) and O (128 columns): 512 columns in all.  While the tensor pipe
+// runs one tile's P V and next S, the other tile's warps form exponentials.
+//
+// Warp roles (384 threads): warp 0 producer, warps 1 and 2 issue the products of tile 0 and 1 (an issuing thread runs
+// only a few products ahead of the tensor pipe), warp 3 owns TMEM; warps 4-7 and 8-11 are the softmax groups of the
+// two tiles, one row per thread.  Persistent CTAs, items dealt out round robin, the longest first.
+#include <type_traits>
+#include "attn.h"
+
+namespace lucid {
+
+static __device__ Control g_attn_fwd_ctl;
+
+constexpr int kFwRing = 5;
+struct AttnFwdSmem {
+  alignas(1024) uint8_t q[2][kTileBytes];
+  alignas(1024) uint8_t ring[kFwRing][kTileBytes];   // K(0), V(0), K(1), V(1), ... of the union of the two tiles' lists
+  alignas(8) uint64_t full[kFwRing];
+  uint64_t empty[kFwRing], q_full[2], q_free[2], s_full[2], p_ready[2], o_full[2], o_free[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+enum AttnFwdBar : int { AF_FULL = 401, AF_EMPTY, AF_Q_FULL, AF_Q_FREE, AF_S_FULL, AF_P_READY, AF_O_FULL, AF_O_FREE };
+
+constexpr int kFwThreads = 384;
+constexpr int kFwS = 0, kFwO = 256;      // + 128 * tile
+constexpr int kFwRegsService = 56, kFwRegsSoftmax = 224;    // 128 * 56 + 256 * 224 = 384 * 168, the launch's total
+constexpr float kFwSlack = 8.f;          // log2 of how far the maximum may outgrow the reference
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kFwThreads, 1)
+attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                const __grid_constant__ CUtensorMap tm_v, const AttnFwdArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  AttnFwdSmem& s = *reinterpret_cast<AttnFwdSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const AttnShape& A = args.a;
+  Control* ctl = &g_attn_fwd_ctl;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const unsigned long long limit = args.wait_ns;
+  volatile int* cta_abort = &s.abort_flag;
+
+  if (tid == 0) {
+    for (int i = 0; i < kFwRing; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.q_full[i], 1);
+      mbar_init(&s.q_free[i], 1);
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_ready[i], 128);
+      mbar_init(&s.o_full[i], 1);
+      mbar_init(&s.o_free[i], 128);
+    }
+    s.abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 3) {
+    tmem_alloc(&s.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = s.tmem_base;
+  auto length_of = [&](int b) -> int { return attn_length(A, args.lengths, b); };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFwRegsService));
+    if (warp == 0) {
+      // =========================== producer (one lane) ===========================
+      if (lane == 0) {
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+        uint32_t r = 0, stage = 0, phase = 0;
+        uint32_t nq[2] = {0, 0};      // Q tiles loaded
+        bool alive = true;
+        FwdItem it;
+        for (int idx = blockIdx.x; alive && fwd_item(A, idx, it); idx += gridDim.x) {
+          const PairTiles pt = pair_tiles(A, it, length_of(it.b));
+          auto load = [&](const CUtensorMap* tm, int tile) -> bool {
+            if (!wait_barrier(&s.empty[stage], phase ^ 1, cta_abort, ctl, limit, idx, (int)r, AF_EMPTY)) return false;
+            mbar_expect_tx(&s.full[stage], kTileBytes);
+            tma_load_4d(s.ring[stage], tm, &s.full[stage], 0, tile * kBlock, it.hk, it.b);
+            tma_load_4d(s.ring[stage] + kHalfBytes, tm, &s.full[stage], 64, tile * kBlock, it.hk, it.b);
+            ++r;
+            if (++stage == kFwRing) {
+              stage = 0;
+              phase ^= 1;
+            }
+            return true;
+          };
+          for (int t = 0; t < 2 && alive; ++t) {
+            if (pt.list(t).n == 0) continue;
+            if (!wait_barrier(&s.q_free[t], (nq[t] & 1) ^ 1, cta_abort, ctl, limit, idx, t, AF_Q_FREE)) {
+              alive = false;
+              break;
+            }
+            ++nq[t];
+            mbar_expect_tx(&s.q_full[t], kTileBytes);
+            tma_load_4d(s.q[t], &tm_q, &s.q_full[t], 0, it.block(t) * kBlock, it.h(t), it.b);
+            tma_load_4d(s.q[t] + kHalfBytes, &tm_q, &s.q_full[t], 64, it.block(t) * kBlock, it.h(t), it.b);
+          }
+          for (int u = 0; u < pt.n && alive; ++u) {
+            const int j = pt.tile(u);
+            alive = load(&tm_k, j) && load(&tm_v, j);
+          }
+        }
+      }
+    } else if (warp < 3) {
+      // =========================== issuer of one tile's products ===========================
+      const int t = warp - 1;
+      constexpr int fmt = kBf16 ? 1 : 0;
+      constexpr uint32_t idesc_s = umma_idesc(fmt, 0, 0, 128, 128);    // Q K^T: both K-major
+      constexpr uint32_t idesc_o = umma_idesc(fmt, 0, 1, 128, 128);    // P V: P from TMEM, V rows = k
+      const uint64_t d_q = umma_smem_desc(smem_u32(s.q[t]), 16, 1024);
+      const uint64_t d_k0 = umma_smem_desc(smem_u32(s.ring[0]), 16, 1024);
+      const uint64_t d_v0 = umma_smem_desc(smem_u32(s.ring[0]), kHalfBytes, 1024);
+      const uint32_t s_tmem = tmem + kFwS + 128 * t, o_tmem = tmem + kFwO + 128 * t;
+      uint32_t r = 0;          // ring uses before this item: K(u) is use r + 2u, V(u) use r + 2u + 1
+      uint32_t nq = 0, np = 0; // items with tiles; weights consumed
+      bool alive = true;
+      FwdItem it;
+      for (int idx = blockIdx.x; alive && fwd_item(A, idx, it); idx += gridDim.x) {
+        const PairTiles pt = pair_tiles(A, it, length_of(it.b));
+        const KeyTiles kt = pt.list(t);
+        const bool mine = kt.n > 0;
+        if (mine && !wait_barrier(&s.q_full[t], nq & 1, cta_abort, ctl, limit, idx, t, AF_Q_FULL)) break;
+        auto wait_full = [&](uint32_t use) -> bool {
+          return wait_barrier(&s.full[use % kFwRing], (use / kFwRing) & 1, cta_abort, ctl, limit, idx, (int)use, AF_FULL);
+        };
+        bool first = true;
+        // O (+)= P(u) V(u), once the softmax group has written P(u)
+        auto issue_pv = [&](int u) -> bool {
+          const uint32_t use = r + 2 * u + 1, st = use % kFwRing;
+          if (!wait_barrier(&s.p_ready[t], np & 1, cta_abort, ctl, limit, idx, u, AF_P_READY)) return false;
+          ++np;
+          if (!wait_full(use)) return false;
+          // the epilogue of this tile's previous item has read O
+          if (first && !wait_barrier(&s.o_free[t], (nq & 1) ^ 1, cta_abort, ctl, limit, idx, u, AF_O_FREE)) return false;
+          tc_fence_after_sync();
+          const uint64_t dv = d_v0 + st * (kTileBytes >> 4);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            umma_ts_w(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, (!first || k) ? 1u : 0u);
+          first = false;
+          umma_commit_w(&s.empty[st]);
+          return true;
+        };
+        int pend = -1, left = kt.n;
+        for (int u = 0; u < pt.n; ++u) {
+          const bool act = pt.active(kt, u);
+          if (pend >= 0) {
+            if (!issue_pv(pend)) { alive = false; break; }
+            pend = -1;
+          }
+          const uint32_t use = r + 2 * u, st = use % kFwRing;
+          if (!wait_full(use)) { alive = false; break; }
+          if (act) {
+            tc_fence_after_sync();
+            const uint64_t dk = d_k0 + st * (kTileBytes >> 4);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
+              umma_ss_w(s_tmem, d_q + off, dk + off, idesc_s, k ? 1u : 0u);
+            }
+            umma_commit_w(&s.s_full[t]);
+            umma_commit_w(&s.empty[st]);
+            if (--left == 0) umma_commit_w(&s.q_free[t]);
+            pend = u;
+          } else {
+            // not this tile's keys: hand both stages on (each only after it has been filled)
+            __syncwarp();
+            mbar_arrive_w(&s.empty[st]);
+            if (!wait_full(use + 1)) { alive = false; break; }
+            __syncwarp();
+            mbar_arrive_w(&s.empty[(use + 1) % kFwRing]);
+          }
+        }
+        if (!alive) break;
+        if (pend >= 0 && !issue_pv(pend)) break;
+        if (mine) {
+          umma_commit_w(&s.o_full[t]);
+          ++nq;
+        }
+        r += 2 * pt.n;
+      }
+    }
+  } else {
+    // =========================== softmax of one tile, then its epilogue ===========================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFwRegsSoftmax));
+    typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
+    const int t = (warp - 4) >> 2;
+    const int row = ((warp & 3) << 5) + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + lanes + kFwS + 128 * t, o_tmem = tmem + lanes + kFwO + 128 * t;
+    const float sl2 = args.scale_log2;
+    uint32_t ns = 0, no = 0, r = 0;
+    bool alive = true;
+    FwdItem it;
+    for (int idx = blockIdx.x; alive && fwd_item(A, idx, it); idx += gridDim.x) {
+      const int len = length_of(it.b);
+      const PairTiles pt = pair_tiles(A, it, len);
+      const KeyTiles kt = pt.list(t);
+      const int i = it.block(t) * kBlock + row;
+      const int p = i + A.off;
+      const bool valid = i < A.Nq && p < len;
+      float ref = -INFINITY, l = 0.f;
+      bool first = true;
+      for (int u = 0; u < pt.n; ++u) {
+        if (!pt.active(kt, u)) continue;
+        const int tile = pt.tile(u), j0 = tile << 7;
+        if (!wait_barrier(&s.s_full[t], ns & 1, cta_abort, ctl, limit, idx, u, AF_S_FULL)) { alive = false; break; }
+        ++ns;
+        tc_fence_after_sync();
+        uint32_t v[128];
+        {
+          uint32_t(&v0)[32] = *reinterpret_cast<uint32_t(*)[32]>(v);
+          uint32_t(&v1)[32] = *reinterpret_cast<uint32_t(*)[32]>(v + 32);
+          uint32_t(&v2)[32] = *reinterpret_cast<uint32_t(*)[32]>(v + 64);
+          uint32_t(&v3)[32] = *reinterpret_cast<uint32_t(*)[32]>(v + 96);
+          tmem_ld32(s_tmem, v0);
+          tmem_ld32(s_tmem + 32, v1);
+          tmem_ld32(s_tmem + 64, v2);
+          tmem_ld32(s_tmem + 96, v3);
+          tmem_wait_ld();
+        }
+        if (tile_masked(A, kt, tile, len)) {
+          const RowMask mask = row_mask(A, p, j0, len);
+#pragma unroll
+          for (int e = 0; e < 128; ++e) v[e] = mask.sees(e) ? v[e] : 0xff800000u;
+          if (j0 + 127 >= len && len < A.Nk) {
+            // rows behind the sequence hold anything, and 0 * NaN is not 0: the value tile's become zero
+            const uint32_t use = r + 2 * u + 1;
+            if (!wait_barrier(&s.full[use % kFwRing], (use / kFwRing) & 1, cta_abort, ctl, limit, idx, (int)use, AF_FULL)) {
+              alive = false;
+              break;
+            }
+            if (j0 + row >= len) zero_tile_row(s.ring[use % kFwRing], row);
+            __syncwarp();
+          }
+          fence_proxy_async_smem();
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(v[c]);
+#pragma unroll
+        for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[e]));
+        const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+        const bool grow = m > ref + kFwSlack;
+        if (first) {
+          ref = m;
+        } else if (__any_sync(0xffffffffu, grow)) {
+          // S(u) is complete, and with it every product issued before it: O holds all earlier tiles
+          const float next = fmaxf(ref, m);
+          const float f = next == -INFINITY ? 1.f : ex2_approx(ref - next);
+          ref = next;
+          l *= f;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_tmem + 16 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(o_tmem + 16 * c, o);
+          }
+        }
+        first = false;
+        const float neg = ref == -INFINITY ? 0.f : -ref;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float a = ex2_approx(fmaf(__uint_as_float(v[32 * c + 2 * e]), sl2, neg));
+            const float b = ex2_approx(fmaf(__uint_as_float(v[32 * c + 2 * e + 1]), sl2, neg));
+            sum[(2 * e) & 3] += a;
+            sum[(2 * e + 1) & 3] += b;
+            pk[e] = pack2<kBf16>(a, b);
+          }
+          tmem_st16(s_tmem + 16 * c, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before_sync();
+        mbar_arrive(&s.p_ready[t]);
+      }
+      if (!alive) break;
+      r += 2 * pt.n;
+
+      // ---- epilogue ----
+      const bool has = kt.n > 0;
+      if (has) {
+        if (!wait_barrier(&s.o_full[t], no & 1, cta_abort, ctl, limit, idx, t, AF_O_FULL)) break;
+        ++no;
+        tc_fence_after_sync();
+      }
+      const bool some = valid && l != 0.f;      // (a NaN sum is written as it is)
+      const float inv = some ? 1.f / l : 0.f;
+      const bool store = i < A.Nq && it.block(t) < A.nqb;
+      elem_t* out = reinterpret_cast<elem_t*>(args.out) + it.b * args.out_strides.b + (long long)i * args.out_strides.n +
+                    it.h(t) * args.out_strides.h;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        if (has) {
+          tmem_ld32(o_tmem + 32 * c, o);
+          tmem_wait_ld();
+        }
+        if (store) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (has && some) {
+              w.x = pack2<kBf16>(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
+              w.y = pack2<kBf16>(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
+              w.z = pack2<kBf16>(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
+              w.w = pack2<kBf16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
+            }
+            *reinterpret_cast<uint4*>(out + 32 * c + 8 * e) = w;
+          }
+        }
+        __syncwarp();
+      }
+      if (has) {
+        tc_fence_before_sync();
+        mbar_arrive(&s.o_free[t]);
+      }
+      if (store)
+        args.lse[((long long)it.b * A.Hq + it.h(t)) * A.Nq + i] =
+            some ? (ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    }
+  }
+
+  if (s.abort_flag) {
+    // a role gave up: leave the copies and products in flight time to land before the CTA's memory goes
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    if (tid == 0) report_error(ctl, kErrAborted, -1, -1, blockIdx.x, 0);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 3) tmem_dealloc(tmem, 512);
+}
+
+cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                            const AttnFwdArgs& args, int sms, cudaStream_t stream) {
+  const int items = fwd_items(args.a), grid = items < sms ? items : sms;
+  const int bytes = (int)sizeof(AttnFwdSmem) + 1024;
+  auto kernel = bf16 ? attn_fwd_kernel<true> : attn_fwd_kernel<false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  kernel<<<grid, kFwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, args);
+  return cudaGetLastError();
+}
+
+cudaError_t attn_fwd_status(cudaStream_t stream, int out[8]) { return take_status(&g_attn_fwd_ctl, stream, out); }
+
+}  // namespace lucid

@@ -1,0 +1,225 @@
+// Which tiles the windowed attention kernels visit, and in which order.  Plain integer arithmetic, usable from host
+// code as well: every role of a kernel derives the same lists from it, so it is checked on the CPU.
+//
+// Query i of Nq sits at position p = i + off with off = Nk - Nq >= 0 (the queries are the last Nq positions).  In a
+// sequence of n valid positions it sees key j when  j <= p,  (j > p - W  or  j < S),  j < n  and  p < n.
+#pragma once
+#include "schedule.h"
+
+namespace lucid {
+
+constexpr int kNoWindow = 1 << 30;   // W of full causality
+constexpr int kMaxSinks = 128;       // S <= 128: visible first keys all lie in key tile 0
+
+LUCID_HD int imax(int a, int b) { return a > b ? a : b; }
+
+struct AttnShape {
+  int B, Nq, Nk, Hq, Hkv;
+  int G;      // query heads per key head
+  int off;    // Nk - Nq
+  int W, S;
+  int nqb, nkb;   // 128-row blocks of queries and keys
+};
+
+// Key tiles of one block of 128 queries: an optional first tile 0 that holds only visible first keys, then lo .. hi.
+struct KeyTiles {
+  int n;         // how many, 0 = no query of the block sees anything
+  int sink;      // 1: tile 0 comes first although the window does not reach it
+  int lo;
+  int p_lo, p_hi;   // positions of the block's first and last valid query
+  LUCID_HD int tile(int u) const { return u < sink ? 0 : lo + u - sink; }
+};
+
+LUCID_HD KeyTiles key_tiles(const AttnShape& a, int block, int len) {
+  KeyTiles t;
+  const int i0 = block * 128;
+  const int last = imin(imin(i0 + 127, a.Nq - 1), len - 1 - a.off);   // last valid query of the block
+  t.p_lo = i0 + a.off;
+  t.p_hi = last + a.off;
+  t.n = 0;
+  t.sink = 0;
+  t.lo = 0;
+  if (last < i0) return t;
+  const int lo_key = a.W >= kNoWindow ? 0 : imax(0, t.p_lo - a.W + 1);
+  const bool near = a.W > 0;                        // W == 0: no key of the window, only first keys
+  t.lo = lo_key >> 7;
+  const int hi = t.p_hi >> 7;
+  t.sink = (a.S > 0 && (!near || t.lo > 0)) ? 1 : 0;
+  t.n = t.sink + (near ? hi - t.lo + 1 : 0);
+  return t;
+}
+
+// Does any (query, key) pair of the tile have to be masked?
+LUCID_HD bool tile_masked(const AttnShape& a, const KeyTiles& t, int tile, int len) {
+  const int j0 = tile << 7;
+  return j0 + 127 > t.p_lo || (a.W < kNoWindow && j0 <= t.p_hi - a.W) || j0 + 127 >= len;
+}
+
+// Columns of a key tile (first key j0) that the query at position p sees: e <= hi and (e >= lo or e < first).
+struct RowMask {
+  int hi, lo, first;
+  LUCID_HD bool sees(int e) const { return e <= hi && (e >= lo || e < first); }
+};
+LUCID_HD RowMask row_mask(const AttnShape& a, int p, int j0, int len) {
+  return RowMask{imin(p, len - 1) - j0, p - a.W + 1 - j0, a.S - j0};
+}
+
+// Transposed: does any pair of key tile j0 and the 128 queries from position p0 on have to be masked, and which columns
+// (queries) lo .. hi see key j.
+LUCID_HD bool block_masked(const AttnShape& a, int j0, int p0, int len) {
+  return p0 < j0 + 127 || p0 + 127 >= len || j0 + 127 >= len || (a.W < kNoWindow && p0 + 127 > j0 + a.W - 1);
+}
+struct ColMask {
+  int lo, hi;
+  LUCID_HD bool sees(int e) const { return e >= lo && e <= hi; }
+};
+LUCID_HD ColMask col_mask(const AttnShape& a, int j, int p0, int len) {
+  ColMask m;
+  m.lo = j - p0;
+  m.hi = len - 1 - p0;
+  if (a.W < kNoWindow && j >= a.S) m.hi = imin(m.hi, j + a.W - 1 - p0);
+  if (j >= len) m.hi = -1;
+  return m;
+}
+
+// Forward work item: two tiles of 128 queries that read the same keys.  With an even number of query heads per key
+// head they are two heads of one block of rows (same keys exactly), otherwise two neighbouring blocks of one head.
+LUCID_HD bool pair_heads(const AttnShape& a) { return (a.G & 1) == 0; }
+LUCID_HD int fwd_items(const AttnShape& a) {
+  return pair_heads(a) ? a.B * (a.Hq / 2) * a.nqb : a.B * a.Hq * ((a.nqb + 1) / 2);
+}
+struct FwdItem {
+  int b, hk;
+  int h0, h1, block0, block1;    // block >= nqb: no such tile
+  LUCID_HD int h(int k) const { return k ? h1 : h0; }
+  LUCID_HD int block(int k) const { return k ? block1 : block0; }
+};
+LUCID_HD bool fwd_item(const AttnShape& a, int idx, FwdItem& it) {
+  if (idx >= fwd_items(a)) return false;
+  // blocks from the last to the first (under full causality the last ones take longest), heads side by side
+  if (pair_heads(a)) {
+    const int per = a.B * (a.Hq / 2);
+    const int blk = a.nqb - 1 - idx / per, r = idx % per;
+    it.b = r / (a.Hq / 2);
+    it.h0 = 2 * (r % (a.Hq / 2));
+    it.h1 = it.h0 + 1;
+    it.block0 = it.block1 = blk;
+  } else {
+    const int per = a.B * a.Hq, nb = (a.nqb + 1) / 2;
+    const int bp = nb - 1 - idx / per, r = idx % per;
+    it.b = r / a.Hq;
+    it.h0 = it.h1 = r % a.Hq;
+    it.block0 = 2 * bp;
+    it.block1 = 2 * bp + 1;
+  }
+  it.hk = it.h0 / a.G;
+  return true;
+}
+// The union of the two tiles' lists, in increasing order; `active` says which of the two visits an entry.
+struct PairTiles {
+  KeyTiles x, y;
+  int n, sink, lo;
+  LUCID_HD KeyTiles list(int k) const { return k ? y : x; }
+  LUCID_HD int tile(int u) const { return u < sink ? 0 : lo + u - sink; }
+  LUCID_HD bool active(const KeyTiles& t, int u) const {
+    const int j = tile(u);
+    if (t.n == 0) return false;
+    if (j == 0 && t.sink) return true;
+    return u >= sink && j >= t.lo && j < t.lo + t.n - t.sink;
+  }
+};
+LUCID_HD PairTiles pair_tiles(const AttnShape& a, const FwdItem& it, int len) {
+  PairTiles p;
+  const KeyTiles x = p.x = key_tiles(a, it.block0, len);
+  const KeyTiles y = p.y = key_tiles(a, it.block1, len);
+  // runs of window tiles: both non-empty, or one of them (x comes first: its rows are the lower ones)
+  const int nx = x.n - x.sink, ny = y.n - y.sink;
+  int hi;
+  if (nx > 0 && ny > 0) {
+    p.lo = imin(x.lo, y.lo);
+    hi = imax(x.lo + nx, y.lo + ny) - 1;
+  } else if (nx > 0) {
+    p.lo = x.lo;
+    hi = x.lo + nx - 1;
+  } else {
+    p.lo = y.lo;
+    hi = y.lo + ny - 1;
+  }
+  const bool any = nx > 0 || ny > 0;
+  // one list's first tile 0 may be the other list's window tile 0
+  p.sink = ((x.n > 0 && x.sink) || (y.n > 0 && y.sink)) && !(any && p.lo == 0) ? 1 : 0;
+  p.n = p.sink + (any ? hi - p.lo + 1 : 0);
+  return p;
+}
+
+// Query blocks whose rows may see a key of key tile `tile` through the window (first .. last; none: first > last).
+struct QueryBlocks {
+  int first, last;
+};
+LUCID_HD QueryBlocks query_blocks(const AttnShape& a, int tile, int len) {
+  QueryBlocks q;
+  const int j0 = tile << 7, j1 = imin(j0 + 127, len - 1);
+  const int i_max = imin(a.Nq, len - a.off) - 1;         // last valid query
+  q.first = imax(0, j0 - a.off) >> 7;
+  q.last = -1;
+  if (j0 >= len || i_max < 0 || a.W == 0) {
+    q.first = 0;
+    return q;
+  }
+  const int i_hi = a.W >= kNoWindow ? i_max : imin(i_max, j1 + a.W - 1 - a.off);
+  if (i_hi < imax(0, j0 - a.off)) {
+    q.first = 0;
+    return q;
+  }
+  q.last = i_hi >> 7;
+  return q;
+}
+// Query blocks that see key tile 0 only through the visible first keys: those behind the window's, up to the last
+// valid query.
+LUCID_HD QueryBlocks sink_blocks(const AttnShape& a, int len) {
+  const QueryBlocks w = query_blocks(a, 0, len);
+  QueryBlocks q;
+  const int i_max = imin(a.Nq, len - a.off) - 1;
+  q.first = w.last + 1;
+  q.last = (a.S > 0 && i_max >= 0 && len > 0) ? i_max >> 7 : -1;
+  return q;
+}
+
+// dK/dV work items.  Every key tile of a (batch, key head) is one item.  The query blocks that see key tile 0 only
+// through the visible first keys would make its item as long as the sequence: they are dealt out in chunks of
+// `chunk` blocks as items of their own, whose sums meet in fp32 and are added in a fixed order.
+LUCID_HD int sink_chunk_blocks(const AttnShape& a) { return a.W >= kNoWindow ? 1 : imax(8, a.W / 128 + 2); }
+LUCID_HD int sink_chunks(const AttnShape& a) {           // per (batch, key head), from the longest possible sequence
+  if (a.S == 0) return 0;
+  const QueryBlocks q = sink_blocks(a, a.Nk);
+  const int n = q.last - q.first + 1, c = sink_chunk_blocks(a);
+  return n > 0 ? (n + c - 1) / c : 0;
+}
+struct KvItem {
+  int b, hk, tile;
+  int chunk;             // -1: the tile's own item; else the chunk of its first-key blocks
+};
+LUCID_HD int kv_items(const AttnShape& a) { return a.B * a.Hkv * (a.nkb + sink_chunks(a)); }
+LUCID_HD bool kv_item(const AttnShape& a, int chunks, int idx, KvItem& it) {
+  const int per = a.B * a.Hkv;
+  if (idx >= per * (a.nkb + chunks)) return false;
+  const int s = idx / per, r = idx % per;
+  it.b = r / a.Hkv;
+  it.hk = r % a.Hkv;
+  it.chunk = s < chunks ? s : -1;
+  it.tile = s < chunks ? 0 : s - chunks;
+  return true;
+}
+// the blocks of an item; for chunks counted from the longest possible sequence, so that they do not depend on `len`
+LUCID_HD QueryBlocks item_blocks(const AttnShape& a, const KvItem& it, int len) {
+  if (it.chunk < 0) return query_blocks(a, it.tile, len);
+  const QueryBlocks all = sink_blocks(a, len);
+  QueryBlocks q;
+  const int c = sink_chunk_blocks(a);
+  const int base = sink_blocks(a, a.Nk).first;
+  q.first = it.chunk == 0 ? all.first : imax(all.first, base + it.chunk * c);
+  q.last = imin(all.last, base + it.chunk * c + c - 1);
+  return q;
+}
+
+}  // namespace lucid

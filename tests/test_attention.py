@@ -1,0 +1,733 @@
+"""Sliding-window attention with visible first keys (forward, backward), the paged cache and its single-token readers,
+against plain 64-bit formulas.
+
+Tolerances.  u = finfo(dtype).eps / 2 is the unit roundoff of the 16-bit type.  The kernels keep scores, statistics and
+sums in fp32; what they round to 16 bits is (a) the weights P (or dS) before the second product and (b) the result.
+(b) is off by at most u |result|.  (a): each weight is off by at most u times itself, so a sum of weights times values is off
+by at most u * (the same sum with absolute values).  fp32 parts (2^-24 per operation, at most ~2^12 of them, and ex2.approx
+at 2 ulp on arguments off by 2^-24 * |score|) stay below u / 4 of the same bound sums for the sizes here.  So every
+comparison is elementwise |got - ref| <= 1.25 u * bound + u |ref|, with `bound` the sum of absolute values that the formula
+itself gives, evaluated in 64 bits; for gradients dS itself carries P's and delta's errors, counted where they arise."""
+import math
+import os
+import subprocess
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+D = 128
+gpu = pytest.mark.gpu
+
+
+def unit(dt):
+    return torch.finfo(dt).eps / 2
+
+
+# ------------------------------------------------------------------------------------------------ references
+def visible(Nq, Nk, window, sinks, n, device="cpu"):
+    p = torch.arange(Nq, device=device)[:, None] + Nk - Nq
+    j = torch.arange(Nk, device=device)[None]
+    near = (j > p - window) if window is not None else torch.ones(1, 1, dtype=torch.bool, device=device)
+    first = (j < sinks) if window is not None else torch.zeros(1, 1, dtype=torch.bool, device=device)
+    return (j <= p) & (near | first) & (j < n) & (p < n)
+
+
+def reference(q, k, v, window, sinks, scale, lengths, dout=None):
+    """Output, lse and gradients in 64 bits, each with the sum of absolute values that its rounding errors scale with."""
+    B, Nq, Hq, _ = q.shape
+    Nk, Hkv = k.shape[1:3]
+    G = Hq // Hkv
+    out, bound = torch.zeros(B, Nq, Hq, D, dtype=torch.float64, device=q.device), torch.zeros(B, Nq, Hq, D, dtype=torch.float64, device=q.device)
+    lse = torch.full((B, Hq, Nq), -math.inf, dtype=torch.float64, device=q.device)
+    grads = [torch.zeros(t.shape, dtype=torch.float64, device=q.device) for t in (q, k, v)] if dout is not None else None
+    gb = [torch.zeros_like(g) for g in grads] if dout is not None else None
+    for b in range(B):
+        n = Nk if lengths is None else int(lengths[b])
+        ok = visible(Nq, Nk, window, sinks, n, q.device)
+        rows = ok.any(1)
+        for h in range(Hq):
+            hk = h // G
+            qq, kk, vv = (torch.where(torch.isfinite(t), t, torch.zeros_like(t)).double() for t in (q[b, :, h], k[b, :, hk], v[b, :, hk]))
+            s = (qq @ kk.T * scale).masked_fill(~ok, -math.inf)
+            lse[b, h] = torch.logsumexp(s, -1)
+            P = torch.where(ok, torch.exp(s - torch.where(rows, lse[b, h], torch.zeros_like(lse[b, h]))[:, None]), torch.zeros_like(s))
+            out[b, :, h] = P @ vv
+            bound[b, :, h] = P @ vv.abs()
+            if dout is not None:
+                do = torch.where(torch.isfinite(dout[b, :, h]), dout[b, :, h], torch.zeros_like(dout[b, :, h])).double()
+                dP = do @ vv.T
+                delta = (do * out[b, :, h]).sum(-1, keepdim=True)
+                dS = P * (dP - delta)
+                # delta is formed from the rounded output: off by u * (|do| . |out|), and by what the output's own
+                # weights' rounding adds, u * (|do| . bound)
+                dd = (do.abs() * (out[b, :, h].abs() + 1.25 * bound[b, :, h])).sum(-1, keepdim=True)
+                eS = dS.abs() + P * dd
+                grads[0][b, :, h] = scale * dS @ kk
+                gb[0][b, :, h] = scale * eS @ kk.abs()
+                grads[1][b, :, hk] += scale * dS.T @ qq
+                gb[1][b, :, hk] += scale * eS.T @ qq.abs()
+                grads[2][b, :, hk] += P.T @ do
+                gb[2][b, :, hk] += P.T @ do.abs()
+    return out, bound, lse, grads, gb
+
+
+def close(got, ref, bound, dt, what=""):
+    u = unit(dt)
+    tiny = torch.finfo(dt).tiny if dt == torch.float16 else 0.0     # fp16 results below its normal range round in steps of 2^-24
+    lim = 1.25 * u * bound + u * ref.abs() + u * tiny + 1e-30
+    err = (got.double() - ref).abs()
+    assert torch.isfinite(got).all(), what
+    bad = err > lim
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((err / lim).max()):.3f} times the bound"
+
+
+def make(B, Nq, Nk, Hq, Hkv, dt, seed=0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g).to(dt)
+    return rnd(B, Nq, Hq, D), rnd(B, Nk, Hkv, D), rnd(B, Nk, Hkv, D), rnd(B, Nq, Hq, D)
+
+
+# ------------------------------------------------------------------------------------------------ host side
+def test_tile_lists_cover_every_visible_pair_once(tmp_path):
+    import shutil
+
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no host compiler")
+    exe = str(tmp_path / "attn_tiles")
+    subprocess.run([gxx, "-O2", "-std=c++17", "-I", os.path.join(ROOT, "lucid_kernels_b200", "csrc"), "-o", exe,
+                    os.path.join(ROOT, "tests", "host", "attn_tiles.cpp")], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout
+    assert out.stdout.startswith("ok ")
+
+
+def test_refusals_of_the_c_entry_points():
+    """Every refused argument is refused on the host, before anything is launched (no device needed)."""
+    import ctypes
+
+    from lucid_kernels_b200 import _cabi
+
+    lib = _cabi.load()
+    buf = ctypes.create_string_buffer(1 << 16)
+    p = (ctypes.addressof(buf) + 1023) // 1024 * 1024
+    I3, I2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
+    st, s2 = I3(512 * 1024, 1024, 128), I2(1024, 128)
+
+    def fwd(q=p, Nq=512, Nk=512, Hq=4, Hkv=2, Dh=128, dt=1, w=128, s=0, scale=0.1, lse=p, qs=st):
+        return lib.lucid_window_attn_fwd(q, p, p, p, lse, qs, st, st, st, 1, Nq, Nk, Hq, Hkv, Dh, dt, w, s, scale, None, None)
+
+    assert fwd(Dh=64) == -1 and fwd(Nq=0) == -1 and fwd(Nq=513) == -1 and fwd(s=129) == -1 and fwd(s=-1) == -1
+    assert fwd(Hq=3) == -10 and fwd(dt=2) == -2 and fwd(q=None) == -5 and fwd(lse=None) == -5 and fwd(q=p + 2) == -3
+    assert fwd(scale=0.0) == -13 and fwd(scale=float("nan")) == -13 and fwd(scale=float("inf")) == -13
+    assert fwd(qs=I3(512 * 1024, 1028, 128)) == -3 and fwd(qs=I3(512 * 1024, 0, 128)) == -9
+    assert fwd(Nk=1 << 29) == -1
+
+    def bwd(ws=p, wsb=1 << 40, dk=p, dv=p, dq=p):
+        return lib.lucid_window_attn_bwd(p, p, p, p, p, p, dq, dk, dv, *[st] * 8, 1, 512, 512, 4, 2, 128, 1, 128, 4, 0.1, None, ws, wsb, None)
+
+    assert bwd(ws=None) == -5 and bwd(ws=p + 4) == -3 and bwd(wsb=100) == -4 and bwd(dk=None) == -5
+    assert lib.lucid_window_attn_bwd_workspace_bytes(1, 512, 512, 4, 2, 128, 0) == 4 * 512 * 8
+    assert lib.lucid_window_attn_bwd_workspace_bytes(1, 512, 512, 4, 3, 128, 0) == 0
+
+    def cache(**kw):
+        a = dict(k=p, v=p, k_strides=I3(64 * 256, 256, 128), v_strides=I3(64 * 256, 256, 128), block_table=p, table_stride=4, table_width=4,
+                 pages=8, page_rows=64)
+        a.update(kw)
+        return ctypes.byref(_cabi.PagedCache(**a))
+
+    def app(c=None, T=3, cu=p, rot=128, freq=p, q=None, q_out=None, dt=1, k=p, lens=p, B=2):
+        return lib.lucid_paged_append(k, p, q, q_out, s2, s2, s2, c or cache(), lens, cu, freq, B, T, 4, 2, 128, rot, 0, dt, None)
+
+    assert app(T=0) == -1 and app(cu=None) == -1 and app(rot=120) == -12 and app(rot=144) == -12 and app(dt=5) == -2
+    assert app(k=None) == -5 and app(lens=None) == -5 and app(q=p) == -5 and app(q=p, q_out=p, freq=None) == -5 and app(k=p + 4) == -3
+    for bad in (dict(page_rows=48), dict(page_rows=0), dict(pages=0), dict(table_width=0), dict(page_rows=131072)):
+        assert app(cache(**bad)) == -11, bad
+    assert app(cache(block_table=None)) == -5 and app(cache(table_stride=3)) == -9 and app(cache(k=p + 8)) == -3
+    assert app(cache(k_strides=I3(0, 256, 128))) == -9 and app(cache(table_width=1 << 26, table_stride=1 << 26)) == -1
+
+    def step(Hq=4, Hkv=2, scale=0.1, ws=p, wsb=1 << 40, B=2, c=None, lens=p, s=0):
+        return lib.lucid_paged_window_attn(p, p, s2, c or cache(), lens, B, Hq, Hkv, 128, 1, 100, s, scale, ws, wsb, None)
+
+    assert step(Hq=5) == -10 and step(scale=-1.0) == -13 and step(B=0) == -1 and step(B=70000) == -1 and step(lens=None) == -5
+    assert step(s=-1) == -1 and step(ws=None) == -5 and step(wsb=8) == -4 and step(c=cache(page_rows=3)) == -11
+
+    def lucid(Hq=4, ks=1.0, v=p):
+        return lib.lucid_paged_lucid_attn(p, v, p, s2, s2, cache(), p, 2, Hq, 2, 128, 1, ks, 0.1, p, 1 << 40, None)
+
+    assert lucid(Hq=32) == -10 and lucid(ks=0.0) == -13 and lucid(v=None) == -5
+    for code in (-10, -11, -12, -13, 4):
+        assert lib.lucid_status_string(code) != b"unknown"
+
+
+def test_refusals_of_the_python_layer():
+    from lucid_kernels_b200 import paged_append, paged_lucid_attention, paged_window_attention, window_attention
+
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)
+    ok = (z(1, 8, 2, D), z(1, 8, 2, D), z(1, 8, 2, D))
+    for args, kw, text in [
+        ((z(1, 8, 2, 64), z(1, 8, 2, 64), z(1, 8, 2, 64)), {}, "head_dim"),
+        ((z(1, 8, 3, D), ok[1], ok[2]), {}, "multiple"),
+        ((z(1, 9, 2, D), ok[1], ok[2]), {}, "more queries"),
+        ((ok[0], ok[1], z(1, 9, 2, D)), {}, "share"),
+        ((ok[0].half(), ok[1], ok[2]), {}, "dtype"),
+        (tuple(t.float() for t in ok), {}, "float16"),
+        (ok, {}, "CUDA"),
+        (ok, dict(window=-1), "window"),
+        (ok, dict(window=4, sinks=-1), "sinks"),
+    ]:
+        with pytest.raises(AssertionError, match=text):
+            window_attention(*args, **kw)
+    pool, table, lens = z(4, 16, 2, D), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    with pytest.raises(AssertionError, match="CUDA"):
+        paged_append(z(1, 2, D), z(1, 2, D), pool, pool, table, lens)
+    with pytest.raises(AssertionError, match="CUDA"):
+        paged_window_attention(z(1, 4, D), pool, pool, table, lens)
+    with pytest.raises(AssertionError, match="share"):
+        paged_lucid_attention(z(1, 4, D), z(1, 2, D), pool, z(4, 16, 1, D), table, lens)
+
+
+# ------------------------------------------------------------------------------------------------ window attention
+SHAPES = [
+    # B, Nq, Nk, Hq, Hkv, window, sinks
+    (1, 1, 1, 1, 1, None, 0),
+    (1, 128, 128, 2, 1, None, 0),
+    (2, 257, 257, 4, 2, 64, 0),
+    (1, 300, 300, 3, 1, 100, 5),
+    (1, 1000, 1000, 2, 2, 128, 128),
+    (1, 1, 700, 4, 2, 37, 3),
+    (2, 130, 901, 6, 2, 300, 4),
+    (1, 513, 640, 8, 1, 1, 0),
+    (1, 385, 385, 2, 1, 1, 1),
+    (1, 400, 400, 5, 5, None, 0),
+    (3, 129, 129, 2, 2, 129, 7),
+    (1, 2300, 2300, 2, 1, 250, 9),
+    (1, 260, 260, 2, 1, 0, 2),        # first keys only
+    (1, 200, 200, 2, 1, 0, 0),        # nothing visible
+]
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(map(str, s)))
+def test_window_attention_forward_and_backward(shape, dt):
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+
+    B, Nq, Nk, Hq, Hkv, window, sinks = shape
+    q, k, v, do = make(B, Nq, Nk, Hq, Hkv, dt, seed=Nq + Nk)
+    scale = D ** -0.5
+    ref, bound, lse_ref, grads, gb = reference(q, k, v, window, sinks, scale, None, do)
+    out, lse = _window_attention_fwd(q, k, v, window, sinks, scale, check=True)
+    close(out, ref, bound, dt, "out")
+    some = torch.isfinite(lse_ref)
+    assert torch.equal(torch.isneginf(lse), ~some)
+    assert float((lse.double() - lse_ref)[some].abs().max() if some.any() else 0) < 1e-5 * 16
+    got = _window_attention_bwd(q, k, v, out, lse, do, window, sinks, scale, check=True)
+    for name, x, r, b in zip(("dq", "dk", "dv"), got, grads, gb):
+        close(x, r, b, dt, name)
+
+
+@gpu
+@pytest.mark.parametrize("window,sinks,Nq", [(200, 4, 600), (None, 0, 600), (64, 128, 350), (0, 3, 600)])
+def test_padded_batch_ignores_whatever_stands_behind_the_sequences(window, sinks, Nq):
+    """Lengths from nothing to all, NaN and infinities in every padded position of every input."""
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+
+    dt, Nk, Hq, Hkv = torch.bfloat16, 600, 4, 2
+    lens = [600, 0, 1, 127, 128, 129, 257, 599, 300]
+    B = len(lens)
+    q, k, v, do = make(B, Nq, Nk, Hq, Hkv, dt, seed=3)
+    for b, n in enumerate(lens):
+        for t in (k, v):
+            t[b, n:] = float("nan")
+            t[b, n::2] = float("inf")
+        for t in (q, do):
+            t[b, max(0, n - (Nk - Nq)):] = float("nan")
+    lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    scale = 0.07
+    ref, bound, lse_ref, grads, gb = reference(q, k, v, window, sinks, scale, lengths, do)
+    out, lse = _window_attention_fwd(q, k, v, window, sinks, scale, lengths, check=True)
+    close(out, ref, bound, dt, "out")
+    assert torch.equal(torch.isneginf(lse), torch.isneginf(lse_ref))
+    for name, x, r, b in zip(("dq", "dk", "dv"), _window_attention_bwd(q, k, v, out, lse, do, window, sinks, scale, lengths, check=True), grads, gb):
+        close(x, r, b, dt, name)
+        for i, n in enumerate(lens):
+            rows = x[i, max(0, n - (Nk - Nq)):] if name == "dq" else x[i, n:]
+            assert not rows.any(), name
+
+
+@gpu
+def test_strided_expanded_and_misaligned_inputs():
+    from lucid_kernels_b200 import window_attention
+
+    dt = torch.float16
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    qkv = torch.randn(2, 333, 8, D, device="cuda", generator=g).to(dt)
+    q, k, v = qkv.split((4, 2, 2), dim=2)
+    want = window_attention(q.contiguous(), k.contiguous(), v.contiguous(), window=90, sinks=2)
+    assert torch.equal(window_attention(q, k, v, window=90, sinks=2), want)
+    # BHSD-backed, an odd base, a transposed last dimension, one key head expanded over the batch
+    assert torch.equal(window_attention(*(t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)), window=90, sinks=2), want)
+    raw = torch.empty(q.numel() + 3, dtype=dt, device="cuda")[3:].view(q.shape).copy_(q)
+    assert torch.equal(window_attention(raw, k, v, window=90, sinks=2), want)
+    turned = q.transpose(1, 3).contiguous().transpose(1, 3)
+    assert turned.stride(-1) != 1 and torch.equal(window_attention(turned, k, v, window=90, sinks=2), want)
+    k1, v1 = (t[:1].clone().requires_grad_(True) for t in (k, v))
+    qg = q.clone().requires_grad_(True)
+    do = torch.randn(q.shape, device="cuda", generator=g).to(dt)
+    window_attention(qg, k1.expand(2, -1, -1, -1), v1.expand(2, -1, -1, -1), window=90, sinks=2).backward(do)
+    kf, vf = (t.detach().repeat(2, 1, 1, 1).requires_grad_(True) for t in (k1, v1))
+    q2 = q.clone().requires_grad_(True)
+    window_attention(q2, kf, vf, window=90, sinks=2).backward(do)
+    assert torch.equal(qg.grad, q2.grad)
+    assert torch.equal(k1.grad[0], kf.grad.sum(0)) and torch.equal(v1.grad[0], vf.grad.sum(0))
+
+
+@gpu
+def test_gradient_against_differences():
+    """Directional derivatives of the kernel's own forward along one perturbed element block: inputs are exact in 16 bits
+    (multiples of 1/8), the step 1/4, central differences; the second-order remainder and the outputs' rounding are bounded
+    by the 64-bit reference evaluated at the same two points."""
+    from lucid_kernels_b200 import window_attention
+
+    dt, N, W, S = torch.float16, 140, 50, 3
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    q, k, v, do = ((torch.randint(-8, 9, (1, N, h, D), device="cuda", generator=g) / 8).to(dt) for h in (2, 1, 1, 2))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    window_attention(*leaves, window=W, sinks=S).backward(do)
+    loss = lambda a, b, c: float((window_attention(a, b, c, window=W, sinks=S).double() * do.double()).sum())
+    exact = lambda a, b, c: float((reference(a, b, c, W, S, D ** -0.5, None)[0] * do.double()).sum())
+    h = 0.25
+    for at in range(3):
+        d = (torch.randint(0, 3, leaves[at].shape, device="cuda", generator=g) - 1).to(dt)
+        plus, minus = ([t + (h * d if i == at else 0) for i, t in enumerate((q, k, v))], [t - (h * d if i == at else 0) for i, t in enumerate((q, k, v))])
+        slope = float((leaves[at].grad.double() * d.double()).sum())
+        got = (loss(*plus) - loss(*minus)) / (2 * h)
+        curve = (exact(*plus) - exact(*minus)) / (2 * h)              # what differences of this width give in 64 bits
+        u = unit(dt)
+        rounding = 2.25 * u * 2 * float(do.double().abs().sum()) / (2 * h)        # two losses of |out| <= 1, weights and result
+        assert abs(got - curve) <= rounding
+        ref = reference(q, k, v, W, S, D ** -0.5, None, do)
+        assert abs(slope - float((ref[3][at] * d.double()).sum())) <= float(((1.25 * u * ref[4][at] + u * ref[3][at].abs()) * d.double().abs()).sum())
+
+
+@gpu
+def test_extreme_scores_and_growing_maxima():
+    """Scores that span +-600 in base 2 and whose running maximum grows from tile to tile, one row at a time."""
+    from lucid_kernels_b200.attention import _window_attention_fwd
+
+    dt, N = torch.bfloat16, 900
+    q, k, v, _ = make(1, N, N, 2, 1, dt, seed=11)
+    ramp = torch.linspace(0.1, 6.0, N, device="cuda")[None, :, None, None]
+    k = (k * ramp).to(dt)
+    q = (q * torch.linspace(6.0, 0.1, N, device="cuda")[None, :, None, None]).to(dt)
+    for window, sinks in ((None, 0), (400, 2)):
+        scale = 1.0
+        ref, bound, lse_ref, _, _ = reference(q, k, v, window, sinks, scale, None)
+        out, lse = _window_attention_fwd(q, k, v, window, sinks, scale, check=True)
+        # a score s carries an fp32 error of up to D products' roundings, 128 * 2^-24 * sum |q||k|, and a weight that
+        # relative error: e^delta - 1 with delta <= 2^-17 * sum |q||k|
+        size = float((q.double().abs().amax() * k.double().abs().amax()) * 0 + (q.double().norm(dim=-1).amax() * k.double().norm(dim=-1).amax()))
+        extra = math.expm1(2 * 2.0 ** -17 * size * scale)
+        err = (out.double() - ref).abs()
+        assert bool((err <= (1.25 * unit(dt) + extra) * bound + unit(dt) * ref.abs()).all())
+        assert float((lse.double() - lse_ref).abs().max()) <= 2.0 ** -17 * size * scale + 1e-4
+
+
+@gpu
+def test_runs_are_identical_and_graphs_replay():
+    from lucid_kernels_b200 import window_attention
+
+    dt = torch.bfloat16
+    q, k, v, do = make(1, 3000, 3000, 4, 2, dt, seed=21)
+    kw = dict(window=500, sinks=4)
+
+    def step(leaves):
+        o = window_attention(*leaves, **kw)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    a, b = step(leaves), step(leaves)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c = step(leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(a, c))
+    gl = [t.detach().clone().requires_grad_(True) for t in leaves]
+    graphs = []
+    for _ in range(2):                      # two graphs, replayed in turn: they share no scratch memory
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            r = step(gl)
+        graphs.append((g, r))
+    with torch.no_grad():
+        gl[1].mul_(0.5)
+    want = step([t.detach().clone().requires_grad_(True) for t in gl])
+    for g, r in graphs * 2:
+        for x in r:
+            x.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(r, want))
+
+
+@gpu
+def test_partial_gradients_and_empty_tensors():
+    from lucid_kernels_b200 import window_attention
+
+    dt = torch.float16
+    q, k, v, do = make(1, 200, 200, 2, 1, dt)
+    full = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    window_attention(*full, window=70).backward(do)
+    for need in range(3):
+        leaves = [t.clone().requires_grad_(i == need) for i, t in enumerate((q, k, v))]
+        window_attention(*leaves, window=70).backward(do)
+        assert torch.equal(leaves[need].grad, full[need].grad)
+    for B, Nq in ((0, 4), (1, 0)):
+        e = [torch.empty(B, n, h, D, device="cuda", dtype=dt, requires_grad=True) for n, h in ((Nq, 2), (4, 1), (4, 1))]
+        o = window_attention(*e, window=3)
+        assert o.shape == e[0].shape
+        o.sum().backward()
+        assert not e[1].grad.any()
+
+
+# ------------------------------------------------------------------------------------------------ paged cache
+def rotated(x, pos, inv_freq, interleaved=False):
+    """64 bits: x (T, H, D), pos (T,)."""
+    a = pos.double()[:, None, None] * inv_freq.double()
+    r = 2 * inv_freq.numel()
+    y, out = x[..., :r].double(), x.double().clone()
+    if interleaved:
+        p, s = y[..., 0::2], y[..., 1::2]
+        out[..., 0:r:2], out[..., 1:r:2] = p * a.cos() - s * a.sin(), s * a.cos() + p * a.sin()
+    else:
+        p, s = y.chunk(2, -1)
+        out[..., :r] = torch.cat((p * a.cos() - s * a.sin(), s * a.cos() + p * a.sin()), -1)
+    return out
+
+
+def frequencies(rot=D):
+    return (10000.0 ** (-torch.arange(rot // 2, dtype=torch.float64) * 2 / rot)).float().cuda()
+
+
+def pool_of(B, cap, page, Hkv, dt, seed=0, fill=None):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    per = -(-cap // page)
+    pages = B * per + 2
+    table = torch.randperm(pages, device="cuda", generator=g)[: B * per].reshape(B, per).to(torch.int32)
+    mk = lambda: torch.randn(pages, page, Hkv, D, device="cuda", generator=g).to(dt) if fill is None else torch.full((pages, page, Hkv, D), fill, device="cuda", dtype=dt)
+    return mk(), mk(), table
+
+
+def close_rotation(got, ref, x, dt):
+    """A rotated element is a sum of two fp32 products, rounded once: u |ref| and fp32 errors of the inputs' size (sines to
+    2^-21, products and sum)."""
+    size = x.double().abs().amax()
+    assert bool(((got.double() - ref).abs() <= unit(dt) * ref.abs() + 2.0 ** -19 * size + (2.0 ** -25 if dt == torch.float16 else 0)).all())
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("page,Hq,Hkv,rot,interleaved", [(16, 8, 4, 128, False), (64, 3, 1, 128, True), (1, 2, 2, 32, False),
+                                                         (256, 4, 1, 48, True), (128, 16, 16, 16, False)])
+def test_append_rotates_and_places(page, Hq, Hkv, rot, interleaved, dt):
+    from lucid_kernels_b200 import paged_append
+
+    new, before = [1, 0, 37, 300, 64], [5, 100, 0, 255, 999_000]
+    B = len(new)
+    per = [-(-(n + m) // page) for n, m in zip(new, before)]
+    width = max(per)
+    pages = sum(-(-n // page) + 1 for n in new) + 3
+    free = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).tolist()
+    table = torch.full((B, width), -7, dtype=torch.int32)                 # only the pages that new tokens reach exist
+    for b in range(B):
+        for i in range(before[b] // page, per[b]):
+            if new[b]:
+                table[b, i] = free.pop()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    T = sum(new) + 3                                                      # three rows of padding behind the last sequence
+    qkv = torch.randn(T, Hq + 2 * Hkv, D, device="cuda", generator=g).to(dt)
+    q, k, v = qkv.split((Hq, Hkv, Hkv), 1)
+    kc = torch.full((pages, page, Hkv, D), 3.0, device="cuda", dtype=dt)
+    vc = kc.clone()
+    f = frequencies(rot)
+    cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    lens = torch.tensor(before, dtype=torch.int32, device="cuda")
+    ver = kc._version
+    got = paged_append(k, v, kc, vc, table.cuda(), lens, cu_seqlens=cu, q=q, inv_freq=f, interleaved=interleaved, check=True)
+    assert kc._version > ver
+    assert not got[sum(new):].any()
+    touched = torch.zeros(pages, page, dtype=torch.bool, device="cuda")
+    for b in range(B):
+        for i in range(new[b]):
+            t, pos = int(cu[b]) + i, before[b] + i
+            touched[int(table[b, pos // page]), pos % page] = True
+    pos = torch.cat([torch.arange(n) + m for n, m in zip(new, before)]).cuda()
+    seq = torch.cat([torch.full((n,), b) for b, n in enumerate(new)])
+    pg = table[seq, (pos.cpu() // page)].long().cuda()
+    n = sum(new)
+    close_rotation(kc[pg, pos % page], rotated(k[:n], pos, f, interleaved), k, dt)
+    close_rotation(got[:n], rotated(q[:n], pos, f, interleaved), q, dt)
+    assert torch.equal(vc[pg, pos % page], v[:n])
+    assert torch.equal(kc[pg, pos % page][..., rot:], k[:n, :, rot:])
+    assert bool((kc[~touched] == 3.0).all()) and bool((vc[~touched] == 3.0).all())
+
+
+@gpu
+def test_append_single_tokens_without_rotation_keys_only_and_interleaved_pools():
+    from lucid_kernels_b200 import paged_append
+
+    dt, B, page, Hkv = torch.bfloat16, 70, 32, 2
+    both = torch.zeros(B * 2, 2, page, Hkv, D, device="cuda", dtype=dt)          # one pool, keys and values side by side
+    kc, vc = both[:, 0], both[:, 1]
+    table = torch.arange(B * 2, device="cuda", dtype=torch.int32).reshape(B, 2)
+    lens = torch.arange(B, device="cuda", dtype=torch.int32) % 64
+    g = torch.Generator(device="cuda")
+    g.manual_seed(0)
+    k, v = (torch.randn(B, Hkv, D, device="cuda", generator=g).to(dt) for _ in range(2))
+    assert paged_append(k, None, kc, vc, table, lens, check=True) is None
+    rows = table.long()[torch.arange(B), (lens // page).long()], (lens % page).long()
+    assert torch.equal(kc[rows], k) and not vc.any()
+    paged_append(k, v, kc, vc, table, lens, check=True)
+    assert torch.equal(vc[rows], v)
+
+
+@gpu
+def test_bad_pages_are_skipped_and_reported():
+    """No address is formed from a page outside the pool or a position beyond the table: the host's view of the bounds is
+    page_of / the append kernel's own check, and the error is reported once."""
+    from lucid_kernels_b200 import _cabi, paged_append, paged_lucid_attention, paged_window_attention
+
+    dt, page, Hkv = torch.bfloat16, 16, 1
+    kc, vc, table = pool_of(2, 64, page, Hkv, dt, seed=4)
+    k0, v0 = kc.clone(), vc.clone()
+    x = torch.ones(2, Hkv, D, device="cuda", dtype=dt)
+    lens = torch.tensor([64, 3], dtype=torch.int32, device="cuda")               # sequence 0: behind the table
+    with pytest.raises(_cabi.LucidKernelError, match="block table"):
+        paged_append(x, x, kc, vc, table, lens, check=True)
+    changed = (kc != k0).any(-1).any(-1)
+    assert int(changed.sum()) == 1 and bool(changed[int(table[1, 0]), 3])
+    bad = table.clone()
+    bad[1, 1] = kc.shape[0]
+    bad[0, 0] = -1
+    q = torch.randn(2, 2, D, device="cuda").to(dt)
+    n = torch.tensor([20, 40], dtype=torch.int32, device="cuda")
+    with pytest.raises(_cabi.LucidKernelError, match="block table"):
+        paged_window_attention(q, kc, vc, bad, n, check=True)
+    v1 = vc.clone()
+    n = torch.tensor([16, 17], dtype=torch.int32, device="cuda")                  # the newest position's page is the bad one
+    with pytest.raises(_cabi.LucidKernelError, match="block table"):
+        paged_lucid_attention(q, x, kc, vc, bad, n, check=True)
+    assert torch.equal(vc, v1)
+    paged_window_attention(q, kc, vc, table, n, check=True)                       # reported once, then forgotten
+
+
+def step_reference(q, kc, vc, table, lens, window, sinks, scale, v=None, k_scale=1.0):
+    """(out, bound, v', its bound) in 64 bits."""
+    B, Hq, _ = q.shape
+    page, Hkv = kc.shape[1:3]
+    G = Hq // Hkv
+    out = torch.zeros(B, Hq, D, dtype=torch.float64, device=q.device)
+    bound, new, nb = torch.zeros_like(out), torch.zeros(B, Hkv, D, dtype=torch.float64, device=q.device), torch.zeros(B, Hkv, D, dtype=torch.float64, device=q.device)
+    for b in range(B):
+        n = int(lens[b])
+        if n == 0:
+            continue
+        pos = torch.arange(n, device=q.device)
+        if window is not None:
+            pos = pos[(pos >= n - window) | (pos < sinks)]
+        pg = table[b].long()[pos // page]
+        kk, vv = kc[pg, pos % page].double(), vc[pg, pos % page].double()
+        for h in range(Hkv):
+            K, V = kk[:, h], vv[:, h].clone()
+            if v is not None:
+                t = K @ K[-1] * k_scale ** 2
+                w = torch.exp(t[:-1] - t[-1])
+                new[b, h] = torch.exp(-t[-1]) * v[b, h].double() - w @ V[:-1]
+                nb[b, h] = w @ V[:-1].abs()
+                V[-1] = new[b, h]
+            if len(pos):
+                P = torch.softmax(q[b, h * G:(h + 1) * G].double() @ K.T * scale, -1)
+                out[b, h * G:(h + 1) * G] = P @ V
+                bound[b, h * G:(h + 1) * G] = P @ V.abs()
+                if v is not None:      # v'_n enters rounded, with its own error
+                    bound[b, h * G:(h + 1) * G] += P[:, -1:] * (nb[b, h] + new[b, h].abs())
+    return out, bound, new, nb
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("page,Hq,Hkv,window,sinks,lens", [
+    (16, 8, 4, None, 0, [1, 0, 17, 64, 500]),
+    (64, 4, 4, 100, 4, [1, 99, 100, 101, 104, 105, 700]),
+    (1, 2, 1, 1, 0, [1, 2, 3]),
+    (32, 6, 2, 5, 300, [4, 5, 6, 250, 305, 306, 1000]),
+    (128, 16, 1, None, 0, [1023]),
+    (256, 40, 2, 64, 1, [3, 70, 2000]),
+    (64, 3, 3, 0, 3, [1, 2, 3, 4, 90]),
+    (64, 3, 3, 0, 0, [1, 90]),
+    (64, 4, 1, None, 0, [9000]),
+])
+def test_paged_window_attention(page, Hq, Hkv, window, sinks, lens, dt):
+    from lucid_kernels_b200 import paged_window_attention
+
+    B = len(lens)
+    kc, vc, table = pool_of(B, max(max(lens), 1), page, Hkv, dt, seed=7)
+    for b, n in enumerate(lens):          # what no sequence owns, or lies behind one's end in its last page, holds anything
+        if n % page:
+            kc[table[b, n // page].long(), n % page:] = float("nan")
+            vc[table[b, n // page].long(), n % page:] = float("inf")
+    q = torch.randn(B, Hq, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(dt)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = paged_window_attention(q, kc, vc, table, sl, window, sinks, check=True)
+    ref, bound, _, _ = step_reference(q, kc, vc, table, lens, window, sinks, D ** -0.5)
+    close(out, ref, bound, dt, "out")
+    # strided queries: a slice of a projection
+    wide = torch.randn(B, Hq + 4, D, device="cuda").to(dt)
+    wide[:, 2:Hq + 2] = q
+    assert torch.equal(paged_window_attention(wide[:, 2:Hq + 2], kc, vc, table, sl, window, sinks), out)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("page,Hq,Hkv,lens", [(16, 8, 4, [1, 0, 2, 17, 64, 500]), (64, 1, 1, [3000]), (128, 15, 1, [129, 128]), (1, 4, 2, [5, 1]),
+                                              (32, 2, 2, [33] * 40)])
+def test_paged_lucid_attention(page, Hq, Hkv, lens, dt):
+    from lucid_kernels_b200 import paged_lucid_attention
+
+    B, ks = len(lens), D ** -0.25
+    kc, vc, table = pool_of(B, max(max(lens), 1), page, Hkv, dt, seed=8)
+    kc.mul_(0.5)
+    vc.mul_(0.1)
+    for b, n in enumerate(lens):
+        if n % page:
+            kc[table[b, n // page].long(), n % page:] = float("nan")
+            vc[table[b, n // page].long(), n % page:] = float("nan")
+        if n:
+            vc[table[b, (n - 1) // page].long(), (n - 1) % page] = float("nan")     # the new row's place is not read
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, v = torch.randn(B, Hq, D, device="cuda", generator=g).to(dt), torch.randn(B, Hkv, D, device="cuda", generator=g).to(dt)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ref, bound, new, nb = step_reference(q, kc, vc, table, lens, None, 0, 0.1, v, ks)
+    before = vc.clone()
+    out = paged_lucid_attention(q, v, kc, vc, table, sl, k_scale=ks, scale=0.1, check=True)
+    close(out, ref, bound, dt, "out")
+    changed = torch.zeros(vc.shape[:2], dtype=torch.bool, device="cuda")
+    for b, n in enumerate(lens):
+        if n:
+            at = int(table[b, (n - 1) // page]), (n - 1) % page
+            close(vc[at], new[b], nb[b], dt, "v'")
+            changed[at] = True
+    assert torch.equal(vc[~changed].view(torch.int16), before[~changed].view(torch.int16))
+    again = paged_lucid_attention(q, v, kc, vc, table, sl, k_scale=ks, scale=0.1, check=True)
+    assert torch.equal(again, out)
+
+
+@gpu
+def test_cache_operators_captured_and_on_another_stream():
+    from lucid_kernels_b200 import paged_append, paged_lucid_attention, paged_window_attention
+
+    dt, B, Hq, Hkv, page = torch.bfloat16, 3, 4, 2, 32
+    kc, vc, table = pool_of(B, 2000, page, Hkv, dt, seed=5)
+    vc.mul_(1e-3)
+    lens = torch.tensor([700, 31, 1999], dtype=torch.int32, device="cuda")
+    q, k, v = (torch.randn(B, h, D, device="cuda").to(dt) for h in (Hq, Hkv, Hkv))
+    f = frequencies()
+
+    def step(kc, vc):
+        qr = paged_append(k, None, kc, vc, table, lens, q=q, inv_freq=f)
+        a = paged_lucid_attention(qr, v, kc, vc, table, lens + 1, k_scale=D ** -0.25)
+        return a, paged_window_attention(qr, kc, vc, table, lens + 1, 300, 4)
+
+    k1, v1 = kc.clone(), vc.clone()
+    want = step(k1, v1)
+    side = torch.cuda.Stream()
+    k2, v2 = kc.clone(), vc.clone()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step(k2, v2)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(want, other)) and torch.equal(k1, k2) and torch.equal(v1, v2)
+    k3, v3 = kc.clone(), vc.clone()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            r = step(k3, v3)
+        graphs.append((g, r))
+    for g, r in graphs * 2:
+        k3.copy_(kc)
+        v3.copy_(vc)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(r, want)) and torch.equal(v3, v1)
+    lens.fill_(5)                                   # a replay reads the lengths of its own time
+    k4, v4 = kc.clone(), vc.clone()
+    want = step(k4, v4)
+    k3.copy_(kc)
+    v3.copy_(vc)
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(graphs[0][1], want))
+
+
+# ------------------------------------------------------------------------------------------------ together
+@gpu
+def test_prompt_and_steps_equal_one_long_run():
+    """A LUCID layer and a window layer, prompt then tokens one by one through the cache, against the whole sequence at once:
+    rotation, solve, V' and attention.  Reference: 64 bits from the 16-bit projections, with the cache's 16-bit keys."""
+    from lucid_kernels_b200 import paged_append, paged_lucid_attention, paged_window_attention, window_attention
+    from lucid_kernels_b200.cute import _forward_sub_fwd
+
+    dt, P, extra, Hq, Hkv, page, W, S = torch.bfloat16, 256, 20, 4, 2, 16, 60, 3
+    N, ks = P + extra, D ** -0.25
+    g = torch.Generator(device="cuda").manual_seed(12)
+    q, k, v = (torch.randn(N, h, D, device="cuda", generator=g).to(dt) for h in (Hq, Hkv, Hkv))
+    k = (k * 0.7).to(dt)
+    f = frequencies()
+    out = {}
+    for kind in ("window", "lucid"):
+        kc, vc, table = pool_of(1, N, page, Hkv, dt, seed=3, fill=float("nan"))
+        zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+        cu = torch.tensor([0, P], dtype=torch.int32, device="cuda")
+        qr = paged_append(k[:P], v[:P], kc, vc, table, zero, cu_seqlens=cu, q=q[:P], inv_freq=f, check=True)
+        pos = torch.arange(N, device="cuda")
+        at = table[0].long()[pos // page], pos % page
+        kr = kc[at][:P]
+        if kind == "window":
+            rows = [window_attention(qr[None], kr[None], v[None, :P], W, S)[0]]
+        else:
+            vp = _forward_sub_fwd(kr[None], v[None, :P], k_scale=ks)
+            vc[at[0][:P], at[1][:P]] = vp[0]
+            rows = [window_attention(qr[None], kr[None], vp, scale=ks * D ** -0.5)[0]]
+        for n in range(P, N):
+            have = torch.full((1,), n, dtype=torch.int32, device="cuda")
+            qn = paged_append(k[n:n + 1], None if kind == "lucid" else v[n:n + 1], kc, vc, table, have, q=q[n:n + 1], inv_freq=f, check=True)
+            if kind == "window":
+                rows.append(paged_window_attention(qn, kc, vc, table, have + 1, W, S, check=True))
+            else:
+                rows.append(paged_lucid_attention(qn, v[n:n + 1], kc, vc, table, have + 1, k_scale=ks, scale=ks * D ** -0.5, check=True))
+        out[kind] = torch.cat(rows).double(), kc[at].double(), vc[at].double()
+    pos = torch.arange(N, device="cuda")
+    qq = rotated(q, pos, f)
+    for kind, (o, kk, vv) in out.items():
+        scale = D ** -0.5 * (ks if kind == "lucid" else 1)
+        for h in range(Hkv):
+            V = v[:, h].double()
+            if kind == "lucid":
+                E = torch.exp(torch.tril(kk[:, h] @ kk[:, h].T * ks * ks)) * torch.tril(torch.ones(N, N, device="cuda", dtype=torch.float64))
+                V = torch.linalg.solve_triangular(E, V, upper=False)
+                assert float((vv[:, h] - V).norm() / V.norm()) < 0.01       # the solve's own tolerance
+            for i in range(Hq // Hkv):
+                x = h * (Hq // Hkv) + i
+                ok = visible(N, N, None if kind == "lucid" else W, S, N, "cuda")
+                ref = torch.softmax((qq[:, x] @ kk[:, h].T * scale).masked_fill(~ok, -math.inf), -1) @ V
+                assert float((o[:, x] - ref).norm() / ref.norm()) < 0.01
