@@ -251,21 +251,25 @@ void lucid_profile_next_call(void* ev_begin, void* ev_after_prep, void* ev_after
  * (`sinks` then has no meaning); 0 <= sinks <= 128.  lengths (B int32 on the device, or NULL): positions at or beyond
  * lengths[b] are neither keys nor queries, whatever the tensors hold there.  A query that sees nothing gives 0 and
  * lse = -infinity; otherwise lse (B, Hq, Nq), fp32, is the natural log of its sum of exponentials of scale * q.k.
+ * What describes a call (sizes, strides, options) is one read-only struct that calls may share.
  * Values at positions inside a sequence must be finite: rows of a 128-row tile share a matrix product. */
-int lucid_window_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int64_t q_strides[3],
-                          const int64_t k_strides[3], const int64_t v_strides[3], const int64_t out_strides[3], int B,
-                          int Nq, int Nk, int Hq, int Hkv, int D, int dtype, int window, int sinks, float scale,
-                          const int32_t* lengths, void* cuda_stream);
+typedef struct {
+  int32_t B, Nq, Nk, Hq, Hkv, D, dtype, window, sinks;
+  float scale;
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];      /* forward and backward */
+  int64_t dout_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];  /* backward */
+} lucid_window_attn_desc;
+
+/* lse may be NULL (not wanted). */
+int lucid_window_attn_fwd(const lucid_window_attn_desc* desc, const void* q, const void* k, const void* v, void* out,
+                          float* lse, const int32_t* lengths, void* cuda_stream);
 
 /* Its gradients, from the forward's out and lse.  dq, or dk and dv together, may be NULL (not computed).  Sums are fp32
  * in a fixed order (no atomics: the same bits on every run).  Workspace 16-byte aligned, contents irrelevant. */
-size_t lucid_window_attn_bwd_workspace_bytes(int B, int Nq, int Nk, int Hq, int Hkv, int window, int sinks);
-int lucid_window_attn_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout,
-                          void* dq, void* dk, void* dv, const int64_t q_strides[3], const int64_t k_strides[3],
-                          const int64_t v_strides[3], const int64_t out_strides[3], const int64_t dout_strides[3],
-                          const int64_t dq_strides[3], const int64_t dk_strides[3], const int64_t dv_strides[3], int B, int Nq,
-                          int Nk, int Hq, int Hkv, int D, int dtype, int window, int sinks, float scale,
-                          const int32_t* lengths, void* workspace, size_t workspace_bytes, void* cuda_stream);
+size_t lucid_window_attn_bwd_workspace_bytes(const lucid_window_attn_desc* desc);
+int lucid_window_attn_bwd(const lucid_window_attn_desc* desc, const void* q, const void* k, const void* v, const void* out,
+                          const float* lse, const void* dout, void* dq, void* dk, void* dv, const int32_t* lengths,
+                          void* workspace, size_t workspace_bytes, void* cuda_stream);
 
 /* A paged key/value cache: pools (pages, page_rows, Hkv, 128) with element strides {page, row, head} (bases 16-byte
  * aligned, strides multiples of 8), page_rows a power of two, and a block table (B, table_width) of page numbers on the
@@ -273,43 +277,50 @@ int lucid_window_attn_bwd(const void* q, const void* k, const void* v, const voi
  * block_table[b][p / page_rows].  A position beyond the table, or a page outside the pool, is skipped and recorded
  * (status 4, lucid_attn_status). */
 typedef struct {
-  void* k;
-  void* v;
-  int64_t k_strides[3];
-  int64_t v_strides[3];
-  const int32_t* block_table;
+  int32_t pages, page_rows, table_width;
   int64_t table_stride;
-  int32_t table_width;
-  int32_t pages;
-  int32_t page_rows;
-} lucid_paged_cache;
+  int64_t k_strides[3], v_strides[3];
+} lucid_paged_cache_desc;
 
 /* Appends T tokens: token t of sequence b (cu_seqlens[b] <= t < cu_seqlens[b+1]; NULL: token b is sequence b's only one,
  * T == B) goes to position cache_lens[b] + t - cu_seqlens[b].  With inv_freq (rotated / 2 fp32 values) the first
  * `rotated` elements of every key, and of every query of q, are rotated by position * inv_freq: pairs (i, i + rotated/2),
  * or (2i, 2i + 1) with `interleaved`.  q_out (T, Hq, 128) contiguous.  v may be NULL (keys only), q may be NULL.  Tokens
  * behind the last sequence write nothing to the cache; their queries come back as zeros.  cache_lens is not changed. */
-int lucid_paged_append(const void* k, const void* v, const void* q, void* q_out, const int64_t k_strides[2],
-                       const int64_t v_strides[2], const int64_t q_strides[2], const lucid_paged_cache* cache,
-                       const int32_t* cache_lens, const int32_t* cu_seqlens, const float* inv_freq, int B, int T, int Hq,
-                       int Hkv, int D, int rotated, int interleaved, int dtype, void* cuda_stream);
+typedef struct {
+  lucid_paged_cache_desc cache;
+  int32_t B, T, Hq, Hkv, D, rotated, interleaved, dtype;
+  int64_t k_strides[2], v_strides[2], q_strides[2];                      /* {token, head} */
+} lucid_paged_append_desc;
+
+int lucid_paged_append(const lucid_paged_append_desc* desc, const void* k, const void* v, const void* q, void* q_out,
+                       void* k_cache, void* v_cache, const int32_t* block_table, const int32_t* cache_lens,
+                       const int32_t* cu_seqlens, const float* inv_freq, void* cuda_stream);
 
 /* One query token per sequence, at position seq_lens[b] - 1, over the cache: the single-token form of
  * lucid_window_attn_fwd (sinks of any size).  seq_lens[b] = 0 gives 0.  out (B, Hq, 128) contiguous. */
-size_t lucid_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int page_rows, int table_width, int window, int sinks,
-                                        int lucid_step);
-int lucid_paged_window_attn(const void* q, void* out, const int64_t q_strides[2], const lucid_paged_cache* cache,
-                            const int32_t* seq_lens, int B, int Hq, int Hkv, int D, int dtype, int window, int sinks,
-                            float scale, void* workspace, size_t workspace_bytes, void* cuda_stream);
+typedef struct {
+  lucid_paged_cache_desc cache;
+  int32_t B, Hq, Hkv, D, dtype;
+  int32_t window, sinks;                 /* lucid_paged_window_attn */
+  float scale;
+  float k_scale;                         /* lucid_paged_lucid_attn  */
+  int64_t q_strides[2], v_strides[2];    /* {sequence, head}        */
+} lucid_paged_attn_desc;
+
+size_t lucid_paged_attn_workspace_bytes(const lucid_paged_attn_desc* desc, int lucid_step);
+int lucid_paged_window_attn(const lucid_paged_attn_desc* desc, const void* q, void* out, const void* k_cache,
+                            const void* v_cache, const int32_t* block_table, const int32_t* seq_lens, void* workspace,
+                            size_t workspace_bytes, void* cuda_stream);
 
 /* The single-token form of lucid_fwd_sub_scaled with the attention on its result.  The cache holds the keys of positions
  * 0 .. n (n = seq_lens[b] - 1, appended before) and V' of positions 0 .. n-1; v (B, Hkv, 128) is the new token's value.
  *   v'_n = exp(-t_n) v_n - sum_{j<n} exp(t_j - t_n) v'_j,  t_j = k_scale^2 k_n.k_j    (written to position n of the cache)
  *   out  = softmax over j <= n of scale q.k_j, applied to V'
  * At most 15 query heads per key head.  seq_lens[b] = 0: out = 0, nothing written. */
-int lucid_paged_lucid_attn(const void* q, const void* v, void* out, const int64_t q_strides[2], const int64_t v_strides[2],
-                           const lucid_paged_cache* cache, const int32_t* seq_lens, int B, int Hq, int Hkv, int D, int dtype,
-                           float k_scale, float scale, void* workspace, size_t workspace_bytes, void* cuda_stream);
+int lucid_paged_lucid_attn(const lucid_paged_attn_desc* desc, const void* q, const void* v, void* out, const void* k_cache,
+                           void* v_cache, const int32_t* block_table, const int32_t* seq_lens, void* workspace,
+                           size_t workspace_bytes, void* cuda_stream);
 
 /* Synchronises the stream and takes the first device-side error of these entry points on the current device since the
  * last call (it is then forgotten): out[0] = 0 ok / 1 a wait ran out / 3 left early after that / 4 bad page; out[1] =

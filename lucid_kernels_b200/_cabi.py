@@ -37,11 +37,31 @@ EXPORTS = ("lucid_workspace_bytes", "lucid_fwd_sub", "lucid_bwd_sub", "lucid_rea
            "lucid_paged_window_attn", "lucid_paged_lucid_attn", "lucid_paged_attn_workspace_bytes", "lucid_attn_status")
 
 
-class PagedCache(ctypes.Structure):
-    """``lucid_paged_cache``"""
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_strides", _I64x3), ("v_strides", _I64x3),
-                ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32),
-                ("pages", ctypes.c_int32), ("page_rows", ctypes.c_int32)]
+class WindowAttnDesc(ctypes.Structure):
+    """``lucid_window_attn_desc``"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "Nq", "Nk", "Hq", "Hkv", "D", "dtype", "window", "sinks")] + \
+        [("scale", ctypes.c_float)] + \
+        [(n + "_strides", _I64x3) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")]
+
+
+class PagedCacheDesc(ctypes.Structure):
+    """``lucid_paged_cache_desc``"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("pages", "page_rows", "table_width")] + \
+        [("table_stride", ctypes.c_int64), ("k_strides", _I64x3), ("v_strides", _I64x3)]
+
+
+class PagedAppendDesc(ctypes.Structure):
+    """``lucid_paged_append_desc``"""
+    _fields_ = [("cache", PagedCacheDesc)] + \
+        [(n, ctypes.c_int32) for n in ("B", "T", "Hq", "Hkv", "D", "rotated", "interleaved", "dtype")] + \
+        [(n + "_strides", _I64x2) for n in ("k", "v", "q")]
+
+
+class PagedAttnDesc(ctypes.Structure):
+    """``lucid_paged_attn_desc``"""
+    _fields_ = [("cache", PagedCacheDesc)] + \
+        [(n, ctypes.c_int32) for n in ("B", "Hq", "Hkv", "D", "dtype", "window", "sinks")] + \
+        [("scale", ctypes.c_float), ("k_scale", ctypes.c_float)] + [(n + "_strides", _I64x2) for n in ("q", "v")]
 
 
 class LucidKernelError(RuntimeError):
@@ -147,21 +167,21 @@ def load() -> ctypes.CDLL:
         lib.lucid_profile_next_call.argtypes = [c.c_void_p, c.c_void_p, c.c_void_p, c.c_void_p]
         lib.lucid_set_wait_limit_ns.restype = None
         lib.lucid_set_wait_limit_ns.argtypes = [c.c_uint64]
-        p, i, f, cache = c.c_void_p, c.c_int, c.c_float, c.POINTER(PagedCache)
+        p, i = c.c_void_p, c.c_int
         lib.lucid_window_attn_fwd.restype = i
-        lib.lucid_window_attn_fwd.argtypes = [p] * 5 + [_I64x3] * 4 + [i] * 9 + [f, p, p]
+        lib.lucid_window_attn_fwd.argtypes = [c.POINTER(WindowAttnDesc)] + [p] * 7
         lib.lucid_window_attn_bwd_workspace_bytes.restype = c.c_size_t
-        lib.lucid_window_attn_bwd_workspace_bytes.argtypes = [i] * 7
+        lib.lucid_window_attn_bwd_workspace_bytes.argtypes = [c.POINTER(WindowAttnDesc)]
         lib.lucid_window_attn_bwd.restype = i
-        lib.lucid_window_attn_bwd.argtypes = [p] * 9 + [_I64x3] * 8 + [i] * 9 + [f, p, p, c.c_size_t, p]
+        lib.lucid_window_attn_bwd.argtypes = [c.POINTER(WindowAttnDesc)] + [p] * 11 + [c.c_size_t, p]
         lib.lucid_paged_append.restype = i
-        lib.lucid_paged_append.argtypes = [p] * 4 + [_I64x2] * 3 + [cache, p, p, p] + [i] * 8 + [p]
+        lib.lucid_paged_append.argtypes = [c.POINTER(PagedAppendDesc)] + [p] * 11
         lib.lucid_paged_attn_workspace_bytes.restype = c.c_size_t
-        lib.lucid_paged_attn_workspace_bytes.argtypes = [i] * 8
+        lib.lucid_paged_attn_workspace_bytes.argtypes = [c.POINTER(PagedAttnDesc), i]
         lib.lucid_paged_window_attn.restype = i
-        lib.lucid_paged_window_attn.argtypes = [p, p, _I64x2, cache, p] + [i] * 7 + [f, p, c.c_size_t, p]
+        lib.lucid_paged_window_attn.argtypes = [c.POINTER(PagedAttnDesc)] + [p] * 7 + [c.c_size_t, p]
         lib.lucid_paged_lucid_attn.restype = i
-        lib.lucid_paged_lucid_attn.argtypes = [p, p, p, _I64x2, _I64x2, cache, p] + [i] * 5 + [f, f, p, c.c_size_t, p]
+        lib.lucid_paged_lucid_attn.argtypes = [c.POINTER(PagedAttnDesc)] + [p] * 8 + [c.c_size_t, p]
         lib.lucid_attn_status.restype = i
         lib.lucid_attn_status.argtypes = [p, c.POINTER(c.c_int32)]
         _lib = lib

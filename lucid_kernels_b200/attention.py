@@ -11,6 +11,10 @@ As with the solve: head dimension 128, fp16 or bf16, launched on torch's current
 a host synchronisation, capturable into CUDA graphs; scratch memory comes from torch's allocator per call (calls on
 different streams and captured graphs share none).  ``check=True`` (or ``LUCID_B200_CHECK=1``) synchronises and raises
 ``LucidKernelError`` if a kernel reported an error - a wait that ran out, a position whose page does not exist.
+
+The checks of a call depend on shapes, strides, types and options only, and so does the descriptor the C entry point
+takes: both are done once per combination and kept (``_plans``); a decoding step on the device takes a few microseconds,
+less than the checks do.
 """
 from __future__ import annotations
 
@@ -28,18 +32,55 @@ __all__ = ["window_attention", "LUCIDWindowAttention", "paged_append", "paged_wi
            "_window_attention_fwd", "_window_attention_bwd"]
 
 _D = 128
+_DTYPES = (torch.float16, torch.bfloat16)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_device_now = torch._C._cuda_getDevice
 
 
-def _usable(t: torch.Tensor) -> torch.Tensor:
+class _Plan:
+    """What a call's shapes, strides, types and options determine."""
+    __slots__ = ("desc", "ref", "device", "copy", "empty", "workspace", "out_shape", "lse_shape", "hq")
+
+    def __init__(self, desc, device: int, copy: bool, empty: bool):
+        self.desc, self.ref = desc, ctypes.byref(desc)
+        self.device = device
+        self.copy = copy          # some tensor's strides have no tensor map: work on contiguous copies
+        self.empty = empty        # nothing to launch
+
+
+_plans: dict = {}
+_MAX_PLANS = 4096
+
+
+def _keep(key, plan: _Plan) -> _Plan:
+    if len(_plans) >= _MAX_PLANS:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _good_strides(t: torch.Tensor) -> bool:
     """The kernels read 16-byte pieces of rows whose last dimension is contiguous; a tensor expanded along a dimension is
     materialised, like one with other strides."""
-    bad = t.stride(-1) != 1 or t.data_ptr() % 16 or any(n > 1 and (s % 8 or s == 0) for s, n in zip(t.stride()[:-1], t.shape[:-1]))
-    return t.clone(memory_format=torch.contiguous_format) if bad else t
+    return t.stride(-1) == 1 and all(n <= 1 or (s % 8 == 0 and s > 0) for s, n in zip(t.stride()[:-1], t.shape[:-1]))
+
+
+def _usable(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if t is None or (_good_strides(t) and t.data_ptr() % 16 == 0):
+        return t
+    return t.detach().clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t: torch.Tensor):
     """Element strides of all but the last dimension (of a dimension of extent 1: any valid one)."""
     st = [s if n > 1 else _D for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+    return (ctypes.c_int64 * len(st))(*st)
+
+
+def _contiguous_strides(*shape):
+    st = [_D]
+    for n in shape[:0:-1]:
+        st.insert(0, st[0] * n)
     return (ctypes.c_int64 * len(st))(*st)
 
 
@@ -54,10 +95,9 @@ def _scale(scale: Optional[float]) -> float:
     return scale
 
 
-def _int32_vector(t: torch.Tensor, n: int, like: torch.Tensor, name: str) -> torch.Tensor:
+def _check_vector(t: torch.Tensor, n: int, device, name: str) -> None:
     assert t.dtype == torch.int32 and t.shape == (n,), f"{name} must be an int32 tensor of shape ({n},)"
-    assert t.device == like.device, f"{name} must be on {like.device}"
-    return t.contiguous()
+    assert t.device == device, f"{name} must be on {device}"
 
 
 def _window(window: Optional[int], sinks: int):
@@ -71,46 +111,75 @@ def _window(window: Optional[int], sinks: int):
     return min(window, 1 << 30), min(sinks, 1 << 30)
 
 
-def _check_qkv(q, k, v, others, lengths, sinks):
+def _plain_options(window, sinks, scale):
+    """Options as hashable numbers (a tensor's hash is its identity)."""
+    return (window if window is None or type(window) is int else int(window), sinks if type(sinks) is int else int(sinks),
+            scale if scale is None or type(scale) is float else float(scale))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# window attention
+# ---------------------------------------------------------------------------------------------------------------------
+def _window_plan(key, q, k, v, out, dout, window, sinks, scale, lengths) -> _Plan:
+    """Checks a forward (out, dout None) or backward call and describes it."""
+    w, s = _window(window, sinks)
     assert q.dim() == 4 and k.dim() == 4, "q and k must be (batch, seqlen, heads, head_dim)"
     B, Nq, Hq, D = q.shape
     _, Nk, Hkv, _ = k.shape
+    others = [t for t in (out, dout) if t is not None]
     assert D == _D, f"this build supports head_dim == {_D}, got {D}"
     assert k.shape == (B, Nk, Hkv, D) and v.shape == k.shape, "k and v must share their shape, and q's batch and head_dim"
     assert Hkv > 0 and Hq % Hkv == 0, f"query heads ({Hq}) must be a multiple of key heads ({Hkv})"
     assert Nq <= Nk, f"more queries ({Nq}) than keys ({Nk})"
     assert all(t.shape == q.shape for t in others), "out and its gradient must have q's shape"
-    assert q.dtype in (torch.float16, torch.bfloat16), "inputs must be float16 or bfloat16"
+    assert q.dtype in _DTYPES, "inputs must be float16 or bfloat16"
     assert all(t.dtype == q.dtype for t in (k, v, *others)), "all tensors must have the same dtype"
     assert q.is_cuda and all(t.device == q.device for t in (k, v, *others)), "inputs must be on one CUDA device"
-    assert sinks <= 128, f"at most 128 first positions stay visible, got {sinks}"
+    assert s <= 128, f"at most 128 first positions stay visible, got {s}"
+    copy = not all(_good_strides(t) for t in (q, k, v, *others))
     if lengths is not None:
-        lengths = _int32_vector(lengths, B, q, "lengths")
-    return lengths
+        _check_vector(lengths, B, q.device, "lengths")
+        copy = copy or not lengths.is_contiguous()
+    desc = _cabi.WindowAttnDesc(B, Nq, Nk, Hq, Hkv, D, _cabi.dtype_code(q.dtype), w, s, _scale(scale))
+    like_q, like_k = _contiguous_strides(B, Nq, Hq), _contiguous_strides(B, Nk, Hkv)
+    desc.q_strides, desc.k_strides, desc.v_strides = _strides(q), _strides(k), _strides(v)
+    desc.out_strides = like_q if out is None else _strides(out)
+    desc.dout_strides = like_q if dout is None else _strides(dout)
+    desc.dq_strides, desc.dk_strides, desc.dv_strides = like_q, like_k, like_k
+    plan = _Plan(desc, q.get_device(), copy, q.numel() == 0)
+    plan.out_shape, plan.lse_shape = (B, Nq, Hq, D), (B, Hq, Nq)
+    plan.workspace = 0 if dout is None or plan.empty else _cabi.load().lucid_window_attn_bwd_workspace_bytes(plan.ref)
+    return _keep(key, plan)
 
 
 def _window_attention_fwd(q, k, v, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
-                          lengths: Optional[torch.Tensor] = None, *, check: Optional[bool] = None):
-    """(out, lse): see ``window_attention``; ``lse`` (B, Hq, Nq) fp32, -inf for a query that sees nothing."""
-    w, s = _window(window, sinks)
-    lengths = _check_qkv(q, k, v, (), lengths, s)
-    scale = _scale(scale)
-    q, k, v = (_usable(t.detach()) for t in (q, k, v))
-    B, Nq, Hq, D = q.shape
-    Nk, Hkv = k.shape[1:3]
-    out = torch.empty((B, Nq, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, Hq, Nq), dtype=torch.float32, device=q.device)
-    if out.numel() == 0:
+                          lengths: Optional[torch.Tensor] = None, *, need_lse: bool = True, check: Optional[bool] = None):
+    """(out, lse): see ``window_attention``; ``lse`` (B, Hq, Nq) fp32, -inf for a query that sees nothing (None unless
+    ``need_lse``)."""
+    window, sinks, scale = _plain_options(window, sinks, scale)
+    key = ("window", q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(),
+           v.dtype, v.get_device(), window, sinks, scale,
+           None if lengths is None else (lengths.shape, lengths.stride(), lengths.dtype, lengths.get_device()))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _window_plan(key, q, k, v, None, None, window, sinks, scale, lengths)
+    qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if plan.copy or (qp | kp | vp) & 15:
+        return _window_attention_fwd(_usable(q), _usable(k), _usable(v), window, sinks, scale,
+                                     None if lengths is None else lengths.contiguous(), need_lse=need_lse, check=check)
+    if _device_now() != plan.device:
+        with torch.cuda.device(plan.device):
+            return _window_attention_fwd(q, k, v, window, sinks, scale, lengths, need_lse=need_lse, check=check)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format, requires_grad=False)
+    lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=q.device) if need_lse else None
+    if plan.empty:
         return out, lse
-    lib = _cabi.load()
-    with torch.cuda.device(q.device):
-        stream = torch.cuda.current_stream().cuda_stream
-        rc = lib.lucid_window_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                                       _strides(q), _strides(k), _strides(v), _strides(out), B, Nq, Nk, Hq, Hkv, D,
-                                       _cabi.dtype_code(q.dtype), w, s, scale,
-                                       None if lengths is None else lengths.data_ptr(), stream)
+    stream = _raw_stream(plan.device)
+    rc = _cabi.load().lucid_window_attn_fwd(plan.ref, qp, kp, vp, out.data_ptr(), None if lse is None else lse.data_ptr(),
+                                            None if lengths is None else lengths.data_ptr(), stream)
+    if rc:
         _cabi.check_rc(rc, "lucid_window_attn_fwd")
-        _finish(check, stream, "_window_attention_fwd")
+    _finish(check, stream, "_window_attention_fwd")
     return out, lse
 
 
@@ -118,34 +187,36 @@ def _window_attention_bwd(q, k, v, out, lse, dout, window: Optional[int] = None,
                           scale: Optional[float] = None, lengths: Optional[torch.Tensor] = None, *, need_dq: bool = True,
                           need_dkv: bool = True, check: Optional[bool] = None):
     """(dq, dk, dv) from the forward's ``out`` and ``lse``; None for what is not needed."""
-    w, s = _window(window, sinks)
-    lengths = _check_qkv(q, k, v, (out, dout), lengths, s)
-    scale = _scale(scale)
-    q, k, v, out, dout = (_usable(t.detach()) for t in (q, k, v, out, dout))
-    B, Nq, Hq, D = q.shape
-    Nk, Hkv = k.shape[1:3]
-    assert lse.shape == (B, Hq, Nq) and lse.dtype == torch.float32 and lse.device == q.device, "lse must be the forward's"
-    lse = lse.contiguous()
-    dq = torch.empty((B, Nq, Hq, D), dtype=q.dtype, device=q.device) if need_dq else None
-    dk = torch.empty((B, Nk, Hkv, D), dtype=q.dtype, device=q.device) if need_dkv else None
-    dv = torch.empty_like(dk) if need_dkv else None
-    if q.numel() == 0:
+    window, sinks, scale = _plain_options(window, sinks, scale)
+    key = ("window bwd", q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(),
+           v.dtype, v.get_device(), out.shape, out.stride(), out.dtype, out.get_device(), dout.shape, dout.stride(), dout.dtype,
+           dout.get_device(), window, sinks, scale,
+           None if lengths is None else (lengths.shape, lengths.stride(), lengths.dtype, lengths.get_device()))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _window_plan(key, q, k, v, out, dout, window, sinks, scale, lengths)
+    qp, kp, vp, op, gp = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr()
+    if plan.copy or (qp | kp | vp | op | gp) & 15:
+        return _window_attention_bwd(*(_usable(t) for t in (q, k, v, out)), lse, _usable(dout), window, sinks, scale,
+                                     None if lengths is None else lengths.contiguous(), need_dq=need_dq, need_dkv=need_dkv, check=check)
+    assert lse.shape == plan.lse_shape and lse.dtype == torch.float32 and lse.device == q.device and lse.is_contiguous(), \
+        "lse must be the forward's"
+    if _device_now() != plan.device:
+        with torch.cuda.device(plan.device):
+            return _window_attention_bwd(q, k, v, out, lse, dout, window, sinks, scale, lengths, need_dq=need_dq, need_dkv=need_dkv,
+                                         check=check)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format, requires_grad=False) if need_dq else None
+    dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format, requires_grad=False) if need_dkv else None for t in (k, v))
+    if plan.empty:
         return dq, dk if dk is None else dk.zero_(), dv if dv is None else dv.zero_()
-    lib = _cabi.load()
-    with torch.cuda.device(q.device):
-        stream = torch.cuda.current_stream().cuda_stream
-        nbytes = lib.lucid_window_attn_bwd_workspace_bytes(B, Nq, Nk, Hq, Hkv, w, s)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        sq, sk, sv = _strides(q), _strides(k), _strides(v)
-        rc = lib.lucid_window_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                                       None if dq is None else dq.data_ptr(), None if dk is None else dk.data_ptr(),
-                                       None if dv is None else dv.data_ptr(), sq, sk, sv, _strides(out), _strides(dout),
-                                       sq if dq is None else _strides(dq), sk if dk is None else _strides(dk),
-                                       sv if dv is None else _strides(dv), B, Nq, Nk, Hq, Hkv, D,
-                                       _cabi.dtype_code(q.dtype), w, s, scale,
-                                       None if lengths is None else lengths.data_ptr(), ws.data_ptr(), nbytes, stream)
+    ws = torch.empty(plan.workspace, dtype=torch.uint8, device=q.device)
+    stream = _raw_stream(plan.device)
+    rc = _cabi.load().lucid_window_attn_bwd(plan.ref, qp, kp, vp, op, lse.data_ptr(), gp, None if dq is None else dq.data_ptr(),
+                                            None if dk is None else dk.data_ptr(), None if dv is None else dv.data_ptr(),
+                                            None if lengths is None else lengths.data_ptr(), ws.data_ptr(), plan.workspace, stream)
+    if rc:
         _cabi.check_rc(rc, "lucid_window_attn_bwd")
-        _finish(check, stream, "_window_attention_bwd")
+    _finish(check, stream, "_window_attention_bwd")
     return dq, dk, dv
 
 
@@ -177,41 +248,78 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     last Nq positions: query i sits at ``p = i + Nk - Nq`` and sees key j when ``j <= p and (j > p - window or j < sinks)``.
     ``window=None``: every key up to p.  ``sinks`` <= 128.  ``scale``: of the scores, 128 ** -0.5 by default.  ``lengths``
     (int32, (B,), on the device): positions from ``lengths[b]`` on are padding, neither keys nor queries, whatever they
-    hold; their outputs and gradients are 0.  So are a query's that sees nothing.
+    hold; their outputs and gradients are 0.  So are a query's that sees nothing.  Values at positions inside a sequence
+    must be finite.
 
     Differentiable in q, k and v (once); gradients come out the same on every run.  In a training step recorded into a CUDA
     graph, record forward and backward together and, as torch asks for every operator, keep no eager graph of the same
     leaves alive while recording."""
-    return LUCIDWindowAttention.apply(q, k, v, window, sinks, scale, lengths)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return LUCIDWindowAttention.apply(q, k, v, window, sinks, scale, lengths)
+    return _window_attention_fwd(q, k, v, window, sinks, scale, lengths, need_lse=False)[0]
 
 
 # ---------------------------------------------------------------------------------------------------------------------
 # paged cache
 # ---------------------------------------------------------------------------------------------------------------------
-def _check_cache(k_cache, v_cache, block_table, B: int, tensors):
+def _cache_desc(k_cache, v_cache, block_table, B: int, tensors):
+    """(descriptor, whether the block table has to be copied)"""
     assert k_cache.dim() == 4 and k_cache.shape[3] == _D, f"caches must be (pages, page_size, heads, {_D})"
     assert v_cache.shape == k_cache.shape, "k_cache and v_cache must share their shape"
     pages, page, Hkv, _ = k_cache.shape
-    assert k_cache.dtype in (torch.float16, torch.bfloat16), "caches must be float16 or bfloat16"
+    assert k_cache.dtype in _DTYPES, "caches must be float16 or bfloat16"
     assert v_cache.dtype == k_cache.dtype and all(t.dtype == k_cache.dtype for t in tensors), "all tensors must have the caches' dtype"
     assert k_cache.is_cuda and all(t.device == k_cache.device for t in (v_cache, block_table, *tensors)), \
         "caches, block table and inputs must be on one CUDA device"
     assert pages > 0 and 0 < page <= 65536 and page & (page - 1) == 0, f"page_size must be a power of two up to 65536, got {page}"
-    for t in (k_cache, v_cache):
-        # written in place: no copy can stand in for it
-        assert t.stride(3) == 1 and t.data_ptr() % 16 == 0 and \
-            all(n == 1 or (s % 8 == 0 and s > 0) for s, n in zip(t.stride()[:3], t.shape[:3])), \
-            "caches must have a contiguous last dimension, a 16-byte aligned base and strides that are multiples of 8"
+    # (written in place: no copy can stand in for it)
+    assert _good_strides(k_cache) and _good_strides(v_cache), \
+        "caches must have a contiguous last dimension and strides that are multiples of 8"
     assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == B and block_table.shape[1] > 0, \
         f"block_table must be an int32 tensor of shape ({B}, pages per sequence)"
-    assert block_table.shape[1] * page <= 1 << 30, "block_table covers more than 2 ** 30 positions"
+    width = block_table.shape[1]
+    assert width * page <= 1 << 30, "block_table covers more than 2 ** 30 positions"
+    copy = (width > 1 and block_table.stride(1) != 1) or (B > 1 and block_table.stride(0) < width)
+    return _cabi.PagedCacheDesc(pages, page, width, width if B == 1 else block_table.stride(0), _strides(k_cache), _strides(v_cache)), copy
+
+
+def _no_gradients(*tensors) -> None:
     if torch.is_grad_enabled():
-        assert not any(t.requires_grad for t in (k_cache, v_cache, *tensors)), "the cache operators have no backward: use torch.no_grad()"
-    if block_table.stride(1) != 1 or (B > 1 and block_table.stride(0) < block_table.shape[1]):
-        block_table = block_table.contiguous()
-    c = _cabi.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), _strides(k_cache), _strides(v_cache), block_table.data_ptr(),
-                         block_table.stride(0), block_table.shape[1], pages, page)
-    return c, block_table
+        assert not any(t is not None and t.requires_grad for t in tensors), "the cache operators have no backward: use torch.no_grad()"
+
+
+def _cache_pointers(k_cache, v_cache):
+    kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
+    assert (kc | vc) & 15 == 0, "caches must be 16-byte aligned"
+    return kc, vc
+
+
+def _append_plan(key, k, v, k_cache, v_cache, block_table, cache_lens, cu_seqlens, q, inv_freq, interleaved) -> _Plan:
+    assert k.dim() == 3 and k.shape[2] == _D, f"k must be (tokens, heads, {_D})"
+    T, Hkv, _ = k.shape
+    assert cache_lens.dim() == 1, "cache_lens must be an int32 tensor of shape (batch,)"
+    B = cache_lens.shape[0]
+    cache, copy = _cache_desc(k_cache, v_cache, block_table, B, [t for t in (k, v, q) if t is not None])
+    assert Hkv == k_cache.shape[2] and (v is None or v.shape == k.shape), "k and v must be (tokens, the caches' heads, head_dim)"
+    assert q is None or (q.dim() == 3 and q.shape[0] == T and q.shape[2] == _D), "q must be (tokens, query heads, head_dim)"
+    assert q is None or inv_freq is not None, "q is only rotated: it needs inv_freq"
+    _check_vector(cache_lens, B, k.device, "cache_lens")
+    copy = copy or not cache_lens.is_contiguous()
+    if cu_seqlens is not None:
+        _check_vector(cu_seqlens, B + 1, k.device, "cu_seqlens")
+        copy = copy or not cu_seqlens.is_contiguous()
+    else:
+        assert T == B, f"without cu_seqlens there is one token per sequence, got {T} for {B}"
+    rot = 0
+    if inv_freq is not None:
+        assert inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.device == k.device, "inv_freq must be an fp32 vector on the device"
+        rot = 2 * inv_freq.numel()
+        assert 0 < rot <= _D and rot % 16 == 0, f"inv_freq must rotate a multiple of 16 elements up to {_D}, got {rot}"
+        copy = copy or not inv_freq.is_contiguous()
+    copy = copy or not all(_good_strides(t) for t in (k, v, q) if t is not None)
+    desc = _cabi.PagedAppendDesc(cache, B, T, 0 if q is None else q.shape[1], Hkv, _D, rot, int(interleaved), _cabi.dtype_code(k.dtype),
+                                 _strides(k), _strides(k if v is None else v), _strides(k if q is None else q))
+    return _keep(key, _Plan(desc, k.get_device(), copy, T == 0 or B == 0))
 
 
 def paged_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -229,52 +337,62 @@ def paged_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tens
     ``position * inv_freq``, in pairs (i, i + r / 2), or (2i, 2i + 1) if ``interleaved``; the angle is formed in 64 bits.  q
     (T, Hq, 128) is rotated likewise and returned as a new tensor.  Tokens behind ``cu_seqlens[-1]`` are padding: nothing is
     written for them, their rows of the returned queries are 0.  A position without a page is skipped and reported."""
-    tensors = [t for t in (k, v, q) if t is not None]
-    assert k.dim() == 3 and k.shape[2] == _D, f"k must be (tokens, heads, {_D})"
-    T, Hkv, _ = k.shape
-    B = cache_lens.shape[0] if cache_lens.dim() == 1 else -1
-    c, block_table = _check_cache(k_cache, v_cache, block_table, B, tensors)
-    assert Hkv == k_cache.shape[2] and (v is None or v.shape == k.shape), "k and v must be (tokens, the caches' heads, head_dim)"
-    assert q is None or (q.dim() == 3 and q.shape[0] == T and q.shape[2] == _D), "q must be (tokens, query heads, head_dim)"
-    assert q is None or inv_freq is not None, "q is only rotated: it needs inv_freq"
-    cache_lens = _int32_vector(cache_lens, B, k, "cache_lens")
-    if cu_seqlens is not None:
-        cu_seqlens = _int32_vector(cu_seqlens, B + 1, k, "cu_seqlens")
-    else:
-        assert T == B, f"without cu_seqlens there is one token per sequence, got {T} for {B}"
-    rot = 0
-    if inv_freq is not None:
-        assert inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.device == k.device, "inv_freq must be an fp32 vector on the device"
-        rot = 2 * inv_freq.numel()
-        assert 0 < rot <= _D and rot % 16 == 0, f"inv_freq must rotate a multiple of 16 elements up to {_D}, got {rot}"
-        inv_freq = inv_freq.contiguous()
-    k, v, q = (None if t is None else _usable(t.detach()) for t in (k, v, q))
-    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if T == 0 or B == 0:
+    key = ("append", k.shape, k.stride(), k.dtype, k.get_device(), None if v is None else (v.shape, v.stride(), v.dtype, v.get_device()),
+           None if q is None else (q.shape, q.stride(), q.dtype, q.get_device()), k_cache.shape, k_cache.stride(), k_cache.dtype,
+           k_cache.get_device(), v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.get_device(), block_table.shape,
+           block_table.stride(), block_table.dtype, block_table.get_device(), cache_lens.shape, cache_lens.stride(), cache_lens.dtype,
+           cache_lens.get_device(),
+           None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.get_device()),
+           None if inv_freq is None else (inv_freq.shape, inv_freq.stride(), inv_freq.dtype, inv_freq.get_device()), bool(interleaved))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _append_plan(key, k, v, k_cache, v_cache, block_table, cache_lens, cu_seqlens, q, inv_freq, interleaved)
+    _no_gradients(k, v, q, k_cache, v_cache)
+    kp, vp, qp = k.data_ptr(), None if v is None else v.data_ptr(), None if q is None else q.data_ptr()
+    if plan.copy or (kp | (vp or 0) | (qp or 0)) & 15:
+        own = lambda t: None if t is None else t.contiguous()
+        return paged_append(_usable(k), _usable(v), k_cache, v_cache, own(block_table), own(cache_lens), own(cu_seqlens), _usable(q),
+                            own(inv_freq), interleaved, check=check)
+    kc, vc = _cache_pointers(k_cache, v_cache)
+    if _device_now() != plan.device:
+        with torch.cuda.device(plan.device):
+            return paged_append(k, v, k_cache, v_cache, block_table, cache_lens, cu_seqlens, q, inv_freq, interleaved, check=check)
+    q_out = None if q is None else torch.empty_like(q, memory_format=torch.contiguous_format)
+    if plan.empty:
         return q_out if q_out is None else q_out.zero_()
-    lib = _cabi.load()
-    ptr = lambda t: None if t is None else t.data_ptr()
-    with torch.cuda.device(k.device):
-        stream = torch.cuda.current_stream().cuda_stream
-        st = _strides(k)
-        rc = lib.lucid_paged_append(ptr(k), ptr(v), ptr(q), ptr(q_out), st, st if v is None else _strides(v),
-                                    st if q is None else _strides(q), ctypes.byref(c), ptr(cache_lens), ptr(cu_seqlens),
-                                    ptr(inv_freq), B, T, 0 if q is None else q.shape[1], Hkv, _D, rot, int(interleaved),
-                                    _cabi.dtype_code(k.dtype), stream)
+    stream = _raw_stream(plan.device)
+    rc = _cabi.load().lucid_paged_append(plan.ref, kp, vp, qp, None if q_out is None else q_out.data_ptr(), kc, vc, block_table.data_ptr(),
+                                         cache_lens.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
+                                         None if inv_freq is None else inv_freq.data_ptr(), stream)
+    if rc:
         _cabi.check_rc(rc, "lucid_paged_append")
-        torch.autograd.graph.increment_version([k_cache] if v is None else [k_cache, v_cache])
-        _finish(check, stream, "paged_append")
+    torch.autograd.graph.increment_version([k_cache] if v is None else [k_cache, v_cache])
+    _finish(check, stream, "paged_append")
     return q_out
 
 
-def _check_step(q, k_cache, v_cache, block_table, seq_lens, more=()):
+def _step_plan(key, q, v, k_cache, v_cache, block_table, seq_lens, window, sinks, scale, k_scale) -> _Plan:
+    """Checks a decoding step (``v`` and ``k_scale``: of a LUCID layer) and describes it."""
+    w, s = _window(window, sinks)
     assert q.dim() == 3 and q.shape[2] == _D, f"q must be (batch, query heads, {_D})"
     B, Hq, _ = q.shape
-    c, block_table = _check_cache(k_cache, v_cache, block_table, B, (q, *more))
+    cache, copy = _cache_desc(k_cache, v_cache, block_table, B, [t for t in (q, v) if t is not None])
     Hkv = k_cache.shape[2]
     assert Hkv > 0 and Hq % Hkv == 0, f"query heads ({Hq}) must be a multiple of key heads ({Hkv})"
     assert B <= 65535, "at most 65535 sequences in a call"
-    return c, block_table, _int32_vector(seq_lens, B, q, "seq_lens"), torch.empty((B, Hq, _D), dtype=q.dtype, device=q.device)
+    _check_vector(seq_lens, B, q.device, "seq_lens")
+    copy = copy or not seq_lens.is_contiguous() or not _good_strides(q)
+    scale = _scale(scale)
+    if v is not None:
+        assert 0.0 < k_scale < 1e18, "k_scale must be positive and finite"
+        assert v.shape == (B, Hkv, _D), f"v must be ({B}, {Hkv}, {_D})"
+        assert Hq // Hkv <= 15, f"at most 15 query heads per key head, got {Hq // Hkv}"
+        copy = copy or not _good_strides(v)
+    desc = _cabi.PagedAttnDesc(cache, B, Hq, Hkv, _D, _cabi.dtype_code(q.dtype), w, s, scale, k_scale, _strides(q),
+                               _strides(q if v is None else v))
+    plan = _Plan(desc, q.get_device(), copy, q.numel() == 0)
+    plan.workspace = 0 if plan.empty else _cabi.load().lucid_paged_attn_workspace_bytes(plan.ref, 0 if v is None else 1)
+    return _keep(key, plan)
 
 
 def paged_window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -283,22 +401,32 @@ def paged_window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     """One decoding step of ``window_attention`` over a paged cache: q (B, Hq, 128) is the query of position
     ``seq_lens[b] - 1`` (int32, (B,); its key has been appended), which sees the last ``window`` positions and the first
     ``sinks``.  Returns (B, Hq, 128); 0 where ``seq_lens[b]`` is 0."""
-    w, s = _window(window, sinks)
-    c, block_table, seq_lens, out = _check_step(q, k_cache, v_cache, block_table, seq_lens)
-    scale = _scale(scale)
-    q = _usable(q.detach())
-    B, Hq, D = q.shape
-    if out.numel() == 0:
+    window, sinks, scale = _plain_options(window, sinks, scale)
+    key = ("step", q.shape, q.stride(), q.dtype, q.get_device(), k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.get_device(),
+           v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.get_device(), block_table.shape, block_table.stride(), block_table.dtype,
+           block_table.get_device(), seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.get_device(), window, sinks, scale)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _step_plan(key, q, None, k_cache, v_cache, block_table, seq_lens, window, sinks, scale, 1.0)
+    _no_gradients(q, k_cache, v_cache)
+    qp = q.data_ptr()
+    if plan.copy or qp & 15:
+        return paged_window_attention(_usable(q), k_cache, v_cache, block_table.contiguous(), seq_lens.contiguous(), window, sinks, scale,
+                                      check=check)
+    kc, vc = _cache_pointers(k_cache, v_cache)
+    if _device_now() != plan.device:
+        with torch.cuda.device(plan.device):
+            return paged_window_attention(q, k_cache, v_cache, block_table, seq_lens, window, sinks, scale, check=check)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if plan.empty:
         return out
-    lib = _cabi.load()
-    with torch.cuda.device(q.device):
-        stream = torch.cuda.current_stream().cuda_stream
-        nbytes = lib.lucid_paged_attn_workspace_bytes(B, Hq, k_cache.shape[2], c.page_rows, c.table_width, w, s, 0)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        rc = lib.lucid_paged_window_attn(q.data_ptr(), out.data_ptr(), _strides(q), ctypes.byref(c), seq_lens.data_ptr(), B, Hq,
-                                         k_cache.shape[2], D, _cabi.dtype_code(q.dtype), w, s, scale, ws.data_ptr(), nbytes, stream)
+    ws = torch.empty(plan.workspace, dtype=torch.uint8, device=q.device) if plan.workspace else None
+    stream = _raw_stream(plan.device)
+    rc = _cabi.load().lucid_paged_window_attn(plan.ref, qp, out.data_ptr(), kc, vc, block_table.data_ptr(), seq_lens.data_ptr(),
+                                              None if ws is None else ws.data_ptr(), plan.workspace, stream)
+    if rc:
         _cabi.check_rc(rc, "lucid_paged_window_attn")
-        _finish(check, stream, "paged_window_attention")
+    _finish(check, stream, "paged_window_attention")
     return out
 
 
@@ -312,25 +440,34 @@ def paged_lucid_attention(q: torch.Tensor, v: torch.Tensor, k_cache: torch.Tenso
     ``t_j = k_scale ** 2 * k_n . k_j``, ``v'_n = exp(-t_n) v_n - sum_{j < n} exp(t_j - t_n) v'_j`` is written to position n of
     v_cache, and softmax attention with scores ``scale * q . k_j`` over j <= n of V' is returned, (B, Hq, 128).  At most 15
     query heads per key head.  ``seq_lens[b] = 0``: the row of the result is 0 and nothing is written."""
-    c, block_table, seq_lens, out = _check_step(q, k_cache, v_cache, block_table, seq_lens, (v,))
-    scale = _scale(scale)
-    assert 0.0 < float(k_scale) < 1e18, "k_scale must be positive and finite"
-    B, Hq, D = q.shape
-    Hkv = k_cache.shape[2]
-    assert v.shape == (B, Hkv, D), f"v must be ({B}, {Hkv}, {D})"
-    assert Hq // Hkv <= 15, f"at most 15 query heads per key head, got {Hq // Hkv}"
-    q, v = _usable(q.detach()), _usable(v.detach())
-    if out.numel() == 0:
+    _, _, scale = _plain_options(None, 0, scale)
+    if type(k_scale) is not float:
+        k_scale = float(k_scale)
+    key = ("lucid step", q.shape, q.stride(), q.dtype, q.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), k_cache.shape,
+           k_cache.stride(), k_cache.dtype, k_cache.get_device(), v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.get_device(),
+           block_table.shape, block_table.stride(), block_table.dtype, block_table.get_device(), seq_lens.shape, seq_lens.stride(),
+           seq_lens.dtype, seq_lens.get_device(), scale, k_scale)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _step_plan(key, q, v, k_cache, v_cache, block_table, seq_lens, None, 0, scale, k_scale)
+    _no_gradients(q, v, k_cache, v_cache)
+    qp, vp = q.data_ptr(), v.data_ptr()
+    if plan.copy or (qp | vp) & 15:
+        return paged_lucid_attention(_usable(q), _usable(v), k_cache, v_cache, block_table.contiguous(), seq_lens.contiguous(), k_scale,
+                                     scale, check=check)
+    kc, vc = _cache_pointers(k_cache, v_cache)
+    if _device_now() != plan.device:
+        with torch.cuda.device(plan.device):
+            return paged_lucid_attention(q, v, k_cache, v_cache, block_table, seq_lens, k_scale, scale, check=check)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if plan.empty:
         return out
-    lib = _cabi.load()
-    with torch.cuda.device(q.device):
-        stream = torch.cuda.current_stream().cuda_stream
-        nbytes = lib.lucid_paged_attn_workspace_bytes(B, Hq, Hkv, c.page_rows, c.table_width, -1, 0, 1)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        rc = lib.lucid_paged_lucid_attn(q.data_ptr(), v.data_ptr(), out.data_ptr(), _strides(q), _strides(v), ctypes.byref(c),
-                                        seq_lens.data_ptr(), B, Hq, Hkv, D, _cabi.dtype_code(q.dtype), float(k_scale), scale,
-                                        ws.data_ptr(), nbytes, stream)
+    ws = torch.empty(plan.workspace, dtype=torch.uint8, device=q.device) if plan.workspace else None
+    stream = _raw_stream(plan.device)
+    rc = _cabi.load().lucid_paged_lucid_attn(plan.ref, qp, vp, out.data_ptr(), kc, vc, block_table.data_ptr(), seq_lens.data_ptr(),
+                                             None if ws is None else ws.data_ptr(), plan.workspace, stream)
+    if rc:
         _cabi.check_rc(rc, "lucid_paged_lucid_attn")
-        torch.autograd.graph.increment_version([v_cache])
-        _finish(check, stream, "paged_lucid_attention")
+    torch.autograd.graph.increment_version([v_cache])
+    _finish(check, stream, "paged_lucid_attention")
     return out

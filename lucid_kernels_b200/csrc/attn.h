@@ -1,6 +1,8 @@
 // Argument blocks and host launchers of the windowed attention kernels (attn_fwd.cu, attn_bwd.cu) and of the paged
 // cache's kernels (paged_append.cu, paged_attn.cu).
 #pragma once
+#include <atomic>
+
 #include "attn_geometry.h"
 #include "common.cuh"
 
@@ -56,6 +58,21 @@ cudaError_t attn_fwd_status(cudaStream_t stream, int out[8]);
 cudaError_t attn_bwd_status(cudaStream_t stream, int out[8]);
 cudaError_t paged_append_status(cudaStream_t stream, int out[8]);
 cudaError_t paged_attn_status(cudaStream_t stream, int out[8]);
+
+// Sets a kernel's dynamic shared memory limit once per device (a kernel's attribute, not a call's).
+struct SmemOnce {
+  std::atomic<unsigned long long> done{0};
+  cudaError_t set(const void* kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
 
 // For the source files' own status records.
 inline cudaError_t take_status(const void* symbol, cudaStream_t stream, int out[8]) {
@@ -123,6 +140,9 @@ struct PagedAttnArgs {
   int B, Hq, Hkv, G, W, S, splits;
   float scale_log2, lucid_log2; // scale * log2(e); k_scale^2 * log2(e)
 };
+
+// up to this many chunks of a sequence are one cluster's CTAs (and then a power of two)
+constexpr int kPagedCluster = 8;
 
 cudaError_t launch_paged_append(bool bf16, const AppendArgs& args, cudaStream_t stream);
 cudaError_t launch_paged_attn(bool bf16, bool lucid, const PagedAttnArgs& args, cudaStream_t stream);

@@ -372,7 +372,8 @@ cudaError_t launch_attn_dq(bool bf16, const CUtensorMap& tm_q, const CUtensorMap
   const int items = args.a.B * args.a.Hq * args.a.nqb, grid = items < sms ? items : sms;
   const int bytes = (int)sizeof(AttnDqSmem) + 1024;
   auto kernel = bf16 ? attn_dq_kernel<true> : attn_dq_kernel<false>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static SmemOnce once[2];
+  cudaError_t e = once[bf16].set(reinterpret_cast<const void*>(kernel), bytes);
   if (e != cudaSuccess) return e;
   kernel<<<grid, kDqThreads, bytes, stream>>>(tm_q, tm_k, tm_v, tm_do, args);
   return cudaGetLastError();
@@ -764,7 +765,8 @@ cudaError_t launch_attn_dkv(bool bf16, const CUtensorMap& tm_q, const CUtensorMa
   const int items = kv_items(a), grid = items < sms ? items : sms;
   const int bytes = (int)sizeof(AttnDkvSmem) + 1024;
   auto kernel = bf16 ? attn_dkv_kernel<true> : attn_dkv_kernel<false>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static SmemOnce once[2];
+  cudaError_t e = once[bf16].set(reinterpret_cast<const void*>(kernel), bytes);
   if (e != cudaSuccess) return e;
   kernel<<<grid, kDkvThreads, bytes, stream>>>(tm_q, tm_k, tm_v, tm_do, args);
   if ((e = cudaGetLastError()) != cudaSuccess || args.chunks == 0) return e;

@@ -340,7 +340,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         tc_fence_before_sync();
         mbar_arrive(&s.o_free[t]);
       }
-      if (store)
+      if (store && args.lse)
         args.lse[((long long)it.b * A.Hq + it.h(t)) * A.Nq + i] =
             some ? (ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
     }
@@ -362,7 +362,8 @@ cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMa
   const int items = fwd_items(args.a), grid = items < sms ? items : sms;
   const int bytes = (int)sizeof(AttnFwdSmem) + 1024;
   auto kernel = bf16 ? attn_fwd_kernel<true> : attn_fwd_kernel<false>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static SmemOnce once[2];
+  cudaError_t e = once[bf16].set(reinterpret_cast<const void*>(kernel), bytes);
   if (e != cudaSuccess) return e;
   kernel<<<grid, kFwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, args);
   return cudaGetLastError();

@@ -10,7 +10,7 @@ namespace lucid {
 unsigned long long wait_limit_ns();
 
 inline int sm_count() {
-  inline int cached[64] = {0};
+  static int cached[64] = {0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   if (dev < 0 || dev >= 64) dev = 0;

@@ -4,8 +4,10 @@
 // query, so the kernel is bound by HBM (long contexts) or by latency (short ones), and the tensor work is small: the
 // G query heads that share a key head are the rows of one 16-row matrix instruction (mma.sync; a tcgen05 tile has 128
 // rows, of which 8 would be in use).  Keys are split over CTAs (`splits` chunks per sequence and key head); each warp
-// streams blocks of 16 keys through a ring of its own (cp.async, page by page) with a running maximum and sum, the
-// warps of a CTA meet in shared memory, the chunks in a second kernel.
+// streams blocks of 16 keys through a ring of its own (cp.async, page by page) with a running maximum and sum, and the
+// warps of a CTA meet in shared memory.  Up to 8 chunks are the CTAs of one cluster and meet there too, each CTA taking a
+// share of the columns from its peers' shared memory: one launch, no scratch memory.  One long sequence alone needs more
+// CTAs than that to draw on the whole HBM; its chunks meet in a second kernel.
 //
 // LUCID: with t_j = k_scale^2 k_n.k_j the solve's newest row is v'_n = exp(-t_n) v_n - sum_{j<n} exp(t_j - t_n) v'_j, an
 // unnormalised attention of k_n over the rows before it.  So k_n is one more row of the same matrix instruction: one
@@ -27,6 +29,8 @@ struct PagedAttnSmem {
   alignas(128) uint8_t ring[kPaWarps][kPaStages][kPaStageBytes];
   int valid[kPaWarps][kPaStages];                              // bit r: row r of the block is a key
   float ml[kPaWarps][16][2];
+  float chunk_ml[16][2];                                       // the CTA's own maximum and sum of each row
+  float self[16];                                              // LUCID: row . k_n, unscaled
 };
 
 // What a sequence shows: positions 0 .. first-1 and lo .. lo+near-1, counted through as 0 .. n-1.
@@ -86,7 +90,36 @@ __device__ __forceinline__ long long page_of(const PagedCache& c, int b, int pos
   return p < c.pages ? p : -1;
 }
 
-template <bool kBf16, bool kLucid>
+template <typename elem_t>
+__device__ __forceinline__ float as_float(elem_t x) {
+  if constexpr (std::is_same<elem_t, __nv_bfloat16>::value) return __bfloat162float(x);
+  else return __half2float(x);
+}
+template <typename elem_t>
+__device__ __forceinline__ elem_t as_elem(float x) {
+  if constexpr (std::is_same<elem_t, __nv_bfloat16>::value) return __float2bfloat16_rn(x);
+  else return __float2half_rn(x);
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
+  return x;
+}
+// LUCID's closing step for one column, given the joined sums over the rows before the newest:
+// v'_n from k_n's row (reference km, sum ka) and t_n; then a query row's result with its weight on v'_n.
+__device__ __forceinline__ float lucid_new_value(float tn, float vn, float km, float ka) {
+  float v = ex2_approx(-tn) * vn;
+  if (km != -INFINITY) v -= ex2_approx(km - tn) * ka;
+  return v;
+}
+__device__ __forceinline__ float lucid_output(float sn, float v_new, float m, float l, float a) {
+  const float mm = fmaxf(m, sn);
+  const float f = m == -INFINITY ? 0.f : ex2_approx(m - mm), w = ex2_approx(sn - mm);
+  return (a * f + w * v_new) / (l * f + w);
+}
+
+// kCluster: the grid's x dimension is one cluster of `splits` CTAs (1, 2, 4 or 8)
+template <bool kBf16, bool kLucid, bool kCluster>
 __global__ void __launch_bounds__(kPaWarps * 32, 2) paged_attn_kernel(const PagedAttnArgs args) {
   typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
   extern __shared__ uint8_t smem_raw[];
@@ -101,7 +134,10 @@ __global__ void __launch_bounds__(kPaWarps * 32, 2) paged_attn_kernel(const Page
   const Visible vis = visible(args, kLucid, len);
   const int chunk = chunk_keys(vis.n, args.splits);
   const int begin = split * chunk, end = imin(vis.n, begin + chunk);
-  if (begin >= end && (args.splits > 1 || kLucid)) return;     // an empty chunk: the second kernel does not read it
+  if constexpr (!kCluster) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (begin >= end) return;                                  // an empty chunk: the second kernel does not read it
+  }
 
   // ---- queries (and k_n) into shared memory, then into fragments ----
   for (int x = tid; x < 256; x += kPaWarps * 32) {
@@ -119,6 +155,18 @@ __global__ void __launch_bounds__(kPaWarps * 32, 2) paged_attn_kernel(const Page
     *reinterpret_cast<uint4*>(s.q + row256(r, ch)) = w;
   }
   __syncthreads();
+  if constexpr (kLucid && kCluster) {
+    for (int r = warp; r < rows; r += kPaWarps) {
+      const uint32_t at = (lane & 1) * 8;
+      const uint2 x = *reinterpret_cast<const uint2*>(s.q + row256(r, lane >> 1) + at);
+      const uint2 y = *reinterpret_cast<const uint2*>(s.q + row256(heads, lane >> 1) + at);
+      const float2 x0 = unpack2<kBf16>(x.x), x1 = unpack2<kBf16>(x.y), y0 = unpack2<kBf16>(y.x), y1 = unpack2<kBf16>(y.y);
+      float dot = (x0.x * y0.x + x0.y * y0.y) + (x1.x * y1.x + x1.y * y1.y);
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, m);
+      if (lane == 0) s.self[r] = dot;
+    }
+  }
   uint32_t qf[8][4];
 #pragma unroll
   for (int k = 0; k < 8; ++k) ldmatrix4(qf[k], smem_u32(s.q) + row256(lane & 15, 2 * k + (lane >> 4)));
@@ -258,6 +306,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, 2) paged_attn_kernel(const Page
     s.ml[warp][r1][1] = l1;
   }
   __syncthreads();
+  float* joined = reinterpret_cast<float*>(s.ring[0][1]);      // rows x 128 of this CTA (the stage behind warp 0's sums)
   for (int r = 0; r < rows; ++r) {
     float m = -INFINITY, l = 0.f, a = 0.f;
 #pragma unroll
@@ -269,11 +318,10 @@ __global__ void __launch_bounds__(kPaWarps * 32, 2) paged_attn_kernel(const Page
       l += f * s.ml[w][r][1];
       a += f * reinterpret_cast<const float*>(s.ring[w][0])[r * 128 + tid];
     }
-    if (args.splits == 1 && !kLucid) {
-      const float o = l != 0.f ? a / l : 0.f;
-      elem_t* out = reinterpret_cast<elem_t*>(args.out) + ((long long)b * args.Hq + hk * args.G + 16 * rc + r) * 128 + tid;
-      if constexpr (kBf16) *out = __float2bfloat16_rn(o);
-      else *out = __float2half_rn(o);
+    if constexpr (kCluster) {
+      joined[r * 128 + tid] = a;
+      if (tid == 0) s.chunk_ml[r][0] = m;
+      if (tid == 1) s.chunk_ml[r][1] = l;
     } else {
       const int total = args.G + (kLucid ? 1 : 0);
       float* p = args.partial + ((((long long)b * args.Hkv + hk) * total + 16 * rc + r) * args.splits + split) * kPaRow;
@@ -281,6 +329,61 @@ __global__ void __launch_bounds__(kPaWarps * 32, 2) paged_attn_kernel(const Page
       if (tid == 0) p[128] = m;
       if (tid == 1) p[129] = l;
     }
+  }
+  if constexpr (kCluster) {
+    cluster_sync_all();
+    // this CTA's share: columns split * per .. + per - 1 of every row
+    const int n = args.splits, per = 128 / n, col = split * per + tid % per;
+    const uint32_t a_joined = smem_u32(joined) + col * 4, a_ml = smem_u32(s.chunk_ml);
+    auto join = [&](int r, float& m, float& l, float& a) {
+      float pm[8], pl[8], pa[8];
+      m = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        if (x < n) {
+          const uint32_t at = mapa_u32(a_ml + r * 8, x);
+          pm[x] = ld_cluster(at);
+          pl[x] = ld_cluster(at + 4);
+          pa[x] = ld_cluster(mapa_u32(a_joined + r * 512, x));
+        } else {
+          pm[x] = -INFINITY;
+          pl[x] = pa[x] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 8; ++x) m = fmaxf(m, pm[x]);
+      const float z = m == -INFINITY ? 0.f : m;
+      l = a = 0.f;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const float f = ex2_approx(pm[x] - z);
+        l += f * pl[x];
+        a += f * pa[x];
+      }
+    };
+    elem_t v_stored = as_elem<elem_t>(0.f);
+    long long page = -1;
+    float m, l, a;
+    if constexpr (kLucid) {
+      if (len > 0) page = page_of(c, b, len - 1);
+      join(heads, m, l, a);
+      if (page >= 0) {
+        const float vn = as_float(reinterpret_cast<const elem_t*>(args.v_new)[b * args.v_b + hk * args.v_h + col]);
+        // the attention reads v'_n as the cache keeps it
+        v_stored = as_elem<elem_t>(lucid_new_value(s.self[heads] * args.lucid_log2, vn, m, a));
+        if (tid < per)
+          reinterpret_cast<elem_t*>(c.v)[page * c.v_page + ((len - 1) & ((1 << c.page_shift) - 1)) * c.v_row + hk * c.v_head + col] = v_stored;
+      } else if (len > 0 && tid == 0) {
+        report_error(&g_paged_ctl, kErrBadPage, b, len - 1, len - 1, 0);
+      }
+    }
+    for (int r = tid / per; r < heads; r += n) {
+      join(r, m, l, a);
+      float o = l != 0.f ? a / l : 0.f;
+      if constexpr (kLucid) o = page >= 0 ? lucid_output(s.self[r] * args.scale_log2, as_float(v_stored), m, l, a) : 0.f;
+      reinterpret_cast<elem_t*>(args.out)[((long long)b * args.Hq + hk * args.G + 16 * rc + r) * 128 + col] = as_elem<elem_t>(o);
+    }
+    cluster_sync_all();                                        // no CTA leaves while a peer reads its sums
   }
 }
 
@@ -333,18 +436,13 @@ __device__ __forceinline__ void join_row(const float* p, int n, float& m, float&
   m = mm;
 }
 
-template <typename elem_t>
-__device__ __forceinline__ float as_float(elem_t x) {
-  if constexpr (std::is_same<elem_t, __nv_bfloat16>::value) return __bfloat162float(x);
-  else return __half2float(x);
-}
-
 template <bool kBf16, bool kLucid>
 __global__ void __launch_bounds__(128 * kJoinGroups) paged_join_kernel(const PagedAttnArgs args) {
   typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
   __shared__ float red[kJoinGroups][3][128];
   __shared__ float red1[4 * kJoinGroups];
   const int row = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, d = threadIdx.x & 127;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int len = __ldg(args.lens + b);
   const Visible vis = visible(args, kLucid, len);
   const int chunk = chunk_keys(vis.n, args.splits);
@@ -370,44 +468,53 @@ __global__ void __launch_bounds__(128 * kJoinGroups) paged_join_kernel(const Pag
       const float vn = as_float(reinterpret_cast<const elem_t*>(args.v_new)[b * args.v_b + hk * args.v_h + d]);
       const float tn = block_sum(kn * kn, red1) * args.lucid_log2;
       const float sn = block_sum(qn * kn, red1) * args.scale_log2;
-      float vp = ex2_approx(-tn) * vn;
-      if (km != -INFINITY) vp -= ex2_approx(km - tn) * ka;
       // the attention reads v'_n as the cache keeps it
-      elem_t stored;
-      if constexpr (kBf16) stored = __float2bfloat16_rn(vp);
-      else stored = __float2half_rn(vp);
+      const elem_t stored = as_elem<elem_t>(lucid_new_value(tn, vn, km, ka));
       if (row == 0 && threadIdx.x < 128)
         reinterpret_cast<elem_t*>(c.v)[page * c.v_page + slot * c.v_row + hk * c.v_head + d] = stored;
-      const float mm = fmaxf(m, sn);
-      const float f = m == -INFINITY ? 0.f : ex2_approx(m - mm), w = ex2_approx(sn - mm);
-      o = (a * f + w * as_float(stored)) / (l * f + w);
+      o = lucid_output(sn, as_float(stored), m, l, a);
     }
   }
-  if (threadIdx.x < 128) {
-    elem_t* out = reinterpret_cast<elem_t*>(args.out) + ((long long)b * args.Hq + hk * args.G + row) * 128 + d;
-    if constexpr (kBf16) *out = __float2bfloat16_rn(o);
-    else *out = __float2half_rn(o);
-  }
+  if (threadIdx.x < 128)
+    reinterpret_cast<elem_t*>(args.out)[((long long)b * args.Hq + hk * args.G + row) * 128 + d] = as_elem<elem_t>(o);
 }
 
 size_t paged_attn_partial_bytes(int B, int Hq, int Hkv, bool lucid, int splits) {
-  if (splits == 1 && !lucid) return 0;
+  if (splits <= kPagedCluster) return 0;
   return (size_t)B * (Hq + (lucid ? Hkv : 0)) * splits * kPaRow * sizeof(float);
 }
 
 template <bool kBf16, bool kLucid>
 static cudaError_t launch_typed(const PagedAttnArgs& args, cudaStream_t stream) {
   const int bytes = (int)sizeof(PagedAttnSmem) + 128;
-  cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<kBf16, kLucid>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const bool cluster = args.splits <= kPagedCluster;
+  auto kernel = cluster ? paged_attn_kernel<kBf16, kLucid, true> : paged_attn_kernel<kBf16, kLucid, false>;
+  static SmemOnce once[2];
+  cudaError_t e = once[cluster].set(reinterpret_cast<const void*>(kernel), bytes);
   if (e != cudaSuccess) return e;
-  const int chunks = (args.G + 15) / 16;
-  paged_attn_kernel<kBf16, kLucid><<<dim3(args.splits, args.Hkv * chunks, args.B), kPaWarps * 32, bytes, stream>>>(args);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if (args.splits > 1 || kLucid) {
-    paged_join_kernel<kBf16, kLucid><<<dim3(args.G, args.Hkv, args.B), 128 * kJoinGroups, 0, stream>>>(args);
-    e = cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(args.splits, args.Hkv * ((args.G + 15) / 16), args.B);
+  cfg.blockDim = dim3(kPaWarps * 32);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  if (cluster) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = args.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
   }
-  return e;
+  if ((e = cudaLaunchKernelEx(&cfg, kernel, args)) != cudaSuccess || cluster) return e;
+  // the second kernel's CTAs may start while the first one's are still at work; they wait for them on the device
+  cfg.gridDim = dim3(args.G, args.Hkv, args.B);
+  cfg.blockDim = dim3(128 * kJoinGroups);
+  cfg.dynamicSmemBytes = 0;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<kBf16, kLucid>, args);
 }
 
 cudaError_t launch_paged_attn(bool bf16, bool lucid, const PagedAttnArgs& args, cudaStream_t stream) {

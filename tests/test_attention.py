@@ -115,47 +115,56 @@ def test_refusals_of_the_c_entry_points():
     p = (ctypes.addressof(buf) + 1023) // 1024 * 1024
     I3, I2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
     st, s2 = I3(512 * 1024, 1024, 128), I2(1024, 128)
+    byref = ctypes.byref
 
-    def fwd(q=p, Nq=512, Nk=512, Hq=4, Hkv=2, Dh=128, dt=1, w=128, s=0, scale=0.1, lse=p, qs=st):
-        return lib.lucid_window_attn_fwd(q, p, p, p, lse, qs, st, st, st, 1, Nq, Nk, Hq, Hkv, Dh, dt, w, s, scale, None, None)
+    def window(Nq=512, Nk=512, Hq=4, Hkv=2, Dh=128, dt=1, w=128, s=0, scale=0.1, qs=st):
+        return byref(_cabi.WindowAttnDesc(1, Nq, Nk, Hq, Hkv, Dh, dt, w, s, scale, qs, *[st] * 7))
+
+    def fwd(q=p, out=p, **kw):
+        return lib.lucid_window_attn_fwd(window(**kw), q, p, p, out, None, None, None)
 
     assert fwd(Dh=64) == -1 and fwd(Nq=0) == -1 and fwd(Nq=513) == -1 and fwd(s=129) == -1 and fwd(s=-1) == -1
-    assert fwd(Hq=3) == -10 and fwd(dt=2) == -2 and fwd(q=None) == -5 and fwd(lse=None) == -5 and fwd(q=p + 2) == -3
+    assert fwd(Hq=3) == -10 and fwd(dt=2) == -2 and fwd(q=None) == -5 and fwd(out=None) == -5 and fwd(q=p + 2) == -3
     assert fwd(scale=0.0) == -13 and fwd(scale=float("nan")) == -13 and fwd(scale=float("inf")) == -13
     assert fwd(qs=I3(512 * 1024, 1028, 128)) == -3 and fwd(qs=I3(512 * 1024, 0, 128)) == -9
-    assert fwd(Nk=1 << 29) == -1
+    assert fwd(Nk=1 << 29) == -1 and lib.lucid_window_attn_fwd(None, p, p, p, p, None, None, None) == -5
 
-    def bwd(ws=p, wsb=1 << 40, dk=p, dv=p, dq=p):
-        return lib.lucid_window_attn_bwd(p, p, p, p, p, p, dq, dk, dv, *[st] * 8, 1, 512, 512, 4, 2, 128, 1, 128, 4, 0.1, None, ws, wsb, None)
+    def bwd(ws=p, wsb=1 << 40, dk=p, dv=p, lse=p):
+        return lib.lucid_window_attn_bwd(window(s=4), p, p, p, p, lse, p, p, dk, dv, None, ws, wsb, None)
 
-    assert bwd(ws=None) == -5 and bwd(ws=p + 4) == -3 and bwd(wsb=100) == -4 and bwd(dk=None) == -5
-    assert lib.lucid_window_attn_bwd_workspace_bytes(1, 512, 512, 4, 2, 128, 0) == 4 * 512 * 8
-    assert lib.lucid_window_attn_bwd_workspace_bytes(1, 512, 512, 4, 3, 128, 0) == 0
+    assert bwd(ws=None) == -5 and bwd(ws=p + 4) == -3 and bwd(wsb=100) == -4 and bwd(dk=None) == -5 and bwd(lse=None) == -5
+    assert lib.lucid_window_attn_bwd_workspace_bytes(window()) == 4 * 512 * 8
+    assert lib.lucid_window_attn_bwd_workspace_bytes(window(Hkv=3)) == 0
 
     def cache(**kw):
-        a = dict(k=p, v=p, k_strides=I3(64 * 256, 256, 128), v_strides=I3(64 * 256, 256, 128), block_table=p, table_stride=4, table_width=4,
-                 pages=8, page_rows=64)
+        a = dict(k_strides=I3(64 * 256, 256, 128), v_strides=I3(64 * 256, 256, 128), table_stride=4, table_width=4, pages=8, page_rows=64)
         a.update(kw)
-        return ctypes.byref(_cabi.PagedCache(**a))
+        return _cabi.PagedCacheDesc(**a)
 
-    def app(c=None, T=3, cu=p, rot=128, freq=p, q=None, q_out=None, dt=1, k=p, lens=p, B=2):
-        return lib.lucid_paged_append(k, p, q, q_out, s2, s2, s2, c or cache(), lens, cu, freq, B, T, 4, 2, 128, rot, 0, dt, None)
+    def app(c=None, T=3, cu=p, rot=128, freq=p, q=None, q_out=None, dt=1, k=p, lens=p, kc=p, table=p):
+        d = _cabi.PagedAppendDesc(c or cache(), 2, T, 4, 2, 128, rot, 0, dt, s2, s2, s2)
+        return lib.lucid_paged_append(byref(d), k, p, q, q_out, kc, p, table, lens, cu, freq, None)
 
     assert app(T=0) == -1 and app(cu=None) == -1 and app(rot=120) == -12 and app(rot=144) == -12 and app(dt=5) == -2
     assert app(k=None) == -5 and app(lens=None) == -5 and app(q=p) == -5 and app(q=p, q_out=p, freq=None) == -5 and app(k=p + 4) == -3
-    for bad in (dict(page_rows=48), dict(page_rows=0), dict(pages=0), dict(table_width=0), dict(page_rows=131072)):
+    bad_pages = (dict(page_rows=48), dict(page_rows=0), dict(pages=0), dict(table_width=0), dict(page_rows=131072))
+    for bad in bad_pages:
         assert app(cache(**bad)) == -11, bad
-    assert app(cache(block_table=None)) == -5 and app(cache(table_stride=3)) == -9 and app(cache(k=p + 8)) == -3
+    assert app(table=None) == -5 and app(cache(table_stride=3)) == -9 and app(kc=p + 8) == -3
     assert app(cache(k_strides=I3(0, 256, 128))) == -9 and app(cache(table_width=1 << 26, table_stride=1 << 26)) == -1
 
-    def step(Hq=4, Hkv=2, scale=0.1, ws=p, wsb=1 << 40, B=2, c=None, lens=p, s=0):
-        return lib.lucid_paged_window_attn(p, p, s2, c or cache(), lens, B, Hq, Hkv, 128, 1, 100, s, scale, ws, wsb, None)
+    def step(Hq=4, Hkv=2, scale=0.1, ws=p, wsb=1 << 40, B=2, c=None, lens=p, s=0, w=100):
+        d = _cabi.PagedAttnDesc(c or cache(), B, Hq, Hkv, 128, 1, w, s, scale, 1.0, s2, s2)
+        return lib.lucid_paged_window_attn(byref(d), p, p, p, p, p, lens, ws, wsb, None)
 
     assert step(Hq=5) == -10 and step(scale=-1.0) == -13 and step(B=0) == -1 and step(B=70000) == -1 and step(lens=None) == -5
-    assert step(s=-1) == -1 and step(ws=None) == -5 and step(wsb=8) == -4 and step(c=cache(page_rows=3)) == -11
+    assert step(s=-1) == -1 and step(ws=p + 4) == -3 and step(c=cache(page_rows=3)) == -11
+    long = cache(table_width=4096, table_stride=4096)
+    assert step(c=long, w=-1, ws=None) == -5 and step(c=long, w=-1, wsb=8) == -4
 
     def lucid(Hq=4, ks=1.0, v=p):
-        return lib.lucid_paged_lucid_attn(p, v, p, s2, s2, cache(), p, 2, Hq, 2, 128, 1, ks, 0.1, p, 1 << 40, None)
+        d = _cabi.PagedAttnDesc(cache(), 2, Hq, 2, 128, 1, -1, 0, 0.1, ks, s2, s2)
+        return lib.lucid_paged_lucid_attn(byref(d), p, v, p, p, p, p, p, p, 1 << 40, None)
 
     assert lucid(Hq=32) == -10 and lucid(ks=0.0) == -13 and lucid(v=None) == -5
     for code in (-10, -11, -12, -13, 4):
