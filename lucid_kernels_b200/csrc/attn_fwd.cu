@@ -11,9 +11,13 @@
 // columns of TMEM; the 16-bit weights P overwrite it) and O (128 columns): 512 columns in all.  While the tensor pipe
 // runs one tile's P V and next S, the other tile's warps form exponentials.
 //
-// Warp roles (384 threads): warp 0 producer, warps 1 and 2 issue the products of tile 0 and 1 (an issuing thread runs
-// only a few products ahead of the tensor pipe), warp 3 owns TMEM; warps 4-7 and 8-11 are the softmax groups of the
-// two tiles, one row per thread.  Persistent CTAs, items dealt out round robin, the longest first.
+// Warp roles (384 threads): warp 0 producer, warp 1 issues all products in the order P V and next S of tile 0, the same of
+// tile 1, ... (one thread's products run in order, so the two tiles' scores become ready half a period apart and their
+// exponentials do not compete; with an issuer per tile the products interleaved and both groups ran in phase), warp 3
+// owns TMEM; warps 4-7 and 8-11 are the softmax groups of the two tiles, one row per thread.  P is handed over in two
+// halves, so that P V starts while the second half's exponentials are formed.  Persistent CTAs, items dealt out round
+// robin, the longest first; results leave through a staging panel per tile and TMA (a thread's own row stores touch 32 lines
+// per instruction and took as long as one and a half tiles).
 #include <type_traits>
 #include "attn.h"
 
@@ -21,27 +25,29 @@ namespace lucid {
 
 static __device__ Control g_attn_fwd_ctl;
 
-constexpr int kFwRing = 5;
+constexpr int kFwRing = 4;
 struct AttnFwdSmem {
   alignas(1024) uint8_t q[2][kTileBytes];
   alignas(1024) uint8_t ring[kFwRing][kTileBytes];   // K(0), V(0), K(1), V(1), ... of the union of the two tiles' lists
+  alignas(1024) uint8_t stage[2][kHalfBytes];         // 128 rows x 64 columns of a tile's result
   alignas(8) uint64_t full[kFwRing];
-  uint64_t empty[kFwRing], q_full[2], q_free[2], s_full[2], p_ready[2], o_full[2], o_free[2];
+  uint64_t empty[kFwRing], q_full[2], q_free[2], s_full[2], p_half[2], p_ready[2], o_full[2], o_free[2];
   uint32_t tmem_base;
   int abort_flag;
 };
 
-enum AttnFwdBar : int { AF_FULL = 401, AF_EMPTY, AF_Q_FULL, AF_Q_FREE, AF_S_FULL, AF_P_READY, AF_O_FULL, AF_O_FREE };
+enum AttnFwdBar : int { AF_FULL = 401, AF_EMPTY, AF_Q_FULL, AF_Q_FREE, AF_S_FULL, AF_P_HALF, AF_P_READY, AF_O_FULL, AF_O_FREE };
 
 constexpr int kFwThreads = 384;
 constexpr int kFwS = 0, kFwO = 256;      // + 128 * tile
-constexpr int kFwRegsService = 56, kFwRegsSoftmax = 224;    // 128 * 56 + 256 * 224 = 384 * 168, the launch's total
+constexpr int kFwRegsService = 88, kFwRegsSoftmax = 208;    // 128 * 88 + 256 * 208 = 384 * 168, the launch's total
 constexpr float kFwSlack = 8.f;          // log2 of how far the maximum may outgrow the reference
 
 template <bool kBf16>
 __global__ void __launch_bounds__(kFwThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                const __grid_constant__ CUtensorMap tm_v, const AttnFwdArgs args) {
+                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_out,
+                const AttnFwdArgs args) {
   extern __shared__ uint8_t smem_raw[];
   AttnFwdSmem& s = *reinterpret_cast<AttnFwdSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const AttnShape& A = args.a;
@@ -53,12 +59,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   if (tid == 0) {
     for (int i = 0; i < kFwRing; ++i) {
       mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], 2);
+      mbar_init(&s.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.q_full[i], 1);
       mbar_init(&s.q_free[i], 1);
       mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_half[i], 128);
       mbar_init(&s.p_ready[i], 128);
       mbar_init(&s.o_full[i], 1);
       mbar_init(&s.o_free[i], 128);
@@ -91,7 +98,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         for (int idx = blockIdx.x; alive && fwd_item(A, idx, it); idx += gridDim.x) {
           const PairTiles pt = pair_tiles(A, it, length_of(it.b));
           auto load = [&](const CUtensorMap* tm, int tile) -> bool {
-            if (!wait_barrier(&s.empty[stage], phase ^ 1, cta_abort, ctl, limit, idx, (int)r, AF_EMPTY)) return false;
+            if (!wait_barrier_soon(&s.empty[stage], phase ^ 1, cta_abort, ctl, limit, idx, (int)r, AF_EMPTY)) return false;
             mbar_expect_tx(&s.full[stage], kTileBytes);
             tma_load_4d(s.ring[stage], tm, &s.full[stage], 0, tile * kBlock, it.hk, it.b);
             tma_load_4d(s.ring[stage] + kHalfBytes, tm, &s.full[stage], 64, tile * kBlock, it.hk, it.b);
@@ -104,7 +111,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           };
           for (int t = 0; t < 2 && alive; ++t) {
             if (pt.list(t).n == 0) continue;
-            if (!wait_barrier(&s.q_free[t], (nq[t] & 1) ^ 1, cta_abort, ctl, limit, idx, t, AF_Q_FREE)) {
+            if (!wait_barrier_soon(&s.q_free[t], (nq[t] & 1) ^ 1, cta_abort, ctl, limit, idx, t, AF_Q_FREE)) {
               alive = false;
               break;
             }
@@ -119,89 +126,118 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         }
       }
-    } else if (warp < 3) {
-      // =========================== issuer of one tile's products ===========================
-      const int t = warp - 1;
+    } else if (warp == 1) {
+      // =========================== issuer of all products ===========================
       constexpr int fmt = kBf16 ? 1 : 0;
-      constexpr uint32_t idesc_s = umma_idesc(fmt, 0, 0, 128, 128);    // Q K^T: both K-major
-      constexpr uint32_t idesc_o = umma_idesc(fmt, 0, 1, 128, 128);    // P V: P from TMEM, V rows = k
-      const uint64_t d_q = umma_smem_desc(smem_u32(s.q[t]), 16, 1024);
+      constexpr uint32_t idesc_s = umma_idesc(fmt, 0, 0, 128, 128);          // Q K^T: both K-major
+      constexpr uint32_t idesc_sn = umma_idesc(fmt, 0, 0, 128, kNarrow);     // the first kNarrow keys only
+      constexpr uint32_t idesc_o = umma_idesc(fmt, 0, 1, 128, 128);          // P V: P from TMEM, V rows = k
+      const uint64_t d_q0 = umma_smem_desc(smem_u32(s.q[0]), 16, 1024);
       const uint64_t d_k0 = umma_smem_desc(smem_u32(s.ring[0]), 16, 1024);
       const uint64_t d_v0 = umma_smem_desc(smem_u32(s.ring[0]), kHalfBytes, 1024);
-      const uint32_t s_tmem = tmem + kFwS + 128 * t, o_tmem = tmem + kFwO + 128 * t;
-      uint32_t r = 0;          // ring uses before this item: K(u) is use r + 2u, V(u) use r + 2u + 1
-      uint32_t nq = 0, np = 0; // items with tiles; weights consumed
+      uint32_t st = 0, phase = 0;        // ring stage and phase of K(u); V(u) is the one behind it
+      uint32_t nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;   // items with tiles; weights consumed
       bool alive = true;
       FwdItem it;
       for (int idx = blockIdx.x; alive && fwd_item(A, idx, it); idx += gridDim.x) {
         const PairTiles pt = pair_tiles(A, it, length_of(it.b));
-        const KeyTiles kt = pt.list(t);
-        const bool mine = kt.n > 0;
-        if (mine && !wait_barrier(&s.q_full[t], nq & 1, cta_abort, ctl, limit, idx, t, AF_Q_FULL)) break;
-        auto wait_full = [&](uint32_t use) -> bool {
-          return wait_barrier(&s.full[use % kFwRing], (use / kFwRing) & 1, cta_abort, ctl, limit, idx, (int)use, AF_FULL);
-        };
-        bool first = true;
-        // O (+)= P(u) V(u), once the softmax group has written P(u)
-        auto issue_pv = [&](int u) -> bool {
-          const uint32_t use = r + 2 * u + 1, st = use % kFwRing;
-          if (!wait_barrier(&s.p_ready[t], np & 1, cta_abort, ctl, limit, idx, u, AF_P_READY)) return false;
-          ++np;
-          if (!wait_full(use)) return false;
+        bool first0 = true, first1 = true;
+        int left0 = pt.x.n, left1 = pt.y.n;
+        bool pend0 = false, pend1 = false;      // weights of tile u - 1 on their way
+        uint32_t v_st = 0, v_phase = 0;         // V(u - 1)
+        // O_t (+)= P_t(u-1) V(u-1)
+        auto issue_pv = [&](int t, uint32_t& np, uint32_t nq, bool& first, bool narrow) -> bool {
+          const uint32_t s_tmem = tmem + kFwS + 128 * t, o_tmem = tmem + kFwO + 128 * t;
+          if (!wait_barrier_soon(&s.p_half[t], np & 1, cta_abort, ctl, limit, idx, t, AF_P_HALF)) return false;
           // the epilogue of this tile's previous item has read O
-          if (first && !wait_barrier(&s.o_free[t], (nq & 1) ^ 1, cta_abort, ctl, limit, idx, u, AF_O_FREE)) return false;
+          if (first && !wait_barrier_soon(&s.o_free[t], (nq & 1) ^ 1, cta_abort, ctl, limit, idx, t, AF_O_FREE)) return false;
           tc_fence_after_sync();
-          const uint64_t dv = d_v0 + st * (kTileBytes >> 4);
+          const uint64_t dv = d_v0 + v_st * (kTileBytes >> 4);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            umma_ts_w(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, (!first || k) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k)
+            if (k < kNarrow / 16 || !narrow)
+              umma_ts_w(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, (!first || k) ? 1u : 0u);
+          if (!wait_barrier_soon(&s.p_ready[t], np & 1, cta_abort, ctl, limit, idx, t, AF_P_READY)) return false;
+          ++np;
+          if (!narrow) {
+            tc_fence_after_sync();
+#pragma unroll
+            for (int k = 4; k < 8; ++k) umma_ts_w(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, 1u);
+          }
           first = false;
-          umma_commit_w(&s.empty[st]);
           return true;
         };
-        int pend = -1, left = kt.n;
-        for (int u = 0; u < pt.n; ++u) {
-          const bool act = pt.active(kt, u);
-          if (pend >= 0) {
-            if (!issue_pv(pend)) { alive = false; break; }
-            pend = -1;
-          }
-          const uint32_t use = r + 2 * u, st = use % kFwRing;
-          if (!wait_full(use)) { alive = false; break; }
-          if (act) {
-            tc_fence_after_sync();
-            const uint64_t dk = d_k0 + st * (kTileBytes >> 4);
+        auto issue_s = [&](int t, uint32_t& nq, int& left, int own, bool narrow) -> bool {
+          if (left == own && !wait_barrier_soon(&s.q_full[t], nq & 1, cta_abort, ctl, limit, idx, t, AF_Q_FULL)) return false;
+          tc_fence_after_sync();
+          const uint64_t dq = d_q0 + t * (kTileBytes >> 4), dk = d_k0 + st * (kTileBytes >> 4);
+          const uint32_t s_tmem = tmem + kFwS + 128 * t;
+          if (narrow) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-              umma_ss_w(s_tmem, d_q + off, dk + off, idesc_s, k ? 1u : 0u);
+              umma_ss_w(s_tmem, dq + off, dk + off, idesc_sn, k ? 1u : 0u);
             }
-            umma_commit_w(&s.s_full[t]);
-            umma_commit_w(&s.empty[st]);
-            if (--left == 0) umma_commit_w(&s.q_free[t]);
-            pend = u;
           } else {
-            // not this tile's keys: hand both stages on (each only after it has been filled)
-            __syncwarp();
-            mbar_arrive_w(&s.empty[st]);
-            if (!wait_full(use + 1)) { alive = false; break; }
-            __syncwarp();
-            mbar_arrive_w(&s.empty[(use + 1) % kFwRing]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
+              umma_ss_w(s_tmem, dq + off, dk + off, idesc_s, k ? 1u : 0u);
+            }
+          }
+          umma_commit_w(&s.s_full[t]);
+          if (--left == 0) umma_commit_w(&s.q_free[t]);
+          return true;
+        };
+        bool was_narrow0 = false, was_narrow1 = false;
+        for (int u = 0; u <= pt.n; ++u) {
+          const bool act0 = u < pt.n && pt.active(pt.x, u), act1 = u < pt.n && pt.active(pt.y, u);
+          const bool narrow0 = u < pt.n && tile_narrow(A, pt.x, pt.tile(u)), narrow1 = u < pt.n && tile_narrow(A, pt.y, pt.tile(u));
+          if (u > 0) {
+            if (!wait_barrier_soon(&s.full[v_st], v_phase, cta_abort, ctl, limit, idx, u, AF_FULL)) { alive = false; break; }
+          }
+          if (pend0 && !issue_pv(0, np0, nq0, first0, was_narrow0)) { alive = false; break; }
+          if (u < pt.n && !wait_barrier_soon(&s.full[st], phase, cta_abort, ctl, limit, idx, u, AF_FULL)) { alive = false; break; }
+          if (act0 && !issue_s(0, nq0, left0, pt.x.n, narrow0)) { alive = false; break; }
+          if (pend1 && !issue_pv(1, np1, nq1, first1, was_narrow1)) { alive = false; break; }
+          if (u > 0) umma_commit_w(&s.empty[v_st]);
+          if (act1 && !issue_s(1, nq1, left1, pt.y.n, narrow1)) { alive = false; break; }
+          if (u < pt.n) umma_commit_w(&s.empty[st]);
+          pend0 = act0;
+          pend1 = act1;
+          was_narrow0 = narrow0;
+          was_narrow1 = narrow1;
+          if (u < pt.n) {
+            v_st = st + 1;
+            v_phase = phase;
+            if (v_st == kFwRing) {
+              v_st = 0;
+              v_phase ^= 1;
+            }
+            st = v_st + 1;
+            phase = v_phase;
+            if (st == kFwRing) {
+              st = 0;
+              phase ^= 1;
+            }
+          }
+          // a tile's last weights have been consumed: its result is complete
+          if (u > 0 && pt.x.n > 0 && left0 == 0 && !pend0) {
+            umma_commit_w(&s.o_full[0]);
+            ++nq0;
+            left0 = -1;
+          }
+          if (u > 0 && pt.y.n > 0 && left1 == 0 && !pend1) {
+            umma_commit_w(&s.o_full[1]);
+            ++nq1;
+            left1 = -1;
           }
         }
-        if (!alive) break;
-        if (pend >= 0 && !issue_pv(pend)) break;
-        if (mine) {
-          umma_commit_w(&s.o_full[t]);
-          ++nq;
-        }
-        r += 2 * pt.n;
       }
     }
   } else {
     // =========================== softmax of one tile, then its epilogue ===========================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFwRegsSoftmax));
-    typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
     const int t = (warp - 4) >> 2;
     const int row = ((warp & 3) << 5) + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -222,82 +258,93 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       for (int u = 0; u < pt.n; ++u) {
         if (!pt.active(kt, u)) continue;
         const int tile = pt.tile(u), j0 = tile << 7;
-        if (!wait_barrier(&s.s_full[t], ns & 1, cta_abort, ctl, limit, idx, u, AF_S_FULL)) { alive = false; break; }
+        if (!wait_barrier_soon(&s.s_full[t], ns & 1, cta_abort, ctl, limit, idx, u, AF_S_FULL)) { alive = false; break; }
         ++ns;
         tc_fence_after_sync();
-        uint32_t v[128];
-        {
-          uint32_t(&v0)[32] = *reinterpret_cast<uint32_t(*)[32]>(v);
-          uint32_t(&v1)[32] = *reinterpret_cast<uint32_t(*)[32]>(v + 32);
-          uint32_t(&v2)[32] = *reinterpret_cast<uint32_t(*)[32]>(v + 64);
-          uint32_t(&v3)[32] = *reinterpret_cast<uint32_t(*)[32]>(v + 96);
-          tmem_ld32(s_tmem, v0);
-          tmem_ld32(s_tmem + 32, v1);
-          tmem_ld32(s_tmem + 64, v2);
-          tmem_ld32(s_tmem + 96, v3);
-          tmem_wait_ld();
-        }
-        if (tile_masked(A, kt, tile, len)) {
-          const RowMask mask = row_mask(A, p, j0, len);
-#pragma unroll
-          for (int e = 0; e < 128; ++e) v[e] = mask.sees(e) ? v[e] : 0xff800000u;
+        const bool masked = tile_masked(A, kt, tile, len);
+        const RowMask mask = row_mask(A, p, j0, len);
+        if (masked) {
           if (j0 + 127 >= len && len < A.Nk) {
             // rows behind the sequence hold anything, and 0 * NaN is not 0: the value tile's become zero
             const uint32_t use = r + 2 * u + 1;
-            if (!wait_barrier(&s.full[use % kFwRing], (use / kFwRing) & 1, cta_abort, ctl, limit, idx, (int)use, AF_FULL)) {
+            if (!wait_barrier_soon(&s.full[use % kFwRing], (use / kFwRing) & 1, cta_abort, ctl, limit, idx, (int)use, AF_FULL)) {
               alive = false;
               break;
             }
             if (j0 + row >= len) zero_tile_row(s.ring[use % kFwRing], row);
             __syncwarp();
-          }
-          fence_proxy_async_smem();
-        }
-        float mx[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(v[c]);
-#pragma unroll
-        for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[e]));
-        const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-        const bool grow = m > ref + kFwSlack;
-        if (first) {
-          ref = m;
-        } else if (__any_sync(0xffffffffu, grow)) {
-          // S(u) is complete, and with it every product issued before it: O holds all earlier tiles
-          const float next = fmaxf(ref, m);
-          const float f = next == -INFINITY ? 1.f : ex2_approx(ref - next);
-          ref = next;
-          l *= f;
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint32_t o[16];
-            tmem_ld16(o_tmem + 16 * c, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st16(o_tmem + 16 * c, o);
+            fence_proxy_async_smem();
           }
         }
-        first = false;
-        const float neg = ref == -INFINITY ? 0.f : -ref;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // the tile's first 32 * kChunks columns (the rest is not visible, and P is not read there)
+        auto weights = [&](auto chunks) {
+          constexpr int kChunks = decltype(chunks)::value;
+          uint32_t v[kChunks][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
+          for (int c = 0; c < kChunks; ++c) tmem_ld32(s_tmem + 32 * c, v[c]);
+          tmem_wait_ld();
+          if (masked) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float a = ex2_approx(fmaf(__uint_as_float(v[32 * c + 2 * e]), sl2, neg));
-            const float b = ex2_approx(fmaf(__uint_as_float(v[32 * c + 2 * e + 1]), sl2, neg));
-            sum[(2 * e) & 3] += a;
-            sum[(2 * e + 1) & 3] += b;
-            pk[e] = pack2<kBf16>(a, b);
+            for (int c = 0; c < kChunks; ++c) {
+              const uint32_t w = mask.word(32 * c);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[c][e] = (w & (1u << e)) ? v[c][e] : 0xff800000u;
+            }
           }
-          tmem_st16(s_tmem + 16 * c, pk);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-        tc_fence_before_sync();
-        mbar_arrive(&s.p_ready[t]);
+          float mx[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mx[x] = __uint_as_float(v[0][x]);
+#pragma unroll
+          for (int x = 4; x < 32 * kChunks; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x >> 5][x & 31]));
+          const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+          const bool grow = m > ref + kFwSlack;
+          if (first) {
+            ref = m;
+          } else if (__any_sync(0xffffffffu, grow)) {
+            // S(u) is complete, and with it every product issued before it: O holds all earlier tiles
+            const float next = fmaxf(ref, m);
+            const float f = next == -INFINITY ? 1.f : ex2_approx(ref - next);
+            ref = next;
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o_tmem + 16 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(o_tmem + 16 * c, o);
+            }
+          }
+          first = false;
+          const float neg = ref == -INFINITY ? 0.f : -ref;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float a = ex2_approx(fmaf(__uint_as_float(v[c][2 * e]), sl2, neg));
+              const float b = ex2_approx(fmaf(__uint_as_float(v[c][2 * e + 1]), sl2, neg));
+              sum[(2 * e) & 3] += a;
+              sum[(2 * e + 1) & 3] += b;
+              pk[e] = pack2<kBf16>(a, b);
+            }
+            tmem_st16(s_tmem + 16 * c, pk);
+            if (c == 1 && kChunks > 2) {
+              tmem_wait_st();
+              tc_fence_before_sync();
+              mbar_arrive(&s.p_half[t]);
+            }
+          }
+          tmem_wait_st();
+          tc_fence_before_sync();
+          if (kChunks <= 2) mbar_arrive(&s.p_half[t]);
+          mbar_arrive(&s.p_ready[t]);
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        };
+        if (tile_narrow(A, kt, tile)) weights(std::integral_constant<int, kNarrow / 32>{});
+        else weights(std::integral_constant<int, 4>{});
       }
       if (!alive) break;
       r += 2 * pt.n;
@@ -305,45 +352,54 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // ---- epilogue ----
       const bool has = kt.n > 0;
       if (has) {
-        if (!wait_barrier(&s.o_full[t], no & 1, cta_abort, ctl, limit, idx, t, AF_O_FULL)) break;
+        if (!wait_barrier_soon(&s.o_full[t], no & 1, cta_abort, ctl, limit, idx, t, AF_O_FULL)) break;
         ++no;
         tc_fence_after_sync();
       }
       const bool some = valid && l != 0.f;      // (a NaN sum is written as it is)
       const float inv = some ? 1.f / l : 0.f;
-      const bool store = i < A.Nq && it.block(t) < A.nqb;
-      elem_t* out = reinterpret_cast<elem_t*>(args.out) + it.b * args.out_strides.b + (long long)i * args.out_strides.n +
-                    it.h(t) * args.out_strides.h;
+      const bool lead = (tid & 127) == 0;
+      if (it.block(t) < A.nqb) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[32];
-        if (has) {
-          tmem_ld32(o_tmem + 32 * c, o);
-          tmem_wait_ld();
-        }
-        if (store) {
+        for (int hf = 0; hf < 2; ++hf) {
+          if (lead) tma_store_wait_read();               // the panel's previous store has read it
+          named_bar_sync(1 + t, 128);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (has && some) {
-              w.x = pack2<kBf16>(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
-              w.y = pack2<kBf16>(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
-              w.z = pack2<kBf16>(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
-              w.w = pack2<kBf16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
+          for (int c = 0; c < 2; ++c) {
+            uint32_t o[32];
+            if (has) {
+              tmem_ld32(o_tmem + 64 * hf + 32 * c, o);
+              tmem_wait_ld();
             }
-            *reinterpret_cast<uint4*>(out + 32 * c + 8 * e) = w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint4 w = make_uint4(0, 0, 0, 0);
+              if (has && some) {
+                w.x = pack2<kBf16>(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
+                w.y = pack2<kBf16>(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
+                w.z = pack2<kBf16>(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
+                w.w = pack2<kBf16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
+              }
+              *reinterpret_cast<uint4*>(s.stage[t] + sw128_off(row, 4 * c + e)) = w;
+            }
+          }
+          fence_proxy_async_smem();
+          named_bar_sync(1 + t, 128);
+          if (lead) {                                    // rows behind Nq lie outside the map and are not written
+            tma_store_4d(&tm_out, s.stage[t], 64 * hf, it.block(t) * kBlock, it.h(t), it.b);
+            tma_store_commit();
           }
         }
-        __syncwarp();
       }
       if (has) {
         tc_fence_before_sync();
         mbar_arrive(&s.o_free[t]);
       }
-      if (store && args.lse)
+      if (i < A.Nq && args.lse)
         args.lse[((long long)it.b * A.Hq + it.h(t)) * A.Nq + i] =
             some ? (ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
     }
+    if ((tid & 127) == 0) tma_store_wait_read();
   }
 
   if (s.abort_flag) {
@@ -358,14 +414,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 }
 
 cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
-                            const AttnFwdArgs& args, int sms, cudaStream_t stream) {
+                            const CUtensorMap& tm_out, const AttnFwdArgs& args, int sms, cudaStream_t stream) {
   const int items = fwd_items(args.a), grid = items < sms ? items : sms;
   const int bytes = (int)sizeof(AttnFwdSmem) + 1024;
   auto kernel = bf16 ? attn_fwd_kernel<true> : attn_fwd_kernel<false>;
   static SmemOnce once[2];
   cudaError_t e = once[bf16].set(reinterpret_cast<const void*>(kernel), bytes);
   if (e != cudaSuccess) return e;
-  kernel<<<grid, kFwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, args);
+  kernel<<<grid, kFwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, tm_out, args);
   return cudaGetLastError();
 }
 

@@ -55,10 +55,19 @@ LUCID_HD bool tile_masked(const AttnShape& a, const KeyTiles& t, int tile, int l
   return j0 + 127 > t.p_lo || (a.W < kNoWindow && j0 <= t.p_hi - a.W) || j0 + 127 >= len;
 }
 
+// A tile visited for its visible first keys alone, few enough for a product of kNarrow keys.
+constexpr int kNarrow = 32;
+LUCID_HD bool tile_narrow(const AttnShape& a, const KeyTiles& t, int tile) { return t.sink && tile == 0 && a.S <= kNarrow; }
+
 // Columns of a key tile (first key j0) that the query at position p sees: e <= hi and (e >= lo or e < first).
 struct RowMask {
   int hi, lo, first;
   LUCID_HD bool sees(int e) const { return e <= hi && (e >= lo || e < first); }
+  // bit e: column base + e, e < 32
+  LUCID_HD unsigned word(int base) const {
+    return below(hi + 1 - base) & (~below(lo - base) | below(first - base));
+  }
+  LUCID_HD static unsigned below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }   // bits 0 .. n-1
 };
 LUCID_HD RowMask row_mask(const AttnShape& a, int p, int j0, int len) {
   return RowMask{imin(p, len - 1) - j0, p - a.W + 1 - j0, a.S - j0};
@@ -72,6 +81,7 @@ LUCID_HD bool block_masked(const AttnShape& a, int j0, int p0, int len) {
 struct ColMask {
   int lo, hi;
   LUCID_HD bool sees(int e) const { return e >= lo && e <= hi; }
+  LUCID_HD unsigned word(int base) const { return RowMask::below(hi + 1 - base) & ~RowMask::below(lo - base); }
 };
 LUCID_HD ColMask col_mask(const AttnShape& a, int j, int p0, int len) {
   ColMask m;

@@ -88,6 +88,15 @@ __device__ __forceinline__ bool wait_barrier(uint64_t* bar, uint32_t parity, vol
   return true;
 }
 
+// The same wait for barriers that usually complete within a microsecond: a few more polls before the clock is looked at for
+// the first time (reading the global timer costs a waiter some hundred cycles).  Same limit, same report.
+__device__ __forceinline__ bool wait_barrier_soon(uint64_t* bar, uint32_t parity, volatile int* cta_abort, Control* ctl,
+                                                  unsigned long long limit_ns, int chain, int row, int bar_id) {
+  for (int i = limit_ns ? 32 : 1; i > 0; --i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return wait_barrier(bar, parity, cta_abort, ctl, limit_ns, chain, row, bar_id);
+}
+
 // A row-block is complete when its flag reaches kFlagComplete: set at once by the thread that stored the
 // block with TMA, or reached by the storing warps (8 or 16 of them) each adding their share with release
 // semantics after their own plain stores.

@@ -30,7 +30,9 @@ static int check(const AttnShape& a, const std::vector<int>& lens) {
         for (int i = blk * 128; i < blk * 128 + 128 && i < a.Nq && i + a.off < len; ++i) {
           const RowMask m = row_mask(a, i + a.off, j0, len);
           for (int e = 0; e < 128; ++e) {
+            if (((m.word(e & ~31) >> (e & 31)) & 1) != (m.sees(e) ? 1u : 0u)) return 16;
             if (masked && !m.sees(e)) continue;
+            if (tile_narrow(a, t, t.tile(u)) && (!masked || e >= kNarrow)) return 17;
             if (j0 + e >= a.Nk) return 2;
             ++seen[(size_t)i * a.Nk + j0 + e];
           }
@@ -80,6 +82,7 @@ static int check(const AttnShape& a, const std::vector<int>& lens) {
       for (int j = j0; j < j0 + 128 && j < a.Nk; ++j) {
         const ColMask c = col_mask(a, j, p0, len);
         for (int e = 0; e < 128; ++e) {
+          if (((c.word(e & ~31) >> (e & 31)) & 1) != (c.sees(e) ? 1u : 0u)) return 18;
           if (masked && !c.sees(e)) continue;
           if (blk * 128 + e >= a.Nq) return 12;
           if (kv.chunk >= 0 && j >= a.S) return 13;     // a chunk holds first keys only
