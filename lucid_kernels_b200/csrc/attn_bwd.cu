@@ -154,21 +154,21 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const KeyTiles kt = key_tiles(A, it.block, attn_length(A, args.lengths, it.b));
         if (kt.n == 0) continue;
         const int hk = it.h / A.G;
-        if (!wait_barrier(&s.q_free, (itn & 1) ^ 1, cta_abort, ctl, limit, idx, 0, AB_Q_FREE)) break;
+        if (!wait_lean(&s.q_free, (itn & 1) ^ 1, cta_abort, limit, AB_Q_FREE)) break;
         mbar_expect_tx(&s.q_full, kTileBytes);
         tma_load_4d(s.q, &tm_q, &s.q_full, 0, it.block * kBlock, it.h, it.b);
         tma_load_4d(s.q + kHalfBytes, &tm_q, &s.q_full, 64, it.block * kBlock, it.h, it.b);
-        if (!wait_barrier(&s.go_free, (itn & 1) ^ 1, cta_abort, ctl, limit, idx, 0, AB_GO_FREE)) break;
+        if (!wait_lean(&s.go_free, (itn & 1) ^ 1, cta_abort, limit, AB_GO_FREE)) break;
         mbar_expect_tx(&s.go_full, kTileBytes);
         tma_load_4d(s.go, &tm_do, &s.go_full, 0, it.block * kBlock, it.h, it.b);
         tma_load_4d(s.go + kHalfBytes, &tm_do, &s.go_full, 64, it.block * kBlock, it.h, it.b);
         for (int u = 0; u < kt.n; ++u, ++g) {
           const int j = kt.tile(u), ks = g % 3, vs = g & 1;
-          if (!wait_barrier(&s.k_empty[ks], ((g / 3) & 1) ^ 1, cta_abort, ctl, limit, idx, u, AB_K_EMPTY)) { alive = false; break; }
+          if (!wait_lean(&s.k_empty[ks], ((g / 3) & 1) ^ 1, cta_abort, limit, AB_K_EMPTY)) { alive = false; break; }
           mbar_expect_tx(&s.k_full[ks], kTileBytes);
           tma_load_4d(s.kring[ks], &tm_k, &s.k_full[ks], 0, j * kBlock, hk, it.b);
           tma_load_4d(s.kring[ks] + kHalfBytes, &tm_k, &s.k_full[ks], 64, j * kBlock, hk, it.b);
-          if (!wait_barrier(&s.v_empty[vs], ((g >> 1) & 1) ^ 1, cta_abort, ctl, limit, idx, u, AB_V_EMPTY)) { alive = false; break; }
+          if (!wait_lean(&s.v_empty[vs], ((g >> 1) & 1) ^ 1, cta_abort, limit, AB_V_EMPTY)) { alive = false; break; }
           mbar_expect_tx(&s.v_full[vs], kTileBytes);
           tma_load_4d(s.vring[vs], &tm_v, &s.v_full[vs], 0, j * kBlock, hk, it.b);
           tma_load_4d(s.vring[vs] + kHalfBytes, &tm_v, &s.v_full[vs], 64, j * kBlock, hk, it.b);
@@ -183,11 +183,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     DQ_ITEMS {
       const KeyTiles kt = key_tiles(A, it.block, attn_length(A, args.lengths, it.b));
       if (kt.n == 0) continue;
-      if (!wait_barrier(&s.go_full, itn & 1, cta_abort, ctl, limit, idx, 0, AB_GO_FULL)) break;
+      if (!wait_lean(&s.go_full, itn & 1, cta_abort, limit, AB_GO_FULL)) break;
       for (int u = 0; u < kt.n; ++u, ++g) {
-        if (g > 0 && !wait_barrier(&s.g_free, (g - 1) & 1, cta_abort, ctl, limit, idx, u, AB_G_FREE)) { alive = false; break; }
+        if (g > 0 && !wait_lean(&s.g_free, (g - 1) & 1, cta_abort, limit, AB_G_FREE)) { alive = false; break; }
         const uint32_t vs = g & 1;
-        if (!wait_barrier(&s.v_full[vs], (g >> 1) & 1, cta_abort, ctl, limit, idx, u, AB_V_FULL)) { alive = false; break; }
+        if (!wait_lean(&s.v_full[vs], (g >> 1) & 1, cta_abort, limit, AB_V_FULL)) { alive = false; break; }
         tc_fence_after_sync();
         const uint64_t db = d_v0 + vs * (kTileBytes >> 4);
 #pragma unroll
@@ -209,11 +209,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     DQ_ITEMS {
       const KeyTiles kt = key_tiles(A, it.block, attn_length(A, args.lengths, it.b));
       if (kt.n == 0) continue;
-      if (!wait_barrier(&s.q_full, itn & 1, cta_abort, ctl, limit, idx, 0, AB_Q_FULL)) break;
+      if (!wait_lean(&s.q_full, itn & 1, cta_abort, limit, AB_Q_FULL)) break;
       for (int u = 0; u < kt.n; ++u, ++g) {
         const uint32_t ks = g % 3, buf = g & 1;
-        if (!wait_barrier(&s.sbuf_free[buf], ((g >> 1) & 1) ^ 1, cta_abort, ctl, limit, idx, u, AB_SBUF_FREE)) { alive = false; break; }
-        if (!wait_barrier(&s.k_full[ks], (g / 3) & 1, cta_abort, ctl, limit, idx, u, AB_K_FULL)) { alive = false; break; }
+        if (!wait_lean(&s.sbuf_free[buf], ((g >> 1) & 1) ^ 1, cta_abort, limit, AB_SBUF_FREE)) { alive = false; break; }
+        if (!wait_lean(&s.k_full[ks], (g / 3) & 1, cta_abort, limit, AB_K_FULL)) { alive = false; break; }
         tc_fence_after_sync();
         const uint64_t db = d_k0 + ks * (kTileBytes >> 4);
 #pragma unroll
@@ -235,8 +235,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       if (kt.n == 0) continue;
       for (int u = 0; u < kt.n; ++u, ++g) {
         const uint32_t ks = g % 3, buf = g & 1;
-        if (!wait_barrier(&s.w_ready[buf], (g >> 1) & 1, cta_abort, ctl, limit, idx, u, AB_W_READY)) { alive = false; break; }
-        if (u == 0 && !wait_barrier(&s.acc_free, (itn & 1) ^ 1, cta_abort, ctl, limit, idx, u, AB_ACC_FREE)) { alive = false; break; }
+        if (!wait_lean(&s.w_ready[buf], (g >> 1) & 1, cta_abort, limit, AB_W_READY)) { alive = false; break; }
+        if (u == 0 && !wait_lean(&s.acc_free, (itn & 1) ^ 1, cta_abort, limit, AB_ACC_FREE)) { alive = false; break; }
         tc_fence_after_sync();
         const uint64_t db = d_k0 + ks * (kTileBytes >> 4);
 #pragma unroll
@@ -266,12 +266,12 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       for (int u = 0; u < kt.n; ++u, ++g) {
         const int tile = kt.tile(u), j0 = tile << 7;
         const uint32_t s_tmem = lanes + kDqS + 128 * (g & 1) + wg * 64, g_tmem = lanes + kDqG + wg * 64;
-        if (!wait_barrier(&s.g_full, g & 1, cta_abort, ctl, limit, idx, u, AB_G_FULL)) { alive = false; break; }
+        if (!wait_lean(&s.g_full, g & 1, cta_abort, limit, AB_G_FULL)) { alive = false; break; }
         tc_fence_after_sync();
         uint32_t gv0[32], gv1[32];
         tmem_ld32(g_tmem, gv0);
         tmem_ld32(g_tmem + 32, gv1);
-        if (!wait_barrier(&s.s_full[g & 1], (g >> 1) & 1, cta_abort, ctl, limit, idx, u, AB_S_FULL)) { alive = false; break; }
+        if (!wait_lean(&s.s_full[g & 1], (g >> 1) & 1, cta_abort, limit, AB_S_FULL)) { alive = false; break; }
         tc_fence_after_sync();
         uint32_t sv0[32], sv1[32];
         tmem_ld32(s_tmem, sv0);
@@ -320,7 +320,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 
       const bool has = kt.n > 0;
       if (has) {
-        if (!wait_barrier(&s.acc_full, itn & 1, cta_abort, ctl, limit, idx, 0, AB_ACC_FULL)) break;
+        if (!wait_lean(&s.acc_full, itn & 1, cta_abort, limit, AB_ACC_FULL)) break;
         tc_fence_after_sync();
       }
       const bool some = has && st.x != INFINITY;
@@ -360,7 +360,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   if (s.abort_flag) {
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-    if (tid == 0) report_error(ctl, kErrAborted, -1, -1, blockIdx.x, 0);
+    if (tid == 0) report_error(ctl, kErrBarrierTimeout, -1, -1, blockIdx.x, s.abort_flag);
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -470,24 +470,24 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       DKV_ITEMS {
         DKV_GEOMETRY
         if (n == 0) continue;
-        if (!wait_barrier(&s.k_free, (itn & 1) ^ 1, cta_abort, ctl, limit, idx, 0, AB_K_EMPTY)) break;
+        if (!wait_lean(&s.k_free, (itn & 1) ^ 1, cta_abort, limit, AB_K_EMPTY)) break;
         mbar_expect_tx(&s.k_full, kTileBytes);
         tma_load_4d(s.k, &tm_k, &s.k_full, 0, it.tile * kBlock, it.hk, it.b);
         tma_load_4d(s.k + kHalfBytes, &tm_k, &s.k_full, 64, it.tile * kBlock, it.hk, it.b);
         for (int q = 0; q < n; ++q, ++g) {
           const int h = it.hk * A.G + q / nb, blk = qb.first + q % nb, st = g & 1;
-          if (!wait_barrier(&s.q_empty[st], ((g >> 1) & 1) ^ 1, cta_abort, ctl, limit, idx, q, AB_Q_FREE)) { alive = false; break; }
+          if (!wait_lean(&s.q_empty[st], ((g >> 1) & 1) ^ 1, cta_abort, limit, AB_Q_FREE)) { alive = false; break; }
           mbar_expect_tx(&s.q_full[st], kTileBytes + kBlock * 8);
           tma_load_4d(s.qring[st], &tm_q, &s.q_full[st], 0, blk * kBlock, h, it.b);
           tma_load_4d(s.qring[st] + kHalfBytes, &tm_q, &s.q_full[st], 64, blk * kBlock, h, it.b);
           bulk_load(s.stat[st], args.stat + (((long long)it.b * A.Hq + h) * A.nqb + blk) * kBlock, kBlock * 8, &s.q_full[st]);
           if (q == 0) {
-            if (!wait_barrier(&s.v_free, (itn & 1) ^ 1, cta_abort, ctl, limit, idx, 0, AB_V_EMPTY)) { alive = false; break; }
+            if (!wait_lean(&s.v_free, (itn & 1) ^ 1, cta_abort, limit, AB_V_EMPTY)) { alive = false; break; }
             mbar_expect_tx(&s.v_full, kTileBytes);
             tma_load_4d(s.v, &tm_v, &s.v_full, 0, it.tile * kBlock, it.hk, it.b);
             tma_load_4d(s.v + kHalfBytes, &tm_v, &s.v_full, 64, it.tile * kBlock, it.hk, it.b);
           }
-          if (!wait_barrier(&s.go_empty[st], ((g >> 1) & 1) ^ 1, cta_abort, ctl, limit, idx, q, AB_GO_FREE)) { alive = false; break; }
+          if (!wait_lean(&s.go_empty[st], ((g >> 1) & 1) ^ 1, cta_abort, limit, AB_GO_FREE)) { alive = false; break; }
           mbar_expect_tx(&s.go_full[st], kTileBytes);
           tma_load_4d(s.gring[st], &tm_do, &s.go_full[st], 0, blk * kBlock, h, it.b);
           tma_load_4d(s.gring[st] + kHalfBytes, &tm_do, &s.go_full[st], 64, blk * kBlock, h, it.b);
@@ -503,9 +503,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     DKV_ITEMS {
       DKV_GEOMETRY
       if (n == 0) continue;
-      if (!wait_barrier(&s.k_full, itn & 1, cta_abort, ctl, limit, idx, 0, AB_K_FULL)) break;
+      if (!wait_lean(&s.k_full, itn & 1, cta_abort, limit, AB_K_FULL)) break;
       auto issue_s = [&](uint32_t gq) -> bool {
-        if (!wait_barrier(&s.q_full[gq & 1], (gq >> 1) & 1, cta_abort, ctl, limit, idx, (int)gq, AB_Q_FULL)) return false;
+        if (!wait_lean(&s.q_full[gq & 1], (gq >> 1) & 1, cta_abort, limit, AB_Q_FULL)) return false;
         tc_fence_after_sync();
         const uint64_t db = d_q0 + (gq & 1) * (kTileBytes >> 4);
 #pragma unroll
@@ -518,9 +518,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       };
       if (!issue_s(g)) break;
       for (int q = 0; q < n; ++q, ++g) {
-        if (!wait_barrier(&s.p_ready, g & 1, cta_abort, ctl, limit, idx, q, AB_P_READY)) { alive = false; break; }
-        if (q == 0 && !wait_barrier(&s.dv_free, (itn & 1) ^ 1, cta_abort, ctl, limit, idx, q, AB_ACC_FREE)) { alive = false; break; }
-        if (!wait_barrier(&s.go_full[g & 1], (g >> 1) & 1, cta_abort, ctl, limit, idx, q, AB_GO_FULL)) { alive = false; break; }
+        if (!wait_lean(&s.p_ready, g & 1, cta_abort, limit, AB_P_READY)) { alive = false; break; }
+        if (q == 0 && !wait_lean(&s.dv_free, (itn & 1) ^ 1, cta_abort, limit, AB_ACC_FREE)) { alive = false; break; }
+        if (!wait_lean(&s.go_full[g & 1], (g >> 1) & 1, cta_abort, limit, AB_GO_FULL)) { alive = false; break; }
         tc_fence_after_sync();
         const uint64_t db = d_g0 + (g & 1) * (kTileBytes >> 4);
 #pragma unroll
@@ -544,9 +544,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     DKV_ITEMS {
       DKV_GEOMETRY
       if (n == 0) continue;
-      if (!wait_barrier(&s.v_full, itn & 1, cta_abort, ctl, limit, idx, 0, AB_V_FULL)) break;
+      if (!wait_lean(&s.v_full, itn & 1, cta_abort, limit, AB_V_FULL)) break;
       auto issue_g = [&](uint32_t gq) -> bool {
-        if (!wait_barrier(&s.go_full[gq & 1], (gq >> 1) & 1, cta_abort, ctl, limit, idx, (int)gq, AB_GO_FULL)) return false;
+        if (!wait_lean(&s.go_full[gq & 1], (gq >> 1) & 1, cta_abort, limit, AB_GO_FULL)) return false;
         tc_fence_after_sync();
         const uint64_t db = d_g0 + (gq & 1) * (kTileBytes >> 4);
 #pragma unroll
@@ -560,8 +560,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       };
       if (!issue_g(g)) break;
       for (int q = 0; q < n; ++q, ++g) {
-        if (!wait_barrier(&s.ds_ready, g & 1, cta_abort, ctl, limit, idx, q, AB_DS_READY)) { alive = false; break; }
-        if (q == 0 && !wait_barrier(&s.dk_free, (itn & 1) ^ 1, cta_abort, ctl, limit, idx, q, AB_ACC_FREE)) { alive = false; break; }
+        if (!wait_lean(&s.ds_ready, g & 1, cta_abort, limit, AB_DS_READY)) { alive = false; break; }
+        if (q == 0 && !wait_lean(&s.dk_free, (itn & 1) ^ 1, cta_abort, limit, AB_ACC_FREE)) { alive = false; break; }
         tc_fence_after_sync();
         const uint64_t db = d_q0 + (g & 1) * (kTileBytes >> 4);
 #pragma unroll
@@ -595,9 +595,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const float2* stat = s.stat[st] + wg * 64;
         const bool masked = block_masked(A, j0, p0, len);
         const ColMask mask = col_mask(A, j, p0 + wg * 64, len);
-        if (!wait_barrier(&s.s_full, g & 1, cta_abort, ctl, limit, idx, q, AB_S_FULL)) { alive = false; break; }
+        if (!wait_lean(&s.s_full, g & 1, cta_abort, limit, AB_S_FULL)) { alive = false; break; }
         // (for this thread's own reads of the statistics: the load that brought Q brought them)
-        if (!wait_barrier(&s.q_full[st], (g >> 1) & 1, cta_abort, ctl, limit, idx, q, AB_Q_FULL)) { alive = false; break; }
+        if (!wait_lean(&s.q_full[st], (g >> 1) & 1, cta_abort, limit, AB_Q_FULL)) { alive = false; break; }
         tc_fence_after_sync();
         uint32_t v0[32], v1[32];
         tmem_ld32(s_tmem, v0);
@@ -636,7 +636,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         // the products that sum over them.  S^T and G^T, which read them as columns, are complete by then.
         const bool stale = p0 + 127 >= len && len < A.Nk;
         if (stale) {
-          if (!wait_barrier(&s.dp_full, g & 1, cta_abort, ctl, limit, idx, q, AB_DP_FULL)) { alive = false; break; }
+          if (!wait_lean(&s.dp_full, g & 1, cta_abort, limit, AB_DP_FULL)) { alive = false; break; }
           if (wg == 0 && p0 + row >= len) {
             zero_tile_row(s.qring[st], row);
             zero_tile_row(s.gring[st], row);
@@ -646,7 +646,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         tc_fence_before_sync();
         mbar_arrive(&s.p_ready);
-        if (!stale && !wait_barrier(&s.dp_full, g & 1, cta_abort, ctl, limit, idx, q, AB_DP_FULL)) { alive = false; break; }
+        if (!stale && !wait_lean(&s.dp_full, g & 1, cta_abort, limit, AB_DP_FULL)) { alive = false; break; }
         tc_fence_after_sync();
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -681,7 +681,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
       for (int which = 0; which < 2; ++which) {       // 0: dV, 1: dK
         if (has) {
-          if (!wait_barrier(which ? &s.dk_full : &s.dv_full, itn & 1, cta_abort, ctl, limit, idx, which, AB_ACC_FULL)) {
+          if (!wait_lean(which ? &s.dk_full : &s.dv_full, itn & 1, cta_abort, limit, AB_ACC_FULL)) {
             alive = false;
             break;
           }
@@ -735,7 +735,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   if (s.abort_flag) {
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-    if (tid == 0) report_error(ctl, kErrAborted, -1, -1, blockIdx.x, 0);
+    if (tid == 0) report_error(ctl, kErrBarrierTimeout, -1, -1, blockIdx.x, s.abort_flag);
   }
   tc_fence_before_sync();
   __syncthreads();

@@ -98,7 +98,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         for (int idx = blockIdx.x; alive && fwd_item(A, idx, it); idx += gridDim.x) {
           const PairTiles pt = pair_tiles(A, it, length_of(it.b));
           auto load = [&](const CUtensorMap* tm, int tile) -> bool {
-            if (!wait_barrier_soon(&s.empty[stage], phase ^ 1, cta_abort, ctl, limit, idx, (int)r, AF_EMPTY)) return false;
+            if (!wait_lean(&s.empty[stage], phase ^ 1, cta_abort, limit, AF_EMPTY)) return false;
             mbar_expect_tx(&s.full[stage], kTileBytes);
             tma_load_4d(s.ring[stage], tm, &s.full[stage], 0, tile * kBlock, it.hk, it.b);
             tma_load_4d(s.ring[stage] + kHalfBytes, tm, &s.full[stage], 64, tile * kBlock, it.hk, it.b);
@@ -111,7 +111,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           };
           for (int t = 0; t < 2 && alive; ++t) {
             if (pt.list(t).n == 0) continue;
-            if (!wait_barrier_soon(&s.q_free[t], (nq[t] & 1) ^ 1, cta_abort, ctl, limit, idx, t, AF_Q_FREE)) {
+            if (!wait_lean(&s.q_free[t], (nq[t] & 1) ^ 1, cta_abort, limit, AF_Q_FREE)) {
               alive = false;
               break;
             }
@@ -148,44 +148,49 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         // O_t (+)= P_t(u-1) V(u-1)
         auto issue_pv = [&](int t, uint32_t& np, uint32_t nq, bool& first, bool narrow) -> bool {
           const uint32_t s_tmem = tmem + kFwS + 128 * t, o_tmem = tmem + kFwO + 128 * t;
-          if (!wait_barrier_soon(&s.p_half[t], np & 1, cta_abort, ctl, limit, idx, t, AF_P_HALF)) return false;
+          if (!wait_lean(&s.p_half[t], np & 1, cta_abort, limit, AF_P_HALF)) return false;
           // the epilogue of this tile's previous item has read O
-          if (first && !wait_barrier_soon(&s.o_free[t], (nq & 1) ^ 1, cta_abort, ctl, limit, idx, t, AF_O_FREE)) return false;
+          if (first && !wait_lean(&s.o_free[t], (nq & 1) ^ 1, cta_abort, limit, AF_O_FREE)) return false;
           tc_fence_after_sync();
           const uint64_t dv = d_v0 + v_st * (kTileBytes >> 4);
+          const uint32_t add = first ? 0u : 1u;
+          if (narrow) {
+            if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (k < kNarrow / 16 || !narrow)
-              umma_ts_w(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, (!first || k) ? 1u : 0u);
-          if (!wait_barrier_soon(&s.p_ready[t], np & 1, cta_abort, ctl, limit, idx, t, AF_P_READY)) return false;
+              for (int k = 0; k < kNarrow / 16; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
+            }
+          } else {
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
+            }
+          }
+          if (!wait_lean(&s.p_ready[t], np & 1, cta_abort, limit, AF_P_READY)) return false;
           ++np;
           if (!narrow) {
             tc_fence_after_sync();
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 4; k < 8; ++k) umma_ts_w(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, 1u);
+              for (int k = 4; k < 8; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, 1u);
+            }
           }
           first = false;
           return true;
         };
         auto issue_s = [&](int t, uint32_t& nq, int& left, int own, bool narrow) -> bool {
-          if (left == own && !wait_barrier_soon(&s.q_full[t], nq & 1, cta_abort, ctl, limit, idx, t, AF_Q_FULL)) return false;
+          if (left == own && !wait_lean(&s.q_full[t], nq & 1, cta_abort, limit, AF_Q_FULL)) return false;
           tc_fence_after_sync();
           const uint64_t dq = d_q0 + t * (kTileBytes >> 4), dk = d_k0 + st * (kTileBytes >> 4);
           const uint32_t s_tmem = tmem + kFwS + 128 * t;
-          if (narrow) {
+          const uint32_t idesc = narrow ? idesc_sn : idesc_s;
+          if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-              umma_ss_w(s_tmem, dq + off, dk + off, idesc_sn, k ? 1u : 0u);
+              umma_ss(s_tmem, dq + off, dk + off, idesc, k ? 1u : 0u);
             }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-              umma_ss_w(s_tmem, dq + off, dk + off, idesc_s, k ? 1u : 0u);
-            }
+            umma_commit(&s.s_full[t]);
           }
-          umma_commit_w(&s.s_full[t]);
           if (--left == 0) umma_commit_w(&s.q_free[t]);
           return true;
         };
@@ -194,10 +199,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const bool act0 = u < pt.n && pt.active(pt.x, u), act1 = u < pt.n && pt.active(pt.y, u);
           const bool narrow0 = u < pt.n && tile_narrow(A, pt.x, pt.tile(u)), narrow1 = u < pt.n && tile_narrow(A, pt.y, pt.tile(u));
           if (u > 0) {
-            if (!wait_barrier_soon(&s.full[v_st], v_phase, cta_abort, ctl, limit, idx, u, AF_FULL)) { alive = false; break; }
+            if (!wait_lean(&s.full[v_st], v_phase, cta_abort, limit, AF_FULL)) { alive = false; break; }
           }
           if (pend0 && !issue_pv(0, np0, nq0, first0, was_narrow0)) { alive = false; break; }
-          if (u < pt.n && !wait_barrier_soon(&s.full[st], phase, cta_abort, ctl, limit, idx, u, AF_FULL)) { alive = false; break; }
+          if (u < pt.n && !wait_lean(&s.full[st], phase, cta_abort, limit, AF_FULL)) { alive = false; break; }
           if (act0 && !issue_s(0, nq0, left0, pt.x.n, narrow0)) { alive = false; break; }
           if (pend1 && !issue_pv(1, np1, nq1, first1, was_narrow1)) { alive = false; break; }
           if (u > 0) umma_commit_w(&s.empty[v_st]);
@@ -258,7 +263,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       for (int u = 0; u < pt.n; ++u) {
         if (!pt.active(kt, u)) continue;
         const int tile = pt.tile(u), j0 = tile << 7;
-        if (!wait_barrier_soon(&s.s_full[t], ns & 1, cta_abort, ctl, limit, idx, u, AF_S_FULL)) { alive = false; break; }
+        if (!wait_lean(&s.s_full[t], ns & 1, cta_abort, limit, AF_S_FULL)) { alive = false; break; }
         ++ns;
         tc_fence_after_sync();
         const bool masked = tile_masked(A, kt, tile, len);
@@ -267,7 +272,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (j0 + 127 >= len && len < A.Nk) {
             // rows behind the sequence hold anything, and 0 * NaN is not 0: the value tile's become zero
             const uint32_t use = r + 2 * u + 1;
-            if (!wait_barrier_soon(&s.full[use % kFwRing], (use / kFwRing) & 1, cta_abort, ctl, limit, idx, (int)use, AF_FULL)) {
+            if (!wait_lean(&s.full[use % kFwRing], (use / kFwRing) & 1, cta_abort, limit, AF_FULL)) {
               alive = false;
               break;
             }
@@ -352,7 +357,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // ---- epilogue ----
       const bool has = kt.n > 0;
       if (has) {
-        if (!wait_barrier_soon(&s.o_full[t], no & 1, cta_abort, ctl, limit, idx, t, AF_O_FULL)) break;
+        if (!wait_lean(&s.o_full[t], no & 1, cta_abort, limit, AF_O_FULL)) break;
         ++no;
         tc_fence_after_sync();
       }
@@ -406,7 +411,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     // a role gave up: leave the copies and products in flight time to land before the CTA's memory goes
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-    if (tid == 0) report_error(ctl, kErrAborted, -1, -1, blockIdx.x, 0);
+    if (tid == 0) report_error(ctl, kErrBarrierTimeout, -1, -1, blockIdx.x, s.abort_flag);
   }
   tc_fence_before_sync();
   __syncthreads();

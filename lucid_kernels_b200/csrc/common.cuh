@@ -88,13 +88,25 @@ __device__ __forceinline__ bool wait_barrier(uint64_t* bar, uint32_t parity, vol
   return true;
 }
 
-// The same wait for barriers that usually complete within a microsecond: a few more polls before the clock is looked at for
-// the first time (reading the global timer costs a waiter some hundred cycles).  Same limit, same report.
-__device__ __forceinline__ bool wait_barrier_soon(uint64_t* bar, uint32_t parity, volatile int* cta_abort, Control* ctl,
-                                                  unsigned long long limit_ns, int chain, int row, int bar_id) {
-  for (int i = limit_ns ? 32 : 1; i > 0; --i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return wait_barrier(bar, parity, cta_abort, ctl, limit_ns, chain, row, bar_id);
+// The same wait in little code, for kernels whose roles wait in many places: a few polls before the clock is looked at for
+// the first time (reading the global timer costs a waiter some hundred cycles), and only the barrier's id is left behind
+// (through the CTA-wide abort word; the kernel reports it when it ends).
+__device__ __forceinline__ bool wait_lean(uint64_t* bar, uint32_t parity, volatile int* cta_abort,
+                                          unsigned long long limit_ns, int bar_id) {
+  if (mbar_try_wait(bar, parity)) return true;
+  unsigned long long t0 = 0;
+  uint32_t spins = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    if ((++spins & 63u) != 0 && limit_ns != 0) continue;
+    if (*cta_abort) return false;
+    const unsigned long long t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    if (t - t0 >= limit_ns) {
+      *cta_abort = bar_id;
+      return false;
+    }
+  }
+  return true;
 }
 
 // A row-block is complete when its flag reaches kFlagComplete: set at once by the thread that stored the
