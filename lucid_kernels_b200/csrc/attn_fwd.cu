@@ -11,9 +11,10 @@
 // columns of TMEM; the 16-bit weights P overwrite it) and O (128 columns): 512 columns in all.  While the tensor pipe
 // runs one tile's P V and next S, the other tile's warps form exponentials.
 //
-// Warp roles (384 threads): warp 0 producer, warp 1 issues all products in the order P V and next S of tile 0, the same of
-// tile 1, ... (one thread's products run in order, so the two tiles' scores become ready half a period apart and their
-// exponentials do not compete; with an issuer per tile the products interleaved and both groups ran in phase), warp 3
+// Warp roles (384 threads): warp 0 producer; warps 1 and 2 issue the products of one tile each, P V and the next S, taking
+// turns: the two tiles' scores become ready half a period apart and their exponentials do not compete (issuers that do not
+// take turns interleave their products, and both groups run in phase), while one issuer's waits and the queue's drain are
+// covered by the other's products (one warp for both tiles took 2320 cycles per tile, 1460 of them for 16 products); warp 3
 // owns TMEM; warps 4-7 and 8-11 are the softmax groups of the two tiles, one row per thread.  P is handed over in two
 // halves, so that P V starts while the second half's exponentials are formed.  Persistent CTAs, items dealt out round
 // robin, the longest first; results leave through a staging panel per tile and TMA (a thread's own row stores touch 32 lines
@@ -31,12 +32,12 @@ struct AttnFwdSmem {
   alignas(1024) uint8_t ring[kFwRing][kTileBytes];   // K(0), V(0), K(1), V(1), ... of the union of the two tiles' lists
   alignas(1024) uint8_t stage[2][kHalfBytes];         // 128 rows x 64 columns of a tile's result
   alignas(8) uint64_t full[kFwRing];
-  uint64_t empty[kFwRing], q_full[2], q_free[2], s_full[2], p_half[2], p_ready[2], o_full[2], o_free[2];
+  uint64_t empty[kFwRing], q_full[2], q_free[2], s_full[2], p_half[2], p_ready[2], turn[2], o_full[2], o_free[2];
   uint32_t tmem_base;
   int abort_flag;
 };
 
-enum AttnFwdBar : int { AF_FULL = 401, AF_EMPTY, AF_Q_FULL, AF_Q_FREE, AF_S_FULL, AF_P_HALF, AF_P_READY, AF_O_FULL, AF_O_FREE };
+enum AttnFwdBar : int { AF_FULL = 401, AF_EMPTY, AF_Q_FULL, AF_Q_FREE, AF_S_FULL, AF_P_HALF, AF_P_READY, AF_TURN, AF_O_FULL, AF_O_FREE };
 
 constexpr int kFwThreads = 384;
 constexpr int kFwS = 0, kFwO = 256;      // + 128 * tile
@@ -59,12 +60,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   if (tid == 0) {
     for (int i = 0; i < kFwRing; ++i) {
       mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], 1);
+      mbar_init(&s.empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.q_full[i], 1);
       mbar_init(&s.q_free[i], 1);
       mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.turn[i], 1);
       mbar_init(&s.p_half[i], 128);
       mbar_init(&s.p_ready[i], 128);
       mbar_init(&s.o_full[i], 1);
@@ -126,93 +128,93 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         }
       }
-    } else if (warp == 1) {
-      // =========================== issuer of all products ===========================
+    } else if (warp < 3) {
+      // =========================== issuer of one tile's products ===========================
+      // Step u of the union: P V of the tile's previous entry and S of entry u, in turns with the other tile's issuer
+      const int t = warp - 1;
       constexpr int fmt = kBf16 ? 1 : 0;
       constexpr uint32_t idesc_s = umma_idesc(fmt, 0, 0, 128, 128);          // Q K^T: both K-major
       constexpr uint32_t idesc_sn = umma_idesc(fmt, 0, 0, 128, kNarrow);     // the first kNarrow keys only
       constexpr uint32_t idesc_o = umma_idesc(fmt, 0, 1, 128, 128);          // P V: P from TMEM, V rows = k
-      const uint64_t d_q0 = umma_smem_desc(smem_u32(s.q[0]), 16, 1024);
+      const uint64_t dq = umma_smem_desc(smem_u32(s.q[t]), 16, 1024);
       const uint64_t d_k0 = umma_smem_desc(smem_u32(s.ring[0]), 16, 1024);
       const uint64_t d_v0 = umma_smem_desc(smem_u32(s.ring[0]), kHalfBytes, 1024);
-      uint32_t st = 0, phase = 0;        // ring stage and phase of K(u); V(u) is the one behind it
-      uint32_t nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;   // items with tiles; weights consumed
+      const uint32_t s_tmem = tmem + kFwS + 128 * t, o_tmem = tmem + kFwO + 128 * t;
+      uint32_t st = 0, phase = 0;        // ring stage and phase of K(u); V(u) is in the stage behind it
+      uint32_t v_st = 0, v_phase = 0;    // V(u - 1)
+      uint32_t nq = 0, np = 0, turns = 0;  // items with tiles; weights consumed; turns taken
       bool alive = true;
       FwdItem it;
       for (int idx = blockIdx.x; alive && fwd_item(A, idx, it); idx += gridDim.x) {
         const PairTiles pt = pair_tiles(A, it, length_of(it.b));
-        bool first0 = true, first1 = true;
-        int left0 = pt.x.n, left1 = pt.y.n;
-        bool pend0 = false, pend1 = false;      // weights of tile u - 1 on their way
-        uint32_t v_st = 0, v_phase = 0;         // V(u - 1)
-        // O_t (+)= P_t(u-1) V(u-1)
-        auto issue_pv = [&](int t, uint32_t& np, uint32_t nq, bool& first, bool narrow) -> bool {
-          const uint32_t s_tmem = tmem + kFwS + 128 * t, o_tmem = tmem + kFwO + 128 * t;
-          if (!wait_lean(&s.p_half[t], np & 1, cta_abort, limit, AF_P_HALF)) return false;
-          // the epilogue of this tile's previous item has read O
-          if (first && !wait_lean(&s.o_free[t], (nq & 1) ^ 1, cta_abort, limit, AF_O_FREE)) return false;
-          tc_fence_after_sync();
-          const uint64_t dv = d_v0 + v_st * (kTileBytes >> 4);
-          const uint32_t add = first ? 0u : 1u;
-          if (narrow) {
-            if (elect_one()) {
-#pragma unroll
-              for (int k = 0; k < kNarrow / 16; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
-            }
-          } else {
-            if (elect_one()) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
-            }
-          }
-          if (!wait_lean(&s.p_ready[t], np & 1, cta_abort, limit, AF_P_READY)) return false;
-          ++np;
-          if (!narrow) {
-            tc_fence_after_sync();
-            if (elect_one()) {
-#pragma unroll
-              for (int k = 4; k < 8; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, 1u);
-            }
-          }
-          first = false;
-          return true;
-        };
-        auto issue_s = [&](int t, uint32_t& nq, int& left, int own, bool narrow) -> bool {
-          if (left == own && !wait_lean(&s.q_full[t], nq & 1, cta_abort, limit, AF_Q_FULL)) return false;
-          tc_fence_after_sync();
-          const uint64_t dq = d_q0 + t * (kTileBytes >> 4), dk = d_k0 + st * (kTileBytes >> 4);
-          const uint32_t s_tmem = tmem + kFwS + 128 * t;
-          const uint32_t idesc = narrow ? idesc_sn : idesc_s;
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-              umma_ss(s_tmem, dq + off, dk + off, idesc, k ? 1u : 0u);
-            }
-            umma_commit(&s.s_full[t]);
-          }
-          if (--left == 0) umma_commit_w(&s.q_free[t]);
-          return true;
-        };
-        bool was_narrow0 = false, was_narrow1 = false;
+        const KeyTiles kt = pt.list(t);
+        bool first = true, pend = false, was_narrow = false;    // pend: the weights of entry u - 1 are this tile's
+        int left = kt.n;
         for (int u = 0; u <= pt.n; ++u) {
-          const bool act0 = u < pt.n && pt.active(pt.x, u), act1 = u < pt.n && pt.active(pt.y, u);
-          const bool narrow0 = u < pt.n && tile_narrow(A, pt.x, pt.tile(u)), narrow1 = u < pt.n && tile_narrow(A, pt.y, pt.tile(u));
-          if (u > 0) {
-            if (!wait_lean(&s.full[v_st], v_phase, cta_abort, limit, AF_FULL)) { alive = false; break; }
+          const bool more = u < pt.n, act = more && pt.active(kt, u), narrow = more && tile_narrow(A, kt, pt.tile(u));
+          if (u > 0 && !wait_lean(&s.full[v_st], v_phase, cta_abort, limit, AF_FULL)) { alive = false; break; }
+          if (more && !wait_lean(&s.full[st], phase, cta_abort, limit, AF_FULL)) { alive = false; break; }
+          if (act && left == kt.n && !wait_lean(&s.q_full[t], nq & 1, cta_abort, limit, AF_Q_FULL)) { alive = false; break; }
+          if (pend) {
+            if (!wait_lean(&s.p_half[t], np & 1, cta_abort, limit, AF_P_HALF)) { alive = false; break; }
+            // the epilogue of this tile's previous item has read O
+            if (first && !wait_lean(&s.o_free[t], (nq & 1) ^ 1, cta_abort, limit, AF_O_FREE)) { alive = false; break; }
           }
-          if (pend0 && !issue_pv(0, np0, nq0, first0, was_narrow0)) { alive = false; break; }
-          if (u < pt.n && !wait_lean(&s.full[st], phase, cta_abort, limit, AF_FULL)) { alive = false; break; }
-          if (act0 && !issue_s(0, nq0, left0, pt.x.n, narrow0)) { alive = false; break; }
-          if (pend1 && !issue_pv(1, np1, nq1, first1, was_narrow1)) { alive = false; break; }
-          if (u > 0) umma_commit_w(&s.empty[v_st]);
-          if (act1 && !issue_s(1, nq1, left1, pt.y.n, narrow1)) { alive = false; break; }
-          if (u < pt.n) umma_commit_w(&s.empty[st]);
-          pend0 = act0;
-          pend1 = act1;
-          was_narrow0 = narrow0;
-          was_narrow1 = narrow1;
-          if (u < pt.n) {
+          const uint64_t dv = d_v0 + v_st * (kTileBytes >> 4), dk = d_k0 + st * (kTileBytes >> 4);
+          if (!wait_lean(&s.turn[t], (turns & 1) ^ (t ^ 1), cta_abort, limit, AF_TURN)) { alive = false; break; }
+          ++turns;
+          tc_fence_after_sync();
+          if (pend) {
+            const uint32_t add = first ? 0u : 1u;
+            if (was_narrow) {
+              if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < kNarrow / 16; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
+              }
+            } else {
+              if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
+              }
+            }
+            if (!wait_lean(&s.p_ready[t], np & 1, cta_abort, limit, AF_P_READY)) { alive = false; break; }
+            ++np;
+            if (!was_narrow) {
+              tc_fence_after_sync();
+              if (elect_one()) {
+#pragma unroll
+                for (int k = 4; k < 8; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, 1u);
+              }
+            }
+            first = false;
+          }
+          if (act) {
+            const uint32_t idesc = narrow ? idesc_sn : idesc_s;
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
+                umma_ss(s_tmem, dq + off, dk + off, idesc, k ? 1u : 0u);
+              }
+            }
+            --left;
+          }
+          __syncwarp();
+          if (elect_one()) {
+            mbar_arrive(&s.turn[t ^ 1]);
+            if (act) umma_commit(&s.s_full[t]);
+            // the stages go back when both issuers' products that read them are complete (an issuer without products
+            // on them only says that it is past them)
+            if (u > 0) umma_commit(&s.empty[v_st]);
+            if (more) umma_commit(&s.empty[st]);
+            if (act && left == 0) umma_commit(&s.q_free[t]);
+            // the tile's last weights have been consumed: its result is complete
+            if (pend && !act && left == 0) umma_commit(&s.o_full[t]);
+          }
+          if (pend && !act && left == 0) ++nq;
+          pend = act;
+          was_narrow = narrow;
+          if (more) {
             v_st = st + 1;
             v_phase = phase;
             if (v_st == kFwRing) {
@@ -225,17 +227,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               st = 0;
               phase ^= 1;
             }
-          }
-          // a tile's last weights have been consumed: its result is complete
-          if (u > 0 && pt.x.n > 0 && left0 == 0 && !pend0) {
-            umma_commit_w(&s.o_full[0]);
-            ++nq0;
-            left0 = -1;
-          }
-          if (u > 0 && pt.y.n > 0 && left1 == 0 && !pend1) {
-            umma_commit_w(&s.o_full[1]);
-            ++nq1;
-            left1 = -1;
           }
         }
       }
