@@ -142,7 +142,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   uint32_t g = 0, itn = 0;                                                             \
   bool alive = true;                                                                   \
   DqItem it;                                                                           \
-  for (int idx = blockIdx.x; alive && dq_item(A, idx, it); idx += gridDim.x)
+  for (int rnd = 0, idx; alive && dq_item(A, idx = snake_item(rnd, blockIdx.x, gridDim.x), it); ++rnd)
 
   if (warp == 0) {
     if (lane == 0) {
@@ -455,7 +455,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint32_t g = 0, itn = 0;                                                                       \
   bool alive = true;                                                                             \
   KvItem it;                                                                                     \
-  for (int idx = blockIdx.x; alive && kv_item(A, args.chunks, idx, it); idx += gridDim.x)
+  for (int rnd = 0, idx; alive && kv_item(A, args.chunks, idx = snake_item(rnd, blockIdx.x, gridDim.x), it); ++rnd)
 #define DKV_GEOMETRY                                                                             \
   const int len = attn_length(A, args.lengths, it.b);                                            \
   const QueryBlocks qb = item_blocks(A, it, len);                                                \

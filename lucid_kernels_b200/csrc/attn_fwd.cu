@@ -32,12 +32,12 @@ struct AttnFwdSmem {
   alignas(1024) uint8_t ring[kFwRing][kTileBytes];   // K(0), V(0), K(1), V(1), ... of the union of the two tiles' lists
   alignas(1024) uint8_t stage[2][kHalfBytes];         // 128 rows x 64 columns of a tile's result
   alignas(8) uint64_t full[kFwRing];
-  uint64_t empty[kFwRing], q_full[2], q_free[2], s_full[2], p_half[2], p_ready[2], turn[2], o_full[2], o_free[2];
+  uint64_t empty[kFwRing], q_full[2], q_free[2], s_full[2], p_half[2], p_ready[2], turn[2], meet[2], o_full[2], o_free[2];
   uint32_t tmem_base;
   int abort_flag;
 };
 
-enum AttnFwdBar : int { AF_FULL = 401, AF_EMPTY, AF_Q_FULL, AF_Q_FREE, AF_S_FULL, AF_P_HALF, AF_P_READY, AF_TURN, AF_O_FULL, AF_O_FREE };
+enum AttnFwdBar : int { AF_FULL = 401, AF_EMPTY, AF_Q_FULL, AF_Q_FREE, AF_S_FULL, AF_P_HALF, AF_P_READY, AF_TURN, AF_MEET, AF_O_FULL, AF_O_FREE };
 
 constexpr int kFwThreads = 384;
 constexpr int kFwS = 0, kFwO = 256;      // + 128 * tile
@@ -67,6 +67,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_init(&s.q_free[i], 1);
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.turn[i], 1);
+      mbar_init(&s.meet[i], 128);
       mbar_init(&s.p_half[i], 128);
       mbar_init(&s.p_ready[i], 128);
       mbar_init(&s.o_full[i], 1);
@@ -97,7 +98,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         uint32_t nq[2] = {0, 0};      // Q tiles loaded
         bool alive = true;
         FwdItem it;
-        for (int idx = blockIdx.x; alive && fwd_item(A, idx, it); idx += gridDim.x) {
+        for (int rnd = 0, idx; alive && fwd_item(A, idx = snake_item(rnd, blockIdx.x, gridDim.x), it); ++rnd) {
           const PairTiles pt = pair_tiles(A, it, length_of(it.b));
           auto load = [&](const CUtensorMap* tm, int tile) -> bool {
             if (!wait_lean(&s.empty[stage], phase ^ 1, cta_abort, limit, AF_EMPTY)) return false;
@@ -145,7 +146,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       uint32_t nq = 0, np = 0, turns = 0;  // items with tiles; weights consumed; turns taken
       bool alive = true;
       FwdItem it;
-      for (int idx = blockIdx.x; alive && fwd_item(A, idx, it); idx += gridDim.x) {
+      for (int rnd = 0, idx; alive && fwd_item(A, idx = snake_item(rnd, blockIdx.x, gridDim.x), it); ++rnd) {
         const PairTiles pt = pair_tiles(A, it, length_of(it.b));
         const KeyTiles kt = pt.list(t);
         bool first = true, pend = false, was_narrow = false;    // pend: the weights of entry u - 1 are this tile's
@@ -239,10 +240,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + kFwS + 128 * t, o_tmem = tmem + lanes + kFwO + 128 * t;
     const float sl2 = args.scale_log2;
-    uint32_t ns = 0, no = 0, r = 0;
+    const unsigned long long sl22 = f32x2(sl2, sl2);
+    uint32_t ns = 0, no = 0, r = 0, meets = 0;
+    // the tile's 128 threads meet (an mbarrier and not a named barrier: this wait, too, has a limit)
+    auto meet = [&]() -> bool {
+      mbar_arrive(&s.meet[t]);
+      return wait_lean(&s.meet[t], meets++ & 1, cta_abort, limit, AF_MEET);
+    };
     bool alive = true;
     FwdItem it;
-    for (int idx = blockIdx.x; alive && fwd_item(A, idx, it); idx += gridDim.x) {
+    for (int rnd = 0, idx; alive && fwd_item(A, idx = snake_item(rnd, blockIdx.x, gridDim.x), it); ++rnd) {
       const int len = length_of(it.b);
       const PairTiles pt = pair_tiles(A, it, len);
       const KeyTiles kt = pt.list(t);
@@ -250,19 +257,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const int p = i + A.off;
       const bool valid = i < A.Nq && p < len;
       float ref = -INFINITY, l = 0.f;
-      bool first = true;
-      for (int u = 0; u < pt.n; ++u) {
-        if (!pt.active(kt, u)) continue;
-        const int tile = pt.tile(u), j0 = tile << 7;
+      for (int x = 0; x < kt.n; ++x, ++ns) {
+        const int tile = kt.tile(x), j0 = tile << 7;
         if (!wait_lean(&s.s_full[t], ns & 1, cta_abort, limit, AF_S_FULL)) { alive = false; break; }
-        ++ns;
         tc_fence_after_sync();
         const bool masked = tile_masked(A, kt, tile, len);
         const RowMask mask = row_mask(A, p, j0, len);
         if (masked) {
           if (j0 + 127 >= len && len < A.Nk) {
             // rows behind the sequence hold anything, and 0 * NaN is not 0: the value tile's become zero
-            const uint32_t use = r + 2 * u + 1;
+            const uint32_t use = r + 2 * (tile == 0 && pt.sink ? 0 : tile - pt.lo + pt.sink) + 1;
             if (!wait_lean(&s.full[use % kFwRing], (use / kFwRing) & 1, cta_abort, limit, AF_FULL)) {
               alive = false;
               break;
@@ -294,7 +298,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           for (int x = 4; x < 32 * kChunks; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x >> 5][x & 31]));
           const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
           const bool grow = m > ref + kFwSlack;
-          if (first) {
+          if (x == 0) {
             ref = m;
           } else if (__any_sync(0xffffffffu, grow)) {
             // S(u) is complete, and with it every product issued before it: O holds all earlier tiles
@@ -312,19 +316,23 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               tmem_st16(o_tmem + 16 * c, o);
             }
           }
-          first = false;
+          // (a part of the exponentials as a polynomial on the FMA pipe, one pair in 2, 3 or 4, took 2 to 12 % longer in all)
           const float neg = ref == -INFINITY ? 0.f : -ref;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const unsigned long long neg2 = f32x2(neg, neg);
+          unsigned long long sum = 0, sum2 = 0;          // two zeros each
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float a = ex2_approx(fmaf(__uint_as_float(v[c][2 * e]), sl2, neg));
-              const float b = ex2_approx(fmaf(__uint_as_float(v[c][2 * e + 1]), sl2, neg));
-              sum[(2 * e) & 3] += a;
-              sum[(2 * e + 1) & 3] += b;
-              pk[e] = pack2<kBf16>(a, b);
+              const unsigned long long y =
+                  f32x2_fma(f32x2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), sl22, neg2);
+              float2 w = f32x2_unpack(y);
+              w.x = ex2_approx(w.x);
+              w.y = ex2_approx(w.y);
+              if (e & 1) sum2 = f32x2_add(sum2, f32x2(w.x, w.y));
+              else sum = f32x2_add(sum, f32x2(w.x, w.y));
+              pk[e] = pack2<kBf16>(w.x, w.y);
             }
             tmem_st16(s_tmem + 16 * c, pk);
             if (c == 1 && kChunks > 2) {
@@ -337,7 +345,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           tc_fence_before_sync();
           if (kChunks <= 2) mbar_arrive(&s.p_half[t]);
           mbar_arrive(&s.p_ready[t]);
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          const float2 both = f32x2_unpack(f32x2_add(sum, sum2));
+          l += both.x + both.y;
         };
         if (tile_narrow(A, kt, tile)) weights(std::integral_constant<int, kNarrow / 32>{});
         else weights(std::integral_constant<int, 4>{});
@@ -359,7 +368,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           if (lead) tma_store_wait_read();               // the panel's previous store has read it
-          named_bar_sync(1 + t, 128);
+          if (!meet()) { alive = false; break; }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t o[32];
@@ -380,7 +389,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             }
           }
           fence_proxy_async_smem();
-          named_bar_sync(1 + t, 128);
+          if (!meet()) { alive = false; break; }
           if (lead) {                                    // rows behind Nq lie outside the map and are not written
             tma_store_4d(&tm_out, s.stage[t], 64 * hf, it.block(t) * kBlock, it.h(t), it.b);
             tma_store_commit();

@@ -98,6 +98,9 @@ LUCID_HD bool pair_heads(const AttnShape& a) { return (a.G & 1) == 0; }
 LUCID_HD int fwd_items(const AttnShape& a) {
   return pair_heads(a) ? a.B * (a.Hq / 2) * a.nqb : a.B * a.Hq * ((a.nqb + 1) / 2);
 }
+// The item that CTA `cta` of `grid` takes in its round `r`: back and forth, so that the CTAs that got the longest items of
+// one round get the shortest of the next (the items are sorted by length).
+LUCID_HD int snake_item(int r, int cta, int grid) { return r * grid + ((r & 1) ? grid - 1 - cta : cta); }
 struct FwdItem {
   int b, hk;
   int h0, h1, block0, block1;    // block >= nqb: no such tile

@@ -9,6 +9,18 @@ namespace lucid {
 // time limit of every device-side wait (lucid_set_wait_limit_ns)
 unsigned long long wait_limit_ns();
 
+// The driver's tensor-map call needs a current context, and a thread that has made no runtime call that needs one (an
+// autograd worker, say) has none: make the current device's primary context current, once per thread and device.
+inline cudaError_t ensure_context() {
+  static thread_local int ready = -1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || ready == dev) return e;
+  if ((e = cudaSetDevice(dev)) != cudaSuccess || (e = cudaFree(nullptr)) != cudaSuccess) return e;
+  ready = dev;
+  return cudaSuccess;
+}
+
 inline int sm_count() {
   static int cached[64] = {0};
   int dev = 0;
@@ -39,6 +51,7 @@ inline int check_tensor(const void* p, const int64_t st[3], int B, int N, int H)
 // (B, N, H, 128) tensor -> 4-D map {d, n, h, b}
 inline int bshd_map(CUtensorMap* m, bool bf16, const void* p, const int64_t st[3], int B, int N, int H,
                     uint32_t box_rows) {
+  if (cudaError_t e = ensure_context()) return (int)e;
   uint64_t dims[4] = {(uint64_t)kBlock, (uint64_t)N, (uint64_t)H, (uint64_t)B};
   // size-1 dimensions may carry any stride; give them a harmless valid one.  (Zero strides of longer
   // dimensions never get here: check_tensor refuses them.)

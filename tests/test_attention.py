@@ -387,6 +387,30 @@ def test_runs_are_identical_and_graphs_replay():
 
 
 @gpu
+def test_calls_from_a_thread_that_has_made_no_cuda_call():
+    """A tensor map can only be made with a current context; a new thread has none until some runtime call gives it one."""
+    import threading
+
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+    from lucid_kernels_b200.cute import _forward_sub_bwd, _forward_sub_fwd
+
+    q, k, v, do = make(1, 256, 256, 2, 2, torch.bfloat16)
+    calls = [lambda: _window_attention_fwd(q, k, v, 64, 2),
+             lambda: _window_attention_bwd(q, k, v, out, lse, do, 64, 2),
+             lambda: (_forward_sub_fwd(k * 0.3, v),),
+             lambda: _forward_sub_bwd(k * 0.3, v, do)]
+    out, lse = calls[0]()
+    for call in calls:
+        want, got = call(), []
+        torch.cuda.synchronize()
+        th = threading.Thread(target=lambda: got.append(call()))
+        th.start()
+        th.join()
+        torch.cuda.synchronize()
+        assert got and all(torch.equal(x, y) for x, y in zip(want, got[0]))
+
+
+@gpu
 def test_partial_gradients_and_empty_tensors():
     from lucid_kernels_b200 import window_attention
 
