@@ -15,6 +15,8 @@ enum : int { kErrBadPage = 4 };
 struct AttnFwdArgs {
   AttnShape a;
   const int* lengths;     // (B) valid positions, or null
+  void* out;              // (B, Nq, Hq, 128)
+  Strides out_strides;
   float* lse;             // or null; (B, Hq, Nq) natural log of the row's sum of exponentials, -inf for an empty row
   float scale_log2;       // scale * log2(e)
   unsigned long long wait_ns;
@@ -44,7 +46,7 @@ struct AttnStatArgs {
 };
 
 cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
-                            const CUtensorMap& tm_out, const AttnFwdArgs& args, int sms, cudaStream_t stream);
+                            const AttnFwdArgs& args, int sms, cudaStream_t stream);
 cudaError_t launch_attn_stat(bool bf16, const AttnStatArgs& args, cudaStream_t stream);
 cudaError_t launch_attn_dq(bool bf16, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                            const CUtensorMap& tm_do, const AttnBwdArgs& args, int sms, cudaStream_t stream);

@@ -121,16 +121,17 @@ int lucid_window_attn_fwd(const lucid_window_attn_desc* d, const void* q, const 
   const int sms = sm_count();
   if (sms <= 0) return LUCID_E_NO_DEVICE;
   const bool bf16 = d->dtype == LUCID_DTYPE_BF16;
-  CUtensorMap tm_q, tm_k, tm_v, tm_out;
+  CUtensorMap tm_q, tm_k, tm_v;
   if ((rc = bshd_map(&tm_q, bf16, q, d->q_strides, B, Nq, Hq, 128)) || (rc = bshd_map(&tm_k, bf16, k, d->k_strides, B, Nk, Hkv, 128)) ||
-      (rc = bshd_map(&tm_v, bf16, v, d->v_strides, B, Nk, Hkv, 128)) ||
-      (rc = bshd_map(&tm_out, bf16, out, d->out_strides, B, Nq, Hq, 128)))
+      (rc = bshd_map(&tm_v, bf16, v, d->v_strides, B, Nk, Hkv, 128)))
     return rc;
   args.lengths = lengths;
+  args.out = out;
+  args.out_strides = Strides{d->out_strides[0], d->out_strides[1], d->out_strides[2]};
   args.lse = lse;
   args.scale_log2 = d->scale * kLog2e;
   args.wait_ns = wait_limit_ns();
-  return (int)launch_attn_fwd(bf16, tm_q, tm_k, tm_v, tm_out, args, sms, static_cast<cudaStream_t>(cuda_stream));
+  return (int)launch_attn_fwd(bf16, tm_q, tm_k, tm_v, args, sms, static_cast<cudaStream_t>(cuda_stream));
 }
 
 size_t lucid_window_attn_bwd_workspace_bytes(const lucid_window_attn_desc* d) {

@@ -11,14 +11,14 @@
 // columns of TMEM; the 16-bit weights P overwrite it) and O (128 columns): 512 columns in all.  While the tensor pipe
 // runs one tile's P V and next S, the other tile's warps form exponentials.
 //
-// Warp roles (384 threads): warp 0 producer; warps 1 and 2 issue the products of one tile each, P V and the next S, taking
+// Warp roles (512 threads): warp 0 producer; warps 1 and 2 issue the products of one tile each, P V and the next S, taking
 // turns: the two tiles' scores become ready half a period apart and their exponentials do not compete (issuers that do not
 // take turns interleave their products, and both groups run in phase), while one issuer's waits and the queue's drain are
 // covered by the other's products (one warp for both tiles took 2320 cycles per tile, 1460 of them for 16 products); warp 3
-// owns TMEM; warps 4-7 and 8-11 are the softmax groups of the two tiles, one row per thread.  P is handed over in two
-// halves, so that P V starts while the second half's exponentials are formed.  Persistent CTAs, items dealt out round
-// robin, the longest first; results leave through a staging panel per tile and TMA (a thread's own row stores touch 32 lines
-// per instruction and took as long as one and a half tiles).
+// owns TMEM; warps 4-7 write finished results (3700 cycles a tile, beside the next item's first
+// tiles); warps 8-11 and 12-15 are the softmax groups of the two tiles, one row per thread.  P is handed over in two
+// halves, so that P V starts while the second half's exponentials are formed.  Persistent CTAs, items dealt out back and forth, the
+// longest first; the steps of consecutive items follow one another without a pause.
 #include <type_traits>
 #include "attn.h"
 
@@ -26,52 +26,79 @@ namespace lucid {
 
 static __device__ Control g_attn_fwd_ctl;
 
-constexpr int kFwRing = 4;
+constexpr int kFwRing = 4, kFwSlots = 4;
+
+// An item as its roles need it, worked out by one thread (the divisions and lists took each role some 1500 cycles an item)
+struct FwdSlot {
+  int n;                  // entries of the union, -1: no more items
+  int b, hk, len, sink, lo;
+  struct Tile {
+    int h, block, n;      // n: entries of its own
+    int first;            // entry 0 is its own, for the visible first keys
+    int from, to;         // and the entries from .. to-1
+    int sink, lo, p_lo, p_hi;
+  } t[2];
+  __device__ __forceinline__ int tile(int u) const { return u < sink ? 0 : lo + u - sink; }
+};
 struct AttnFwdSmem {
   alignas(1024) uint8_t q[2][kTileBytes];
   alignas(1024) uint8_t ring[kFwRing][kTileBytes];   // K(0), V(0), K(1), V(1), ... of the union of the two tiles' lists
-  alignas(1024) uint8_t stage[2][kHalfBytes];         // 128 rows x 64 columns of a tile's result
+  alignas(1024) uint8_t stage[kTileBytes];            // a tile's result: per warp two panels of 32 rows x 64 columns
   alignas(8) uint64_t full[kFwRing];
-  uint64_t empty[kFwRing], q_full[2], q_free[2], s_full[2], p_half[2], p_ready[2], turn[2], meet[2], o_full[2], o_free[2];
+  uint64_t empty[kFwRing], q_full[2], q_free[2], s_full[2], p_half[2], p_ready[2], turn[2], o_full[2], o_free[2], l_full[2], l_free[2];
+  uint64_t slot_full[kFwSlots], slot_free[kFwSlots];
+  FwdSlot slot[kFwSlots];
+  alignas(16) float2 l[2][kBlock];                                // a finished row's sum and the reference of its exponents
   uint32_t tmem_base;
   int abort_flag;
 };
 
-enum AttnFwdBar : int { AF_FULL = 401, AF_EMPTY, AF_Q_FULL, AF_Q_FREE, AF_S_FULL, AF_P_HALF, AF_P_READY, AF_TURN, AF_MEET, AF_O_FULL, AF_O_FREE };
+static_assert(sizeof(AttnFwdSmem) <= 232448, "shared memory of a CTA");
 
-constexpr int kFwThreads = 384;
+enum AttnFwdBar : int { AF_FULL = 401, AF_EMPTY, AF_Q_FULL, AF_Q_FREE, AF_S_FULL, AF_P_HALF, AF_P_READY, AF_TURN, AF_O_FULL, AF_O_FREE, AF_L_FULL, AF_L_FREE, AF_SLOT_FULL, AF_SLOT_FREE };
+
+constexpr int kFwThreads = 512;
 constexpr int kFwS = 0, kFwO = 256;      // + 128 * tile
-constexpr int kFwRegsService = 88, kFwRegsSoftmax = 208;    // 128 * 88 + 256 * 208 = 384 * 168, the launch's total
+constexpr int kFwRegsService = 80, kFwRegsSoftmax = 176;    // 256 * 80 + 256 * 176 = 512 * 128, the launch's total
 constexpr float kFwSlack = 8.f;          // log2 of how far the maximum may outgrow the reference
 
 template <bool kBf16>
 __global__ void __launch_bounds__(kFwThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_out,
-                const AttnFwdArgs args) {
-  extern __shared__ uint8_t smem_raw[];
-  AttnFwdSmem& s = *reinterpret_cast<AttnFwdSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+                const __grid_constant__ CUtensorMap tm_v, const AttnFwdArgs args) {
+  // (no room to round the base up: the kernel has no static shared memory, and the window starts on 1 KiB)
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  AttnFwdSmem& s = *reinterpret_cast<AttnFwdSmem*>(smem_raw);
   const AttnShape& A = args.a;
   Control* ctl = &g_attn_fwd_ctl;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const unsigned long long limit = args.wait_ns;
   volatile int* cta_abort = &s.abort_flag;
 
+  if (smem_u32(smem_raw) & 1023) {       // (operand tiles would be misread)
+    if (tid == 0) report_error(ctl, kErrAborted, -1, -1, blockIdx.x, 0);
+    return;
+  }
   if (tid == 0) {
     for (int i = 0; i < kFwRing; ++i) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], 2);
+    }
+    for (int i = 0; i < kFwSlots; ++i) {
+      mbar_init(&s.slot_full[i], 1);
+      mbar_init(&s.slot_free[i], 15);      // producer, two issuers, four epilogue and eight softmax warps
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.q_full[i], 1);
       mbar_init(&s.q_free[i], 1);
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.turn[i], 1);
-      mbar_init(&s.meet[i], 128);
       mbar_init(&s.p_half[i], 128);
       mbar_init(&s.p_ready[i], 128);
       mbar_init(&s.o_full[i], 1);
       mbar_init(&s.o_free[i], 128);
+      mbar_init(&s.l_full[i], 128);
+      mbar_init(&s.l_free[i], 128);
     }
     s.abort_flag = 0;
     mbar_fence_init();
@@ -84,7 +111,19 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = s.tmem_base;
-  auto length_of = [&](int b) -> int { return attn_length(A, args.lengths, b); };
+  // The items of this CTA, one after another: `next` waits for the slot, `done` hands it back (per warp; whoever reads it
+  // later keeps copies).
+  uint32_t slots = 0;
+  auto next = [&]() -> const FwdSlot* {
+    if (!wait_lean(&s.slot_full[slots % kFwSlots], (slots / kFwSlots) & 1, cta_abort, limit, AF_SLOT_FULL)) return nullptr;
+    const FwdSlot* slot = &s.slot[slots % kFwSlots];
+    return slot->n < 0 ? nullptr : slot;
+  };
+  auto done = [&](bool one_thread) {
+    if (!one_thread) __syncwarp();
+    if (one_thread || lane == 0) mbar_arrive(&s.slot_free[slots % kFwSlots]);
+    ++slots;
+  };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFwRegsService));
@@ -94,44 +133,85 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         tma_prefetch_desc(&tm_q);
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
-        uint32_t r = 0, stage = 0, phase = 0;
+        uint32_t stage = 0, phase = 0;
         uint32_t nq[2] = {0, 0};      // Q tiles loaded
         bool alive = true;
-        FwdItem it;
-        for (int rnd = 0, idx; alive && fwd_item(A, idx = snake_item(rnd, blockIdx.x, gridDim.x), it); ++rnd) {
-          const PairTiles pt = pair_tiles(A, it, length_of(it.b));
+        while (alive) {
+          const FwdSlot* it = next();
+          if (!it) break;
+          const int b = it->b, hk = it->hk;
           auto load = [&](const CUtensorMap* tm, int tile) -> bool {
             if (!wait_lean(&s.empty[stage], phase ^ 1, cta_abort, limit, AF_EMPTY)) return false;
             mbar_expect_tx(&s.full[stage], kTileBytes);
-            tma_load_4d(s.ring[stage], tm, &s.full[stage], 0, tile * kBlock, it.hk, it.b);
-            tma_load_4d(s.ring[stage] + kHalfBytes, tm, &s.full[stage], 64, tile * kBlock, it.hk, it.b);
-            ++r;
+            tma_load_4d(s.ring[stage], tm, &s.full[stage], 0, tile * kBlock, hk, b);
+            tma_load_4d(s.ring[stage] + kHalfBytes, tm, &s.full[stage], 64, tile * kBlock, hk, b);
             if (++stage == kFwRing) {
               stage = 0;
               phase ^= 1;
             }
             return true;
           };
-          for (int t = 0; t < 2 && alive; ++t) {
-            if (pt.list(t).n == 0) continue;
+          for (int t = 0; t < 2; ++t) {
+            if (it->t[t].n == 0) continue;
             if (!wait_lean(&s.q_free[t], (nq[t] & 1) ^ 1, cta_abort, limit, AF_Q_FREE)) {
               alive = false;
               break;
             }
             ++nq[t];
             mbar_expect_tx(&s.q_full[t], kTileBytes);
-            tma_load_4d(s.q[t], &tm_q, &s.q_full[t], 0, it.block(t) * kBlock, it.h(t), it.b);
-            tma_load_4d(s.q[t] + kHalfBytes, &tm_q, &s.q_full[t], 64, it.block(t) * kBlock, it.h(t), it.b);
+            tma_load_4d(s.q[t], &tm_q, &s.q_full[t], 0, it->t[t].block * kBlock, it->t[t].h, b);
+            tma_load_4d(s.q[t] + kHalfBytes, &tm_q, &s.q_full[t], 64, it->t[t].block * kBlock, it->t[t].h, b);
           }
-          for (int u = 0; u < pt.n && alive; ++u) {
-            const int j = pt.tile(u);
+          for (int u = 0, n = it->n; u < n && alive; ++u) {
+            const int j = it->tile(u);
             alive = load(&tm_k, j) && load(&tm_v, j);
           }
+          done(true);
+        }
+      }
+    } else if (warp == 3) {
+      // =========================== the items (one lane) ===========================
+      if (lane == 0) {
+        FwdItem it;
+        for (int rnd = 0;; ++rnd) {
+          const int k = rnd % kFwSlots;
+          if (!wait_lean(&s.slot_free[k], ((rnd / kFwSlots) & 1) ^ 1, cta_abort, limit, AF_SLOT_FREE)) break;
+          FwdSlot& x = s.slot[k];
+          const bool more = fwd_item(A, snake_item(rnd, blockIdx.x, gridDim.x), it);
+          if (more) {
+            x.len = attn_length(A, args.lengths, it.b);
+            const PairTiles pt = pair_tiles(A, it, x.len);
+            x.n = pt.n;
+            x.b = it.b;
+            x.hk = it.hk;
+            x.sink = pt.sink;
+            x.lo = pt.lo;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const KeyTiles kt = pt.list(t);
+              FwdSlot::Tile& y = x.t[t];
+              y.h = it.h(t);
+              y.block = it.block(t);
+              y.n = kt.n;
+              y.first = kt.n > 0 && kt.sink;
+              y.from = kt.n > kt.sink ? kt.lo - pt.lo + pt.sink : 0;
+              y.to = y.from + (kt.n > kt.sink ? kt.n - kt.sink : 0);
+              y.sink = kt.sink;
+              y.lo = kt.lo;
+              y.p_lo = kt.p_lo;
+              y.p_hi = kt.p_hi;
+            }
+          } else {
+            x.n = -1;
+          }
+          mbar_arrive(&s.slot_full[k]);
+          if (!more) break;
         }
       }
     } else if (warp < 3) {
       // =========================== issuer of one tile's products ===========================
-      // Step u of the union: P V of the tile's previous entry and S of entry u, in turns with the other tile's issuer
+      // A step per entry of the items' unions, one after another, and one at the end: P V of this tile's previous entry (it
+      // may be the last of the item before), then S of this entry, in turns with the other tile's issuer.
       const int t = warp - 1;
       constexpr int fmt = kBf16 ? 1 : 0;
       constexpr uint32_t idesc_s = umma_idesc(fmt, 0, 0, 128, 128);          // Q K^T: both K-major
@@ -141,121 +221,212 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const uint64_t d_k0 = umma_smem_desc(smem_u32(s.ring[0]), 16, 1024);
       const uint64_t d_v0 = umma_smem_desc(smem_u32(s.ring[0]), kHalfBytes, 1024);
       const uint32_t s_tmem = tmem + kFwS + 128 * t, o_tmem = tmem + kFwO + 128 * t;
-      uint32_t st = 0, phase = 0;        // ring stage and phase of K(u); V(u) is in the stage behind it
-      uint32_t v_st = 0, v_phase = 0;    // V(u - 1)
-      uint32_t nq = 0, np = 0, turns = 0;  // items with tiles; weights consumed; turns taken
-      bool alive = true;
-      FwdItem it;
-      for (int rnd = 0, idx; alive && fwd_item(A, idx = snake_item(rnd, blockIdx.x, gridDim.x), it); ++rnd) {
-        const PairTiles pt = pair_tiles(A, it, length_of(it.b));
-        const KeyTiles kt = pt.list(t);
-        bool first = true, pend = false, was_narrow = false;    // pend: the weights of entry u - 1 are this tile's
-        int left = kt.n;
-        for (int u = 0; u <= pt.n; ++u) {
-          const bool more = u < pt.n, act = more && pt.active(kt, u), narrow = more && tile_narrow(A, kt, pt.tile(u));
-          if (u > 0 && !wait_lean(&s.full[v_st], v_phase, cta_abort, limit, AF_FULL)) { alive = false; break; }
-          if (more && !wait_lean(&s.full[st], phase, cta_abort, limit, AF_FULL)) { alive = false; break; }
-          if (act && left == kt.n && !wait_lean(&s.q_full[t], nq & 1, cta_abort, limit, AF_Q_FULL)) { alive = false; break; }
-          if (pend) {
-            if (!wait_lean(&s.p_half[t], np & 1, cta_abort, limit, AF_P_HALF)) { alive = false; break; }
-            // the epilogue of this tile's previous item has read O
-            if (first && !wait_lean(&s.o_free[t], (nq & 1) ^ 1, cta_abort, limit, AF_O_FREE)) { alive = false; break; }
-          }
-          const uint64_t dv = d_v0 + v_st * (kTileBytes >> 4), dk = d_k0 + st * (kTileBytes >> 4);
-          if (!wait_lean(&s.turn[t], (turns & 1) ^ (t ^ 1), cta_abort, limit, AF_TURN)) { alive = false; break; }
-          ++turns;
-          tc_fence_after_sync();
-          if (pend) {
-            const uint32_t add = first ? 0u : 1u;
-            if (was_narrow) {
-              if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < kNarrow / 16; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
-              }
-            } else {
-              if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
-              }
-            }
-            if (!wait_lean(&s.p_ready[t], np & 1, cta_abort, limit, AF_P_READY)) { alive = false; break; }
-            ++np;
-            if (!was_narrow) {
-              tc_fence_after_sync();
-              if (elect_one()) {
-#pragma unroll
-                for (int k = 4; k < 8; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, 1u);
-              }
-            }
-            first = false;
-          }
-          if (act) {
-            const uint32_t idesc = narrow ? idesc_sn : idesc_s;
+      uint32_t st = 0, phase = 0;             // ring stage and phase of this entry's K; its V is in the stage behind it
+      uint32_t v_st = 0, v_phase = 0;         // V of the entry before
+      uint32_t nq = 0, no = 0, np = 0, turns = 0;   // items begun and results begun (with tiles); weights consumed; turns taken
+      bool before = false;                    // is there an entry before
+      bool pend = false, pend_first = false, pend_last = false, pend_narrow = false;   // its weights are this tile's
+      auto step = [&](bool more, bool act, bool first, bool last, bool narrow) -> bool {
+        if (before && !wait_lean(&s.full[v_st], v_phase, cta_abort, limit, AF_FULL)) return false;
+        if (more && !wait_lean(&s.full[st], phase, cta_abort, limit, AF_FULL)) return false;
+        if (act && first && !wait_lean(&s.q_full[t], nq++ & 1, cta_abort, limit, AF_Q_FULL)) return false;
+        if (pend) {
+          if (!wait_lean(&s.p_half[t], np & 1, cta_abort, limit, AF_P_HALF)) return false;
+          // the epilogue of this tile's previous item has read O
+          if (pend_first && !wait_lean(&s.o_free[t], (no++ & 1) ^ 1, cta_abort, limit, AF_O_FREE)) return false;
+        }
+        const uint64_t dv = d_v0 + v_st * (kTileBytes >> 4), dk = d_k0 + st * (kTileBytes >> 4);
+        if (!wait_lean(&s.turn[t], (turns++ & 1) ^ (t ^ 1), cta_abort, limit, AF_TURN)) return false;
+        tc_fence_after_sync();
+        if (pend) {
+          const uint32_t add = pend_first ? 0u : 1u;
+          if (pend_narrow) {
             if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-                umma_ss(s_tmem, dq + off, dk + off, idesc, k ? 1u : 0u);
-              }
+              for (int k = 0; k < kNarrow / 16; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
             }
-            --left;
+          } else {
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
+            }
           }
-          __syncwarp();
+          if (!wait_lean(&s.p_ready[t], np++ & 1, cta_abort, limit, AF_P_READY)) return false;
+          if (!pend_narrow) {
+            tc_fence_after_sync();
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 4; k < 8; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, 1u);
+            }
+          }
+          if (pend_last) umma_commit_w(&s.o_full[t]);
+        }
+        if (act) {
+          const uint32_t idesc = narrow ? idesc_sn : idesc_s;
           if (elect_one()) {
-            mbar_arrive(&s.turn[t ^ 1]);
-            if (act) umma_commit(&s.s_full[t]);
-            // the stages go back when both issuers' products that read them are complete (an issuer without products
-            // on them only says that it is past them)
-            if (u > 0) umma_commit(&s.empty[v_st]);
-            if (more) umma_commit(&s.empty[st]);
-            if (act && left == 0) umma_commit(&s.q_free[t]);
-            // the tile's last weights have been consumed: its result is complete
-            if (pend && !act && left == 0) umma_commit(&s.o_full[t]);
-          }
-          if (pend && !act && left == 0) ++nq;
-          pend = act;
-          was_narrow = narrow;
-          if (more) {
-            v_st = st + 1;
-            v_phase = phase;
-            if (v_st == kFwRing) {
-              v_st = 0;
-              v_phase ^= 1;
-            }
-            st = v_st + 1;
-            phase = v_phase;
-            if (st == kFwRing) {
-              st = 0;
-              phase ^= 1;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
+              umma_ss(s_tmem, dq + off, dk + off, idesc, k ? 1u : 0u);
             }
           }
         }
+        __syncwarp();
+        if (elect_one()) {
+          mbar_arrive(&s.turn[t ^ 1]);
+          if (act) umma_commit(&s.s_full[t]);
+          // the stages go back when both issuers' products that read them are complete (an issuer without products on
+          // them only says that it is past them)
+          if (before) umma_commit(&s.empty[v_st]);
+          if (more) umma_commit(&s.empty[st]);
+          if (act && last) umma_commit(&s.q_free[t]);
+        }
+        pend = act;
+        pend_first = first;
+        pend_last = last;
+        pend_narrow = narrow;
+        before = true;
+        v_st = st + 1;
+        v_phase = phase;
+        if (v_st == kFwRing) {
+          v_st = 0;
+          v_phase ^= 1;
+        }
+        st = v_st + 1;
+        phase = v_phase;
+        if (st == kFwRing) {
+          st = 0;
+          phase ^= 1;
+        }
+        return true;
+      };
+      bool alive = true;
+      while (alive) {
+        const FwdSlot* it = next();
+        if (!it) break;
+        const int n = it->n, own = it->t[t].n, own_first = it->t[t].first, from = it->t[t].from, to = it->t[t].to;
+        done(false);
+        const bool narrow0 = own_first && A.S <= kNarrow;       // (tile_narrow)
+        int at = 0;
+        for (int u = 0; u < n && alive; ++u) {
+          const bool act = (u == 0 && own_first) || (u >= from && u < to);
+          alive = step(true, act, at == 0, at == own - 1, narrow0 && u == 0);
+          if (act) ++at;
+        }
       }
+      if (alive && before) step(false, false, false, false, false);
+    }
+  } else if (warp < 8) {
+    // =========================== epilogue of both tiles ===========================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFwRegsService));
+    typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
+    const int row = ((warp & 3) << 5) + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    // Through two staging panels of the warp's own, 32 rows x 64 columns each: a thread has a row, but its own stores would
+    // touch 32 lines per instruction; read back in rows, one instruction writes four lines.  O is handed back as soon as it
+    // stands in the panels: the next item's first P V waits for it.
+    uint8_t* panel = s.stage + (warp & 3) * 8192;
+    uint32_t no0 = 0, no1 = 0;
+    bool alive = true;
+    while (alive) {
+      const FwdSlot* it = next();
+      if (!it) break;
+      const int len = it->len, b = it->b;
+#pragma unroll 1
+      for (int t = 0; t < 2; ++t) {
+        const int block = it->t[t].block, h = it->t[t].h;
+        if (block >= A.nqb) continue;
+        const bool has = it->t[t].n > 0;
+        const int i = block * kBlock + row;
+        float l = 0.f, ref = 0.f;
+        if (has) {
+          const uint32_t n = t ? no1++ : no0++;
+          if (!wait_lean(&s.l_full[t], n & 1, cta_abort, limit, AF_L_FULL)) { alive = false; break; }
+          const float2 x = s.l[t][row];
+          l = x.x;
+          ref = x.y;
+          mbar_arrive(&s.l_free[t]);
+          if (!wait_lean(&s.o_full[t], n & 1, cta_abort, limit, AF_O_FULL)) { alive = false; break; }
+          tc_fence_after_sync();
+        }
+        const bool some = i + A.off < len && l != 0.f;     // (a NaN sum is written as it is)
+        const float inv = some ? 1.f / l : 0.f;
+        elem_t* out = reinterpret_cast<elem_t*>(args.out) + b * args.out_strides.b + h * args.out_strides.h + (lane & 7) * 8;
+        const int r0 = block * kBlock + (warp & 3) * 32 + (lane >> 3);
+        const uint32_t o_tmem = tmem + lanes + kFwO + 128 * t;
+        if (has) {
+          uint32_t oa[16], ob[16];
+          auto put = [&](const uint32_t (&o)[16], int c) {        // columns 16c .. 16c+15
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint4 w = make_uint4(0, 0, 0, 0);
+              if (some) {
+                w.x = pack2<kBf16>(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
+                w.y = pack2<kBf16>(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
+                w.z = pack2<kBf16>(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
+                w.w = pack2<kBf16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
+              }
+              *reinterpret_cast<uint4*>(panel + (c >> 2) * 4096 + sw128_off(lane, 2 * (c & 3) + e)) = w;
+            }
+          };
+          tmem_ld16(o_tmem, oa);
+          tmem_wait_ld();
+#pragma unroll 1
+          for (int c = 0; c < 8; c += 2) {
+            tmem_ld16(o_tmem + 16 * (c + 1), ob);
+            put(oa, c);
+            tmem_wait_ld();
+            if (c < 6) tmem_ld16(o_tmem + 16 * (c + 2), oa);
+            else {
+              // (all of O is in registers)
+              tc_fence_before_sync();
+              mbar_arrive(&s.o_free[t]);
+            }
+            put(ob, c + 1);
+            if (c < 6) tmem_wait_ld();
+          }
+        }
+        __syncwarp();
+#pragma unroll 1
+        for (int y = 0; y < 8; ++y) {
+          const uint4 w0 = *reinterpret_cast<const uint4*>(panel + sw128_off(4 * y + (lane >> 3), lane & 7));
+          const uint4 w1 = *reinterpret_cast<const uint4*>(panel + 4096 + sw128_off(4 * y + (lane >> 3), lane & 7));
+          const uint4 zero = make_uint4(0, 0, 0, 0);
+          if (r0 + 4 * y < A.Nq) {
+            elem_t* at = out + (long long)(r0 + 4 * y) * args.out_strides.n;
+            *reinterpret_cast<uint4*>(at) = has ? w0 : zero;
+            *reinterpret_cast<uint4*>(at + 64) = has ? w1 : zero;
+          }
+        }
+        __syncwarp();
+        if (i < A.Nq && args.lse)
+          args.lse[((long long)b * A.Hq + h) * A.Nq + i] = some ? (ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      }
+      done(false);
     }
   } else {
-    // =========================== softmax of one tile, then its epilogue ===========================
+    // =========================== softmax of one tile ===========================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFwRegsSoftmax));
-    const int t = (warp - 4) >> 2;
+    const int t = (warp - 8) >> 2;
     const int row = ((warp & 3) << 5) + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + kFwS + 128 * t, o_tmem = tmem + lanes + kFwO + 128 * t;
     const float sl2 = args.scale_log2;
     const unsigned long long sl22 = f32x2(sl2, sl2);
-    uint32_t ns = 0, no = 0, r = 0, meets = 0;
-    // the tile's 128 threads meet (an mbarrier and not a named barrier: this wait, too, has a limit)
-    auto meet = [&]() -> bool {
-      mbar_arrive(&s.meet[t]);
-      return wait_lean(&s.meet[t], meets++ & 1, cta_abort, limit, AF_MEET);
-    };
+    uint32_t ns = 0, nl = 0, r = 0;
     bool alive = true;
-    FwdItem it;
-    for (int rnd = 0, idx; alive && fwd_item(A, idx = snake_item(rnd, blockIdx.x, gridDim.x), it); ++rnd) {
-      const int len = length_of(it.b);
-      const PairTiles pt = pair_tiles(A, it, len);
-      const KeyTiles kt = pt.list(t);
-      const int i = it.block(t) * kBlock + row;
-      const int p = i + A.off;
-      const bool valid = i < A.Nq && p < len;
+    while (alive) {
+      const FwdSlot* it = next();
+      if (!it) break;
+      const int len = it->len, u_sink = it->sink, u_lo = it->lo, u_n = it->n;
+      KeyTiles kt;
+      kt.n = it->t[t].n;
+      kt.sink = it->t[t].sink;
+      kt.lo = it->t[t].lo;
+      kt.p_lo = it->t[t].p_lo;
+      kt.p_hi = it->t[t].p_hi;
+      const int p = it->t[t].block * kBlock + row + A.off;
+      done(false);
       float ref = -INFINITY, l = 0.f;
       for (int x = 0; x < kt.n; ++x, ++ns) {
         const int tile = kt.tile(x), j0 = tile << 7;
@@ -266,7 +437,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (masked) {
           if (j0 + 127 >= len && len < A.Nk) {
             // rows behind the sequence hold anything, and 0 * NaN is not 0: the value tile's become zero
-            const uint32_t use = r + 2 * (tile == 0 && pt.sink ? 0 : tile - pt.lo + pt.sink) + 1;
+            const uint32_t use = r + 2 * (tile == 0 && u_sink ? 0 : tile - u_lo + u_sink) + 1;
             if (!wait_lean(&s.full[use % kFwRing], (use / kFwRing) & 1, cta_abort, limit, AF_FULL)) {
               alive = false;
               break;
@@ -277,25 +448,34 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         }
         // the tile's first 32 * kChunks columns (the rest is not visible, and P is not read there)
-        auto weights = [&](auto chunks) {
+        auto weights = [&](auto chunks, auto some_masked) {
           constexpr int kChunks = decltype(chunks)::value;
+          constexpr bool kMasked = decltype(some_masked)::value;
           uint32_t v[kChunks][32];
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) tmem_ld32(s_tmem + 32 * c, v[c]);
           tmem_wait_ld();
-          if (masked) {
+          // most chunks of a masked tile are whole or empty for all rows of a warp
+          bool empty[kChunks];
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
+          for (int c = 0; c < kChunks; ++c) {
+            empty[c] = false;
+            if constexpr (kMasked) {
               const uint32_t w = mask.word(32 * c);
+              empty[c] = __all_sync(0xffffffffu, w == 0u);
+              if (!empty[c] && !__all_sync(0xffffffffu, w == ~0u)) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[c][e] = (w & (1u << e)) ? v[c][e] : 0xff800000u;
+                for (int e = 0; e < 32; ++e) v[c][e] = (w & (1u << e)) ? v[c][e] : 0xff800000u;
+              }
             }
           }
-          float mx[4];
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int x = 0; x < 4; ++x) mx[x] = __uint_as_float(v[0][x]);
+          for (int c = 0; c < kChunks; ++c) {
+            if (kMasked && empty[c]) continue;
 #pragma unroll
-          for (int x = 4; x < 32 * kChunks; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x >> 5][x & 31]));
+            for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[c][e]));
+          }
           const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
           const bool grow = m > ref + kFwSlack;
           if (x == 0) {
@@ -323,6 +503,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             uint32_t pk[16];
+            if (kMasked && empty[c]) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) pk[e] = 0u;
+            } else {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const unsigned long long y =
@@ -333,6 +517,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               if (e & 1) sum2 = f32x2_add(sum2, f32x2(w.x, w.y));
               else sum = f32x2_add(sum, f32x2(w.x, w.y));
               pk[e] = pack2<kBf16>(w.x, w.y);
+            }
             }
             tmem_st16(s_tmem + 16 * c, pk);
             if (c == 1 && kChunks > 2) {
@@ -348,63 +533,19 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const float2 both = f32x2_unpack(f32x2_add(sum, sum2));
           l += both.x + both.y;
         };
-        if (tile_narrow(A, kt, tile)) weights(std::integral_constant<int, kNarrow / 32>{});
-        else weights(std::integral_constant<int, 4>{});
+        if (!masked) weights(std::integral_constant<int, 4>{}, std::false_type{});
+        else if (tile_narrow(A, kt, tile)) weights(std::integral_constant<int, kNarrow / 32>{}, std::true_type{});
+        else weights(std::integral_constant<int, 4>{}, std::true_type{});
       }
       if (!alive) break;
-      r += 2 * pt.n;
+      r += 2 * u_n;
 
-      // ---- epilogue ----
-      const bool has = kt.n > 0;
-      if (has) {
-        if (!wait_lean(&s.o_full[t], no & 1, cta_abort, limit, AF_O_FULL)) break;
-        ++no;
-        tc_fence_after_sync();
+      if (kt.n > 0) {
+        if (!wait_lean(&s.l_free[t], (nl++ & 1) ^ 1, cta_abort, limit, AF_L_FREE)) break;
+        s.l[t][row] = make_float2(l, ref);
+        mbar_arrive(&s.l_full[t]);
       }
-      const bool some = valid && l != 0.f;      // (a NaN sum is written as it is)
-      const float inv = some ? 1.f / l : 0.f;
-      const bool lead = (tid & 127) == 0;
-      if (it.block(t) < A.nqb) {
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          if (lead) tma_store_wait_read();               // the panel's previous store has read it
-          if (!meet()) { alive = false; break; }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t o[32];
-            if (has) {
-              tmem_ld32(o_tmem + 64 * hf + 32 * c, o);
-              tmem_wait_ld();
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint4 w = make_uint4(0, 0, 0, 0);
-              if (has && some) {
-                w.x = pack2<kBf16>(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
-                w.y = pack2<kBf16>(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
-                w.z = pack2<kBf16>(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
-                w.w = pack2<kBf16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
-              }
-              *reinterpret_cast<uint4*>(s.stage[t] + sw128_off(row, 4 * c + e)) = w;
-            }
-          }
-          fence_proxy_async_smem();
-          if (!meet()) { alive = false; break; }
-          if (lead) {                                    // rows behind Nq lie outside the map and are not written
-            tma_store_4d(&tm_out, s.stage[t], 64 * hf, it.block(t) * kBlock, it.h(t), it.b);
-            tma_store_commit();
-          }
-        }
-      }
-      if (has) {
-        tc_fence_before_sync();
-        mbar_arrive(&s.o_free[t]);
-      }
-      if (i < A.Nq && args.lse)
-        args.lse[((long long)it.b * A.Hq + it.h(t)) * A.Nq + i] =
-            some ? (ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
     }
-    if ((tid & 127) == 0) tma_store_wait_read();
   }
 
   if (s.abort_flag) {
@@ -419,14 +560,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 }
 
 cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
-                            const CUtensorMap& tm_out, const AttnFwdArgs& args, int sms, cudaStream_t stream) {
+                            const AttnFwdArgs& args, int sms, cudaStream_t stream) {
   const int items = fwd_items(args.a), grid = items < sms ? items : sms;
-  const int bytes = (int)sizeof(AttnFwdSmem) + 1024;
+  const int bytes = (int)sizeof(AttnFwdSmem);
   auto kernel = bf16 ? attn_fwd_kernel<true> : attn_fwd_kernel<false>;
   static SmemOnce once[2];
   cudaError_t e = once[bf16].set(reinterpret_cast<const void*>(kernel), bytes);
   if (e != cudaSuccess) return e;
-  kernel<<<grid, kFwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, tm_out, args);
+  kernel<<<grid, kFwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, args);
   return cudaGetLastError();
 }
 
