@@ -25,7 +25,7 @@ struct AttnFwdArgs {
 struct AttnBwdArgs {
   AttnShape a;
   const int* lengths;
-  const float2* stat;     // (B, Hq, nqb * 128) {lse in base 2 (+inf: row without weight), delta}
+  const float* stat;      // (B, Hq, nqb, 2, 128): lse in base 2 (+inf: row without weight), delta
   void* dq;
   Strides dq_strides;
   void *dk, *dv;
@@ -42,7 +42,7 @@ struct AttnStatArgs {
   const void *out, *dout;
   Strides out_strides, dout_strides;
   const float* lse;
-  float2* stat;
+  float* stat;
 };
 
 cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,

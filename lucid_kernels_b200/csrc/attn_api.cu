@@ -33,7 +33,7 @@ static int make_shape(AttnShape* a, const lucid_window_attn_desc* d) {
   return 0;
 }
 
-static size_t stat_bytes(const AttnShape& a) { return (size_t)a.B * a.Hq * a.nqb * kBlock * sizeof(float2); }
+static size_t stat_bytes(const AttnShape& a) { return (size_t)a.B * a.Hq * a.nqb * 2 * kBlock * sizeof(float); }
 static size_t partial_bytes(const AttnShape& a) {
   const int c = sink_chunks(a);
   return c ? (size_t)a.B * a.Hkv * (1 + c) * 2 * a.S * kBlock * sizeof(float) : 0;
@@ -168,7 +168,7 @@ int lucid_window_attn_bwd(const lucid_window_attn_desc* d, const void* q, const 
       (rc = bshd_map(&tm_v, bf16, v, d->v_strides, B, Nk, Hkv, 128)) ||
       (rc = bshd_map(&tm_do, bf16, dout, d->dout_strides, B, Nq, Hq, 128)))
     return rc;
-  float2* stat = static_cast<float2*>(workspace);
+  float* stat = static_cast<float*>(workspace);
   AttnStatArgs sa;
   sa.a = args.a;
   sa.lengths = lengths;

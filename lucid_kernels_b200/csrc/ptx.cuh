@@ -422,6 +422,11 @@ __device__ __forceinline__ unsigned long long f32x2_add(unsigned long long a, un
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ unsigned long long f32x2_mul(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // Element e of a row uses the polynomial when e % kExpPolyPeriod == kExpPolyPeriod - 1 (0 disables it).
 // Measured on B200 (B=2, N=32768, H=8): periods 2, 3 and 4 were all slower than 0, because a polynomial
 // costs about as many FMA + ALU issue cycles per warp as the 8 cycles of one MUFU instruction, so it
