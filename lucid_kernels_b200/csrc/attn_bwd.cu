@@ -83,6 +83,18 @@ __device__ __forceinline__ void issue_ts(uint32_t d_tmem, uint32_t a_tmem, uint6
   }
 }
 
+// The same in two parts: k-steps 0, 1, 4, 5 (the first 32 columns of both halves' threads), then 2, 3, 6, 7
+template <int kPart>
+__device__ __forceinline__ void issue_ts_part(uint32_t d_tmem, uint32_t a_tmem, uint64_t db, uint32_t idesc, uint32_t add) {
+  if (elect_one()) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int k = 2 * kPart + (x & 1) + 4 * (x >> 1);
+      umma_ts(d_tmem, a_tmem + (k < 4 ? 8 * k : 32 + 8 * k), db + k * (2048 >> 4), idesc, x ? 1u : add);
+    }
+  }
+}
+
 // 64 fp32 columns of this thread's row, from tensor memory, times `f`, as 16-bit values into the warp's panel (32 rows x 64
 // columns; zeros unless `some`); `loaded` is called when the tensor memory has been read.
 template <bool kBf16, class Loaded>
@@ -520,7 +532,7 @@ struct AttnDkvSmem {
   alignas(8) uint64_t q_full[2];
   uint64_t q_empty[2], go_full[2], go_empty[2], slot_full[2], slot_free[2];
   uint64_t k_full, k_free, v_full, v_free;
-  uint64_t s_full, p_ready, dp_full, ds_ready, dv_full, dv_free, dk_full, dk_free;
+  uint64_t s_full, p_half, p_ready, dp_full, ds_ready, dv_full, dv_free, dk_full, dk_free;
   DkvSlot slot[2];
   uint32_t tmem_base;
   int abort_flag;
@@ -560,6 +572,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     mbar_init(&s.v_full, 1);
     mbar_init(&s.v_free, 1);
     mbar_init(&s.s_full, 1);
+    mbar_init(&s.p_half, 256);
     mbar_init(&s.p_ready, 256);
     mbar_init(&s.dp_full, 1);
     mbar_init(&s.ds_ready, 256);
@@ -675,9 +688,13 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       for (int q = 0; q < n; ++q, ++g) {
         if (!wait_lean(&s.go_full[g & 1], (g >> 1) & 1, cta_abort, limit, AB_GO_FULL)) { alive = false; break; }
         if (q == 0 && !wait_lean(&s.dv_free, (itn & 1) ^ 1, cta_abort, limit, AB_ACC_FREE)) { alive = false; break; }
+        if (!wait_lean(&s.p_half, g & 1, cta_abort, limit, AB_P_READY)) { alive = false; break; }
+        tc_fence_after_sync();
+        const uint64_t db = d_g0 + (g & 1) * (kTileBytes >> 4);
+        issue_ts_part<0>(tmem + kKvDv, tmem + kKvS, db, idesc_mn, q ? 1u : 0u);
         if (!wait_lean(&s.p_ready, g & 1, cta_abort, limit, AB_P_READY)) { alive = false; break; }
         tc_fence_after_sync();
-        issue_ts(tmem + kKvDv, tmem + kKvS, d_g0 + (g & 1) * (kTileBytes >> 4), idesc_mn, q ? 1u : 0u);
+        issue_ts_part<1>(tmem + kKvDv, tmem + kKvS, db, idesc_mn, 1u);
         umma_commit_w(&s.go_empty[g & 1]);
         if (q + 1 < n && !issue_s(g + 1)) { alive = false; break; }
       }
@@ -753,13 +770,35 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           tmem_ld32(s_tmem, v[0]);
           tmem_ld32(s_tmem + 32, v[1]);
           tmem_wait_ld();
+          // Query rows behind the sequence hold anything, and 0 * NaN is not 0: they become zero in Q and dO before
+          // the products that sum over them.  S^T and G^T, which read them as columns, are complete by then.
+          const bool stale = kMasked && p0 + 127 >= len && len < A.Nk;
+          if (stale) {
+            if (!wait_lean(&s.dp_full, g & 1, cta_abort, limit, AB_DP_FULL)) return false;
+            if (wg == 0 && p0 + row >= len) {
+              zero_tile_row(s.qring[st], row);
+              zero_tile_row(s.gring[st], row);
+            }
+            __syncwarp();
+            fence_proxy_async_smem();
+          }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t pk[16];
+            bool empty = false;
             if constexpr (kMasked) {
+              empty = __all_sync(0xffffffffu, words[c] == 0u);
+              if (!__all_sync(0xffffffffu, words[c] == ~0u)) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[c][e] = (words[c] & (1u << e)) ? v[c][e] : 0xff800000u;
+                for (int e = 0; e < 32; ++e) v[c][e] = (words[c] & (1u << e)) ? v[c][e] : 0xff800000u;
+              }
             }
+            if (kMasked && empty) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[c][e] = 0u;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) pk[e] = 0u;
+            } else {
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
               const float4 t = *reinterpret_cast<const float4*>(stat + 32 * c + 2 * e);
@@ -778,23 +817,12 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               pk[e] = pack2<kBf16>(w.x, w.y);
               pk[e + 1] = pack2<kBf16>(y.x, y.y);
             }
-            tmem_st16(s_tmem + 16 * c, pk);
-          }
-          tmem_wait_st();
-          // Query rows behind the sequence hold anything, and 0 * NaN is not 0: they become zero in Q and dO before
-          // the products that sum over them.  S^T and G^T, which read them as columns, are complete by then.
-          const bool stale = kMasked && p0 + 127 >= len && len < A.Nk;
-          if (stale) {
-            if (!wait_lean(&s.dp_full, g & 1, cta_abort, limit, AB_DP_FULL)) return false;
-            if (wg == 0 && p0 + row >= len) {
-              zero_tile_row(s.qring[st], row);
-              zero_tile_row(s.gring[st], row);
             }
-            __syncwarp();
-            fence_proxy_async_smem();
+            tmem_st16(s_tmem + 16 * c, pk);
+            tmem_wait_st();
+            tc_fence_before_sync();
+            mbar_arrive(c ? &s.p_ready : &s.p_half);
           }
-          tc_fence_before_sync();
-          mbar_arrive(&s.p_ready);
           if (!stale && !wait_lean(&s.dp_full, g & 1, cta_abort, limit, AB_DP_FULL)) return false;
           tc_fence_after_sync();
           uint32_t ga[16], gb[16];
@@ -809,7 +837,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                                                 f32x2_fma(f32x2(t.x, t.y), minus, f32x2(__uint_as_float(cur[2 * e]), __uint_as_float(cur[2 * e + 1])))));
               float2 d = f32x2_unpack(f32x2_mul(f32x2(__uint_as_float(pv[2 * e + 2]), __uint_as_float(pv[2 * e + 3])),
                                                 f32x2_fma(f32x2(t.z, t.w), minus, f32x2(__uint_as_float(cur[2 * e + 2]), __uint_as_float(cur[2 * e + 3])))));
-              if constexpr (kMasked) {
+              if (kMasked && stale) {          // (elsewhere G is finite, and 0 * G is 0)
                 const uint32_t m = words[c >> 1] >> (16 * (c & 1) + 2 * e);
                 a.x = (m & 1u) ? a.x : 0.f;
                 a.y = (m & 2u) ? a.y : 0.f;
