@@ -94,7 +94,7 @@ static int paged_splits(int B, int Hkv, int G, long long keys) {
   }
   long long n = full, most = (keys + 255) / 256;
   if (n > most) n = most;
-  return (int)(n > 128 ? 128 : n);
+  return (int)(n > kPagedMaxSplits ? kPagedMaxSplits : n);
 }
 static int paged_splits(const lucid_paged_attn_desc* d, bool lucid_step) {
   long long keys = (long long)d->cache.page_rows * d->cache.table_width;

@@ -13,7 +13,7 @@ namespace lucid {
 
 static __device__ Control g_append_ctl;
 
-constexpr int kApWarps = 4;
+constexpr int kApWarps = 4, kAhead = 4;
 
 // Last b with cu[b] <= tok < cu[b + 1], or -1 (behind the last sequence).  Whole warp; a 32-way search.
 __device__ __forceinline__ int find_sequence(const int* cu, int B, int tok, int lane) {
@@ -59,6 +59,29 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Appen
   const long long unit = (long long)blockIdx.x * kApWarps + warp;
   const int tok = (int)(unit / parts), part = (int)(unit % parts);
   if (tok >= args.T) return;
+  // rows of the token: Hkv keys, Hkv values, Hq queries; a lane's two pieces of its row in each of kAhead rounds are
+  // requested first, everything that says where they go and how they turn is worked out meanwhile
+  const int half = args.inv_freq ? args.rot / 16 : 0, l8 = lane & 7;
+  const bool turn = l8 < half;
+  const int ca = turn ? l8 : 2 * half + 2 * (l8 - half), cb = turn ? l8 + half : ca + 1;
+  const int nv = args.v ? args.Hkv : 0, rows = args.Hkv + nv + (args.q ? args.Hq : 0);
+  const int row0 = part * 4 + (lane >> 3), step = parts * 4;
+  auto source = [&](int r) -> const elem_t* {
+    if (r < args.Hkv) return reinterpret_cast<const elem_t*>(args.k) + tok * args.k_tok + r * args.k_head;
+    if (r < args.Hkv + nv) return reinterpret_cast<const elem_t*>(args.v) + tok * args.v_tok + (r - args.Hkv) * args.v_head;
+    return reinterpret_cast<const elem_t*>(args.q) + tok * args.q_tok + (r - args.Hkv - nv) * args.q_head;
+  };
+  uint4 x[kAhead], y[kAhead];
+  auto request = [&](int r) {
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      if (r + e * step >= rows) break;
+      const elem_t* src = source(r + e * step);
+      x[e] = *reinterpret_cast<const uint4*>(src + 8 * ca);
+      y[e] = *reinterpret_cast<const uint4*>(src + 8 * cb);
+    }
+  };
+  request(row0);
   const int b = args.cu ? find_sequence(args.cu, args.B, tok, lane) : tok;
   long long pos = -1;
   if (b >= 0) pos = (long long)__ldg(args.cache_lens + b) + (args.cu ? tok - __ldg(args.cu + b) : 0);
@@ -84,38 +107,26 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Appen
     }
   }
   __syncwarp();
-  // rows of the token: Hkv keys, Hkv values, Hq queries
-  const int half = args.inv_freq ? args.rot / 16 : 0, l8 = lane & 7;
-  const bool turn = l8 < half;
-  const int ca = turn ? l8 : 2 * half + 2 * (l8 - half), cb = turn ? l8 + half : ca + 1;
-  const int nv = args.v ? args.Hkv : 0, rows = args.Hkv + nv + (args.q ? args.Hq : 0);
-#pragma unroll 2
-  for (int r = part * 4 + (lane >> 3); r < rows; r += parts * 4) {
-    const elem_t* src;
-    elem_t* dst = nullptr;
-    bool rotated = turn;
-    if (r < args.Hkv) {
-      src = reinterpret_cast<const elem_t*>(args.k) + tok * args.k_tok + r * args.k_head;
-      if (ok) dst = reinterpret_cast<elem_t*>(c.k) + page * c.k_page + slot * c.k_row + r * c.k_head;
-    } else if (r < args.Hkv + nv) {
-      const int h = r - args.Hkv;
-      src = reinterpret_cast<const elem_t*>(args.v) + tok * args.v_tok + h * args.v_head;
-      if (ok) dst = reinterpret_cast<elem_t*>(c.v) + page * c.v_page + slot * c.v_row + h * c.v_head;
-      rotated = false;
-    } else {
-      const int h = r - args.Hkv - nv;
-      src = reinterpret_cast<const elem_t*>(args.q) + tok * args.q_tok + h * args.q_head;
-      dst = reinterpret_cast<elem_t*>(args.q_out) + ((long long)tok * args.Hq + h) * 128;
+  for (int r = row0; r < rows; r += kAhead * step) {
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const int re = r + e * step;
+      if (re >= rows) break;
+      elem_t* dst = nullptr;
+      if (re < args.Hkv) {
+        if (ok) dst = reinterpret_cast<elem_t*>(c.k) + page * c.k_page + slot * c.k_row + re * c.k_head;
+      } else if (re < args.Hkv + nv) {
+        if (ok) dst = reinterpret_cast<elem_t*>(c.v) + page * c.v_page + slot * c.v_row + (re - args.Hkv) * c.v_head;
+      } else {
+        dst = reinterpret_cast<elem_t*>(args.q_out) + ((long long)tok * args.Hq + re - args.Hkv - nv) * 128;
+      }
+      if (!dst) continue;
+      if (b < 0) x[e] = y[e] = make_uint4(0, 0, 0, 0);        // queries behind the last sequence come back as zeros
+      else if (turn && (re < args.Hkv || re >= args.Hkv + nv)) rotate_pieces<kBf16>(x[e], y[e], cs, ca, cb, args.interleaved != 0);
+      *reinterpret_cast<uint4*>(dst + 8 * ca) = x[e];
+      *reinterpret_cast<uint4*>(dst + 8 * cb) = y[e];
     }
-    if (!dst) continue;
-    uint4 x = make_uint4(0, 0, 0, 0), y = x;
-    if (b >= 0) {                                     // queries behind the last sequence come back as zeros
-      x = *reinterpret_cast<const uint4*>(src + 8 * ca);
-      y = *reinterpret_cast<const uint4*>(src + 8 * cb);
-      if (rotated) rotate_pieces<kBf16>(x, y, cs, ca, cb, args.interleaved != 0);
-    }
-    *reinterpret_cast<uint4*>(dst + 8 * ca) = x;
-    *reinterpret_cast<uint4*>(dst + 8 * cb) = y;
+    request(r + kAhead * step);
   }
 }
 

@@ -139,7 +139,43 @@ __global__ void __launch_bounds__(kPaWarps * 32, 2) paged_attn_kernel(const Page
     if (begin >= end) return;                                  // an empty chunk: the second kernel does not read it
   }
 
-  // ---- queries (and k_n) into shared memory, then into fragments ----
+  // ---- this warp's blocks: begin + (4 i + warp) * 16 ----
+  const int first = begin + warp * kPaKeys, stride = kPaWarps * kPaKeys;
+  const int blocks = first < end ? (end - first + stride - 1) / stride : 0;
+  uint8_t* ring = s.ring[warp][0];
+  auto load = [&](int i) {
+    const int st = i % kPaStages;
+    if (i < blocks) {
+      // lanes 0-15: the row of the cache of one key each
+      const int v = first + i * stride + (lane & 15);
+      long long page = -1;
+      int pos = 0;
+      if (v < end) {
+        pos = vis.pos(v);
+        page = page_of(c, b, pos);
+        if (page < 0 && lane < 16) report_error(&g_paged_ctl, kErrBadPage, b, pos, pos, 0);
+      }
+      const bool ok = page >= 0;
+      const long long slot = pos & ((1 << c.page_shift) - 1);
+      const long long ko = ok ? page * c.k_page + slot * c.k_row + hk * c.k_head : 0;
+      const long long vo = ok ? page * c.v_page + slot * c.v_row + hk * c.v_head : 0;
+      const unsigned mask = __ballot_sync(0xffffffffu, ok);
+      if (lane == 0) s.valid[warp][st] = mask & 0xffff;
+      const uint32_t dst = smem_u32(ring + st * kPaStageBytes);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int r = 2 * x + (lane >> 4), ch = lane & 15;
+        const long long kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+        const int bytes = (mask >> r) & 1 ? 16 : 0;
+        cp_async16(dst + row256(r, ch), reinterpret_cast<const elem_t*>(c.k) + kr + 8 * ch, bytes);
+        cp_async16(dst + kPaKeys * 256 + row256(r, ch), reinterpret_cast<const elem_t*>(c.v) + vr + 8 * ch, bytes);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kPaStages - 1; ++i) load(i);
+  // ---- queries (and k_n) into shared memory, then into fragments, while the first blocks are on their way ----
   for (int x = tid; x < 256; x += kPaWarps * 32) {
     const int r = x >> 4, ch = x & 15;
     uint4 w = make_uint4(0, 0, 0, 0);
@@ -181,42 +217,6 @@ __global__ void __launch_bounds__(kPaWarps * 32, 2) paged_attn_kernel(const Page
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
 
-  // ---- this warp's blocks: begin + (4 i + warp) * 16 ----
-  const int first = begin + warp * kPaKeys, stride = kPaWarps * kPaKeys;
-  const int blocks = first < end ? (end - first + stride - 1) / stride : 0;
-  uint8_t* ring = s.ring[warp][0];
-  auto load = [&](int i) {
-    const int st = i % kPaStages;
-    if (i < blocks) {
-      // lanes 0-15: the row of the cache of one key each
-      const int v = first + i * stride + (lane & 15);
-      long long page = -1;
-      int pos = 0;
-      if (v < end) {
-        pos = vis.pos(v);
-        page = page_of(c, b, pos);
-        if (page < 0 && lane < 16) report_error(&g_paged_ctl, kErrBadPage, b, pos, pos, 0);
-      }
-      const bool ok = page >= 0;
-      const long long slot = pos & ((1 << c.page_shift) - 1);
-      const long long ko = ok ? page * c.k_page + slot * c.k_row + hk * c.k_head : 0;
-      const long long vo = ok ? page * c.v_page + slot * c.v_row + hk * c.v_head : 0;
-      const unsigned mask = __ballot_sync(0xffffffffu, ok);
-      if (lane == 0) s.valid[warp][st] = mask & 0xffff;
-      const uint32_t dst = smem_u32(ring + st * kPaStageBytes);
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const int r = 2 * x + (lane >> 4), ch = lane & 15;
-        const long long kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-        const int bytes = (mask >> r) & 1 ? 16 : 0;
-        cp_async16(dst + row256(r, ch), reinterpret_cast<const elem_t*>(c.k) + kr + 8 * ch, bytes);
-        cp_async16(dst + kPaKeys * 256 + row256(r, ch), reinterpret_cast<const elem_t*>(c.v) + vr + 8 * ch, bytes);
-      }
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kPaStages - 1; ++i) load(i);
   for (int i = 0; i < blocks; ++i) {
     cp_async_wait<kPaStages - 2>();
     __syncwarp();
@@ -389,9 +389,10 @@ __global__ void __launch_bounds__(kPaWarps * 32, 2) paged_attn_kernel(const Page
 
 // ------------------------------------------------------------------------------------------------------------------
 // Joins the chunks of one row; LUCID: also of k_n's row, from which v'_n follows, and adds v'_n's own share.
-// One CTA per (query head of a key head, key head, sequence), four groups of 128 threads (one column each).
+// One CTA per (query head of a key head, key head, sequence), eight groups of 128 threads (one column each); LUCID: half of
+// them on k_n's row.
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int kJoinGroups = 4;
+constexpr int kJoinGroups = 8, kPaMaxSplits = kPagedMaxSplits;
 
 __device__ __forceinline__ float block_sum(float x, float* red) {       // 128 threads of one group use the result
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -404,44 +405,57 @@ __device__ __forceinline__ float block_sum(float x, float* red) {       // 128 t
   return (red[g] + red[g + 1]) + (red[g + 2] + red[g + 3]);
 }
 
-// maximum, sum and column `d` of a row's chunks; every thread returns the row's values for its column
-__device__ __forceinline__ void join_row(const float* p, int n, float& m, float& l, float& a, float (*red)[3][128]) {
-  const int d = threadIdx.x & 127, g = threadIdx.x >> 7;
-  m = -INFINITY;
-  l = a = 0.f;
-  for (int c = g; c < n; c += kJoinGroups) m = fmaxf(m, p[(long long)c * kPaRow + 128]);
-  const float z = m == -INFINITY ? 0.f : m;
-#pragma unroll 8
-  for (int c = g; c < n; c += kJoinGroups) {
-    const float f = ex2_approx(p[(long long)c * kPaRow + 128] - z);
-    l += f * p[(long long)c * kPaRow + 129];
-    a += f * p[(long long)c * kPaRow + d];
+// Maximum, sum and this thread's column of a row's chunks, joined by `groups` groups of 128 threads (this thread is in
+// group `g`; every thread of the CTA calls it with its own row).  w: this row's weights, red: the groups' sums.
+__device__ __forceinline__ void join_row(const float* p, int n, int g, int groups, float& m, float& l, float& a,
+                                         float* w, float (*red)[128], float* ml) {
+  const int d = threadIdx.x & 127, t = g * 128 + d, lane = threadIdx.x & 31;
+  // the chunks' maxima and sums, all at once; a warp of each row's first group joins them
+  if (t < n) {
+    w[t] = p[(long long)t * kPaRow + 128];
+    w[kPaMaxSplits + t] = p[(long long)t * kPaRow + 129];
   }
   __syncthreads();
-  red[g][0][d] = m;
-  red[g][1][d] = l;
-  red[g][2][d] = a;
-  __syncthreads();
-  float mm = -INFINITY;
+  if (t < 32) {
+    float mm = -INFINITY;
+    for (int c = lane; c < n; c += 32) mm = fmaxf(mm, w[c]);
 #pragma unroll
-  for (int x = 0; x < kJoinGroups; ++x) mm = fmaxf(mm, red[x][0][d]);
-  const float zz = mm == -INFINITY ? 0.f : mm;
-  l = a = 0.f;
+    for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+    const float z = mm == -INFINITY ? 0.f : mm;
+    float sum = 0.f;
+    for (int c = lane; c < n; c += 32) {
+      const float f = ex2_approx(w[c] - z);
+      w[c] = f;
+      sum += f * w[kPaMaxSplits + c];
+    }
 #pragma unroll
-  for (int x = 0; x < kJoinGroups; ++x) {
-    const float f = ex2_approx(red[x][0][d] - zz);
-    l += f * red[x][1][d];
-    a += f * red[x][2][d];
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (lane == 0) {
+      ml[0] = mm;
+      ml[1] = sum;
+    }
   }
-  m = mm;
+  __syncthreads();
+  float acc = 0.f;
+#pragma unroll 16
+  for (int c = g; c < n; c += groups) acc += w[c] * p[(long long)c * kPaRow + d];
+  red[g][d] = acc;
+  __syncthreads();
+  m = ml[0];
+  l = ml[1];
+  a = 0.f;
+  for (int x = 0; x < groups; ++x) a += red[x][d];
 }
 
 template <bool kBf16, bool kLucid>
 __global__ void __launch_bounds__(128 * kJoinGroups) paged_join_kernel(const PagedAttnArgs args) {
   typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
-  __shared__ float red[kJoinGroups][3][128];
+  constexpr int kRows = kLucid ? 2 : 1, kGroups = kJoinGroups / kRows;
+  __shared__ float red[kRows][kGroups][128];
+  __shared__ float weights[kRows][2 * kPaMaxSplits], ml[kRows][2], sums[kRows][128];
   __shared__ float red1[4 * kJoinGroups];
   const int row = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, d = threadIdx.x & 127;
+  const int which = (threadIdx.x >> 7) / kGroups, g = (threadIdx.x >> 7) % kGroups;     // which row this group joins
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int len = __ldg(args.lens + b);
   const Visible vis = visible(args, kLucid, len);
@@ -450,7 +464,7 @@ __global__ void __launch_bounds__(128 * kJoinGroups) paged_join_kernel(const Pag
   const int total = args.G + (kLucid ? 1 : 0);
   const float* part = args.partial + (((long long)b * args.Hkv + hk) * total) * args.splits * kPaRow;
   float m, l, a;
-  join_row(part + (long long)row * args.splits * kPaRow, n, m, l, a, red);
+  join_row(part + (long long)(which ? args.G : row) * args.splits * kPaRow, n, g, kGroups, m, l, a, weights[which], red[which], ml[which]);
   float o;
   if constexpr (!kLucid) {
     o = l != 0.f ? a / l : 0.f;
@@ -459,8 +473,12 @@ __global__ void __launch_bounds__(128 * kJoinGroups) paged_join_kernel(const Pag
     const long long page = len > 0 ? page_of(c, b, len - 1) : -1;
     const long long slot = len > 0 ? (len - 1) & ((1 << c.page_shift) - 1) : 0;
     if (len > 0 && page < 0 && threadIdx.x == 0) report_error(&g_paged_ctl, kErrBadPage, b, len - 1, len - 1, 0);
-    float km, kl, ka;
-    join_row(part + (long long)args.G * args.splits * kPaRow, n, km, kl, ka, red);
+    if (g == 0) sums[which][d] = a;
+    __syncthreads();
+    const float km = ml[1][0], ka = sums[1][d];
+    m = ml[0][0];
+    l = ml[0][1];
+    a = sums[0][d];
     o = 0.f;
     if (page >= 0) {                                           // (uniform in the CTA)
       const float kn = as_float(reinterpret_cast<const elem_t*>(c.k)[page * c.k_page + slot * c.k_row + hk * c.k_head + d]);
