@@ -78,14 +78,14 @@ static int check_rows(const void* p, const int64_t st[2], long long T, int H) {
 
 // How many chunks a sequence's keys are dealt out in, from what the host knows: the capacity of the block table, not the
 // lengths.  A cluster's worth (8, or what leaves a chunk 64 keys) where that fills the SMs or the keys are so few that a second launch
-// costs more than it gains; otherwise one wave of CTAs, two per SM.
+// costs more than it gains; otherwise one wave of CTAs.
 static int paged_splits(int B, int Hkv, int G, long long keys) {
   int sms = sm_count();
   if (sms <= 0) {
     (void)cudaGetLastError();
     sms = 148;
   }
-  const long long base = (long long)B * Hkv * ((G + 15) / 16), wave = 2ll * sms;
+  const long long base = (long long)B * Hkv * ((G + 15) / 16), wave = (long long)kPagedPerSm * sms;
   const long long full = (wave + base - 1) / base;
   if (full <= kPagedCluster || keys <= 4096) {
     int n = 1;
