@@ -14,6 +14,7 @@ enum : int { kErrBadPage = 4 };
 
 struct AttnFwdArgs {
   AttnShape a;
+  int split;              // items are single tiles of queries whose keys are split between the CTA's two halves
   const int* lengths;     // (B) valid positions, or null
   void* out;              // (B, Nq, Hq, 128)
   Strides out_strides;

@@ -38,7 +38,11 @@ struct FwdSlot {
     int from, to;         // and the entries from .. to-1
     int sink, lo, p_lo, p_hi;
   } t[2];
-  __device__ __forceinline__ int tile(int u) const { return u < sink ? 0 : lo + u - sink; }
+  __device__ __forceinline__ int tile(int u, bool split) const {
+    if (!split) return u < sink ? 0 : lo + u - sink;
+    const Tile& y = t[u & 1];
+    return (u >> 1) < y.sink ? 0 : y.lo + (u >> 1) - y.sink;
+  }
 };
 struct AttnFwdSmem {
   alignas(1024) uint8_t q[2][kTileBytes];
@@ -111,6 +115,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = s.tmem_base;
+  const bool split = args.split != 0;
   // The items of this CTA, one after another: `next` waits for the slot, `done` hands it back (per warp; whoever reads it
   // later keeps copies).
   uint32_t slots = 0;
@@ -163,7 +168,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             tma_load_4d(s.q[t] + kHalfBytes, &tm_q, &s.q_full[t], 64, it->t[t].block * kBlock, it->t[t].h, b);
           }
           for (int u = 0, n = it->n; u < n && alive; ++u) {
-            const int j = it->tile(u);
+            const int j = it->tile(u, split);
             alive = load(&tm_k, j) && load(&tm_v, j);
           }
           done(true);
@@ -177,7 +182,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const int k = rnd % kFwSlots;
           if (!wait_lean(&s.slot_free[k], ((rnd / kFwSlots) & 1) ^ 1, cta_abort, limit, AF_SLOT_FREE)) break;
           FwdSlot& x = s.slot[k];
-          const bool more = fwd_item(A, snake_item(rnd, blockIdx.x, gridDim.x), it);
+          const bool more = fwd_item(A, split, snake_item(rnd, blockIdx.x, gridDim.x), it);
           if (more) {
             x.len = attn_length(A, args.lengths, it.b);
             const PairTiles pt = pair_tiles(A, it, x.len);
@@ -188,7 +193,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             x.lo = pt.lo;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              const KeyTiles kt = pt.list(t);
+              const KeyTiles kt = split ? half_list(pt.x, t) : pt.list(t);
               FwdSlot::Tile& y = x.t[t];
               y.h = it.h(t);
               y.block = it.block(t);
@@ -309,7 +314,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const bool narrow0 = own_first && A.S <= kNarrow;       // (tile_narrow)
         int at = 0;
         for (int u = 0; u < n && alive; ++u) {
-          const bool act = (u == 0 && own_first) || (u >= from && u < to);
+          const bool act = split ? (u & 1) == t : (u == 0 && own_first) || (u >= from && u < to);
           alive = step(true, act, at == 0, at == own - 1, narrow0 && u == 0);
           if (act) ++at;
         }
@@ -335,17 +340,37 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll 1
       for (int t = 0; t < 2; ++t) {
         const int block = it->t[t].block, h = it->t[t].h;
-        if (block >= A.nqb) continue;
+        if (block >= A.nqb || (split && t)) continue;
         const bool has = it->t[t].n > 0;
         const int i = block * kBlock + row;
         float l = 0.f, ref = 0.f;
+        // split: the other half's sum and reference, and the factors that bring both halves to a common reference
+        const bool two = split && it->t[1].n > 0;
+        float f0 = 1.f, f1 = 0.f;
+        if (two) {
+          if (!wait_lean(&s.l_full[1], no1 & 1, cta_abort, limit, AF_L_FULL)) { alive = false; break; }
+          const float2 x = s.l[1][row];
+          mbar_arrive(&s.l_free[1]);
+          if (!wait_lean(&s.o_full[1], no1 & 1, cta_abort, limit, AF_O_FULL)) { alive = false; break; }
+          ++no1;
+          l = x.x;
+          ref = x.y;
+        }
         if (has) {
           const uint32_t n = t ? no1++ : no0++;
           if (!wait_lean(&s.l_full[t], n & 1, cta_abort, limit, AF_L_FULL)) { alive = false; break; }
           const float2 x = s.l[t][row];
-          l = x.x;
-          ref = x.y;
           mbar_arrive(&s.l_free[t]);
+          if (two) {
+            const float both = fmaxf(x.y, ref), z = both == -INFINITY ? 0.f : both;
+            f0 = ex2_approx(x.y - z);
+            f1 = ex2_approx(ref - z);
+            l = x.x * f0 + l * f1;
+            ref = both;
+          } else {
+            l = x.x;
+            ref = x.y;
+          }
           if (!wait_lean(&s.o_full[t], n & 1, cta_abort, limit, AF_O_FULL)) { alive = false; break; }
           tc_fence_after_sync();
         }
@@ -369,6 +394,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               *reinterpret_cast<uint4*>(panel + (c >> 2) * 4096 + sw128_off(lane, 2 * (c & 3) + e)) = w;
             }
           };
+          if (two) {
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              tmem_ld16(o_tmem + 16 * c, oa);
+              tmem_ld16(o_tmem + 128 + 16 * c, ob);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) oa[e] = __float_as_uint(__uint_as_float(oa[e]) * f0 + __uint_as_float(ob[e]) * f1);
+              put(oa, c);
+            }
+            tc_fence_before_sync();
+            mbar_arrive(&s.o_free[0]);
+            mbar_arrive(&s.o_free[1]);
+          } else {
           tmem_ld16(o_tmem, oa);
           tmem_wait_ld();
 #pragma unroll 1
@@ -384,6 +423,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             }
             put(ob, c + 1);
             if (c < 6) tmem_wait_ld();
+          }
           }
         }
         __syncwarp();
@@ -437,7 +477,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (masked) {
           if (j0 + 127 >= len && len < A.Nk) {
             // rows behind the sequence hold anything, and 0 * NaN is not 0: the value tile's become zero
-            const uint32_t use = r + 2 * (tile == 0 && u_sink ? 0 : tile - u_lo + u_sink) + 1;
+            const uint32_t use = r + 2 * (split ? 2 * x + t : tile == 0 && u_sink ? 0 : tile - u_lo + u_sink) + 1;
             if (!wait_lean(&s.full[use % kFwRing], (use / kFwRing) & 1, cta_abort, limit, AF_FULL)) {
               alive = false;
               break;
@@ -561,7 +601,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
 cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                             const AttnFwdArgs& args, int sms, cudaStream_t stream) {
-  const int items = fwd_items(args.a), grid = items < sms ? items : sms;
+  const int items = fwd_items(args.a, args.split != 0), grid = items < sms ? items : sms;
   const int bytes = (int)sizeof(AttnFwdSmem);
   auto kernel = bf16 ? attn_fwd_kernel<true> : attn_fwd_kernel<false>;
   static SmemOnce once[2];

@@ -95,7 +95,8 @@ LUCID_HD ColMask col_mask(const AttnShape& a, int j, int p0, int len) {
 // Forward work item: two tiles of 128 queries that read the same keys.  With an even number of query heads per key
 // head they are two heads of one block of rows (same keys exactly), otherwise two neighbouring blocks of one head.
 LUCID_HD bool pair_heads(const AttnShape& a) { return (a.G & 1) == 0; }
-LUCID_HD int fwd_items(const AttnShape& a) {
+LUCID_HD int fwd_items(const AttnShape& a, bool split) {
+  if (split) return a.B * a.Hq * a.nqb;
   return pair_heads(a) ? a.B * (a.Hq / 2) * a.nqb : a.B * a.Hq * ((a.nqb + 1) / 2);
 }
 // The item that CTA `cta` of `grid` takes in its round `r`: back and forth, so that the CTAs that got the longest items of
@@ -107,10 +108,15 @@ struct FwdItem {
   LUCID_HD int h(int k) const { return k ? h1 : h0; }
   LUCID_HD int block(int k) const { return k ? block1 : block0; }
 };
-LUCID_HD bool fwd_item(const AttnShape& a, int idx, FwdItem& it) {
-  if (idx >= fwd_items(a)) return false;
+LUCID_HD bool fwd_item(const AttnShape& a, bool split, int idx, FwdItem& it) {
+  if (idx >= fwd_items(a, split)) return false;
   // blocks from the last to the first (under full causality the last ones take longest), heads side by side
-  if (pair_heads(a)) {
+  if (split) {
+    const int per = a.B * a.Hq, r = idx % per;
+    it.b = r / a.Hq;
+    it.h0 = it.h1 = r % a.Hq;
+    it.block0 = it.block1 = a.nqb - 1 - idx / per;
+  } else if (pair_heads(a)) {
     const int per = a.B * (a.Hq / 2);
     const int blk = a.nqb - 1 - idx / per, r = idx % per;
     it.b = r / (a.Hq / 2);
@@ -127,6 +133,20 @@ LUCID_HD bool fwd_item(const AttnShape& a, int idx, FwdItem& it) {
   }
   it.hk = it.h0 / a.G;
   return true;
+}
+// With fewer such pairs than SMs the item is ONE tile of queries, and its list is split: the first half goes to tile 0, the
+// rest to tile 1, entries of the two in turn; their results are joined at the end.
+LUCID_HD KeyTiles half_list(const KeyTiles& t, int k) {
+  KeyTiles h = t;
+  const int n0 = (t.n + 1) / 2;
+  h.n = k ? t.n - n0 : n0;
+  if (k) {
+    h.sink = 0;
+    h.lo = t.n > 0 ? t.tile(n0) : 0;
+  } else if (h.n == 0) {
+    h.sink = 0;
+  }
+  return h;
 }
 // The union of the two tiles' lists, in increasing order; `active` says which of the two visits an entry.
 struct PairTiles {

@@ -47,7 +47,7 @@ static int check(const AttnShape& a, const std::vector<int>& lens) {
   std::vector<int> tiles((size_t)a.B * a.Hq * a.nqb, 0);
   FwdItem it;
   int n = 0;
-  for (; fwd_item(a, n, it); ++n) {
+  for (; fwd_item(a, false, n, it); ++n) {
     if (it.b < 0 || it.b >= a.B || it.hk != it.h(0) / a.G || it.hk != it.h(1) / a.G) return 4;
     const PairTiles pt = pair_tiles(a, it, lens[it.b]);
     for (int k = 0; k < 2; ++k) {
@@ -63,7 +63,20 @@ static int check(const AttnShape& a, const std::vector<int>& lens) {
       if (at != t.n) return 7;
     }
   }
-  if (n != fwd_items(a)) return 8;
+  if (n != fwd_items(a, false)) return 8;
+  // split items: every (b, head, block) once, the halves one after the other make the list, tile 0's first
+  std::vector<int> halves((size_t)a.B * a.Hq * a.nqb, 0);
+  for (n = 0; fwd_item(a, true, n, it); ++n) {
+    if (it.hk != it.h(0) / a.G || it.h(0) != it.h(1) || it.block(0) != it.block(1)) return 19;
+    ++halves[((size_t)it.b * a.Hq + it.h(0)) * a.nqb + it.block(0)];
+    const KeyTiles t = key_tiles(a, it.block(0), lens[it.b]), x = half_list(t, 0), y = half_list(t, 1);
+    if (x.n + y.n != t.n || x.n < y.n || x.n > y.n + 1) return 20;
+    for (int e = 0; e < t.n; ++e)
+      if ((e < x.n ? x.tile(e) : y.tile(e - x.n)) != t.tile(e)) return 21;
+  }
+  if (n != fwd_items(a, true)) return 22;
+  for (int v : halves)
+    if (v != 1) return 23;
   for (int x : tiles)
     if (x != 1) return 9;
   // by keys: dK/dV's items

@@ -215,6 +215,12 @@ SHAPES = [
     (1, 2300, 2300, 2, 1, 250, 9),
     (1, 260, 260, 2, 1, 0, 2),        # first keys only
     (1, 200, 200, 2, 1, 0, 0),        # nothing visible
+    # more tiles of queries than SMs: two tiles to an item, several items to a CTA
+    (3, 500, 500, 16, 4, 130, 5),
+    (3, 500, 500, 15, 5, 200, 100),
+    (2, 1000, 1100, 10, 10, None, 0),
+    (1, 2500, 2500, 24, 8, 600, 4),
+    (2, 2500, 2500, 16, 4, 300, 33),
 ]
 
 
@@ -239,12 +245,13 @@ def test_window_attention_forward_and_backward(shape, dt):
 
 
 @gpu
+@pytest.mark.parametrize("Hq,Hkv", [(4, 2), (5, 1), (1, 1)])
 @pytest.mark.parametrize("window,sinks,Nq", [(200, 4, 600), (None, 0, 600), (64, 128, 350), (0, 3, 600)])
-def test_padded_batch_ignores_whatever_stands_behind_the_sequences(window, sinks, Nq):
+def test_padded_batch_ignores_whatever_stands_behind_the_sequences(window, sinks, Nq, Hq, Hkv):
     """Lengths from nothing to all, NaN and infinities in every padded position of every input."""
     from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
 
-    dt, Nk, Hq, Hkv = torch.bfloat16, 600, 4, 2
+    dt, Nk = torch.bfloat16, 600
     lens = [600, 0, 1, 127, 128, 129, 257, 599, 300]
     B = len(lens)
     q, k, v, do = make(B, Nq, Nk, Hq, Hkv, dt, seed=3)
