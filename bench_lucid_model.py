@@ -13,6 +13,12 @@ Everything around the LUCID solve is plain PyTorch (cuBLAS GEMMs, torch SDPA): p
 in both variants, so that the difference between the two is the cost of the solve and its call-site glue.
 
     python bench_lucid_model.py [--seqlens 2048 8192 32768 65536] [--iters 5] [--vprime-residency]
+                                [--attention kernels] [--decode-tokens 64]
+
+With --attention kernels the attention of all layers runs on this package's kernels (window_attention) instead of
+torch SDPA.  --decode-tokens T also generates T tokens after each prompt through a paged key/value cache
+(paged_append, paged_window_attention; in LUCID layers paged_lucid_attention, which extends the solve by a row) and
+prints a line with the time per token.
 
 Prints one JSON line per sequence length: tokens/s of both variants and the LUCID overhead.  With
 --vprime-residency it also times, per sequence length, a global layer's attention call straight after the
@@ -79,6 +85,25 @@ def sliding_window_attention(q, k, v, window):
     return torch.cat((first, rest), dim=2)
 
 
+class KVCache:
+    """Paged keys and values of every layer for B sequences of up to `capacity` positions.  A sequence's pages lie one
+    after another here, so that its prompt is also a plain (B, N, heads, D) view of the pool."""
+
+    def __init__(self, B, capacity, device, dtype=torch.bfloat16, page=64):
+        c = CFG
+        self.B, self.page, self.per = B, page, -(-capacity // page)
+        pool = (B * self.per, page, c["kv_heads"], c["head_dim"])
+        self.k = [torch.zeros(pool, device=device, dtype=dtype) for _ in range(c["layers"])]
+        self.v = [torch.zeros(pool, device=device, dtype=dtype) for _ in range(c["layers"])]
+        self.table = torch.arange(B * self.per, device=device, dtype=torch.int32).reshape(B, self.per)
+        self.lens = torch.zeros(B, device=device, dtype=torch.int32)
+        D = c["head_dim"]
+        self.inv_freq = c["rope_base"] ** (-torch.arange(0, D // 2, device=device, dtype=torch.float32) / (D // 2))
+
+    def rows(self, pool, N):
+        return pool.view(self.B, self.per * self.page, *pool.shape[2:])[:, :N]
+
+
 class Model:
     def __init__(self, device, dtype=torch.bfloat16, seed=0):
         g = torch.Generator(device=device)
@@ -98,11 +123,72 @@ class Model:
                 wgu=w(2 * c["mlp"], c["hidden"]), wd=w(c["hidden"], c["mlp"])))
         self.norm = torch.ones(c["hidden"], device=device, dtype=dtype)
 
+    def _mlp(self, L, x):
+        h = rms_norm(x, L["n2"])
+        gate, up = (h @ L["wgu"].T).split(CFG["mlp"], dim=-1)
+        return x + (F.gelu(gate, approximate="tanh") * up) @ L["wd"].T
+
     @torch.no_grad()
-    def prefill(self, ids, lucid: bool, tap=None):
-        """Returns the last position's logits.  `lucid`: apply the LUCID solve to K/V of the global layers.
+    def prefill_cached(self, ids, lucid: bool, cache: KVCache):
+        """The prompt through the cache (empty before): keys are rotated into it, LUCID layers keep V' there.  Returns
+        the last position's logits."""
+        from lucid_kernels_b200 import paged_append, window_attention
+        from lucid_kernels_b200.cute import _forward_sub_fwd
+
+        c = CFG
+        B, N = ids.shape
+        D, Hq, Hkv = c["head_dim"], c["q_heads"], c["kv_heads"]
+        x = self.embed[ids] * math.sqrt(c["hidden"])
+        cu = torch.arange(B + 1, device=ids.device, dtype=torch.int32) * N
+        for li, L in enumerate(self.layers):
+            is_global = (li + 1) % c["global_every"] == 0
+            qkv = (rms_norm(x, L["n1"]) @ L["wqkv"].T).view(B * N, Hq + 2 * Hkv, D)
+            q, k, v = qkv.split((Hq, Hkv, Hkv), dim=1)
+            solve = is_global and lucid
+            q = paged_append(k, None if solve else v, cache.k[li], cache.v[li], cache.table, cache.lens, cu_seqlens=cu, q=q,
+                             inv_freq=cache.inv_freq).view(B, N, Hq, D)
+            k, v = cache.rows(cache.k[li], N), v.view(B, N, Hkv, D)
+            if solve:
+                ks = D ** -0.25
+                v = _forward_sub_fwd(k, v, k_scale=ks)
+                cache.rows(cache.v[li], N).copy_(v)
+                a = window_attention(q, k, v, scale=ks / math.sqrt(D))
+            else:
+                a = window_attention(q, k, v, window=None if is_global else c["window"])
+            x = self._mlp(L, x + a.reshape(B, N, Hq * D) @ L["wo"].T)
+        cache.lens += N
+        return rms_norm(x[:, -1], self.norm) @ self.embed.T
+
+    @torch.no_grad()
+    def decode(self, ids, lucid: bool, cache: KVCache):
+        """One token per sequence, ids (B,): appends it to the cache and returns the next token's logits."""
+        from lucid_kernels_b200 import paged_append, paged_lucid_attention, paged_window_attention
+
+        c = CFG
+        B = ids.shape[0]
+        D, Hq, Hkv = c["head_dim"], c["q_heads"], c["kv_heads"]
+        x = self.embed[ids] * math.sqrt(c["hidden"])
+        now = cache.lens + 1
+        for li, L in enumerate(self.layers):
+            is_global = (li + 1) % c["global_every"] == 0
+            q, k, v = (rms_norm(x, L["n1"]) @ L["wqkv"].T).view(B, Hq + 2 * Hkv, D).split((Hq, Hkv, Hkv), dim=1)
+            kc, vc, solve = cache.k[li], cache.v[li], is_global and lucid
+            q = paged_append(k, None if solve else v, kc, vc, cache.table, cache.lens, q=q, inv_freq=cache.inv_freq)
+            if solve:
+                ks = D ** -0.25
+                a = paged_lucid_attention(q, v, kc, vc, cache.table, now, k_scale=ks, scale=ks / math.sqrt(D))
+            else:
+                a = paged_window_attention(q, kc, vc, cache.table, now, window=None if is_global else c["window"])
+            x = self._mlp(L, x + a.reshape(B, Hq * D) @ L["wo"].T)
+        cache.lens.copy_(now)
+        return rms_norm(x, self.norm) @ self.embed.T
+
+    @torch.no_grad()
+    def prefill(self, ids, lucid: bool, tap=None, attention="torch"):
+        """Returns the last position's logits.  `attention`: torch SDPA, or this package's `kernels`.  `lucid`: apply the LUCID solve to K/V of the global layers.
         `tap`: a list that receives (layer index, k, v, v_prime, k_scale) of every solve, k and v being the
         BSHD views handed to it."""
+        from lucid_kernels_b200 import window_attention
         from lucid_kernels_b200.cute import _forward_sub_fwd
 
         c = CFG
@@ -134,7 +220,12 @@ class Model:
                         tap.append((li, k.transpose(1, 2), v.transpose(1, 2), v_prime, ks))
                     v = v_prime.transpose(1, 2)
                     scale = ks / math.sqrt(D)                          # q . (ks k) / sqrt(d)
-                a = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True, scale=scale)
+                if attention == "kernels":
+                    a = window_attention(*(t.transpose(1, 2) for t in (q, k, v)), scale=scale).transpose(1, 2)
+                else:
+                    a = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True, scale=scale)
+            elif attention == "kernels":
+                a = window_attention(*(t.transpose(1, 2) for t in (q, k, v)), window=c["window"]).transpose(1, 2)
             else:
                 a = sliding_window_attention(q, k, v, c["window"])
             x = x + a.transpose(1, 2).reshape(B, N, Hq * D) @ L["wo"].T
@@ -182,11 +273,34 @@ def vprime_residency_probe(N, dev, iters=10):
                 hbm_round_trip_ms_at_6_5_TBps=2 * vp_bytes / 6.5e12 * 1e3)
 
 
+@torch.no_grad()
+def decode_probe(model, ids, tokens):
+    """Milliseconds per generated token after the prompt `ids`, all-softmax and LUCID."""
+    res = {}
+    B, N = ids.shape
+    for name, lucid in (("softmax", False), ("lucid", True)):
+        cache = KVCache(B, N + tokens + 8, ids.device)
+        out = model.prefill_cached(ids, lucid, cache)
+        for _ in range(4):
+            out = model.decode(out.argmax(-1), lucid, cache)
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        torch.cuda.synchronize()
+        a.record()
+        for _ in range(tokens):
+            out = model.decode(out.argmax(-1), lucid, cache)
+        b.record()
+        torch.cuda.synchronize()
+        res[name] = dict(ms_per_token=a.elapsed_time(b) / tokens, finite=bool(torch.isfinite(out.float()).all()))
+    return dict(seqlen=N, batch=B, tokens=tokens, **res)
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--seqlens", type=int, nargs="+", default=[2048, 8192, 32768, 65536])
     ap.add_argument("--iters", type=int, default=5)
     ap.add_argument("--vprime-residency", action="store_true")
+    ap.add_argument("--attention", choices=("torch", "kernels"), default="torch")
+    ap.add_argument("--decode-tokens", type=int, default=0)
     args = ap.parse_args()
     assert torch.cuda.is_available(), "needs a CUDA device"
     dev = torch.device("cuda", 0)
@@ -197,14 +311,14 @@ def main():
         ids = torch.randint(0, CFG["vocab"], (1, N), device=dev, generator=g)
         res = {}
         for lucid in (False, True, False, True):      # warm both variants before either is timed
-            model.prefill(ids, lucid)
+            model.prefill(ids, lucid, attention=args.attention)
         for name, lucid in (("softmax", False), ("lucid", True)):
-            model.prefill(ids, lucid)
+            model.prefill(ids, lucid, attention=args.attention)
             torch.cuda.synchronize()
             a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             a.record()
             for _ in range(args.iters):
-                out = model.prefill(ids, lucid)
+                out = model.prefill(ids, lucid, attention=args.attention)
             b.record()
             torch.cuda.synchronize()
             ms = a.elapsed_time(b) / args.iters
@@ -213,9 +327,12 @@ def main():
         print(json.dumps(dict(metric="prefill_tok_s", seqlen=N, batch=1, dtype="bf16", data="synthetic",
                               config="Gemma-3-4B-style: 34 layers (5 global + LUCID, 29 sliding window 1024), "
                                      "hidden 2560, 8q/4kv heads, d 128, GeGLU 10240, vocab 262144",
-                              softmax=res["softmax"], lucid=res["lucid"], lucid_overhead=over)), flush=True)
+                              attention=args.attention, softmax=res["softmax"], lucid=res["lucid"], lucid_overhead=over)),
+              flush=True)
         if args.vprime_residency:
             print(json.dumps(dict(metric="vprime_residency", **vprime_residency_probe(N, dev))), flush=True)
+        if args.decode_tokens:
+            print(json.dumps(dict(metric="decode_ms_per_token", **decode_probe(model, ids, args.decode_tokens))), flush=True)
 
 
 if __name__ == "__main__":
