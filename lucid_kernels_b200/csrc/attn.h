@@ -2,6 +2,7 @@
 // cache's kernels (paged_append.cu, paged_attn.cu).
 #pragma once
 #include <atomic>
+#include <utility>
 
 #include "attn_geometry.h"
 #include "common.cuh"
@@ -33,6 +34,7 @@ struct AttnBwdArgs {
   Strides dk_strides, dv_strides;
   float* partial;         // (B * Hkv, 1 + chunks, 2, S, 128) fp32 sums of the first keys' rows {dK, dV}
   int chunks;
+  int after_dq;           // dK/dV: launched behind the dQ kernel (else behind the statistics)
   float scale, scale_log2;
   unsigned long long wait_ns;
 };
@@ -74,6 +76,22 @@ struct SmemOnce {
     return e;
   }
 };
+
+// A launch that may begin before the kernel in front of it has ended (the kernel itself waits for what it needs).
+template <class... P, class... A>
+inline cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, int bytes, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
 
 // For the source files' own status records.
 inline cudaError_t take_status(const void* symbol, cudaStream_t stream, int out[8]) {

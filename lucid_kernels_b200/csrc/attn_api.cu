@@ -195,6 +195,7 @@ int lucid_window_attn_bwd(const lucid_window_attn_desc* d, const void* q, const 
     if ((e = launch_attn_dq(bf16, tm_q, tm_k, tm_v, tm_do, args, sms, stream)) != cudaSuccess) return (int)e;
   }
   if (dk) {
+    args.after_dq = dq ? 1 : 0;
     args.dk = dk;
     args.dv = dv;
     args.dk_strides = Strides{d->dk_strides[0], d->dk_strides[1], d->dk_strides[2]};

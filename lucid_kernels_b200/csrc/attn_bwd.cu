@@ -19,6 +19,7 @@ static __device__ Control g_attn_bwd_ctl;
 template <bool kBf16>
 __global__ void __launch_bounds__(256) attn_stat_kernel(const AttnStatArgs args) {
   typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
+  launch_dependents();
   const AttnShape& A = args.a;
   const int lane = threadIdx.x & 31;
   const int rows = A.nqb * kBlock;                       // padded rows per head
@@ -233,6 +234,10 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  // The statistics' kernel may still be running until here.  From here on the dK/dV kernel, which needs them too but
+  // nothing of this one, may take SMs that have no items left.
+  wait_for_primary();
+  launch_dependents();
   const uint32_t tmem = s.tmem_base;
   constexpr int fmt = kBf16 ? 1 : 0;
   constexpr uint32_t idesc_kk = umma_idesc(fmt, 0, 0, 128, 128);
@@ -506,8 +511,7 @@ cudaError_t launch_attn_dq(bool bf16, const CUtensorMap& tm_q, const CUtensorMap
   static SmemOnce once[2];
   cudaError_t e = once[bf16].set(reinterpret_cast<const void*>(kernel), bytes);
   if (e != cudaSuccess) return e;
-  kernel<<<grid, kBwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, tm_do, args);
-  return cudaGetLastError();
+  return launch_early(kernel, dim3(grid), kBwThreads, bytes, stream, tm_q, tm_k, tm_v, tm_do, args);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -590,6 +594,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  if (!args.after_dq) wait_for_primary();
+  launch_dependents();
   const uint32_t tmem = s.tmem_base;
   constexpr int fmt = kBf16 ? 1 : 0;
   constexpr uint32_t idesc_kk = umma_idesc(fmt, 0, 0, 128, 128);
@@ -913,6 +919,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     }
   }
 
+  if (args.after_dq) wait_for_primary();       // what follows this kernel follows the dQ kernel as well
   if (s.abort_flag) {
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
@@ -927,6 +934,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 template <bool kBf16>
 __global__ void __launch_bounds__(128) attn_first_keys_kernel(const AttnBwdArgs args) {
   typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
+  wait_for_primary();
   const AttnShape& A = args.a;
   const int j = blockIdx.x, which = blockIdx.y, bh = blockIdx.z, b = bh / A.Hkv, hk = bh % A.Hkv;
   const float* p = args.partial + (((long long)bh * (1 + args.chunks) * 2 + which) * A.S + j) * 128 + threadIdx.x;
@@ -949,12 +957,10 @@ cudaError_t launch_attn_dkv(bool bf16, const CUtensorMap& tm_q, const CUtensorMa
   static SmemOnce once[2];
   cudaError_t e = once[bf16].set(reinterpret_cast<const void*>(kernel), bytes);
   if (e != cudaSuccess) return e;
-  kernel<<<grid, kBwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, tm_do, args);
-  if ((e = cudaGetLastError()) != cudaSuccess || args.chunks == 0) return e;
+  e = launch_early(kernel, dim3(grid), kBwThreads, bytes, stream, tm_q, tm_k, tm_v, tm_do, args);
+  if (e != cudaSuccess || args.chunks == 0) return e;
   const dim3 sum_grid(a.S < a.Nk ? a.S : a.Nk, 2, a.B * a.Hkv);
-  if (bf16) attn_first_keys_kernel<true><<<sum_grid, 128, 0, stream>>>(args);
-  else attn_first_keys_kernel<false><<<sum_grid, 128, 0, stream>>>(args);
-  return cudaGetLastError();
+  return launch_early(bf16 ? attn_first_keys_kernel<true> : attn_first_keys_kernel<false>, sum_grid, 128, 0, stream, args);
 }
 
 cudaError_t attn_bwd_status(cudaStream_t stream, int out[8]) { return take_status(&g_attn_bwd_ctl, stream, out); }

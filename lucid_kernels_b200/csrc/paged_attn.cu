@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, kPagedPerSm) paged_attn_kernel(
   const int chunk = chunk_keys(vis.n, args.splits);
   const int begin = split * chunk, end = imin(vis.n, begin + chunk);
   if constexpr (!kCluster) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    launch_dependents();
     if (begin >= end) return;                                  // an empty chunk: the second kernel does not read it
   }
 
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(128 * kJoinGroups) paged_join_kernel(const Pag
   __shared__ float red1[4 * kJoinGroups];
   const int row = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, d = threadIdx.x & 127;
   const int which = (threadIdx.x >> 7) / kGroups, g = (threadIdx.x >> 7) % kGroups;     // which row this group joins
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_primary();
   const int len = __ldg(args.lens + b);
   const Visible vis = visible(args, kLucid, len);
   const int chunk = chunk_keys(vis.n, args.splits);

@@ -34,6 +34,11 @@ __device__ __forceinline__ bool elect_one() {
   return pred != 0;
 }
 
+// Programmatic dependent launch: let the next kernel's CTAs start as soon as there is room / wait until the kernel before
+// is complete and its writes are visible (returns at once in a kernel launched without that attribute).
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------------------------
 // mbarrier (CTA-local shared memory)
 // ---------------------------------------------------------------------------------------------
