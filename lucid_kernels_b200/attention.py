@@ -35,6 +35,13 @@ _D = 128
 _DTYPES = (torch.float16, torch.bfloat16)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _device_now = torch._C._cuda_getDevice
+_grad_enabled = torch.is_grad_enabled
+_empty, _empty_like, _uint8 = torch.empty, torch.empty_like, torch.uint8
+_increment_version = torch.autograd.graph.increment_version
+
+
+def _new_like(t: torch.Tensor) -> torch.Tensor:
+    return _empty_like(t) if t.is_contiguous() else _empty_like(t, memory_format=torch.contiguous_format)
 
 
 class _Plan:
@@ -84,9 +91,6 @@ def _contiguous_strides(*shape):
     return (ctypes.c_int64 * len(st))(*st)
 
 
-def _finish(check: Optional[bool], stream: int, what: str) -> None:
-    if _CHECK_DEFAULT if check is None else check:
-        _cabi.raise_on_attention_error(stream, what)
 
 
 def _scale(scale: Optional[float]) -> float:
@@ -170,7 +174,7 @@ def _window_attention_fwd(q, k, v, window: Optional[int] = None, sinks: int = 0,
     if _device_now() != plan.device:
         with torch.cuda.device(plan.device):
             return _window_attention_fwd(q, k, v, window, sinks, scale, lengths, need_lse=need_lse, check=check)
-    out = torch.empty_like(q, memory_format=torch.contiguous_format, requires_grad=False)
+    out = _new_like(q)
     lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=q.device) if need_lse else None
     if plan.empty:
         return out, lse
@@ -179,7 +183,8 @@ def _window_attention_fwd(q, k, v, window: Optional[int] = None, sinks: int = 0,
                                             None if lengths is None else lengths.data_ptr(), stream)
     if rc:
         _cabi.check_rc(rc, "lucid_window_attn_fwd")
-    _finish(check, stream, "_window_attention_fwd")
+    if check or (check is None and _CHECK_DEFAULT):
+        _cabi.raise_on_attention_error(stream, "_window_attention_fwd")
     return out, lse
 
 
@@ -205,18 +210,19 @@ def _window_attention_bwd(q, k, v, out, lse, dout, window: Optional[int] = None,
         with torch.cuda.device(plan.device):
             return _window_attention_bwd(q, k, v, out, lse, dout, window, sinks, scale, lengths, need_dq=need_dq, need_dkv=need_dkv,
                                          check=check)
-    dq = torch.empty_like(q, memory_format=torch.contiguous_format, requires_grad=False) if need_dq else None
-    dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format, requires_grad=False) if need_dkv else None for t in (k, v))
+    dq = _new_like(q) if need_dq else None
+    dk, dv = (_new_like(t) if need_dkv else None for t in (k, v))
     if plan.empty:
         return dq, dk if dk is None else dk.zero_(), dv if dv is None else dv.zero_()
-    ws = torch.empty(plan.workspace, dtype=torch.uint8, device=q.device)
+    ws = _empty(plan.workspace, dtype=_uint8, device=q.device)
     stream = _raw_stream(plan.device)
     rc = _cabi.load().lucid_window_attn_bwd(plan.ref, qp, kp, vp, op, lse.data_ptr(), gp, None if dq is None else dq.data_ptr(),
                                             None if dk is None else dk.data_ptr(), None if dv is None else dv.data_ptr(),
                                             None if lengths is None else lengths.data_ptr(), ws.data_ptr(), plan.workspace, stream)
     if rc:
         _cabi.check_rc(rc, "lucid_window_attn_bwd")
-    _finish(check, stream, "_window_attention_bwd")
+    if check or (check is None and _CHECK_DEFAULT):
+        _cabi.raise_on_attention_error(stream, "_window_attention_bwd")
     return dq, dk, dv
 
 
@@ -254,7 +260,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     Differentiable in q, k and v (once); gradients come out the same on every run.  In a training step recorded into a CUDA
     graph, record forward and backward together and, as torch asks for every operator, keep no eager graph of the same
     leaves alive while recording."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return LUCIDWindowAttention.apply(q, k, v, window, sinks, scale, lengths)
     return _window_attention_fwd(q, k, v, window, sinks, scale, lengths, need_lse=False)[0]
 
@@ -283,9 +289,7 @@ def _cache_desc(k_cache, v_cache, block_table, B: int, tensors):
     return _cabi.PagedCacheDesc(pages, page, width, width if B == 1 else block_table.stride(0), _strides(k_cache), _strides(v_cache)), copy
 
 
-def _no_gradients(*tensors) -> None:
-    if torch.is_grad_enabled():
-        assert not any(t is not None and t.requires_grad for t in tensors), "the cache operators have no backward: use torch.no_grad()"
+_NO_BACKWARD = "the cache operators have no backward: use torch.no_grad()"
 
 
 def _cache_pointers(k_cache, v_cache):
@@ -347,7 +351,9 @@ def paged_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tens
     plan = _plans.get(key)
     if plan is None:
         plan = _append_plan(key, k, v, k_cache, v_cache, block_table, cache_lens, cu_seqlens, q, inv_freq, interleaved)
-    _no_gradients(k, v, q, k_cache, v_cache)
+    if _grad_enabled():
+        assert not (k.requires_grad or (v is not None and v.requires_grad) or (q is not None and q.requires_grad) or
+                    k_cache.requires_grad or v_cache.requires_grad), _NO_BACKWARD
     kp, vp, qp = k.data_ptr(), None if v is None else v.data_ptr(), None if q is None else q.data_ptr()
     if plan.copy or (kp | (vp or 0) | (qp or 0)) & 15:
         own = lambda t: None if t is None else t.contiguous()
@@ -357,7 +363,7 @@ def paged_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tens
     if _device_now() != plan.device:
         with torch.cuda.device(plan.device):
             return paged_append(k, v, k_cache, v_cache, block_table, cache_lens, cu_seqlens, q, inv_freq, interleaved, check=check)
-    q_out = None if q is None else torch.empty_like(q, memory_format=torch.contiguous_format)
+    q_out = None if q is None else _new_like(q)
     if plan.empty:
         return q_out if q_out is None else q_out.zero_()
     stream = _raw_stream(plan.device)
@@ -366,8 +372,9 @@ def paged_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tens
                                          None if inv_freq is None else inv_freq.data_ptr(), stream)
     if rc:
         _cabi.check_rc(rc, "lucid_paged_append")
-    torch.autograd.graph.increment_version([k_cache] if v is None else [k_cache, v_cache])
-    _finish(check, stream, "paged_append")
+    _increment_version([k_cache] if v is None else [k_cache, v_cache])
+    if check or (check is None and _CHECK_DEFAULT):
+        _cabi.raise_on_attention_error(stream, "paged_append")
     return q_out
 
 
@@ -408,7 +415,8 @@ def paged_window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     plan = _plans.get(key)
     if plan is None:
         plan = _step_plan(key, q, None, k_cache, v_cache, block_table, seq_lens, window, sinks, scale, 1.0)
-    _no_gradients(q, k_cache, v_cache)
+    if _grad_enabled():
+        assert not (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad), _NO_BACKWARD
     qp = q.data_ptr()
     if plan.copy or qp & 15:
         return paged_window_attention(_usable(q), k_cache, v_cache, block_table.contiguous(), seq_lens.contiguous(), window, sinks, scale,
@@ -417,16 +425,17 @@ def paged_window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     if _device_now() != plan.device:
         with torch.cuda.device(plan.device):
             return paged_window_attention(q, k_cache, v_cache, block_table, seq_lens, window, sinks, scale, check=check)
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    out = _new_like(q)
     if plan.empty:
         return out
-    ws = torch.empty(plan.workspace, dtype=torch.uint8, device=q.device) if plan.workspace else None
+    ws = _empty(plan.workspace, dtype=_uint8, device=q.device) if plan.workspace else None
     stream = _raw_stream(plan.device)
     rc = _cabi.load().lucid_paged_window_attn(plan.ref, qp, out.data_ptr(), kc, vc, block_table.data_ptr(), seq_lens.data_ptr(),
                                               None if ws is None else ws.data_ptr(), plan.workspace, stream)
     if rc:
         _cabi.check_rc(rc, "lucid_paged_window_attn")
-    _finish(check, stream, "paged_window_attention")
+    if check or (check is None and _CHECK_DEFAULT):
+        _cabi.raise_on_attention_error(stream, "paged_window_attention")
     return out
 
 
@@ -450,7 +459,8 @@ def paged_lucid_attention(q: torch.Tensor, v: torch.Tensor, k_cache: torch.Tenso
     plan = _plans.get(key)
     if plan is None:
         plan = _step_plan(key, q, v, k_cache, v_cache, block_table, seq_lens, None, 0, scale, k_scale)
-    _no_gradients(q, v, k_cache, v_cache)
+    if _grad_enabled():
+        assert not (q.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad), _NO_BACKWARD
     qp, vp = q.data_ptr(), v.data_ptr()
     if plan.copy or (qp | vp) & 15:
         return paged_lucid_attention(_usable(q), _usable(v), k_cache, v_cache, block_table.contiguous(), seq_lens.contiguous(), k_scale,
@@ -459,15 +469,16 @@ def paged_lucid_attention(q: torch.Tensor, v: torch.Tensor, k_cache: torch.Tenso
     if _device_now() != plan.device:
         with torch.cuda.device(plan.device):
             return paged_lucid_attention(q, v, k_cache, v_cache, block_table, seq_lens, k_scale, scale, check=check)
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    out = _new_like(q)
     if plan.empty:
         return out
-    ws = torch.empty(plan.workspace, dtype=torch.uint8, device=q.device) if plan.workspace else None
+    ws = _empty(plan.workspace, dtype=_uint8, device=q.device) if plan.workspace else None
     stream = _raw_stream(plan.device)
     rc = _cabi.load().lucid_paged_lucid_attn(plan.ref, qp, vp, out.data_ptr(), kc, vc, block_table.data_ptr(), seq_lens.data_ptr(),
                                              None if ws is None else ws.data_ptr(), plan.workspace, stream)
     if rc:
         _cabi.check_rc(rc, "lucid_paged_lucid_attn")
-    torch.autograd.graph.increment_version([v_cache])
-    _finish(check, stream, "paged_lucid_attention")
+    _increment_version([v_cache])
+    if check or (check is None and _CHECK_DEFAULT):
+        _cabi.raise_on_attention_error(stream, "paged_lucid_attention")
     return out

@@ -16,7 +16,8 @@ inline cudaError_t ensure_context() {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || ready == dev) return e;
-  if ((e = cudaSetDevice(dev)) != cudaSuccess || (e = cudaFree(nullptr)) != cudaSuccess) return e;
+  // (makes and binds the context since CUDA 12, and is allowed while a stream is being captured)
+  if ((e = cudaSetDevice(dev)) != cudaSuccess) return e;
   ready = dev;
   return cudaSuccess;
 }

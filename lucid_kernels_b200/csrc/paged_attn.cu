@@ -44,6 +44,8 @@ __device__ __forceinline__ Visible visible(const PagedAttnArgs& a, bool lucid, i
   Visible v;
   if (lucid) --len;                                            // the rows before the newest one
   if (len < 0) len = 0;
+  // a length beyond the block table (reported where the newest position is looked up) does not make a longer loop
+  len = imin(len, a.c.table_width << a.c.page_shift);
   v.lo = a.W < len ? len - a.W : 0;
   v.first = a.S < v.lo ? a.S : v.lo;
   v.n = v.first + len - v.lo;
@@ -136,6 +138,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, kPagedPerSm) paged_attn_kernel(
   const Visible vis = visible(args, kLucid, len);
   const int chunk = chunk_keys(vis.n, args.splits);
   const int begin = split * chunk, end = imin(vis.n, begin + chunk);
+  if (!kLucid && split == 0 && tid == 0 && len > (c.table_width << c.page_shift)) report_error(&g_paged_ctl, kErrBadPage, b, len - 1, len - 1, 0);
   if constexpr (!kCluster) {
     launch_dependents();
     if (begin >= end) return;                                  // an empty chunk: the second kernel does not read it

@@ -418,6 +418,56 @@ def test_calls_from_a_thread_that_has_made_no_cuda_call():
 
 
 @gpu
+def test_a_thread_may_make_its_first_call_while_a_stream_is_captured():
+    import threading
+
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+
+    q, k, v, do = make(1, 256, 256, 2, 2, torch.bfloat16)
+    want = _window_attention_fwd(q, k, v, 64, 2)
+    grads = _window_attention_bwd(q, k, v, *want, do, 64, 2)
+    got = []
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        stream = torch.cuda.current_stream()
+
+        def work():
+            with torch.cuda.stream(stream):
+                got.append(_window_attention_bwd(q, k, v, *want, do, 64, 2))
+
+        th = threading.Thread(target=work)
+        th.start()
+        th.join()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got[0], grads))
+
+
+@gpu
+def test_expired_waits_end_and_are_reported():
+    """A wait limit of 0 (a wait that is not satisfied at once has run out): every kernel ends, the error is reported,
+    and the next call is right."""
+    from lucid_kernels_b200 import _cabi
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+
+    lib = _cabi.load()
+    q, k, v, do = make(2, 700, 700, 4, 2, torch.bfloat16)
+    out, lse = _window_attention_fwd(q, k, v, 200, 4, check=True)
+    grads = _window_attention_bwd(q, k, v, out, lse, do, 200, 4, check=True)
+    try:
+        lib.lucid_set_wait_limit_ns(0)
+        with pytest.raises(_cabi.LucidKernelError, match="timed out"):
+            _window_attention_fwd(q, k, v, 200, 4, check=True)
+        with pytest.raises(_cabi.LucidKernelError, match="timed out"):
+            _window_attention_bwd(q, k, v, out, lse, do, 200, 4, check=True)
+    finally:
+        lib.lucid_set_wait_limit_ns(2_000_000_000)
+    again = _window_attention_fwd(q, k, v, 200, 4, check=True)
+    assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+    assert all(torch.equal(x, y) for x, y in zip(grads, _window_attention_bwd(q, k, v, out, lse, do, 200, 4, check=True)))
+
+
+@gpu
 def test_partial_gradients_and_empty_tensors():
     from lucid_kernels_b200 import window_attention
 
@@ -541,6 +591,72 @@ def test_append_single_tokens_without_rotation_keys_only_and_interleaved_pools()
 
 
 @gpu
+@pytest.mark.parametrize("Hq,Hkv,B,most", [(16, 16, 3, 4400), (3, 1, 100, 150), (5, 1, 40, 300)])
+def test_append_many_tokens(Hq, Hkv, B, most):
+    """A warp per token and several rounds of head rows; many sequences, some of them without tokens."""
+    from lucid_kernels_b200 import paged_append
+
+    dt, page = torch.bfloat16, 16
+    h = torch.Generator().manual_seed(B)
+    new = torch.randint(0, most + 1, (B,), generator=h)
+    new[torch.randint(0, B, (B // 3,), generator=h)] = 0
+    new[B // 2] = most
+    T = int(new.sum())
+    assert T >= 4096
+    before = torch.randint(0, 50, (B,), generator=h)
+    per = -(-int((new + before).max()) // page)
+    table = torch.randperm(B * per, generator=h).reshape(B, per).to(torch.int32)
+    kc = torch.zeros(B * per, page, Hkv, D, device="cuda", dtype=dt)
+    vc = torch.zeros_like(kc)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(T, n, D, device="cuda", generator=g).to(dt) for n in (Hq, Hkv, Hkv))
+    cu = torch.cat((torch.zeros(1, dtype=torch.int64), new.cumsum(0)))
+    f = frequencies()
+    got = paged_append(k, v, kc, vc, table.cuda(), before.to(torch.int32).cuda(), cu_seqlens=cu.to(torch.int32).cuda(), q=q, inv_freq=f, check=True)
+    seq = torch.repeat_interleave(torch.arange(B), new)
+    pos = before[seq] + torch.arange(T) - cu[:-1][seq]
+    at = table[seq, pos // page].long().cuda(), (pos % page).cuda()
+    close_rotation(kc[at], rotated(k, pos.cuda(), f), k, dt)
+    close_rotation(got, rotated(q, pos.cuda(), f), q, dt)
+    assert torch.equal(vc[at], v)
+    assert int((vc != 0).any(-1).any(-1).sum()) == T
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """Pools of more than 2^31 elements, the sequence's pages at their end; inputs whose rows lie that far apart."""
+    from lucid_kernels_b200 import paged_append, paged_lucid_attention, paged_window_attention, window_attention
+
+    dt, page, Hkv, Hq, n = torch.bfloat16, 64, 4, 8, 300
+    pages = 2 ** 31 // (page * Hkv * D) + 40
+    kc, vc = (torch.empty(pages, page, Hkv, D, device="cuda", dtype=dt) for _ in range(2))
+    per = -(-n // page)
+    table = torch.arange(pages - 1, pages - 1 - per, -1, device="cuda", dtype=torch.int32)[None]
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v = (torch.randn(n, h, D, device="cuda", generator=g).to(dt) for h in (Hq, Hkv, Hkv))
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    paged_append(k, v, kc, vc, table, zero, cu_seqlens=cu, check=True)
+    small_k, small_v = kc[table[0].long()].clone(), vc[table[0].long()].clone()
+    small = torch.arange(per, device="cuda", dtype=torch.int32)[None]
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    a = paged_window_attention(q[-1:], kc, vc, table, lens, 100, 4, check=True)
+    assert torch.equal(a, paged_window_attention(q[-1:], small_k, small_v, small, lens, 100, 4, check=True))
+    small_v.mul_(1e-3)
+    vc[table[0].long()] = small_v
+    a = paged_lucid_attention(q[-1:], v[-1:], kc, vc, table, lens, k_scale=0.2, check=True)
+    assert torch.equal(a, paged_lucid_attention(q[-1:], v[-1:], small_k, small_v, small, lens, k_scale=0.2, check=True))
+    assert torch.equal(vc[table[0].long()], small_v)
+    del kc, vc
+    width = (2 ** 31 // (n - 1) // 8 + 1) * 8
+    far = torch.empty(n, width, device="cuda", dtype=dt)[:, : Hq * D]
+    far.copy_(q.reshape(n, Hq * D))
+    fq = far.unflatten(1, (Hq, D))[None]
+    assert fq.stride(1) * (n - 1) >= 2 ** 31
+    assert torch.equal(window_attention(fq, k[None], v[None], 100, 4), window_attention(q[None], k[None], v[None], 100, 4))
+
+
+@gpu
 def test_bad_pages_are_skipped_and_reported():
     """No address is formed from a page outside the pool or a position beyond the table: the host's view of the bounds is
     page_of / the append kernel's own check, and the error is reported once."""
@@ -568,6 +684,13 @@ def test_bad_pages_are_skipped_and_reported():
         paged_lucid_attention(q, x, kc, vc, bad, n, check=True)
     assert torch.equal(vc, v1)
     paged_window_attention(q, kc, vc, table, n, check=True)                       # reported once, then forgotten
+    n = torch.tensor([2 ** 31 - 1, 40], dtype=torch.int32, device="cuda")         # a length far beyond the table ends, too
+    with pytest.raises(_cabi.LucidKernelError, match="block table"):
+        paged_window_attention(q, kc, vc, table, n, check=True)
+    with pytest.raises(_cabi.LucidKernelError, match="block table"):
+        paged_lucid_attention(q, x, kc, vc, table, n, check=True)
+    n = torch.tensor([-5, 40], dtype=torch.int32, device="cuda")                  # and a negative one is none
+    assert not paged_window_attention(q, kc, vc, table, n, check=True)[0].any()
 
 
 def step_reference(q, kc, vc, table, lens, window, sinks, scale, v=None, k_scale=1.0):
