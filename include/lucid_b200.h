@@ -260,16 +260,19 @@ typedef struct {
   int64_t dout_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];  /* backward */
 } lucid_window_attn_desc;
 
-/* lse may be NULL (not wanted). */
+/* lse may be NULL (not wanted).  For a backward to come, `rest` (lucid_window_attn_rest_bytes(), 16-byte aligned, opaque;
+ * NULL: not wanted) receives what the rounding of `out` to 16 bits took off; out, lse and rest then fit together so that
+ * dO . out is accurate where one key has nearly all the weight. */
+size_t lucid_window_attn_rest_bytes(const lucid_window_attn_desc* desc);
 int lucid_window_attn_fwd(const lucid_window_attn_desc* desc, const void* q, const void* k, const void* v, void* out,
-                          float* lse, const int32_t* lengths, void* cuda_stream);
+                          void* rest, float* lse, const int32_t* lengths, void* cuda_stream);
 
-/* Its gradients, from the forward's out and lse.  dq, or dk and dv together, may be NULL (not computed).  Sums are fp32
+/* Its gradients, from the forward's out, rest (may be NULL: less accurate) and lse.  dq, or dk and dv together, may be NULL (not computed).  Sums are fp32
  * in a fixed order (no atomics: the same bits on every run).  Workspace 16-byte aligned, contents irrelevant. */
 size_t lucid_window_attn_bwd_workspace_bytes(const lucid_window_attn_desc* desc);
 int lucid_window_attn_bwd(const lucid_window_attn_desc* desc, const void* q, const void* k, const void* v, const void* out,
-                          const float* lse, const void* dout, void* dq, void* dk, void* dv, const int32_t* lengths,
-                          void* workspace, size_t workspace_bytes, void* cuda_stream);
+                          const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv,
+                          const int32_t* lengths, void* workspace, size_t workspace_bytes, void* cuda_stream);
 
 /* A paged key/value cache: pools (pages, page_rows, Hkv, 128) with element strides {page, row, head} (bases 16-byte
  * aligned, strides multiples of 8), page_rows a power of two, and a block table (B, table_width) of page numbers on the

@@ -33,7 +33,8 @@ EXPORTS = ("lucid_workspace_bytes", "lucid_fwd_sub", "lucid_bwd_sub", "lucid_rea
            "lucid_set_fused_backward", "lucid_fwd_sub_scaled", "lucid_bwd_sub_scaled",
            "lucid_set_pair_solve", "lucid_set_pair_limits", "lucid_fwd_workspace_bytes", "lucid_stream_capture_id", "lucid_query_pair_solve", "lucid_set_solve_variant", "lucid_set_upper_in_solve", "lucid_query_upper_in_solve",
            "lucid_probe_tma_delivery", "lucid_query_chain_group",
-           "lucid_window_attn_fwd", "lucid_window_attn_bwd", "lucid_window_attn_bwd_workspace_bytes", "lucid_paged_append",
+           "lucid_window_attn_fwd", "lucid_window_attn_bwd", "lucid_window_attn_bwd_workspace_bytes", "lucid_window_attn_rest_bytes",
+           "lucid_paged_append",
            "lucid_paged_window_attn", "lucid_paged_lucid_attn", "lucid_paged_attn_workspace_bytes", "lucid_attn_status")
 
 
@@ -169,11 +170,13 @@ def load() -> ctypes.CDLL:
         lib.lucid_set_wait_limit_ns.argtypes = [c.c_uint64]
         p, i = c.c_void_p, c.c_int
         lib.lucid_window_attn_fwd.restype = i
-        lib.lucid_window_attn_fwd.argtypes = [c.POINTER(WindowAttnDesc)] + [p] * 7
+        lib.lucid_window_attn_fwd.argtypes = [c.POINTER(WindowAttnDesc)] + [p] * 8
+        lib.lucid_window_attn_rest_bytes.restype = c.c_size_t
+        lib.lucid_window_attn_rest_bytes.argtypes = [c.POINTER(WindowAttnDesc)]
         lib.lucid_window_attn_bwd_workspace_bytes.restype = c.c_size_t
         lib.lucid_window_attn_bwd_workspace_bytes.argtypes = [c.POINTER(WindowAttnDesc)]
         lib.lucid_window_attn_bwd.restype = i
-        lib.lucid_window_attn_bwd.argtypes = [c.POINTER(WindowAttnDesc)] + [p] * 11 + [c.c_size_t, p]
+        lib.lucid_window_attn_bwd.argtypes = [c.POINTER(WindowAttnDesc)] + [p] * 12 + [c.c_size_t, p]
         lib.lucid_paged_append.restype = i
         lib.lucid_paged_append.argtypes = [c.POINTER(PagedAppendDesc)] + [p] * 11
         lib.lucid_paged_attn_workspace_bytes.restype = c.c_size_t

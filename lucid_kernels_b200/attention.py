@@ -152,14 +152,16 @@ def _window_plan(key, q, k, v, out, dout, window, sinks, scale, lengths) -> _Pla
     desc.dq_strides, desc.dk_strides, desc.dv_strides = like_q, like_k, like_k
     plan = _Plan(desc, q.get_device(), copy, q.numel() == 0)
     plan.out_shape, plan.lse_shape = (B, Nq, Hq, D), (B, Hq, Nq)
-    plan.workspace = 0 if dout is None or plan.empty else _cabi.load().lucid_window_attn_bwd_workspace_bytes(plan.ref)
+    plan.workspace = 0
+    if not plan.empty:       # backward: its scratch memory; forward: the size of `rest`
+        plan.workspace = getattr(_cabi.load(), "lucid_window_attn_rest_bytes" if dout is None else "lucid_window_attn_bwd_workspace_bytes")(plan.ref)
     return _keep(key, plan)
 
 
 def _window_attention_fwd(q, k, v, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
-                          lengths: Optional[torch.Tensor] = None, *, need_lse: bool = True, check: Optional[bool] = None):
-    """(out, lse): see ``window_attention``; ``lse`` (B, Hq, Nq) fp32, -inf for a query that sees nothing (None unless
-    ``need_lse``)."""
+                          lengths: Optional[torch.Tensor] = None, *, training: bool = True, check: Optional[bool] = None):
+    """(out, lse, rest): see ``window_attention``; ``lse`` (B, Hq, Nq) fp32, -inf for a query that sees nothing; ``rest``, what
+    the rounding of ``out`` took off, opaque.  Both are for the backward and None unless ``training``."""
     window, sinks, scale = _plain_options(window, sinks, scale)
     key = ("window", q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(),
            v.dtype, v.get_device(), window, sinks, scale,
@@ -170,28 +172,32 @@ def _window_attention_fwd(q, k, v, window: Optional[int] = None, sinks: int = 0,
     qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if plan.copy or (qp | kp | vp) & 15:
         return _window_attention_fwd(_usable(q), _usable(k), _usable(v), window, sinks, scale,
-                                     None if lengths is None else lengths.contiguous(), need_lse=need_lse, check=check)
+                                     None if lengths is None else lengths.contiguous(), training=training, check=check)
     if _device_now() != plan.device:
         with torch.cuda.device(plan.device):
-            return _window_attention_fwd(q, k, v, window, sinks, scale, lengths, need_lse=need_lse, check=check)
+            return _window_attention_fwd(q, k, v, window, sinks, scale, lengths, training=training, check=check)
     out = _new_like(q)
-    lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=q.device) if need_lse else None
+    lse = rest = None
+    if training:
+        lse = _empty(plan.lse_shape, dtype=torch.float32, device=q.device)
+        rest = _empty(plan.workspace, dtype=_uint8, device=q.device)
     if plan.empty:
-        return out, lse
+        return out, lse, rest
     stream = _raw_stream(plan.device)
-    rc = _cabi.load().lucid_window_attn_fwd(plan.ref, qp, kp, vp, out.data_ptr(), None if lse is None else lse.data_ptr(),
+    rc = _cabi.load().lucid_window_attn_fwd(plan.ref, qp, kp, vp, out.data_ptr(), None if rest is None else rest.data_ptr(),
+                                            None if lse is None else lse.data_ptr(),
                                             None if lengths is None else lengths.data_ptr(), stream)
     if rc:
         _cabi.check_rc(rc, "lucid_window_attn_fwd")
     if check or (check is None and _CHECK_DEFAULT):
         _cabi.raise_on_attention_error(stream, "_window_attention_fwd")
-    return out, lse
+    return out, lse, rest
 
 
-def _window_attention_bwd(q, k, v, out, lse, dout, window: Optional[int] = None, sinks: int = 0,
+def _window_attention_bwd(q, k, v, out, lse, rest, dout, window: Optional[int] = None, sinks: int = 0,
                           scale: Optional[float] = None, lengths: Optional[torch.Tensor] = None, *, need_dq: bool = True,
                           need_dkv: bool = True, check: Optional[bool] = None):
-    """(dq, dk, dv) from the forward's ``out`` and ``lse``; None for what is not needed."""
+    """(dq, dk, dv) from the forward's ``out``, ``lse`` and ``rest`` (None: a less accurate delta); None for what is not needed."""
     window, sinks, scale = _plain_options(window, sinks, scale)
     key = ("window bwd", q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(),
            v.dtype, v.get_device(), out.shape, out.stride(), out.dtype, out.get_device(), dout.shape, dout.stride(), dout.dtype,
@@ -202,13 +208,13 @@ def _window_attention_bwd(q, k, v, out, lse, dout, window: Optional[int] = None,
         plan = _window_plan(key, q, k, v, out, dout, window, sinks, scale, lengths)
     qp, kp, vp, op, gp = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr()
     if plan.copy or (qp | kp | vp | op | gp) & 15:
-        return _window_attention_bwd(*(_usable(t) for t in (q, k, v, out)), lse, _usable(dout), window, sinks, scale,
+        return _window_attention_bwd(*(_usable(t) for t in (q, k, v, out)), lse, rest, _usable(dout), window, sinks, scale,
                                      None if lengths is None else lengths.contiguous(), need_dq=need_dq, need_dkv=need_dkv, check=check)
     assert lse.shape == plan.lse_shape and lse.dtype == torch.float32 and lse.device == q.device and lse.is_contiguous(), \
         "lse must be the forward's"
     if _device_now() != plan.device:
         with torch.cuda.device(plan.device):
-            return _window_attention_bwd(q, k, v, out, lse, dout, window, sinks, scale, lengths, need_dq=need_dq, need_dkv=need_dkv,
+            return _window_attention_bwd(q, k, v, out, lse, rest, dout, window, sinks, scale, lengths, need_dq=need_dq, need_dkv=need_dkv,
                                          check=check)
     dq = _new_like(q) if need_dq else None
     dk, dv = (_new_like(t) if need_dkv else None for t in (k, v))
@@ -216,7 +222,7 @@ def _window_attention_bwd(q, k, v, out, lse, dout, window: Optional[int] = None,
         return dq, dk if dk is None else dk.zero_(), dv if dv is None else dv.zero_()
     ws = _empty(plan.workspace, dtype=_uint8, device=q.device)
     stream = _raw_stream(plan.device)
-    rc = _cabi.load().lucid_window_attn_bwd(plan.ref, qp, kp, vp, op, lse.data_ptr(), gp, None if dq is None else dq.data_ptr(),
+    rc = _cabi.load().lucid_window_attn_bwd(plan.ref, qp, kp, vp, op, None if rest is None else rest.data_ptr(), lse.data_ptr(), gp, None if dq is None else dq.data_ptr(),
                                             None if dk is None else dk.data_ptr(), None if dv is None else dv.data_ptr(),
                                             None if lengths is None else lengths.data_ptr(), ws.data_ptr(), plan.workspace, stream)
     if rc:
@@ -231,17 +237,17 @@ class LUCIDWindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, window=None, sinks=0, scale=None, lengths=None):
-        out, lse = _window_attention_fwd(q, k, v, window, sinks, scale, lengths)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        out, lse, rest = _window_attention_fwd(q, k, v, window, sinks, scale, lengths)
+        ctx.save_for_backward(q, k, v, out, lse, rest, lengths)
         ctx.args = (window, sinks, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
+        q, k, v, out, lse, rest, lengths = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dv = _window_attention_bwd(q, k, v, out, lse, dout, *ctx.args, lengths, need_dq=need[0],
+        dq, dk, dv = _window_attention_bwd(q, k, v, out, lse, rest, dout, *ctx.args, lengths, need_dq=need[0],
                                            need_dkv=need[1] or need[2])
         return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
@@ -262,7 +268,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     leaves alive while recording."""
     if _grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return LUCIDWindowAttention.apply(q, k, v, window, sinks, scale, lengths)
-    return _window_attention_fwd(q, k, v, window, sinks, scale, lengths, need_lse=False)[0]
+    return _window_attention_fwd(q, k, v, window, sinks, scale, lengths, training=False)[0]
 
 
 # ---------------------------------------------------------------------------------------------------------------------

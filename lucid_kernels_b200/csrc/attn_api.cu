@@ -109,7 +109,7 @@ using namespace lucid;
 extern "C" {
 
 int lucid_window_attn_fwd(const lucid_window_attn_desc* d, const void* q, const void* k, const void* v, void* out,
-                          float* lse, const int32_t* lengths, void* cuda_stream) {
+                          void* rest, float* lse, const int32_t* lengths, void* cuda_stream) {
   AttnFwdArgs args;
   int rc;
   if ((rc = make_shape(&args.a, d))) return rc;
@@ -118,6 +118,8 @@ int lucid_window_attn_fwd(const lucid_window_attn_desc* d, const void* q, const 
   if ((rc = check_tensor(q, d->q_strides, B, Nq, Hq)) || (rc = check_tensor(k, d->k_strides, B, Nk, Hkv)) ||
       (rc = check_tensor(v, d->v_strides, B, Nk, Hkv)) || (rc = check_tensor(out, d->out_strides, B, Nq, Hq)))
     return rc;
+  if (rest && !lse) return LUCID_E_NULL_POINTER;
+  if (reinterpret_cast<uintptr_t>(rest) % 16) return LUCID_E_BAD_ALIGNMENT;
   const int sms = sm_count();
   if (sms <= 0) return LUCID_E_NO_DEVICE;
   const bool bf16 = d->dtype == LUCID_DTYPE_BF16;
@@ -128,12 +130,19 @@ int lucid_window_attn_fwd(const lucid_window_attn_desc* d, const void* q, const 
   args.lengths = lengths;
   args.out = out;
   args.out_strides = Strides{d->out_strides[0], d->out_strides[1], d->out_strides[2]};
+  args.rest = rest;
   args.lse = lse;
   args.scale_log2 = d->scale * kLog2e;
   args.wait_ns = wait_limit_ns();
   // Single tiles with split keys where all of them fit the SMs at once: a CTA then has half as many steps in a row
-  args.split = fwd_items(args.a, true) <= sms ? 1 : 0;
+  args.split = !rest && fwd_items(args.a, true) <= sms ? 1 : 0;
   return (int)launch_attn_fwd(bf16, tm_q, tm_k, tm_v, args, sms, static_cast<cudaStream_t>(cuda_stream));
+}
+
+size_t lucid_window_attn_rest_bytes(const lucid_window_attn_desc* d) {
+  AttnShape a;
+  if (make_shape(&a, d)) return 0;
+  return (size_t)a.B * a.Hq * a.nqb * kBlock * kBlock * 2;
 }
 
 size_t lucid_window_attn_bwd_workspace_bytes(const lucid_window_attn_desc* d) {
@@ -143,7 +152,7 @@ size_t lucid_window_attn_bwd_workspace_bytes(const lucid_window_attn_desc* d) {
 }
 
 int lucid_window_attn_bwd(const lucid_window_attn_desc* d, const void* q, const void* k, const void* v, const void* out,
-                          const float* lse, const void* dout, void* dq, void* dk, void* dv, const int32_t* lengths,
+                          const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, const int32_t* lengths,
                           void* workspace, size_t workspace_bytes, void* cuda_stream) {
   AttnBwdArgs args;
   memset(&args, 0, sizeof(args));
@@ -159,7 +168,7 @@ int lucid_window_attn_bwd(const lucid_window_attn_desc* d, const void* q, const 
   if ((dk == nullptr) != (dv == nullptr)) return LUCID_E_NULL_POINTER;
   if (dk && ((rc = check_tensor(dk, d->dk_strides, B, Nk, Hkv)) || (rc = check_tensor(dv, d->dv_strides, B, Nk, Hkv)))) return rc;
   if (!lse || !workspace) return LUCID_E_NULL_POINTER;
-  if (reinterpret_cast<uintptr_t>(workspace) % 16) return LUCID_E_BAD_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 || reinterpret_cast<uintptr_t>(rest) % 16) return LUCID_E_BAD_ALIGNMENT;
   if (workspace_bytes < stat_bytes(args.a) + partial_bytes(args.a)) return LUCID_E_WORKSPACE_TOO_SMALL;
   const int sms = sm_count();
   if (sms <= 0) return LUCID_E_NO_DEVICE;
@@ -175,6 +184,7 @@ int lucid_window_attn_bwd(const lucid_window_attn_desc* d, const void* q, const 
   sa.a = args.a;
   sa.lengths = lengths;
   sa.out = out;
+  sa.rest = rest;
   sa.dout = dout;
   sa.out_strides = Strides{d->out_strides[0], d->out_strides[1], d->out_strides[2]};
   sa.dout_strides = Strides{d->dout_strides[0], d->dout_strides[1], d->dout_strides[2]};

@@ -14,41 +14,59 @@ namespace lucid {
 static __device__ Control g_attn_bwd_ctl;
 
 // ------------------------------------------------------------------------------------------------------------------
-// Row statistics {lse in base 2, delta}, one row per warp: reads O and dO once, bound by HBM.
+// Row statistics {lse in base 2, delta}: delta = dO . (O + what its rounding took off).  Reads each once, bound by HBM.
+// Eight lanes per row, four rows per warp and round.
 // ------------------------------------------------------------------------------------------------------------------
+constexpr int kStatRows = 16;            // rows of a warp
+
 template <bool kBf16>
 __global__ void __launch_bounds__(256) attn_stat_kernel(const AttnStatArgs args) {
   typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
   launch_dependents();
   const AttnShape& A = args.a;
-  const int lane = threadIdx.x & 31;
-  const int rows = A.nqb * kBlock;                       // padded rows per head
-  const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (r >= (long long)A.B * A.Hq * rows) return;
-  const int i = (int)(r % rows), bh = (int)(r / rows), b = bh / A.Hq, h = bh % A.Hq;
-  float st_lse = INFINITY, st_delta = 0.f;               // a row without weight
-  if (i < A.Nq) {
-    const float lse = args.lse[(long long)bh * A.Nq + i];
-    const elem_t* o = reinterpret_cast<const elem_t*>(args.out) + b * args.out_strides.b + (long long)i * args.out_strides.n +
-                      h * args.out_strides.h;
-    const elem_t* g = reinterpret_cast<const elem_t*>(args.dout) + b * args.dout_strides.b +
-                      (long long)i * args.dout_strides.n + h * args.dout_strides.h;
-    const uint2 ov = *reinterpret_cast<const uint2*>(o + lane * 4), gv = *reinterpret_cast<const uint2*>(g + lane * 4);
-    const float2 o0 = unpack2<kBf16>(ov.x), o1 = unpack2<kBf16>(ov.y), g0 = unpack2<kBf16>(gv.x), g1 = unpack2<kBf16>(gv.y);
-    float d = o0.x * g0.x + o0.y * g0.y + o1.x * g1.x + o1.y * g1.y;
+  const int lane = threadIdx.x & 31, ch = lane & 7;
+  const long long base = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kStatRows;     // of the padded rows of all heads
+  if (base >= (long long)A.B * A.Hq * A.nqb * kBlock) return;
+  const int rows = A.nqb * kBlock;
+  const int i0 = (int)(base % rows), bh = (int)(base / rows), b = bh / A.Hq, h = bh % A.Hq;
+  const elem_t* o = reinterpret_cast<const elem_t*>(args.out) + b * args.out_strides.b + h * args.out_strides.h + ch * 8;
+  const elem_t* g = reinterpret_cast<const elem_t*>(args.dout) + b * args.dout_strides.b + h * args.dout_strides.h + ch * 8;
+  const long long tile = base >> 7;
+  const elem_t* rest = reinterpret_cast<const elem_t*>(args.rest) + tile * (16 * kBlock * 8) + ch * (kBlock * 8);
 #pragma unroll
-    for (int m = 16; m > 0; m >>= 1) d += __shfl_xor_sync(0xffffffffu, d, m);
-    if (lse != -INFINITY) {
-      st_lse = lse * kLog2e;
-      st_delta = d;
+  for (int y = 0; y < kStatRows / 4; ++y) {
+    const int r = 4 * y + (lane >> 3), i = i0 + r;
+    float d = 0.f;
+    if (i < A.Nq) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint4 ov = *reinterpret_cast<const uint4*>(o + (long long)i * args.out_strides.n + 64 * c);
+        const uint4 gv = *reinterpret_cast<const uint4*>(g + (long long)i * args.dout_strides.n + 64 * c);
+        uint4 rv = make_uint4(0, 0, 0, 0);
+        if (args.rest) rv = *reinterpret_cast<const uint4*>(rest + 8 * c * (kBlock * 8) + (i & 127) * 8);
+        const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w}, gw[4] = {gv.x, gv.y, gv.z, gv.w}, rw[4] = {rv.x, rv.y, rv.z, rv.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = unpack2<kBf16>(ow[e]), q = unpack2<kBf16>(gw[e]), l = unpack2<kBf16>(rw[e]);
+          d += (a.x + l.x) * q.x + (a.y + l.y) * q.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 4; m > 0; m >>= 1) d += __shfl_xor_sync(0xffffffffu, d, m);
+    if (ch == 0) {
+      const float lse = i < A.Nq ? args.lse[(long long)bh * A.Nq + i] : -INFINITY;
+      const bool weight = lse != -INFINITY;                // (a row without weight: P = 0 from +infinity)
+      float* st = args.stat + tile * (2 * kBlock) + (i & 127);
+      st[0] = weight ? lse * kLog2e : INFINITY;
+      st[kBlock] = weight ? d : 0.f;
     }
   }
-  if (lane < 2) args.stat[(r >> 7) * (2 * kBlock) + lane * kBlock + (r & 127)] = lane ? st_delta : st_lse;
 }
 
 cudaError_t launch_attn_stat(bool bf16, const AttnStatArgs& args, cudaStream_t stream) {
   const long long rows = (long long)args.a.B * args.a.Hq * args.a.nqb * kBlock;
-  const unsigned grid = (unsigned)((rows + 7) / 8);
+  const unsigned grid = (unsigned)((rows + 8 * kStatRows - 1) / (8 * kStatRows));
   if (bf16) attn_stat_kernel<true><<<grid, 256, 0, stream>>>(args);
   else attn_stat_kernel<false><<<grid, 256, 0, stream>>>(args);
   return cudaGetLastError();
@@ -400,10 +418,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     while (const DqSlot* x = next()) {
       const KeyTiles kt = x->list();
       const int len = x->len, block = x->block, b = x->b, h = x->h;
-      const float lse2 = s.stat[slots & 1][row], delta = s.stat[slots & 1][kBlock + row];
+      const int i = block * kBlock + row, p = i + A.off;
+      // (a query that sees one key has dS = 0 exactly, not the difference of two nearly equal sums)
+      const float lse2 = sees_one(A, p) ? INFINITY : s.stat[slots & 1][row], delta = s.stat[slots & 1][kBlock + row];
       done();
       const unsigned long long nlse2 = f32x2(-lse2, -lse2), ndelta = f32x2(-delta, -delta);
-      const int i = block * kBlock + row, p = i + A.off;
       for (int u = 0; u < kt.n; ++u, ++g) {
         const int tile = kt.tile(u), j0 = tile << 7;
         const uint32_t s_tmem = lanes + kDqS + 128 * (g & 1) + wg * 64, g_tmem = lanes + kDqG + wg * 64;
@@ -777,13 +796,15 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           tmem_ld32(s_tmem + 32, v[1]);
           tmem_wait_ld();
           // Query rows behind the sequence hold anything, and 0 * NaN is not 0: they become zero in Q and dO before
-          // the products that sum over them.  S^T and G^T, which read them as columns, are complete by then.
+          // the products that sum over them; so do, in Q, those of queries that see one key, whose dS is 0 exactly.  S^T and
+          // G^T, which read them as columns, are complete by then.
           const bool stale = kMasked && p0 + 127 >= len && len < A.Nk;
-          if (stale) {
+          const bool cleared = stale || (kMasked && (sees_one(A, p0) || sees_one(A, p0 + 127)));
+          if (cleared) {
             if (!wait_lean(&s.dp_full, g & 1, cta_abort, limit, AB_DP_FULL)) return false;
-            if (wg == 0 && p0 + row >= len) {
-              zero_tile_row(s.qring[st], row);
-              zero_tile_row(s.gring[st], row);
+            if (wg == 0) {
+              if (p0 + row >= len || sees_one(A, p0 + row)) zero_tile_row(s.qring[st], row);
+              if (p0 + row >= len) zero_tile_row(s.gring[st], row);
             }
             __syncwarp();
             fence_proxy_async_smem();
@@ -829,7 +850,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             tc_fence_before_sync();
             mbar_arrive(c ? &s.p_ready : &s.p_half);
           }
-          if (!stale && !wait_lean(&s.dp_full, g & 1, cta_abort, limit, AB_DP_FULL)) return false;
+          if (!cleared && !wait_lean(&s.dp_full, g & 1, cta_abort, limit, AB_DP_FULL)) return false;
           tc_fence_after_sync();
           uint32_t ga[16], gb[16];
           auto ds = [&](uint32_t (&cur)[16], uint32_t (&nxt)[16], int c) {

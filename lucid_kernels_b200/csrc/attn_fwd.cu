@@ -52,7 +52,7 @@ struct AttnFwdSmem {
   uint64_t empty[kFwRing], q_full[2], q_free[2], s_full[2], p_half[2], p_ready[2], turn[2], o_full[2], o_free[2], l_full[2], l_free[2];
   uint64_t slot_full[kFwSlots], slot_free[kFwSlots];
   FwdSlot slot[kFwSlots];
-  alignas(16) float2 l[2][kBlock];                                // a finished row's sum and the reference of its exponents
+  alignas(16) float2 l[2][kBlock];       // a finished row's sum and the reference of its exponents (kTrain: and its lse in base 2)
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -66,7 +66,10 @@ constexpr int kFwS = 0, kFwO = 256;      // + 128 * tile
 constexpr int kFwRegsService = 80, kFwRegsSoftmax = 176;    // 256 * 80 + 256 * 176 = 512 * 128, the launch's total
 constexpr float kFwSlack = 8.f;          // log2 of how far the maximum may outgrow the reference
 
-template <bool kBf16>
+// kTrain: for a backward to come.  The result is normalised by the sum of the weights as they are rounded (so that it is a
+// mean of values even where one weight is nearly all), lse comes from the sum of the weights themselves, and what the
+// rounding of the result takes off is kept: delta = dO . O is subtracted from a nearly equal dO . v_j where a row is peaked.
+template <bool kBf16, bool kTrain>
 __global__ void __launch_bounds__(kFwThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const AttnFwdArgs args) {
@@ -379,6 +382,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         elem_t* out = reinterpret_cast<elem_t*>(args.out) + b * args.out_strides.b + h * args.out_strides.h + (lane & 7) * 8;
         const int r0 = block * kBlock + (warp & 3) * 32 + (lane >> 3);
         const uint32_t o_tmem = tmem + lanes + kFwO + 128 * t;
+        elem_t* rest = kTrain ? reinterpret_cast<elem_t*>(args.rest) + ((((long long)b * A.Hq + h) * A.nqb + block) * 16 * kBlock + row) * 8 : nullptr;
         if (has) {
           uint32_t oa[16], ob[16];
           auto put = [&](const uint32_t (&o)[16], int c) {        // columns 16c .. 16c+15
@@ -392,6 +396,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 w.w = pack2<kBf16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
               }
               *reinterpret_cast<uint4*>(panel + (c >> 2) * 4096 + sw128_off(lane, 2 * (c & 3) + e)) = w;
+              if constexpr (kTrain) {
+                const uint32_t hi[4] = {w.x, w.y, w.z, w.w};
+                uint32_t lo[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const float2 h2 = unpack2<kBf16>(hi[y]);
+                  lo[y] = some ? pack2<kBf16>(__uint_as_float(o[8 * e + 2 * y]) * inv - h2.x, __uint_as_float(o[8 * e + 2 * y + 1]) * inv - h2.y) : 0u;
+                }
+                *reinterpret_cast<uint4*>(rest + (2 * c + e) * (kBlock * 8)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              }
             }
           };
           if (two) {
@@ -426,6 +440,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
           }
         }
+        if (kTrain && !has) {
+#pragma unroll 1
+          for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(rest + c * (kBlock * 8)) = make_uint4(0, 0, 0, 0);
+        }
         __syncwarp();
 #pragma unroll 1
         for (int y = 0; y < 8; ++y) {
@@ -440,7 +458,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         __syncwarp();
         if (i < A.Nq && args.lse)
-          args.lse[((long long)b * A.Hq + h) * A.Nq + i] = some ? (ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
+          args.lse[((long long)b * A.Hq + h) * A.Nq + i] = some ? (kTrain ? ref : ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
       }
       done(false);
     }
@@ -468,6 +486,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const int p = it->t[t].block * kBlock + row + A.off;
       done(false);
       float ref = -INFINITY, l = 0.f;
+      [[maybe_unused]] float l16 = 0.f;
       for (int x = 0; x < kt.n; ++x, ++ns) {
         const int tile = kt.tile(x), j0 = tile << 7;
         if (!wait_lean(&s.s_full[t], ns & 1, cta_abort, limit, AF_S_FULL)) { alive = false; break; }
@@ -526,6 +545,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             const float f = next == -INFINITY ? 1.f : ex2_approx(ref - next);
             ref = next;
             l *= f;
+            if constexpr (kTrain) l16 *= f;
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
               uint32_t o[16];
@@ -540,6 +560,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const float neg = ref == -INFINITY ? 0.f : -ref;
           const unsigned long long neg2 = f32x2(neg, neg);
           unsigned long long sum = 0, sum2 = 0;          // two zeros each
+          [[maybe_unused]] unsigned long long rounded = 0;
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             uint32_t pk[16];
@@ -557,6 +578,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               if (e & 1) sum2 = f32x2_add(sum2, f32x2(w.x, w.y));
               else sum = f32x2_add(sum, f32x2(w.x, w.y));
               pk[e] = pack2<kBf16>(w.x, w.y);
+              if constexpr (kTrain) {
+                const float2 y2 = unpack2<kBf16>(pk[e]);
+                rounded = f32x2_add(rounded, f32x2(y2.x, y2.y));
+              }
             }
             }
             tmem_st16(s_tmem + 16 * c, pk);
@@ -572,6 +597,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           mbar_arrive(&s.p_ready[t]);
           const float2 both = f32x2_unpack(f32x2_add(sum, sum2));
           l += both.x + both.y;
+          if constexpr (kTrain) {
+            const float2 r2 = f32x2_unpack(rounded);
+            l16 += r2.x + r2.y;
+          }
         };
         if (!masked) weights(std::integral_constant<int, 4>{}, std::false_type{});
         else if (tile_narrow(A, kt, tile)) weights(std::integral_constant<int, kNarrow / 32>{}, std::true_type{});
@@ -582,7 +611,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
       if (kt.n > 0) {
         if (!wait_lean(&s.l_free[t], (nl++ & 1) ^ 1, cta_abort, limit, AF_L_FREE)) break;
-        s.l[t][row] = make_float2(l, ref);
+        if constexpr (kTrain) s.l[t][row] = make_float2(l16, ref + log2f(l));
+        else s.l[t][row] = make_float2(l, ref);
         mbar_arrive(&s.l_full[t]);
       }
     }
@@ -603,9 +633,11 @@ cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMa
                             const AttnFwdArgs& args, int sms, cudaStream_t stream) {
   const int items = fwd_items(args.a, args.split != 0), grid = items < sms ? items : sms;
   const int bytes = (int)sizeof(AttnFwdSmem);
-  auto kernel = bf16 ? attn_fwd_kernel<true> : attn_fwd_kernel<false>;
-  static SmemOnce once[2];
-  cudaError_t e = once[bf16].set(reinterpret_cast<const void*>(kernel), bytes);
+  const bool train = args.rest != nullptr;
+  auto kernel = train ? (bf16 ? attn_fwd_kernel<true, true> : attn_fwd_kernel<false, true>)
+                      : (bf16 ? attn_fwd_kernel<true, false> : attn_fwd_kernel<false, false>);
+  static SmemOnce once[4];
+  cudaError_t e = once[2 * train + bf16].set(reinterpret_cast<const void*>(kernel), bytes);
   if (e != cudaSuccess) return e;
   kernel<<<grid, kFwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, args);
   return cudaGetLastError();

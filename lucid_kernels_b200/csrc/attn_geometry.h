@@ -55,6 +55,13 @@ LUCID_HD bool tile_masked(const AttnShape& a, const KeyTiles& t, int tile, int l
   return j0 + 127 > t.p_lo || (a.W < kNoWindow && j0 <= t.p_hi - a.W) || j0 + 127 >= len;
 }
 
+// Does the query at position p see exactly one key?  Its weight is 1 whatever the scores are: no gradient reaches q or k.
+LUCID_HD bool sees_one(const AttnShape& a, int p) {
+  const int near = a.W >= kNoWindow ? p + 1 : imin(a.W, p + 1);
+  const int first = a.W >= kNoWindow ? 0 : imin(a.S, p + 1 - near);
+  return near + first == 1;
+}
+
 // A tile visited for its visible first keys alone, few enough for a product of kNarrow keys.
 constexpr int kNarrow = 32;
 LUCID_HD bool tile_narrow(const AttnShape& a, const KeyTiles& t, int tile) { return t.sink && tile == 0 && a.S <= kNarrow; }

@@ -39,9 +39,17 @@ static int check(const AttnShape& a, const std::vector<int>& lens) {
         }
       }
     }
-    for (int i = 0; i < a.Nq; ++i)
-      for (int j = 0; j < a.Nk; ++j)
+    for (int i = 0; i < a.Nq; ++i) {
+      int keys = 0;
+      for (int j = 0; j < a.Nk; ++j) {
         if (seen[(size_t)i * a.Nk + j] != (sees(a, i, j, len) ? 1 : 0)) return 3;
+        keys += seen[(size_t)i * a.Nk + j];
+      }
+      if (i + a.off < len && sees_one(a, i + a.off) != (keys == 1)) return 24;
+      // a block that holds such a row shows it at one of its ends, and only in masked pairs of tiles
+      const int p0 = (i & ~127) + a.off;
+      if (i + a.off < len && keys == 1 && !sees_one(a, p0) && !sees_one(a, p0 + 127)) return 25;
+    }
   }
   // forward items: every (b, head, block) once, its own list in order
   std::vector<int> tiles((size_t)a.B * a.Hq * a.nqb, 0);
@@ -92,6 +100,7 @@ static int check(const AttnShape& a, const std::vector<int>& lens) {
       if (blk < 0 || blk >= a.nqb) return 11;
       const int p0 = blk * 128 + a.off, j0 = kv.tile * 128;
       const bool masked = block_masked(a, j0, p0, len);
+      if (!masked && (sees_one(a, p0) || sees_one(a, p0 + 127))) return 26;
       for (int j = j0; j < j0 + 128 && j < a.Nk; ++j) {
         const ColMask c = col_mask(a, j, p0, len);
         for (int e = 0; e < 128; ++e) {

@@ -120,17 +120,19 @@ def test_refusals_of_the_c_entry_points():
     def window(Nq=512, Nk=512, Hq=4, Hkv=2, Dh=128, dt=1, w=128, s=0, scale=0.1, qs=st):
         return byref(_cabi.WindowAttnDesc(1, Nq, Nk, Hq, Hkv, Dh, dt, w, s, scale, qs, *[st] * 7))
 
-    def fwd(q=p, out=p, **kw):
-        return lib.lucid_window_attn_fwd(window(**kw), q, p, p, out, None, None, None)
+    def fwd(q=p, out=p, rest=None, **kw):
+        return lib.lucid_window_attn_fwd(window(**kw), q, p, p, out, rest, None, None, None)
 
     assert fwd(Dh=64) == -1 and fwd(Nq=0) == -1 and fwd(Nq=513) == -1 and fwd(s=129) == -1 and fwd(s=-1) == -1
     assert fwd(Hq=3) == -10 and fwd(dt=2) == -2 and fwd(q=None) == -5 and fwd(out=None) == -5 and fwd(q=p + 2) == -3
     assert fwd(scale=0.0) == -13 and fwd(scale=float("nan")) == -13 and fwd(scale=float("inf")) == -13
     assert fwd(qs=I3(512 * 1024, 1028, 128)) == -3 and fwd(qs=I3(512 * 1024, 0, 128)) == -9
-    assert fwd(Nk=1 << 29) == -1 and lib.lucid_window_attn_fwd(None, p, p, p, p, None, None, None) == -5
+    assert fwd(Nk=1 << 29) == -1 and lib.lucid_window_attn_fwd(None, p, p, p, p, None, None, None, None) == -5
+    assert fwd(rest=p) == -5                                   # without lse
+    assert lib.lucid_window_attn_rest_bytes(window(Nq=300)) == 4 * 3 * 128 * 128 * 2
 
     def bwd(ws=p, wsb=1 << 40, dk=p, dv=p, lse=p):
-        return lib.lucid_window_attn_bwd(window(s=4), p, p, p, p, lse, p, p, dk, dv, None, ws, wsb, None)
+        return lib.lucid_window_attn_bwd(window(s=4), p, p, p, p, p, lse, p, p, dk, dv, None, ws, wsb, None)
 
     assert bwd(ws=None) == -5 and bwd(ws=p + 4) == -3 and bwd(wsb=100) == -4 and bwd(dk=None) == -5 and bwd(lse=None) == -5
     assert lib.lucid_window_attn_bwd_workspace_bytes(window()) == 4 * 512 * 8
@@ -234,12 +236,13 @@ def test_window_attention_forward_and_backward(shape, dt):
     q, k, v, do = make(B, Nq, Nk, Hq, Hkv, dt, seed=Nq + Nk)
     scale = D ** -0.5
     ref, bound, lse_ref, grads, gb = reference(q, k, v, window, sinks, scale, None, do)
-    out, lse = _window_attention_fwd(q, k, v, window, sinks, scale, check=True)
+    out, lse, rest = _window_attention_fwd(q, k, v, window, sinks, scale, check=True)
     close(out, ref, bound, dt, "out")
+    close(_window_attention_fwd(q, k, v, window, sinks, scale, training=False, check=True)[0], ref, bound, dt, "out, inference")
     some = torch.isfinite(lse_ref)
     assert torch.equal(torch.isneginf(lse), ~some)
     assert float((lse.double() - lse_ref)[some].abs().max() if some.any() else 0) < 1e-5 * 16
-    got = _window_attention_bwd(q, k, v, out, lse, do, window, sinks, scale, check=True)
+    got = _window_attention_bwd(q, k, v, out, lse, rest, do, window, sinks, scale, check=True)
     for name, x, r, b in zip(("dq", "dk", "dv"), got, grads, gb):
         close(x, r, b, dt, name)
 
@@ -264,10 +267,11 @@ def test_padded_batch_ignores_whatever_stands_behind_the_sequences(window, sinks
     lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
     scale = 0.07
     ref, bound, lse_ref, grads, gb = reference(q, k, v, window, sinks, scale, lengths, do)
-    out, lse = _window_attention_fwd(q, k, v, window, sinks, scale, lengths, check=True)
+    out, lse, rest = _window_attention_fwd(q, k, v, window, sinks, scale, lengths, check=True)
     close(out, ref, bound, dt, "out")
+    close(_window_attention_fwd(q, k, v, window, sinks, scale, lengths, training=False, check=True)[0], ref, bound, dt, "out, inference")
     assert torch.equal(torch.isneginf(lse), torch.isneginf(lse_ref))
-    for name, x, r, b in zip(("dq", "dk", "dv"), _window_attention_bwd(q, k, v, out, lse, do, window, sinks, scale, lengths, check=True), grads, gb):
+    for name, x, r, b in zip(("dq", "dk", "dv"), _window_attention_bwd(q, k, v, out, lse, rest, do, window, sinks, scale, lengths, check=True), grads, gb):
         close(x, r, b, dt, name)
         for i, n in enumerate(lens):
             rows = x[i, max(0, n - (Nk - Nq)):] if name == "dq" else x[i, n:]
@@ -300,6 +304,28 @@ def test_strided_expanded_and_misaligned_inputs():
     window_attention(q2, kf, vf, window=90, sinks=2).backward(do)
     assert torch.equal(qg.grad, q2.grad)
     assert torch.equal(k1.grad[0], kf.grad.sum(0)) and torch.equal(v1.grad[0], vf.grad.sum(0))
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("shape,window,sinks,sharp", [((1, 1, 1, 2, 1), None, 0, 1), ((2, 300, 300, 4, 2), 1, 0, 1), ((1, 200, 260, 3, 3), 0, 1, 1),
+                                                      ((1, 400, 400, 4, 2), 2, 0, 1), ((1, 400, 400, 4, 2), 5, 1, 1), ((1, 500, 500, 4, 2), 200, 4, 12)])
+def test_gradients_of_rows_with_few_or_peaked_weights(shape, window, sinks, sharp, dt):
+    """Where one key has (nearly) all the weight, dS is a difference of nearly equal numbers.  One visible key: exactly 0.
+    Otherwise in the 2-norm: dS rounded (u / sqrt 3 on average), the result rounded (the same), and delta from weights
+    rounded but normalised, whose error is again at most u times dS's own size: sqrt(3) u / sqrt(3) = u together."""
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+
+    q, k, v, do = make(*shape, dt, seed=31)
+    scale = sharp * D ** -0.5
+    _, _, _, grads, _ = reference(q, k, v, window, sinks, scale, None, do)
+    out, lse, rest = _window_attention_fwd(q, k, v, window, sinks, scale, check=True)
+    got = _window_attention_bwd(q, k, v, out, lse, rest, do, window, sinks, scale, check=True)
+    for name, x, r in zip(("dq", "dk"), got, grads):
+        if float(r.abs().max()) < 1e-12:
+            assert not x.any(), name
+        else:
+            assert float((x.double() - r).norm() / r.norm()) <= unit(dt), name
 
 
 @gpu
@@ -344,7 +370,7 @@ def test_extreme_scores_and_growing_maxima():
     for window, sinks in ((None, 0), (400, 2)):
         scale = 1.0
         ref, bound, lse_ref, _, _ = reference(q, k, v, window, sinks, scale, None)
-        out, lse = _window_attention_fwd(q, k, v, window, sinks, scale, check=True)
+        out, lse, _ = _window_attention_fwd(q, k, v, window, sinks, scale, check=True)
         # a score s carries an fp32 error of up to D products' roundings, 128 * 2^-24 * sum |q||k|, and a weight that
         # relative error: e^delta - 1 with delta <= 2^-17 * sum |q||k|
         size = float((q.double().abs().amax() * k.double().abs().amax()) * 0 + (q.double().norm(dim=-1).amax() * k.double().norm(dim=-1).amax()))
@@ -403,10 +429,10 @@ def test_calls_from_a_thread_that_has_made_no_cuda_call():
 
     q, k, v, do = make(1, 256, 256, 2, 2, torch.bfloat16)
     calls = [lambda: _window_attention_fwd(q, k, v, 64, 2),
-             lambda: _window_attention_bwd(q, k, v, out, lse, do, 64, 2),
+             lambda: _window_attention_bwd(q, k, v, out, lse, rest, do, 64, 2),
              lambda: (_forward_sub_fwd(k * 0.3, v),),
              lambda: _forward_sub_bwd(k * 0.3, v, do)]
-    out, lse = calls[0]()
+    out, lse, rest = calls[0]()
     for call in calls:
         want, got = call(), []
         torch.cuda.synchronize()
@@ -452,19 +478,19 @@ def test_expired_waits_end_and_are_reported():
 
     lib = _cabi.load()
     q, k, v, do = make(2, 700, 700, 4, 2, torch.bfloat16)
-    out, lse = _window_attention_fwd(q, k, v, 200, 4, check=True)
-    grads = _window_attention_bwd(q, k, v, out, lse, do, 200, 4, check=True)
+    out, lse, rest = _window_attention_fwd(q, k, v, 200, 4, check=True)
+    grads = _window_attention_bwd(q, k, v, out, lse, rest, do, 200, 4, check=True)
     try:
         lib.lucid_set_wait_limit_ns(0)
         with pytest.raises(_cabi.LucidKernelError, match="timed out"):
             _window_attention_fwd(q, k, v, 200, 4, check=True)
         with pytest.raises(_cabi.LucidKernelError, match="timed out"):
-            _window_attention_bwd(q, k, v, out, lse, do, 200, 4, check=True)
+            _window_attention_bwd(q, k, v, out, lse, rest, do, 200, 4, check=True)
     finally:
         lib.lucid_set_wait_limit_ns(2_000_000_000)
     again = _window_attention_fwd(q, k, v, 200, 4, check=True)
     assert torch.equal(again[0], out) and torch.equal(again[1], lse)
-    assert all(torch.equal(x, y) for x, y in zip(grads, _window_attention_bwd(q, k, v, out, lse, do, 200, 4, check=True)))
+    assert all(torch.equal(x, y) for x, y in zip(grads, _window_attention_bwd(q, k, v, out, lse, rest, do, 200, 4, check=True)))
 
 
 @gpu
