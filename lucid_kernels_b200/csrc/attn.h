@@ -15,11 +15,11 @@ enum : int { kErrBadPage = 4 };
 
 struct AttnFwdArgs {
   AttnShape a;
-  int split;              // items are single tiles of queries whose keys are split between the CTA's two halves
+  int split;              // (without lse) items are single tiles of queries whose keys are split between the CTA's two halves
   const int* lengths;     // (B) valid positions, or null
   void* out;              // (B, Nq, Hq, 128)
   Strides out_strides;
-  void* rest;             // or null: (B, Hq, nqb, 16, 128, 8) 16-bit, what the rounding of `out` took off (needs lse, no split)
+  void* rest;             // or null: (B, Hq, nqb, 16, 128, 8) 16-bit, what the rounding of `out` took off (needs lse)
   float* lse;             // or null; (B, Hq, Nq) natural log of the row's sum of exponentials, -inf for an empty row
   float scale_log2;       // scale * log2(e)
   unsigned long long wait_ns;

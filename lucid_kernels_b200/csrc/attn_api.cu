@@ -134,8 +134,8 @@ int lucid_window_attn_fwd(const lucid_window_attn_desc* d, const void* q, const 
   args.lse = lse;
   args.scale_log2 = d->scale * kLog2e;
   args.wait_ns = wait_limit_ns();
-  // Single tiles with split keys where all of them fit the SMs at once: a CTA then has half as many steps in a row
-  args.split = !rest && fwd_items(args.a, true) <= sms ? 1 : 0;
+  // (inference) single tiles with split keys where all of them fit the SMs at once: a CTA then has half as many steps in a row
+  args.split = !lse && fwd_items(args.a, true) <= sms ? 1 : 0;
   return (int)launch_attn_fwd(bf16, tm_q, tm_k, tm_v, args, sms, static_cast<cudaStream_t>(cuda_stream));
 }
 

@@ -66,9 +66,10 @@ constexpr int kFwS = 0, kFwO = 256;      // + 128 * tile
 constexpr int kFwRegsService = 80, kFwRegsSoftmax = 176;    // 256 * 80 + 256 * 176 = 512 * 128, the launch's total
 constexpr float kFwSlack = 8.f;          // log2 of how far the maximum may outgrow the reference
 
-// kTrain: for a backward to come.  The result is normalised by the sum of the weights as they are rounded (so that it is a
-// mean of values even where one weight is nearly all), lse comes from the sum of the weights themselves, and what the
-// rounding of the result takes off is kept: delta = dO . O is subtracted from a nearly equal dO . v_j where a row is peaked.
+// The result is normalised by the sum of the weights as they are rounded, so that it is a mean of values even where one
+// weight is nearly all (the mixed-precision adds cost nothing measurable; unpacking the halves first took 8 % longer).
+// kTrain: lse is wanted, for a backward to come.  lse comes from the sum of the weights themselves, and what the rounding of the result
+// takes off is kept (if `rest` is given): delta = dO . O is subtracted from a nearly equal dO . v_j where a row is peaked.
 template <bool kBf16, bool kTrain>
 __global__ void __launch_bounds__(kFwThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -396,7 +397,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 w.w = pack2<kBf16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
               }
               *reinterpret_cast<uint4*>(panel + (c >> 2) * 4096 + sw128_off(lane, 2 * (c & 3) + e)) = w;
-              if constexpr (kTrain) {
+              if (kTrain && args.rest) {
                 const uint32_t hi[4] = {w.x, w.y, w.z, w.w};
                 uint32_t lo[4];
 #pragma unroll
@@ -440,7 +441,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
           }
         }
-        if (kTrain && !has) {
+        if (kTrain && args.rest && !has) {
 #pragma unroll 1
           for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(rest + c * (kBlock * 8)) = make_uint4(0, 0, 0, 0);
         }
@@ -457,8 +458,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         }
         __syncwarp();
-        if (i < A.Nq && args.lse)
-          args.lse[((long long)b * A.Hq + h) * A.Nq + i] = some ? (kTrain ? ref : ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
+        if (kTrain && i < A.Nq) args.lse[((long long)b * A.Hq + h) * A.Nq + i] = some ? ref * 0.6931471805599453f : -INFINITY;
       }
       done(false);
     }
@@ -485,8 +485,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       kt.p_hi = it->t[t].p_hi;
       const int p = it->t[t].block * kBlock + row + A.off;
       done(false);
-      float ref = -INFINITY, l = 0.f;
-      [[maybe_unused]] float l16 = 0.f;
+      float ref = -INFINITY, l16 = 0.f;                // l16: the sum of the weights as they are rounded
+      [[maybe_unused]] float l = 0.f;
       for (int x = 0; x < kt.n; ++x, ++ns) {
         const int tile = kt.tile(x), j0 = tile << 7;
         if (!wait_lean(&s.s_full[t], ns & 1, cta_abort, limit, AF_S_FULL)) { alive = false; break; }
@@ -544,8 +544,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             const float next = fmaxf(ref, m);
             const float f = next == -INFINITY ? 1.f : ex2_approx(ref - next);
             ref = next;
-            l *= f;
-            if constexpr (kTrain) l16 *= f;
+            l16 *= f;
+            if constexpr (kTrain) l *= f;
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
               uint32_t o[16];
@@ -559,8 +559,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           // (a part of the exponentials as a polynomial on the FMA pipe, one pair in 2, 3 or 4, took 2 to 12 % longer in all)
           const float neg = ref == -INFINITY ? 0.f : -ref;
           const unsigned long long neg2 = f32x2(neg, neg);
-          unsigned long long sum = 0, sum2 = 0;          // two zeros each
-          [[maybe_unused]] unsigned long long rounded = 0;
+          [[maybe_unused]] unsigned long long sum = 0, sum2 = 0;     // two zeros each
+          float rounded0 = 0.f, rounded1 = 0.f;
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             uint32_t pk[16];
@@ -575,13 +575,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               float2 w = f32x2_unpack(y);
               w.x = ex2_approx(w.x);
               w.y = ex2_approx(w.y);
-              if (e & 1) sum2 = f32x2_add(sum2, f32x2(w.x, w.y));
-              else sum = f32x2_add(sum, f32x2(w.x, w.y));
-              pk[e] = pack2<kBf16>(w.x, w.y);
               if constexpr (kTrain) {
-                const float2 y2 = unpack2<kBf16>(pk[e]);
-                rounded = f32x2_add(rounded, f32x2(y2.x, y2.y));
+                if (e & 1) sum2 = f32x2_add(sum2, f32x2(w.x, w.y));
+                else sum = f32x2_add(sum, f32x2(w.x, w.y));
               }
+              pk[e] = pack2<kBf16>(w.x, w.y);
+              add_halves<kBf16>(rounded0, rounded1, pk[e]);
             }
             }
             tmem_st16(s_tmem + 16 * c, pk);
@@ -595,11 +594,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           tc_fence_before_sync();
           if (kChunks <= 2) mbar_arrive(&s.p_half[t]);
           mbar_arrive(&s.p_ready[t]);
-          const float2 both = f32x2_unpack(f32x2_add(sum, sum2));
-          l += both.x + both.y;
+          l16 += rounded0 + rounded1;
           if constexpr (kTrain) {
-            const float2 r2 = f32x2_unpack(rounded);
-            l16 += r2.x + r2.y;
+            const float2 both = f32x2_unpack(f32x2_add(sum, sum2));
+            l += both.x + both.y;
           }
         };
         if (!masked) weights(std::integral_constant<int, 4>{}, std::false_type{});
@@ -612,7 +610,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (kt.n > 0) {
         if (!wait_lean(&s.l_free[t], (nl++ & 1) ^ 1, cta_abort, limit, AF_L_FREE)) break;
         if constexpr (kTrain) s.l[t][row] = make_float2(l16, ref + log2f(l));
-        else s.l[t][row] = make_float2(l, ref);
+        else s.l[t][row] = make_float2(l16, ref);
         mbar_arrive(&s.l_full[t]);
       }
     }
@@ -633,7 +631,7 @@ cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMa
                             const AttnFwdArgs& args, int sms, cudaStream_t stream) {
   const int items = fwd_items(args.a, args.split != 0), grid = items < sms ? items : sms;
   const int bytes = (int)sizeof(AttnFwdSmem);
-  const bool train = args.rest != nullptr;
+  const bool train = args.lse != nullptr;
   auto kernel = train ? (bf16 ? attn_fwd_kernel<true, true> : attn_fwd_kernel<false, true>)
                       : (bf16 ? attn_fwd_kernel<true, false> : attn_fwd_kernel<false, false>);
   static SmemOnce once[4];

@@ -276,10 +276,16 @@ __global__ void __launch_bounds__(kPaWarps * 32, kPagedPerSm) paged_attn_kernel(
       sa[e + 2] = ex2_approx(sa[e + 2] - z1);
       sb[e + 2] = ex2_approx(sb[e + 2] - z1);
     }
-    l0 += (sa[0] + sa[1]) + (sb[0] + sb[1]);
-    l1 += (sa[2] + sa[3]) + (sb[2] + sb[3]);
     const uint32_t pf[4] = {pack2<kBf16>(sa[0], sa[1]), pack2<kBf16>(sa[2], sa[3]), pack2<kBf16>(sb[0], sb[1]),
                             pack2<kBf16>(sb[2], sb[3])};
+    // the sums of the weights as they are rounded: the result is a mean of values even where one weight is nearly all
+    float e0 = 0.f, e1 = 0.f, f0 = 0.f, f1 = 0.f;
+    add_halves<kBf16>(e0, e1, pf[0]);
+    add_halves<kBf16>(e0, e1, pf[2]);
+    add_halves<kBf16>(f0, f1, pf[1]);
+    add_halves<kBf16>(f0, f1, pf[3]);
+    l0 += e0 + e1;
+    l1 += f0 + f1;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       uint32_t bv[4];      // keys 0-7 and 8-15 of columns 16n .. 16n+7, then of 16n+8 .. 16n+15

@@ -477,6 +477,15 @@ __device__ __forceinline__ uint32_t pack2_fast(float lo, float hi) {
   else return pack2<kBf16>(lo, hi);
 }
 
+// a += the low, b += the high 16-bit value of `w` (mixed-precision adds)
+template <bool kBf16>
+__device__ __forceinline__ void add_halves(float& a, float& b, uint32_t w) {
+  if constexpr (kBf16)
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\nadd.rn.f32.bf16 %0, l, %0;\nadd.rn.f32.bf16 %1, h, %1;\n}" : "+f"(a), "+f"(b) : "r"(w));
+  else
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\nadd.rn.f32.f16 %0, l, %0;\nadd.rn.f32.f16 %1, h, %1;\n}" : "+f"(a), "+f"(b) : "r"(w));
+}
+
 template <bool kBf16>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
   float2 f;
