@@ -79,7 +79,8 @@ __global__ void __launch_bounds__(128) diag_prep_kernel(const __grid_constant__ 
   uint32_t phase = 0;        // completed waits on bar_mma
   // every thread waits for the product just committed; false after a timeout (anybody's)
   auto product_done = [&](int id) -> bool {
-    const bool ok = wait_barrier(&s.bar_mma, phase & 1, cta_abort, args.ctl, args.wait_ns, chain, i, id);
+    // (one outcome per warp: what follows are warp-wide instructions)
+    const bool ok = __all_sync(0xffffffffu, wait_barrier(&s.bar_mma, phase & 1, cta_abort, args.ctl, args.wait_ns, chain, i, id));
     ++phase;
     tc_fence_after_sync();
     return ok;
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(128) diag_prep_kernel(const __grid_constant__ 
   }
   tc_fence_before_sync();
   __syncthreads();             // every thread has read S (also: the MMA has finished reading K_i)
-  ok = !s.abort_flag;
+  ok = __all_sync(0xffffffffu, !s.abort_flag);
 
   // ---- step 2: invert the unit lower-triangular sub-blocks, one column per thread ----
   if (ok) {
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(128) diag_prep_kernel(const __grid_constant__ 
     fence_proxy_async_smem();
     tc_fence_before_sync();
     __syncthreads();
-    ok = !s.abort_flag;
+    ok = __all_sync(0xffffffffu, !s.abort_flag);
     if (ok && tid == 0) {
       tc_fence_after_sync();
       issue_product(s.n, s.x);                                 // T = N X_d
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(128) diag_prep_kernel(const __grid_constant__ 
     fence_proxy_async_smem();
     tc_fence_before_sync();
     __syncthreads();
-    ok = !s.abort_flag;
+    ok = __all_sync(0xffffffffu, !s.abort_flag);
     if (ok && tid == 0) {
       tc_fence_after_sync();
       issue_product(s.x, s.k);                                 // U = X_d T
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(128) diag_prep_kernel(const __grid_constant__ 
   }
   tc_fence_before_sync();
   __syncthreads();
-  ok = !s.abort_flag;
+  ok = __all_sync(0xffffffffu, !s.abort_flag);
   if (!ok) {
     // a wait ran out: give a tile load or product that may still be in flight time to land before this
     // CTA's shared memory and tensor memory are handed to another CTA

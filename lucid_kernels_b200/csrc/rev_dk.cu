@@ -642,8 +642,10 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
       }
       fence_proxy_async_smem();
       mbar_arrive(&s.stage_full);
-      if (tid == 128) {
-        if (!wait_barrier(&s.stage_full, it & 1, cta_abort, ctl, limit, chain, i, RD_STAGE_FULL)) break;
+      // (if the publishing thread's wait runs out, its warp leaves with it below: the others would go on to warp-wide
+      // instructions that it never reaches)
+      auto publish = [&]() -> bool {
+        if (!wait_barrier(&s.stage_full, it & 1, cta_abort, ctl, limit, chain, i, RD_STAGE_FULL)) return false;
         tma_store_4d(&tm_dv, s.rhs, 0, i * kBlock, h, b);
         tma_store_4d(&tm_dv, s.rhs + kHalfBytes, 64, i * kBlock, h, b);
         tma_store_commit();
@@ -652,10 +654,14 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
         tma_store_wait_all();
         fence_proxy_async_all();
         st_release_gpu(args.flags + chain * T + i, kFlagComplete);
-      }
+        return true;
+      };
+      bool published = true;
+      if (tid == 128) published = publish();
 
       // ---- the upper-triangle dK sums of this row-block (tiles j >= i + 2), fp32, to the workspace ----
-      if (!wait_barrier(&s.acck_full, it & 1, cta_abort, ctl, limit, chain, i, RD_ACCK_FULL)) break;
+      const bool summed = wait_barrier(&s.acck_full, it & 1, cta_abort, ctl, limit, chain, i, RD_ACCK_FULL);
+      if (!__all_sync(0xffffffffu, summed && published)) break;
       float* up = args.upper + ((long long)(chain * T + i) * kBlock + row) * kBlock + wg * 32;
       if (n >= 2) {
         tc_fence_after_sync();

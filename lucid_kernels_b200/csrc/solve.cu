@@ -578,15 +578,18 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
     uint32_t nq = 0;             // items finished through Q so far (phase of pq_full / q_full)
     uint32_t u_peer = 0;         // pair mode, CTA 0: half-tiles the peer CTA's rings have seen so far
     bool alive = true;
+    bool published = true;       // the publishing thread's: false after a wait that ran out
     int trc = 0;
     (void)trc;
     const bool tr_lead = (tid == 128 || tid == 256) && wg < 2;
     (void)tr_lead;
     for (int it = 0; alive; ++it) {
       const int slot = it & 1;
-      if (!wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, BAR_TK_FULL)) break;
+      const bool posted = wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, BAR_TK_FULL);
       const int ticket = s.tk_slot[slot];
-      __syncwarp();
+      // a warp goes on or leaves as one: lanes that went on without the publishing one, whose wait for the block before
+      // ran out, would stand for ever in a warp-wide instruction
+      if (!__all_sync(0xffffffffu, posted && published)) break;
       if (lane == 0) mbar_arrive(&s.tk_empty[slot]);
       int chain, i, n, jfirst;
       if (!item_geometry(ticket, chain, i, n, jfirst)) break;
@@ -797,9 +800,10 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
         // after it has acquired the barrier: a cluster-wide proxy fence here cost 4000 cycles per row-block.
         fence_proxy_async_smem();
         mbar_arrive(&s.stage_full);
-        if (tid == 128) {
+        // (the publishing thread's waits may run out like any other: it leaves with its warp, at the next item's start)
+        auto publish = [&]() -> bool {
           if (hand_over) {
-            if (!wait_barrier(&s.stage_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_STAGE_FULL)) break;
+            if (!wait_barrier(&s.stage_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_STAGE_FULL)) return false;
             // Has the peer claimed its stages for this item?  A counter, not a barrier phase: the peer's
             // producer may run an item ahead.  Only this thread needs to know (cluster-scope acquire loads
             // are expensive), and normally the answer has been yes for a while.
@@ -818,7 +822,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
                   }
                 }
               }
-              if (!ok) break;
+              if (!ok) return false;
             }
             // The staged tile (two 64-column panels of 128 rows) goes to the peer as four 8 KiB bulk copies:
             // rows 0-63 of both panels into stage st0, rows 64-127 into st1 - the layout of a ring stage, and
@@ -833,7 +837,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
                                 mapa_u32(smem_u32(&s.v_full[st]), 1));
             }
           } else if (!wait_barrier(&s.stage_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_STAGE_FULL)) {
-            break;
+            return false;
           }
           LUCID_TR(args.trace, 3, trc, 47, i);
           tma_store_4d(&tm_st, s.rhs, 0, i * kBlock, h, b);
@@ -846,7 +850,9 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
           LUCID_TR(args.trace, 3, trc, 49, i);
           fence_proxy_async_all();
           st_release_gpu(args.flags + chain * T + i, kFlagComplete);
-        }
+          return true;
+        };
+        if (tid == 128) published = publish();
       } else {
         // ---- publish (identity diagonal: the result was stored with plain stores above) ----
         // Each warp orders its lanes' stores with a warp barrier and then adds its share to the flag with
