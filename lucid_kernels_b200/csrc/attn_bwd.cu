@@ -286,7 +286,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const int per = A.B * A.Hq;
       for (int rnd = 0; alive; ++rnd, ++slots) {
         const int idx = snake_item(rnd, blockIdx.x, gridDim.x), sl = rnd & 1;
-        if (!wait_lean(&s.slot_free[sl], ((rnd >> 1) & 1) ^ 1, cta_abort, limit, AB_SLOT_FREE)) break;
+        if (!wait_lane(&s.slot_free[sl], ((rnd >> 1) & 1) ^ 1, cta_abort, limit, AB_SLOT_FREE)) break;
         DqSlot& x = s.slot[sl];
         if (idx >= per * A.nqb) {
           x.n = -1;
@@ -309,24 +309,24 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         mbar_expect_tx(&s.slot_full[sl], 2 * kBlock * 4);
         bulk_load(s.stat[sl], args.stat + (((long long)b * A.Hq + h) * A.nqb + block) * (2 * kBlock), 2 * kBlock * 4, &s.slot_full[sl]);
         if (kt.n == 0) continue;
-        if (!wait_lean(&s.q_free, (itn & 1) ^ 1, cta_abort, limit, AB_Q_FREE)) break;
+        if (!wait_lane(&s.q_free, (itn & 1) ^ 1, cta_abort, limit, AB_Q_FREE)) break;
         mbar_expect_tx(&s.q_full, kTileBytes);
         tma_load_4d(s.q, &tm_q, &s.q_full, 0, block * kBlock, h, b);
         tma_load_4d(s.q + kHalfBytes, &tm_q, &s.q_full, 64, block * kBlock, h, b);
-        if (!wait_lean(&s.go_free, (itn & 1) ^ 1, cta_abort, limit, AB_GO_FREE)) break;
+        if (!wait_lane(&s.go_free, (itn & 1) ^ 1, cta_abort, limit, AB_GO_FREE)) break;
         mbar_expect_tx(&s.go_full, kTileBytes);
         tma_load_4d(s.go, &tm_do, &s.go_full, 0, block * kBlock, h, b);
         tma_load_4d(s.go + kHalfBytes, &tm_do, &s.go_full, 64, block * kBlock, h, b);
         for (int u = 0; u < kt.n; ++u, ++g) {
           const int j = kt.tile(u), ks = g % 3, vs = vt.stage();
-          if (!wait_lean(&s.k_empty[ks], ((g / 3) & 1) ^ 1, cta_abort, limit, AB_K_EMPTY)) { alive = false; break; }
+          if (!wait_lane(&s.k_empty[ks], ((g / 3) & 1) ^ 1, cta_abort, limit, AB_K_EMPTY)) { alive = false; break; }
           mbar_expect_tx(&s.k_full[ks], kTileBytes);
           tma_load_4d(s.kring[ks], &tm_k, &s.k_full[ks], 0, j * kBlock, hk, b);
           tma_load_4d(s.kring[ks] + kHalfBytes, &tm_k, &s.k_full[ks], 64, j * kBlock, hk, b);
-          if (!wait_lean(&s.v_empty[vs], (vt.used() & 1) ^ 1, cta_abort, limit, AB_V_EMPTY)) { alive = false; break; }
+          if (!wait_lane(&s.v_empty[vs], (vt.used() & 1) ^ 1, cta_abort, limit, AB_V_EMPTY)) { alive = false; break; }
           if (vs == passed) {
             // (itn items have passed a stage so far; the last of them has to be through with it)
-            if (!wait_lean(&s.panel_done, (itn - 1) & 1, cta_abort, limit, AB_PANEL)) { alive = false; break; }
+            if (!wait_lane(&s.panel_done, (itn - 1) & 1, cta_abort, limit, AB_PANEL)) { alive = false; break; }
             passed = -1;
           }
           mbar_expect_tx(&s.v_full[vs], kTileBytes);
@@ -335,7 +335,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           vt.use();
         }
         // (an item of one tile that did not come to the stage the item before passed over: wait here, one at a time)
-        if (alive && passed >= 0 && !wait_lean(&s.panel_done, (itn - 1) & 1, cta_abort, limit, AB_PANEL)) break;
+        if (alive && passed >= 0 && !wait_lane(&s.panel_done, (itn - 1) & 1, cta_abort, limit, AB_PANEL)) break;
         passed = vt.stage();
         ++vt.at;
         ++itn;
@@ -643,7 +643,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       KvItem it;
       for (int rnd = 0; alive; ++rnd) {
         const int sl = rnd & 1;
-        if (!wait_lean(&s.slot_free[sl], ((rnd >> 1) & 1) ^ 1, cta_abort, limit, AB_SLOT_FREE)) break;
+        if (!wait_lane(&s.slot_free[sl], ((rnd >> 1) & 1) ^ 1, cta_abort, limit, AB_SLOT_FREE)) break;
         DkvSlot& x = s.slot[sl];
         if (!kv_item(A, args.chunks, snake_item(rnd, blockIdx.x, gridDim.x), it)) {
           x.nb = -1;
@@ -662,7 +662,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         x.len = len;
         mbar_arrive(&s.slot_full[sl]);
         if (nb == 0) continue;
-        if (!wait_lean(&s.k_free, (itn & 1) ^ 1, cta_abort, limit, AB_K_EMPTY)) break;
+        if (!wait_lane(&s.k_free, (itn & 1) ^ 1, cta_abort, limit, AB_K_EMPTY)) break;
         mbar_expect_tx(&s.k_full, kTileBytes);
         tma_load_4d(s.k, &tm_k, &s.k_full, 0, it.tile * kBlock, it.hk, it.b);
         tma_load_4d(s.k + kHalfBytes, &tm_k, &s.k_full, 64, it.tile * kBlock, it.hk, it.b);
@@ -671,19 +671,19 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const float* stat = args.stat + ((long long)it.b * A.Hq + h) * A.nqb * (2 * kBlock);
           for (int blk = qb.first; blk <= qb.last; ++blk, ++g) {
             const int st = g & 1;
-            if (!wait_lean(&s.q_empty[st], ((g >> 1) & 1) ^ 1, cta_abort, limit, AB_Q_FREE)) { alive = false; break; }
+            if (!wait_lane(&s.q_empty[st], ((g >> 1) & 1) ^ 1, cta_abort, limit, AB_Q_FREE)) { alive = false; break; }
             mbar_expect_tx(&s.q_full[st], kTileBytes + 2 * kBlock * 4);
             tma_load_4d(s.qring[st], &tm_q, &s.q_full[st], 0, blk * kBlock, h, it.b);
             tma_load_4d(s.qring[st] + kHalfBytes, &tm_q, &s.q_full[st], 64, blk * kBlock, h, it.b);
             bulk_load(s.stat[st], stat + (long long)blk * (2 * kBlock), 2 * kBlock * 4, &s.q_full[st]);
             if (!v_loaded) {
-              if (!wait_lean(&s.v_free, (itn & 1) ^ 1, cta_abort, limit, AB_V_EMPTY)) { alive = false; break; }
+              if (!wait_lane(&s.v_free, (itn & 1) ^ 1, cta_abort, limit, AB_V_EMPTY)) { alive = false; break; }
               mbar_expect_tx(&s.v_full, kTileBytes);
               tma_load_4d(s.v, &tm_v, &s.v_full, 0, it.tile * kBlock, it.hk, it.b);
               tma_load_4d(s.v + kHalfBytes, &tm_v, &s.v_full, 64, it.tile * kBlock, it.hk, it.b);
               v_loaded = true;
             }
-            if (!wait_lean(&s.go_empty[st], ((g >> 1) & 1) ^ 1, cta_abort, limit, AB_GO_FREE)) { alive = false; break; }
+            if (!wait_lane(&s.go_empty[st], ((g >> 1) & 1) ^ 1, cta_abort, limit, AB_GO_FREE)) { alive = false; break; }
             mbar_expect_tx(&s.go_full[st], kTileBytes);
             tma_load_4d(s.gring[st], &tm_do, &s.go_full[st], 0, blk * kBlock, h, it.b);
             tma_load_4d(s.gring[st] + kHalfBytes, &tm_do, &s.go_full[st], 64, blk * kBlock, h, it.b);

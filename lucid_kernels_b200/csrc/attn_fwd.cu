@@ -123,8 +123,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   // The items of this CTA, one after another: `next` waits for the slot, `done` hands it back (per warp; whoever reads it
   // later keeps copies).
   uint32_t slots = 0;
-  auto next = [&]() -> const FwdSlot* {
-    if (!wait_lean(&s.slot_full[slots % kFwSlots], (slots / kFwSlots) & 1, cta_abort, limit, AF_SLOT_FULL)) return nullptr;
+  auto next = [&](bool one_thread = false) -> const FwdSlot* {
+    uint64_t* bar = &s.slot_full[slots % kFwSlots];
+    const uint32_t parity = (slots / kFwSlots) & 1;
+    if (!(one_thread ? wait_lane(bar, parity, cta_abort, limit, AF_SLOT_FULL) : wait_lean(bar, parity, cta_abort, limit, AF_SLOT_FULL)))
+      return nullptr;
     const FwdSlot* slot = &s.slot[slots % kFwSlots];
     return slot->n < 0 ? nullptr : slot;
   };
@@ -146,11 +149,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         uint32_t nq[2] = {0, 0};      // Q tiles loaded
         bool alive = true;
         while (alive) {
-          const FwdSlot* it = next();
+          const FwdSlot* it = next(true);
           if (!it) break;
           const int b = it->b, hk = it->hk;
           auto load = [&](const CUtensorMap* tm, int tile) -> bool {
-            if (!wait_lean(&s.empty[stage], phase ^ 1, cta_abort, limit, AF_EMPTY)) return false;
+            if (!wait_lane(&s.empty[stage], phase ^ 1, cta_abort, limit, AF_EMPTY)) return false;
             mbar_expect_tx(&s.full[stage], kTileBytes);
             tma_load_4d(s.ring[stage], tm, &s.full[stage], 0, tile * kBlock, hk, b);
             tma_load_4d(s.ring[stage] + kHalfBytes, tm, &s.full[stage], 64, tile * kBlock, hk, b);
@@ -162,7 +165,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           };
           for (int t = 0; t < 2; ++t) {
             if (it->t[t].n == 0) continue;
-            if (!wait_lean(&s.q_free[t], (nq[t] & 1) ^ 1, cta_abort, limit, AF_Q_FREE)) {
+            if (!wait_lane(&s.q_free[t], (nq[t] & 1) ^ 1, cta_abort, limit, AF_Q_FREE)) {
               alive = false;
               break;
             }
@@ -184,7 +187,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         FwdItem it;
         for (int rnd = 0;; ++rnd) {
           const int k = rnd % kFwSlots;
-          if (!wait_lean(&s.slot_free[k], ((rnd / kFwSlots) & 1) ^ 1, cta_abort, limit, AF_SLOT_FREE)) break;
+          if (!wait_lane(&s.slot_free[k], ((rnd / kFwSlots) & 1) ^ 1, cta_abort, limit, AF_SLOT_FREE)) break;
           FwdSlot& x = s.slot[k];
           const bool more = fwd_item(A, split, snake_item(rnd, blockIdx.x, gridDim.x), it);
           if (more) {
@@ -220,68 +223,60 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     } else if (warp < 3) {
       // =========================== issuer of one tile's products ===========================
       // A step per entry of the items' unions, one after another, and one at the end: P V of this tile's previous entry (it
-      // may be the last of the item before), then S of this entry, in turns with the other tile's issuer.
-      const int t = warp - 1;
-      constexpr int fmt = kBf16 ? 1 : 0;
-      constexpr uint32_t idesc_s = umma_idesc(fmt, 0, 0, 128, 128);          // Q K^T: both K-major
-      constexpr uint32_t idesc_sn = umma_idesc(fmt, 0, 0, 128, kNarrow);     // the first kNarrow keys only
-      constexpr uint32_t idesc_o = umma_idesc(fmt, 0, 1, 128, 128);          // P V: P from TMEM, V rows = k
-      const uint64_t dq = umma_smem_desc(smem_u32(s.q[t]), 16, 1024);
-      const uint64_t d_k0 = umma_smem_desc(smem_u32(s.ring[0]), 16, 1024);
-      const uint64_t d_v0 = umma_smem_desc(smem_u32(s.ring[0]), kHalfBytes, 1024);
-      const uint32_t s_tmem = tmem + kFwS + 128 * t, o_tmem = tmem + kFwO + 128 * t;
-      uint32_t st = 0, phase = 0;             // ring stage and phase of this entry's K; its V is in the stage behind it
-      uint32_t v_st = 0, v_phase = 0;         // V of the entry before
-      uint32_t nq = 0, no = 0, np = 0, turns = 0;   // items begun and results begun (with tiles); weights consumed; turns taken
-      bool before = false;                    // is there an entry before
-      bool pend = false, pend_first = false, pend_last = false, pend_narrow = false;   // its weights are this tile's
-      auto step = [&](bool more, bool act, bool first, bool last, bool narrow) -> bool {
-        if (before && !wait_lean(&s.full[v_st], v_phase, cta_abort, limit, AF_FULL)) return false;
-        if (more && !wait_lean(&s.full[st], phase, cta_abort, limit, AF_FULL)) return false;
-        if (act && first && !wait_lean(&s.q_full[t], nq++ & 1, cta_abort, limit, AF_Q_FULL)) return false;
-        if (pend) {
-          if (!wait_lean(&s.p_half[t], np & 1, cta_abort, limit, AF_P_HALF)) return false;
-          // the epilogue of this tile's previous item has read O
-          if (pend_first && !wait_lean(&s.o_free[t], (no++ & 1) ^ 1, cta_abort, limit, AF_O_FREE)) return false;
-        }
-        const uint64_t dv = d_v0 + v_st * (kTileBytes >> 4), dk = d_k0 + st * (kTileBytes >> 4);
-        if (!wait_lean(&s.turn[t], (turns++ & 1) ^ (t ^ 1), cta_abort, limit, AF_TURN)) return false;
-        tc_fence_after_sync();
-        if (pend) {
-          const uint32_t add = pend_first ? 0u : 1u;
-          if (pend_narrow) {
-            if (elect_one()) {
+      // may be the last of the item before), then S of this entry, in turns with the other tile's issuer.  One thread has
+      // the role to itself (votes of the whole warp at each wait took 2.5 % longer in the 64k prefill).
+      if (elect_one()) {
+        const int t = warp - 1;
+        constexpr int fmt = kBf16 ? 1 : 0;
+        constexpr uint32_t idesc_s = umma_idesc(fmt, 0, 0, 128, 128);          // Q K^T: both K-major
+        constexpr uint32_t idesc_sn = umma_idesc(fmt, 0, 0, 128, kNarrow);     // the first kNarrow keys only
+        constexpr uint32_t idesc_o = umma_idesc(fmt, 0, 1, 128, 128);          // P V: P from TMEM, V rows = k
+        const uint64_t dq = umma_smem_desc(smem_u32(s.q[t]), 16, 1024);
+        const uint64_t d_k0 = umma_smem_desc(smem_u32(s.ring[0]), 16, 1024);
+        const uint64_t d_v0 = umma_smem_desc(smem_u32(s.ring[0]), kHalfBytes, 1024);
+        const uint32_t s_tmem = tmem + kFwS + 128 * t, o_tmem = tmem + kFwO + 128 * t;
+        uint32_t st = 0, phase = 0;             // ring stage and phase of this entry's K; its V is in the stage behind it
+        uint32_t v_st = 0, v_phase = 0;         // V of the entry before
+        uint32_t nq = 0, no = 0, np = 0, turns = 0;   // items begun and results begun (with tiles); weights consumed; turns taken
+        bool before = false;                    // is there an entry before
+        bool pend = false, pend_first = false, pend_last = false, pend_narrow = false;   // its weights are this tile's
+        auto step = [&](bool more, bool act, bool first, bool last, bool narrow) -> bool {
+          if (before && !wait_lane(&s.full[v_st], v_phase, cta_abort, limit, AF_FULL)) return false;
+          if (more && !wait_lane(&s.full[st], phase, cta_abort, limit, AF_FULL)) return false;
+          if (act && first && !wait_lane(&s.q_full[t], nq++ & 1, cta_abort, limit, AF_Q_FULL)) return false;
+          if (pend) {
+            if (!wait_lane(&s.p_half[t], np & 1, cta_abort, limit, AF_P_HALF)) return false;
+            // the epilogue of this tile's previous item has read O
+            if (pend_first && !wait_lane(&s.o_free[t], (no++ & 1) ^ 1, cta_abort, limit, AF_O_FREE)) return false;
+          }
+          const uint64_t dv = d_v0 + v_st * (kTileBytes >> 4), dk = d_k0 + st * (kTileBytes >> 4);
+          if (!wait_lane(&s.turn[t], (turns++ & 1) ^ (t ^ 1), cta_abort, limit, AF_TURN)) return false;
+          tc_fence_after_sync();
+          if (pend) {
+            const uint32_t add = pend_first ? 0u : 1u;
+            if (pend_narrow) {
 #pragma unroll
               for (int k = 0; k < kNarrow / 16; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
-            }
-          } else {
-            if (elect_one()) {
+            } else {
 #pragma unroll
               for (int k = 0; k < 4; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, k ? 1u : add);
             }
-          }
-          if (!wait_lean(&s.p_ready[t], np++ & 1, cta_abort, limit, AF_P_READY)) return false;
-          if (!pend_narrow) {
-            tc_fence_after_sync();
-            if (elect_one()) {
+            if (!wait_lane(&s.p_ready[t], np++ & 1, cta_abort, limit, AF_P_READY)) return false;
+            if (!pend_narrow) {
+              tc_fence_after_sync();
 #pragma unroll
               for (int k = 4; k < 8; ++k) umma_ts(o_tmem, s_tmem + 8 * k, dv + k * (2048 >> 4), idesc_o, 1u);
             }
+            if (pend_last) umma_commit(&s.o_full[t]);
           }
-          if (pend_last) umma_commit_w(&s.o_full[t]);
-        }
-        if (act) {
-          const uint32_t idesc = narrow ? idesc_sn : idesc_s;
-          if (elect_one()) {
+          if (act) {
+            const uint32_t idesc = narrow ? idesc_sn : idesc_s;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
               umma_ss(s_tmem, dq + off, dk + off, idesc, k ? 1u : 0u);
             }
           }
-        }
-        __syncwarp();
-        if (elect_one()) {
           mbar_arrive(&s.turn[t ^ 1]);
           if (act) umma_commit(&s.s_full[t]);
           // the stages go back when both issuers' products that read them are complete (an issuer without products on
@@ -289,41 +284,41 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (before) umma_commit(&s.empty[v_st]);
           if (more) umma_commit(&s.empty[st]);
           if (act && last) umma_commit(&s.q_free[t]);
+          pend = act;
+          pend_first = first;
+          pend_last = last;
+          pend_narrow = narrow;
+          before = true;
+          v_st = st + 1;
+          v_phase = phase;
+          if (v_st == kFwRing) {
+            v_st = 0;
+            v_phase ^= 1;
+          }
+          st = v_st + 1;
+          phase = v_phase;
+          if (st == kFwRing) {
+            st = 0;
+            phase ^= 1;
+          }
+          return true;
+        };
+        bool alive = true;
+        while (alive) {
+          const FwdSlot* it = next(true);
+          if (!it) break;
+          const int n = it->n, own = it->t[t].n, own_first = it->t[t].first, from = it->t[t].from, to = it->t[t].to;
+          done(true);
+          const bool narrow0 = own_first && A.S <= kNarrow;       // (tile_narrow)
+          int at = 0;
+          for (int u = 0; u < n && alive; ++u) {
+            const bool act = split ? (u & 1) == t : (u == 0 && own_first) || (u >= from && u < to);
+            alive = step(true, act, at == 0, at == own - 1, narrow0 && u == 0);
+            if (act) ++at;
+          }
         }
-        pend = act;
-        pend_first = first;
-        pend_last = last;
-        pend_narrow = narrow;
-        before = true;
-        v_st = st + 1;
-        v_phase = phase;
-        if (v_st == kFwRing) {
-          v_st = 0;
-          v_phase ^= 1;
-        }
-        st = v_st + 1;
-        phase = v_phase;
-        if (st == kFwRing) {
-          st = 0;
-          phase ^= 1;
-        }
-        return true;
-      };
-      bool alive = true;
-      while (alive) {
-        const FwdSlot* it = next();
-        if (!it) break;
-        const int n = it->n, own = it->t[t].n, own_first = it->t[t].first, from = it->t[t].from, to = it->t[t].to;
-        done(false);
-        const bool narrow0 = own_first && A.S <= kNarrow;       // (tile_narrow)
-        int at = 0;
-        for (int u = 0; u < n && alive; ++u) {
-          const bool act = split ? (u & 1) == t : (u == 0 && own_first) || (u >= from && u < to);
-          alive = step(true, act, at == 0, at == own - 1, narrow0 && u == 0);
-          if (act) ++at;
-        }
+        if (alive && before) step(false, false, false, false, false);
       }
-      if (alive && before) step(false, false, false, false, false);
     }
   } else if (warp < 8) {
     // =========================== epilogue of both tiles ===========================

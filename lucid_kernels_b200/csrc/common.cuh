@@ -90,23 +90,36 @@ __device__ __forceinline__ bool wait_barrier(uint64_t* bar, uint32_t parity, vol
 
 // The same wait in little code, for kernels whose roles wait in many places: a few polls before the clock is looked at for
 // the first time (reading the global timer costs a waiter some hundred cycles), and only the barrier's id is left behind
-// (through the CTA-wide abort word; the kernel reports it when it ends).
-__device__ __forceinline__ bool wait_lean(uint64_t* bar, uint32_t parity, volatile int* cta_abort,
-                                          unsigned long long limit_ns, int bar_id) {
-  if (mbar_try_wait(bar, parity)) return true;
+// (through the CTA-wide abort word; the kernel reports it when it ends).  wait_lean is called by a whole warp, which gets
+// one answer: if lanes went their own ways when a limit runs out, some would wait for ever in a warp-wide instruction that
+// the others never reach.  wait_lane is called by one thread that has its role to itself.
+template <bool kWarp>
+__device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, volatile int* cta_abort,
+                                             unsigned long long limit_ns, int bar_id) {
+  auto ready = [&]() { return kWarp ? __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) != 0 : mbar_try_wait(bar, parity); };
+  auto agreed = [&](bool x) { return kWarp ? __any_sync(0xffffffffu, x) != 0 : x; };
+  if (ready()) return true;
   unsigned long long t0 = 0;
   uint32_t spins = 0;
-  while (!mbar_try_wait(bar, parity)) {
+  while (!ready()) {
     if ((++spins & 63u) != 0 && limit_ns != 0) continue;
-    if (*cta_abort) return false;
+    if (agreed(*cta_abort != 0)) return false;
     const unsigned long long t = globaltimer_ns();
     if (t0 == 0) t0 = t;
-    if (t - t0 >= limit_ns) {
+    if (agreed(t - t0 >= limit_ns)) {
       *cta_abort = bar_id;
       return false;
     }
   }
   return true;
+}
+__device__ __forceinline__ bool wait_lean(uint64_t* bar, uint32_t parity, volatile int* cta_abort,
+                                          unsigned long long limit_ns, int bar_id) {
+  return wait_bounded<true>(bar, parity, cta_abort, limit_ns, bar_id);
+}
+__device__ __forceinline__ bool wait_lane(uint64_t* bar, uint32_t parity, volatile int* cta_abort,
+                                          unsigned long long limit_ns, int bar_id) {
+  return wait_bounded<false>(bar, parity, cta_abort, limit_ns, bar_id);
 }
 
 // A row-block is complete when its flag reaches kFlagComplete: set at once by the thread that stored the
