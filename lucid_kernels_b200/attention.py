@@ -399,6 +399,7 @@ def _step_plan(key, q, v, k_cache, v_cache, block_table, seq_lens, window, sinks
     if v is not None:
         assert 0.0 < k_scale < 1e18, "k_scale must be positive and finite"
         assert v.shape == (B, Hkv, _D), f"v must be ({B}, {Hkv}, {_D})"
+        assert Hq > 0, "a LUCID step needs query heads"       # (nothing would be launched, and the new row not written)
         assert Hq // Hkv <= 15, f"at most 15 query heads per key head, got {Hq // Hkv}"
         copy = copy or not _good_strides(v)
     desc = _cabi.PagedAttnDesc(cache, B, Hq, Hkv, _D, _cabi.dtype_code(q.dtype), w, s, scale, k_scale, _strides(q),

@@ -16,6 +16,7 @@ enum : int { kErrBadPage = 4 };
 struct AttnFwdArgs {
   AttnShape a;
   int split;              // (without lse) items are single tiles of queries whose keys are split between the CTA's two halves
+  int parts;              // (with split) CTAs of a cluster that share an item's keys: 1, 2, 4 or 8
   const int* lengths;     // (B) valid positions, or null
   void* out;              // (B, Nq, Hq, 128)
   Strides out_strides;
@@ -49,6 +50,8 @@ struct AttnStatArgs {
   float* stat;
 };
 
+// The most CTAs that share an item's keys, for few items of long lists (split, without lse).
+int fwd_parts(const AttnShape& a, bool bf16, int sms);
 cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                             const AttnFwdArgs& args, int sms, cudaStream_t stream);
 cudaError_t launch_attn_stat(bool bf16, const AttnStatArgs& args, cudaStream_t stream);

@@ -136,6 +136,7 @@ int lucid_window_attn_fwd(const lucid_window_attn_desc* d, const void* q, const 
   args.wait_ns = wait_limit_ns();
   // (inference) single tiles with split keys where all of them fit the SMs at once: a CTA then has half as many steps in a row
   args.split = !lse && fwd_items(args.a, true) <= sms ? 1 : 0;
+  args.parts = args.split ? fwd_parts(args.a, bf16, sms) : 1;
   return (int)launch_attn_fwd(bf16, tm_q, tm_k, tm_v, args, sms, static_cast<cudaStream_t>(cuda_stream));
 }
 

@@ -66,11 +66,58 @@ constexpr int kFwS = 0, kFwO = 256;      // + 128 * tile
 constexpr int kFwRegsService = 80, kFwRegsSoftmax = 176;    // 256 * 80 + 256 * 176 = 512 * 128, the launch's total
 constexpr float kFwSlack = 8.f;          // log2 of how far the maximum may outgrow the reference
 
+// A part's O in the ring: rows of 128 fp32, 16-byte pieces permuted by the row (threads of a warp write equal pieces of 32 rows)
+__device__ __forceinline__ uint32_t join_off(int row, int piece) { return row * 512 + ((piece ^ (row & 31)) << 4); }
+
+// This CTA's share of a tile's rows, joined from the parts of all CTAs of the cluster.  One warp per row, four columns per lane;
+// 8 warps call it.
+template <bool kBf16>
+__device__ __forceinline__ void join_rows(AttnFwdSmem& s, const AttnFwdArgs& args, int warp, int lane) {
+  typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
+  const AttnShape& A = args.a;
+  const int parts = args.parts, part = blockIdx.x % parts, per = kBlock / parts;
+  FwdItem it;
+  if (!fwd_item(A, true, blockIdx.x / parts, it)) return;
+  const int len = attn_length(A, args.lengths, it.b);
+  const uint32_t sums = smem_u32(s.ring[2]), tile = smem_u32(s.ring[0]);
+  elem_t* out = reinterpret_cast<elem_t*>(args.out) + it.b * args.out_strides.b + it.h0 * args.out_strides.h + 4 * lane;
+  for (int y = warp; y < per; y += 8) {
+    const int r = part * per + y, i = it.block0 * kBlock + r;
+    if (i >= A.Nq) break;
+    float l[8], ref[8], top = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      l[p] = 0.f;
+      ref[p] = -INFINITY;
+      if (p < parts) ld_cluster2(mapa_u32(sums + 8 * r, p), l[p], ref[p]);
+      top = fmaxf(top, ref[p]);
+    }
+    float sum = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      if (l[p] == 0.f) continue;            // (no weight: nothing was written there; a NaN sum goes on)
+      const float f = top == -INFINITY ? 1.f : ex2_approx(ref[p] - top);
+      float o[4];
+      ld_cluster4(mapa_u32(tile + join_off(r, lane), p), o);
+      sum += f * l[p];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[e] += f * o[e];
+    }
+    const bool some = i + A.off < len && sum != 0.f;
+    const float inv = some ? 1.f / sum : 0.f;
+    uint2 w = make_uint2(0u, 0u);
+    if (some) w = make_uint2(pack2<kBf16>(a[0] * inv, a[1] * inv), pack2<kBf16>(a[2] * inv, a[3] * inv));
+    *reinterpret_cast<uint2*>(out + (long long)i * args.out_strides.n) = w;
+  }
+}
+
 // The result is normalised by the sum of the weights as they are rounded, so that it is a mean of values even where one
 // weight is nearly all (the mixed-precision adds cost nothing measurable; unpacking the halves first took 8 % longer).
 // kTrain: lse is wanted, for a backward to come.  lse comes from the sum of the weights themselves, and what the rounding of the result
 // takes off is kept (if `rest` is given): delta = dO . O is subtracted from a nearly equal dO . v_j where a row is peaked.
-template <bool kBf16, bool kTrain>
+// kJoin: a cluster of `parts` CTAs owns one tile of queries, each CTA a run of its keys; they leave O (fp32, unnormalised),
+// sums and references in the ring, which is free by then, and each joins a share of the rows from all CTAs' shared memory.
+template <bool kBf16, bool kTrain, bool kJoin>
 __global__ void __launch_bounds__(kFwThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const AttnFwdArgs args) {
@@ -189,18 +236,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const int k = rnd % kFwSlots;
           if (!wait_lane(&s.slot_free[k], ((rnd / kFwSlots) & 1) ^ 1, cta_abort, limit, AF_SLOT_FREE)) break;
           FwdSlot& x = s.slot[k];
-          const bool more = fwd_item(A, split, snake_item(rnd, blockIdx.x, gridDim.x), it);
+          const bool more = kJoin ? rnd == 0 && fwd_item(A, true, blockIdx.x / args.parts, it)
+                                  : fwd_item(A, split, snake_item(rnd, blockIdx.x, gridDim.x), it);
           if (more) {
             x.len = attn_length(A, args.lengths, it.b);
             const PairTiles pt = pair_tiles(A, it, x.len);
-            x.n = pt.n;
+            const KeyTiles run = kJoin ? part_list(pt.x, blockIdx.x % args.parts, args.parts) : pt.x;
+            x.n = kJoin ? run.n : pt.n;
             x.b = it.b;
             x.hk = it.hk;
             x.sink = pt.sink;
             x.lo = pt.lo;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              const KeyTiles kt = split ? half_list(pt.x, t) : pt.list(t);
+              const KeyTiles kt = split ? half_list(run, t) : pt.list(t);
               FwdSlot::Tile& y = x.t[t];
               y.h = it.h(t);
               y.block = it.block(t);
@@ -382,6 +431,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (has) {
           uint32_t oa[16], ob[16];
           auto put = [&](const uint32_t (&o)[16], int c) {        // columns 16c .. 16c+15
+            if constexpr (kJoin) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint4*>(s.ring[0] + join_off(row, 4 * c + e)) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              return;
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               uint4 w = make_uint4(0, 0, 0, 0);
@@ -439,6 +494,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (kTrain && args.rest && !has) {
 #pragma unroll 1
           for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(rest + c * (kBlock * 8)) = make_uint4(0, 0, 0, 0);
+        }
+        if constexpr (kJoin) {
+          reinterpret_cast<float2*>(s.ring[2])[row] = has ? make_float2(l, ref) : make_float2(0.f, -INFINITY);
+          continue;
         }
         __syncwarp();
 #pragma unroll 1
@@ -618,22 +677,93 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (tid == 0) report_error(ctl, kErrBarrierTimeout, -1, -1, blockIdx.x, s.abort_flag);
   }
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (kJoin) {
+    __syncwarp();
+    cluster_sync_all();               // (also after an abort: every role comes here)
+    if (warp >= 8) join_rows<kBf16>(s, args, warp - 8, lane);
+    __syncwarp();
+    cluster_sync_all();               // nobody leaves while its memory is being read
+  } else {
+    __syncthreads();
+  }
   if (warp == 3) tmem_dealloc(tmem, 512);
+}
+
+template <bool kBf16>
+static cudaError_t join_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int items, int parts, cudaStream_t stream) {
+  const int bytes = (int)sizeof(AttnFwdSmem);
+  static SmemOnce once;
+  const cudaError_t e = once.set(reinterpret_cast<const void*>(attn_fwd_kernel<kBf16, false, true>), bytes);
+  if (e != cudaSuccess) return e;
+  cfg->gridDim = dim3(items * parts);
+  cfg->blockDim = dim3(kFwThreads);
+  cfg->dynamicSmemBytes = bytes;
+  cfg->stream = stream;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = parts;
+  attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = 1;
+  return cudaSuccess;
+}
+
+// How many clusters of `parts` CTAs the device holds at once (its groups of SMs are not multiples of 8); asked once.
+template <bool kBf16>
+static int clusters_at_once(int parts) {
+  static std::atomic<int> known[64][4];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::atomic<int>& k = known[dev][parts >= 8 ? 3 : parts >= 4 ? 2 : 1];
+  if ((n = k.load(std::memory_order_relaxed)) > 0) return n - 1;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  if (join_config<kBf16>(&cfg, attr, 1, parts, nullptr) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, attn_fwd_kernel<kBf16, false, true>, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  k.store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
+// Sharing a list costs a cluster launch and the join, some 4 us, and saves up to (1 - 1/parts) of the list's steps: as many CTAs
+// as there is room for, two tiles each or more, from 8 tiles on - for two CTAs, which save least, from 12 on.  One query on 65536
+// keys, 8 heads: 594 us alone, 85 us in eights; 256 queries on 2048 keys: 26 and 17 us in eights; 1024 queries on 4096 keys: 44 and
+// 32 us in twos; 4 tiles: 12.9 and 16 us in twos (alone it is); 1000 queries, 8 tiles: 17.7 and 18.5 us in twos.
+int fwd_parts(const AttnShape& a, bool bf16, int sms) {
+  const int items = fwd_items(a, true), list = longest_list(a);
+  if (list < 8) return 1;
+  int parts = 1;
+  while (parts < 8 && items * parts * 2 <= sms && list >= parts * 4 &&
+         items <= (bf16 ? clusters_at_once<true>(parts * 2) : clusters_at_once<false>(parts * 2)))
+    parts *= 2;
+  return parts == 2 && list < 12 ? 1 : parts;
+}
+
+template <bool kBf16>
+static cudaError_t launch_typed(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttnFwdArgs& args,
+                                int sms, cudaStream_t stream) {
+  const int items = fwd_items(args.a, args.split != 0), grid = items < sms ? items : sms;
+  const int bytes = (int)sizeof(AttnFwdSmem);
+  if (args.parts > 1) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    const cudaError_t e = join_config<kBf16>(&cfg, attr, items, args.parts, stream);
+    if (e != cudaSuccess) return e;
+    return cudaLaunchKernelEx(&cfg, attn_fwd_kernel<kBf16, false, true>, tm_q, tm_k, tm_v, args);
+  }
+  const bool train = args.lse != nullptr;
+  auto kernel = train ? attn_fwd_kernel<kBf16, true, false> : attn_fwd_kernel<kBf16, false, false>;
+  static SmemOnce once[2];
+  const cudaError_t e = once[train].set(reinterpret_cast<const void*>(kernel), bytes);
+  if (e != cudaSuccess) return e;
+  kernel<<<grid, kFwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, args);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_attn_fwd(bool bf16, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                             const AttnFwdArgs& args, int sms, cudaStream_t stream) {
-  const int items = fwd_items(args.a, args.split != 0), grid = items < sms ? items : sms;
-  const int bytes = (int)sizeof(AttnFwdSmem);
-  const bool train = args.lse != nullptr;
-  auto kernel = train ? (bf16 ? attn_fwd_kernel<true, true> : attn_fwd_kernel<false, true>)
-                      : (bf16 ? attn_fwd_kernel<true, false> : attn_fwd_kernel<false, false>);
-  static SmemOnce once[4];
-  cudaError_t e = once[2 * train + bf16].set(reinterpret_cast<const void*>(kernel), bytes);
-  if (e != cudaSuccess) return e;
-  kernel<<<grid, kFwThreads, bytes, stream>>>(tm_q, tm_k, tm_v, args);
-  return cudaGetLastError();
+  return bf16 ? launch_typed<true>(tm_q, tm_k, tm_v, args, sms, stream) : launch_typed<false>(tm_q, tm_k, tm_v, args, sms, stream);
 }
 
 cudaError_t attn_fwd_status(cudaStream_t stream, int out[8]) { return take_status(&g_attn_fwd_ctl, stream, out); }

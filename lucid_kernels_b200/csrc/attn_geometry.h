@@ -155,6 +155,20 @@ LUCID_HD KeyTiles half_list(const KeyTiles& t, int k) {
   }
   return h;
 }
+// And with fewer still the list is first dealt out in `parts` runs, one per CTA of a cluster.
+LUCID_HD KeyTiles part_list(const KeyTiles& t, int k, int parts) {
+  KeyTiles h = t;
+  const int from = (int)((long long)t.n * k / parts), to = (int)((long long)t.n * (k + 1) / parts);
+  h.n = to - from;
+  if (h.n == 0 || from > 0) h.sink = 0;
+  if (h.n > 0 && from > 0) h.lo = t.tile(from);
+  return h;
+}
+// The most key tiles a block of queries visits.
+LUCID_HD int longest_list(const AttnShape& a) {
+  const int near = a.W >= kNoWindow ? a.nkb : imin(a.nkb, (a.W + 253) / 128 + 1);
+  return near + (a.S > 0 ? 1 : 0);
+}
 // The union of the two tiles' lists, in increasing order; `active` says which of the two visits an entry.
 struct PairTiles {
   KeyTiles x, y;

@@ -81,6 +81,20 @@ static int check(const AttnShape& a, const std::vector<int>& lens) {
     if (x.n + y.n != t.n || x.n < y.n || x.n > y.n + 1) return 20;
     for (int e = 0; e < t.n; ++e)
       if ((e < x.n ? x.tile(e) : y.tile(e - x.n)) != t.tile(e)) return 21;
+    // runs for a cluster's CTAs: one after the other they make the list too
+    if (t.n > longest_list(a)) return 27;
+    for (int parts = 1; parts <= 8; parts *= 2) {
+      int at = 0;
+      for (int k = 0; k < parts; ++k) {
+        const KeyTiles run = part_list(t, k, parts);
+        const KeyTiles r0 = half_list(run, 0), r1 = half_list(run, 1);
+        if (run.n < 0 || run.n > t.n / parts + 1 || run.p_lo != t.p_lo || run.p_hi != t.p_hi || r0.n + r1.n != run.n) return 28;
+        for (int e = 0; e < run.n; ++e, ++at)
+          if (run.tile(e) != t.tile(at) || (e < r0.n ? r0.tile(e) : r1.tile(e - r0.n)) != t.tile(at)) return 29;
+        if (run.sink && !(t.sink && at == run.n)) return 30;
+      }
+      if (at != t.n) return 31;
+    }
   }
   if (n != fwd_items(a, true)) return 22;
   for (int v : halves)

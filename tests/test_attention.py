@@ -248,6 +248,38 @@ def test_window_attention_forward_and_backward(shape, dt):
 
 
 @gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("Nq,Nk,Hq,Hkv,window,sinks,lens", [
+    (1, 5000, 2, 1, None, 0, None),                       # one tile of queries, eight CTAs on its keys
+    (1, 65, 1, 1, None, 0, None),                         # too short to share
+    (300, 9000, 3, 1, None, 0, None),                     # nine tiles, eight CTAs each
+    (100, 4000, 8, 4, 1024, 4, None),
+    (130, 3100, 12, 2, 700, 128, None),                   # two CTAs each
+    (128, 1300, 1, 1, 900, 40, None),
+    (200, 2600, 2, 2, None, 0, [2600, 0, 1, 2400, 2401]), # no query, no key, the last row of a tile
+    (257, 3000, 2, 1, 1500, 3, [3000, 2800, 2999]),
+])
+def test_few_queries_of_long_sequences(Nq, Nk, Hq, Hkv, window, sinks, lens, dt):
+    """Inference: the keys of a tile of queries are dealt out to the CTAs of a cluster.  Stale rows hold NaN."""
+    from lucid_kernels_b200 import window_attention
+
+    B = len(lens) if lens else 1
+    q, k, v, do = make(B, Nq, Nk, Hq, Hkv, dt, seed=Nq + Nk)
+    lengths = None
+    if lens:
+        lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        for b, n in enumerate(lens):
+            k[b, n:] = v[b, n:] = float("nan")
+    scale = D ** -0.5
+    with torch.no_grad():
+        out = window_attention(q, k, v, window, sinks, scale, lengths)
+        again = window_attention(q, k, v, window, sinks, scale, lengths)
+    ref, bound = reference(q, torch.nan_to_num(k), torch.nan_to_num(v), window, sinks, scale, lens, do)[:2]
+    close(out, ref, bound, dt, "out")
+    assert torch.equal(out, again)
+
+
+@gpu
 @pytest.mark.parametrize("Hq,Hkv", [(4, 2), (5, 1), (1, 1)])
 @pytest.mark.parametrize("window,sinks,Nq", [(200, 4, 600), (None, 0, 600), (64, 128, 350), (0, 3, 600)])
 def test_padded_batch_ignores_whatever_stands_behind_the_sequences(window, sinks, Nq, Hq, Hkv):
@@ -491,6 +523,74 @@ def test_expired_waits_end_and_are_reported():
     again = _window_attention_fwd(q, k, v, 200, 4, check=True)
     assert torch.equal(again[0], out) and torch.equal(again[1], lse)
     assert all(torch.equal(x, y) for x, y in zip(grads, _window_attention_bwd(q, k, v, out, lse, rest, do, 200, 4, check=True)))
+
+
+@gpu
+def test_an_expired_wait_in_a_cluster_ends_it():
+    from lucid_kernels_b200 import _cabi
+    from lucid_kernels_b200.attention import _window_attention_fwd
+
+    lib = _cabi.load()
+    q, k, v, _ = make(1, 200, 4000, 2, 1, torch.bfloat16)
+    out = _window_attention_fwd(q, k, v, training=False, check=True)[0]
+    try:
+        lib.lucid_set_wait_limit_ns(0)
+        with pytest.raises(_cabi.LucidKernelError, match="timed out"):
+            _window_attention_fwd(q, k, v, training=False, check=True)
+    finally:
+        lib.lucid_set_wait_limit_ns(2_000_000_000)
+    assert torch.equal(_window_attention_fwd(q, k, v, training=False, check=True)[0], out)
+
+
+@gpu
+def test_calls_at_once_on_two_streams():
+    """Nothing is shared between calls: the same bits as one after another."""
+    from lucid_kernels_b200 import paged_lucid_attention
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+
+    a, c = make(1, 300, 3000, 4, 2, torch.bfloat16, seed=1), make(2, 900, 900, 8, 2, torch.bfloat16, seed=2)
+    pages, page = 40, 64
+    kc = torch.randn(pages, page, 2, D, device="cuda").bfloat16() * 0.1
+    vc = torch.randn(pages, page, 2, D, device="cuda").bfloat16()
+    table = torch.randperm(pages, device="cuda", dtype=torch.int32).view(1, -1)
+    lens = torch.tensor([2500], dtype=torch.int32, device="cuda")
+
+    def work():
+        x = _window_attention_fwd(*a[:3], None, 0, training=False)[0]
+        out, lse, rest = _window_attention_fwd(*c[:3], 300, 4)
+        grads = _window_attention_bwd(*c[:3], out, lse, rest, c[3], 300, 4)
+        pools = kc.clone(), vc.clone()
+        y = paged_lucid_attention(a[0][:, 0], a[1][:, 0], *pools, table, lens, k_scale=0.3, scale=0.1)
+        return [x, out, lse, *grads, y, pools[1]]
+
+    want = work()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(work())
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(x, y) for x, y in zip(g, want))
+    with pytest.raises(AssertionError, match="query heads"):
+        paged_lucid_attention(a[0][:, 0, :0], a[1][:, 0], kc, vc, table, lens)
+
+
+@gpu
+def test_one_tensor_as_queries_keys_and_values():
+    from lucid_kernels_b200 import window_attention
+
+    x, _, _, do = make(1, 300, 300, 2, 2, torch.bfloat16, seed=5)
+    leaves = [x.clone().requires_grad_() for _ in range(3)]
+    window_attention(*leaves, window=70, sinks=2).backward(do)
+    one = x.clone().requires_grad_()
+    window_attention(one, one, one, window=70, sinks=2).backward(do)
+    parts = [t.grad.double() for t in leaves]
+    # two additions in 16 bits, in any order: each off by u = 2^-8 of at most |dq| + |dk| + |dv|, and the first's error on top
+    u = torch.finfo(x.dtype).eps / 2
+    assert ((one.grad.double() - sum(parts)).abs() <= 2 * u * (1 + u) * sum(t.abs() for t in parts)).all()
 
 
 @gpu
