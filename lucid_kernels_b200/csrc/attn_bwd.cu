@@ -957,7 +957,7 @@ __global__ void __launch_bounds__(128) attn_first_keys_kernel(const AttnBwdArgs 
   typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
   wait_for_primary();
   const AttnShape& A = args.a;
-  const int j = blockIdx.x, which = blockIdx.y, bh = blockIdx.z, b = bh / A.Hkv, hk = bh % A.Hkv;
+  const int bh = blockIdx.x, which = blockIdx.y, j = blockIdx.z, b = bh / A.Hkv, hk = bh % A.Hkv;
   const float* p = args.partial + (((long long)bh * (1 + args.chunks) * 2 + which) * A.S + j) * 128 + threadIdx.x;
   const long long step = (long long)2 * A.S * 128;
   float sum = 0.f;
@@ -980,7 +980,7 @@ cudaError_t launch_attn_dkv(bool bf16, const CUtensorMap& tm_q, const CUtensorMa
   if (e != cudaSuccess) return e;
   e = launch_early(kernel, dim3(grid), kBwThreads, bytes, stream, tm_q, tm_k, tm_v, tm_do, args);
   if (e != cudaSuccess || args.chunks == 0) return e;
-  const dim3 sum_grid(a.S < a.Nk ? a.S : a.Nk, 2, a.B * a.Hkv);
+  const dim3 sum_grid(a.B * a.Hkv, 2, a.S < a.Nk ? a.S : a.Nk);     // (S <= 128; batch times heads may pass 65535)
   return launch_early(bf16 ? attn_first_keys_kernel<true> : attn_first_keys_kernel<false>, sum_grid, 128, 0, stream, args);
 }
 

@@ -579,6 +579,26 @@ def test_calls_at_once_on_two_streams():
 
 
 @gpu
+def test_first_keys_of_more_than_65535_heads():
+    """One query on its own key and the first one, for 8200 sequences of 8 heads."""
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+
+    B, H, Nk, dt = 8200, 8, 129, torch.bfloat16
+    q, k, v, do = make(B, 1, Nk, H, H, dt, seed=7)
+    out, lse, rest = _window_attention_fwd(q, k, v, 1, 1, 0.1, check=True)
+    dk, dv = _window_attention_bwd(q, k, v, out, lse, rest, do, 1, 1, 0.1, check=True)[1:]
+    u = torch.finfo(dt).eps / 2
+    for lo in range(0, B, 1025):
+        part = slice(lo, lo + 1025)
+        s = 0.1 * (q[part].double() * k[part, [0, -1]].double()).sum(-1, keepdim=True)
+        want = torch.softmax(s, 1) * do[part].double()
+        # the weight and the result are rounded (u each); the exponential and the sum of the weights add less than u
+        assert ((dv[part, [0, -1]].double() - want).abs() <= 3 * u * want.abs() + 1e-30).all()
+        assert torch.isfinite(dk[part]).all() and dk[part, [0, -1]].any()
+    assert not dv[:, 1:-1].any() and not dk[:, 1:-1].any()
+
+
+@gpu
 def test_one_tensor_as_queries_keys_and_values():
     from lucid_kernels_b200 import window_attention
 
