@@ -23,6 +23,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _cabi
@@ -42,6 +43,12 @@ _increment_version = torch.autograd.graph.increment_version
 
 def _new_like(t: torch.Tensor) -> torch.Tensor:
     return _empty_like(t) if t.is_contiguous() else _empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _refuse_tangents(name: str, *tensors) -> None:
+    """The kernels see values only: a forward-mode tangent (whose tensor need not require a gradient) would be lost."""
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 class _Plan:
@@ -263,9 +270,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     hold; their outputs and gradients are 0.  So are a query's that sees nothing.  Values at positions inside a sequence
     must be finite.
 
-    Differentiable in q, k and v (once); gradients come out the same on every run.  In a training step recorded into a CUDA
+    Differentiable in q, k and v (once, in reverse mode; forward-mode tangents are refused); gradients come out the same on every run.  In a training step recorded into a CUDA
     graph, record forward and backward together and, as torch asks for every operator, keep no eager graph of the same
     leaves alive while recording."""
+    _refuse_tangents("window_attention", q, k, v)
     if _grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return LUCIDWindowAttention.apply(q, k, v, window, sinks, scale, lengths)
     return _window_attention_fwd(q, k, v, window, sinks, scale, lengths, training=False)[0]
@@ -347,6 +355,7 @@ def paged_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tens
     ``position * inv_freq``, in pairs (i, i + r / 2), or (2i, 2i + 1) if ``interleaved``; the angle is formed in 64 bits.  q
     (T, Hq, 128) is rotated likewise and returned as a new tensor.  Tokens behind ``cu_seqlens[-1]`` are padding: nothing is
     written for them, their rows of the returned queries are 0.  A position without a page is skipped and reported."""
+    _refuse_tangents("paged_append", k, v, q, k_cache, v_cache, inv_freq)
     key = ("append", k.shape, k.stride(), k.dtype, k.get_device(), None if v is None else (v.shape, v.stride(), v.dtype, v.get_device()),
            None if q is None else (q.shape, q.stride(), q.dtype, q.get_device()), k_cache.shape, k_cache.stride(), k_cache.dtype,
            k_cache.get_device(), v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.get_device(), block_table.shape,
@@ -415,6 +424,7 @@ def paged_window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     """One decoding step of ``window_attention`` over a paged cache: q (B, Hq, 128) is the query of position
     ``seq_lens[b] - 1`` (int32, (B,); its key has been appended), which sees the last ``window`` positions and the first
     ``sinks``.  Returns (B, Hq, 128); 0 where ``seq_lens[b]`` is 0."""
+    _refuse_tangents("paged_window_attention", q, k_cache, v_cache)
     window, sinks, scale = _plain_options(window, sinks, scale)
     key = ("step", q.shape, q.stride(), q.dtype, q.get_device(), k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.get_device(),
            v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.get_device(), block_table.shape, block_table.stride(), block_table.dtype,
@@ -456,6 +466,7 @@ def paged_lucid_attention(q: torch.Tensor, v: torch.Tensor, k_cache: torch.Tenso
     ``t_j = k_scale ** 2 * k_n . k_j``, ``v'_n = exp(-t_n) v_n - sum_{j < n} exp(t_j - t_n) v'_j`` is written to position n of
     v_cache, and softmax attention with scores ``scale * q . k_j`` over j <= n of V' is returned, (B, Hq, 128).  At most 15
     query heads per key head.  ``seq_lens[b] = 0``: the row of the result is 0 and nothing is written."""
+    _refuse_tangents("paged_lucid_attention", q, v, k_cache, v_cache)
     _, _, scale = _plain_options(None, 0, scale)
     if type(k_scale) is not float:
         k_scale = float(k_scale)

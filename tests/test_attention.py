@@ -200,6 +200,39 @@ def test_refusals_of_the_python_layer():
         paged_lucid_attention(z(1, 4, D), z(1, 2, D), pool, z(4, 16, 1, D), table, lens)
 
 
+@pytest.mark.parametrize("mode", ["dual", "jvp"])
+def test_forward_mode_is_refused(mode):
+    """A tangent must not vanish: no operator has a forward-mode derivative.  (A dual tensor does not require a gradient.)"""
+    from torch.autograd import forward_ad
+
+    from lucid_kernels_b200 import paged_append, paged_lucid_attention, paged_window_attention, window_attention
+
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)
+    x, pool, new, row = z(1, 8, 2, D), z(4, 16, 2, D), z(1, 2, D), z(1, 4, D)
+    table, lens, freq = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32), z(64, dt=torch.float32)
+    calls = [
+        (x, lambda t: window_attention(t, x, x)), (x, lambda t: window_attention(x, t, x)), (x, lambda t: window_attention(x, x, t)),
+        (new, lambda t: paged_append(t, new, pool, pool, table, lens)), (new, lambda t: paged_append(new, t, pool, pool, table, lens)),
+        (pool, lambda t: paged_append(new, new, t, pool, table, lens)), (pool, lambda t: paged_append(new, new, pool, t, table, lens)),
+        (row, lambda t: paged_append(new, new, pool, pool, table, lens, q=t, inv_freq=freq)),
+        (freq, lambda t: paged_append(new, new, pool, pool, table, lens, inv_freq=t)),
+        (row, lambda t: paged_window_attention(t, pool, pool, table, lens)), (pool, lambda t: paged_window_attention(row, t, pool, table, lens)),
+        (pool, lambda t: paged_window_attention(row, pool, t, table, lens)),
+        (row, lambda t: paged_lucid_attention(t, new, pool, pool, table, lens)), (new, lambda t: paged_lucid_attention(row, t, pool, pool, table, lens)),
+        (pool, lambda t: paged_lucid_attention(row, new, t, pool, table, lens)), (pool, lambda t: paged_lucid_attention(row, new, pool, t, table, lens)),
+    ]
+    for at, call in calls:
+        with pytest.raises(NotImplementedError, match="forward-mode"), torch.no_grad():
+            if mode == "jvp":
+                torch.func.jvp(call, (at,), (torch.ones_like(at),))
+            else:
+                with forward_ad.dual_level():
+                    call(forward_ad.make_dual(at, torch.ones_like(at)))
+    # inside the mode, tensors without a tangent go their usual way (here to the check of the device)
+    with forward_ad.dual_level(), pytest.raises(AssertionError, match="CUDA"):
+        window_attention(x, x, x)
+
+
 # ------------------------------------------------------------------------------------------------ window attention
 SHAPES = [
     # B, Nq, Nk, Hq, Hkv, window, sinks
