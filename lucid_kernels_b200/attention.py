@@ -368,7 +368,7 @@ def paged_append(k: torch.Tensor, v: Optional[torch.Tensor], k_cache: torch.Tens
         plan = _append_plan(key, k, v, k_cache, v_cache, block_table, cache_lens, cu_seqlens, q, inv_freq, interleaved)
     if _grad_enabled():
         assert not (k.requires_grad or (v is not None and v.requires_grad) or (q is not None and q.requires_grad) or
-                    k_cache.requires_grad or v_cache.requires_grad), _NO_BACKWARD
+                    k_cache.requires_grad or v_cache.requires_grad or (inv_freq is not None and inv_freq.requires_grad)), _NO_BACKWARD
     kp, vp, qp = k.data_ptr(), None if v is None else v.data_ptr(), None if q is None else q.data_ptr()
     if plan.copy or (kp | (vp or 0) | (qp or 0)) & 15:
         own = lambda t: None if t is None else t.contiguous()

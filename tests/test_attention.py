@@ -233,6 +233,26 @@ def test_forward_mode_is_refused(mode):
         window_attention(x, x, x)
 
 
+def test_cache_operators_refuse_gradients_of_every_input(monkeypatch):
+    """(What a call's shapes determine is stubbed: the refusal comes before anything is launched.)"""
+    import lucid_kernels_b200.attention as A
+
+    monkeypatch.setattr(A, "_append_plan", lambda *a: A._Plan(A._cabi.PagedAppendDesc(), 0, False, True))
+    monkeypatch.setattr(A, "_step_plan", lambda *a: A._Plan(A._cabi.PagedAttnDesc(), 0, False, True))
+    monkeypatch.setattr(A, "_plans", {})
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)
+    pool, new, row, table, lens = z(4, 16, 2, D), z(1, 2, D), z(1, 4, D), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    append = [new, new.clone(), pool, pool.clone(), row, z(64, dt=torch.float32)]
+    step = [row, new, pool, pool.clone()]
+    calls = [(append, i, lambda k, v, kc, vc, q, f: A.paged_append(k, v, kc, vc, table, lens, q=q, inv_freq=f)) for i in range(6)] + \
+        [(step, i, lambda q, v, kc, vc: A.paged_lucid_attention(q, v, kc, vc, table, lens)) for i in range(4)] + \
+        [(step, i, lambda q, v, kc, vc: A.paged_window_attention(q, kc, vc, table, lens)) for i in (0, 2, 3)]
+    for inputs, i, call in calls:
+        args = [t.clone().requires_grad_(True) if x == i else t for x, t in enumerate(inputs)]
+        with pytest.raises(AssertionError, match="no backward"):
+            call(*args)
+
+
 # ------------------------------------------------------------------------------------------------ window attention
 SHAPES = [
     # B, Nq, Nk, Hq, Hkv, window, sinks
