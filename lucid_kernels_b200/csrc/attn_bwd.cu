@@ -515,10 +515,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   if (s.abort_flag) {
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-    if (tid == 0) report_error(ctl, kErrBarrierTimeout, -1, -1, blockIdx.x, s.abort_flag);
   }
   tc_fence_before_sync();
   __syncthreads();
+  // (reported once every role is here: this thread's own role may have ended long before another's wait ran out)
+  if (tid == 0 && s.abort_flag) report_error(ctl, kErrBarrierTimeout, -1, -1, blockIdx.x, s.abort_flag);
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
@@ -944,10 +945,11 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   if (s.abort_flag) {
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-    if (tid == 0) report_error(ctl, kErrBarrierTimeout, -1, -1, blockIdx.x, s.abort_flag);
   }
   tc_fence_before_sync();
   __syncthreads();
+  // (reported once every role is here: this thread's own role may have ended long before another's wait ran out)
+  if (tid == 0 && s.abort_flag) report_error(ctl, kErrBarrierTimeout, -1, -1, blockIdx.x, s.abort_flag);
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 

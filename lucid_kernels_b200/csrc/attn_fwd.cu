@@ -674,7 +674,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     // a role gave up: leave the copies and products in flight time to land before the CTA's memory goes
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-    if (tid == 0) report_error(ctl, kErrBarrierTimeout, -1, -1, blockIdx.x, s.abort_flag);
   }
   tc_fence_before_sync();
   if constexpr (kJoin) {
@@ -686,6 +685,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   } else {
     __syncthreads();
   }
+  // (reported once every role is here: this thread's own role may have ended long before another's wait ran out)
+  if (tid == 0 && s.abort_flag) report_error(ctl, kErrBarrierTimeout, -1, -1, blockIdx.x, s.abort_flag);
   if (warp == 3) tmem_dealloc(tmem, 512);
 }
 

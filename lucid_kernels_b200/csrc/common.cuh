@@ -90,7 +90,7 @@ __device__ __forceinline__ bool wait_barrier(uint64_t* bar, uint32_t parity, vol
 
 // The same wait in little code, for kernels whose roles wait in many places: a few polls before the clock is looked at for
 // the first time (reading the global timer costs a waiter some hundred cycles), and only the barrier's id is left behind
-// (through the CTA-wide abort word; the kernel reports it when it ends).  wait_lean is called by a whole warp, which gets
+// (through the CTA-wide abort word; the kernel reports it when all its roles have come to their end).  wait_lean is called by a whole warp, which gets
 // one answer: if lanes went their own ways when a limit runs out, some would wait for ever in a warp-wide instruction that
 // the others never reach.  wait_lane is called by one thread that has its role to itself.
 template <bool kWarp>

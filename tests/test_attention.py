@@ -595,6 +595,87 @@ def test_an_expired_wait_in_a_cluster_ends_it():
     assert torch.equal(_window_attention_fwd(q, k, v, training=False, check=True)[0], out)
 
 
+def attention_failed(lib):
+    """Whether an attention kernel has reported an error since the last look."""
+    import ctypes
+
+    status = (ctypes.c_int32 * 8)()
+    assert lib.lucid_attn_status(torch.cuda.current_stream().cuda_stream, status) == 0
+    assert status[0] in (0, 1, 3), list(status)
+    return status[0] != 0
+
+
+@gpu
+def test_a_wait_that_runs_out_at_the_very_end_is_reported():
+    """One tile of queries on more and more keys: the warps that write results wait for all of them.  With the shortest limit
+    above 0 (64 polls pass before the clock is looked at, and 64 more before the limit counts) that wait, and no other, runs
+    out from some number of keys on; next to that number it runs out when every other role has just ended.  A call that reports
+    nothing has given the right result, bit for bit."""
+    from lucid_kernels_b200 import _cabi
+    from lucid_kernels_b200.attention import _window_attention_fwd
+
+    lib, most = _cabi.load(), 1500
+    q, k, v, _ = make(1, 128, 128 * most, 1, 1, torch.bfloat16)
+    call = lambda n: _window_attention_fwd(q, k[:, :128 * n], v[:, :128 * n])[:2]
+    right = {}
+
+    def reported(n):
+        if n not in right:
+            lib.lucid_set_wait_limit_ns(2_000_000_000)
+            right[n] = call(n)
+            assert not attention_failed(lib)
+        lib.lucid_set_wait_limit_ns(1)
+        got = call(n)
+        bad = attention_failed(lib)
+        assert bad or all(torch.equal(x, y) for x, y in zip(got, right[n])), n
+        return bad
+
+    try:
+        lo, hi = 1, most
+        assert reported(hi)
+        while hi - lo > 1:
+            mid = (lo + hi) // 2
+            lo, hi = (lo, mid) if reported(mid) else (mid, hi)
+        for n in range(max(1, hi - 12), min(most, hi + 12) + 1):
+            for _ in range(8):
+                reported(n)
+    finally:
+        lib.lucid_set_wait_limit_ns(2_000_000_000)
+    assert all(torch.equal(x, y) for x, y in zip(call(hi), right[hi])) and not attention_failed(lib)
+
+
+@gpu
+@pytest.mark.parametrize("shape,window,sinks", [((1, 128, 128, 1, 1), None, 0), ((1, 100, 256, 2, 1), None, 0), ((1, 256, 256, 3, 1), 60, 3),
+                                                ((2, 300, 300, 2, 2), 100, 4), ((1, 64, 1536, 1, 1), None, 0), ((4, 256, 256, 80, 80), None, 0)])
+def test_with_no_time_to_wait_small_calls_are_right_or_report(shape, window, sinks):
+    from lucid_kernels_b200 import _cabi
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+
+    lib = _cabi.load()
+    q, k, v, do = make(*shape, torch.bfloat16)
+    out, lse, rest = _window_attention_fwd(q, k, v, window, sinks, check=True)
+    calls = [lambda: _window_attention_fwd(q, k, v, window, sinks)[:2],
+             lambda: _window_attention_fwd(q, k, v, window, sinks, training=False)[:1],
+             lambda: _window_attention_bwd(q, k, v, out, lse, rest, do, window, sinks),
+             lambda: _window_attention_bwd(q, k, v, out, lse, rest, do, window, sinks, need_dkv=False)[:1],
+             lambda: _window_attention_bwd(q, k, v, out, lse, rest, do, window, sinks, need_dq=False)[1:]]
+    right = [call() for call in calls]
+    assert not attention_failed(lib)
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    try:
+        lib.lucid_set_wait_limit_ns(0)
+        for n in range(10):
+            for i, call in enumerate(calls):
+                flush.fill_(n)                  # operands from memory: their loads take longest
+                got = call()
+                assert attention_failed(lib) or all(torch.equal(x, y) for x, y in zip(got, right[i])), i
+    finally:
+        lib.lucid_set_wait_limit_ns(2_000_000_000)
+    for call, ref in zip(calls, right):
+        assert all(torch.equal(x, y) for x, y in zip(call(), ref))
+    assert not attention_failed(lib)
+
+
 @gpu
 def test_calls_at_once_on_two_streams():
     """Nothing is shared between calls: the same bits as one after another."""
