@@ -88,6 +88,27 @@ __device__ __forceinline__ bool wait_barrier(uint64_t* bar, uint32_t parity, vol
   return true;
 }
 
+// The same for a whole warp, which gets one answer: lanes that went their own ways when a limit runs out would stand for
+// ever in a warp-wide instruction (tensor-memory access, elect, vote) that the others never reach.
+__device__ __forceinline__ bool wait_barrier_warp(uint64_t* bar, uint32_t parity, volatile int* cta_abort, Control* ctl,
+                                                  unsigned long long limit_ns, int chain, int row, int bar_id) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  unsigned long long t0 = 0;
+  uint32_t spins = 0;
+  while (limit_ns == 0 || !__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+    if ((++spins & 255u) != 0 && limit_ns != 0) continue;
+    if (__any_sync(0xffffffffu, *cta_abort != 0)) return false;
+    const unsigned long long t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    if (__any_sync(0xffffffffu, t - t0 >= limit_ns)) {
+      *cta_abort = 1;
+      report_error(ctl, kErrBarrierTimeout, chain, row, 0, bar_id);
+      return false;
+    }
+  }
+  return true;
+}
+
 // The same wait in little code, for kernels whose roles wait in many places: a few polls before the clock is looked at for
 // the first time (reading the global timer costs a waiter some hundred cycles), and only the barrier's id is left behind
 // (through the CTA-wide abort word; the kernel reports it when all its roles have come to their end).  wait_lean is called by a whole warp, which gets

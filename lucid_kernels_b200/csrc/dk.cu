@@ -44,6 +44,7 @@ struct DkSmem {
   uint64_t ki_full, ki_free, ai_full, ai_free;
   uint64_t s_full[2], g_full, g_free, w_ready[2], sbuf_free[2];
   uint64_t acc_full, acc_free;
+  uint64_t claimed, other_done, sums_left;     // split items
   uint64_t tk_full[2], tk_empty[2];
   int tk_slot[2];
   uint32_t tmem_base;
@@ -53,7 +54,8 @@ struct DkSmem {
 
 enum DkBar : int {
   DK_K_FULL = 201, DK_K_EMPTY, DK_Z_FULL, DK_Z_EMPTY, DK_KI_FULL, DK_KI_FREE, DK_AI_FULL, DK_AI_FREE, DK_S_FULL,
-  DK_G_FULL, DK_G_FREE, DK_ACC_FULL, DK_ACC_FREE, DK_TK_FULL, DK_TK_EMPTY, DK_SBUF_FREE, DK_W_READY
+  DK_G_FULL, DK_G_FREE, DK_ACC_FULL, DK_ACC_FREE, DK_TK_FULL, DK_TK_EMPTY, DK_SBUF_FREE, DK_W_READY,
+  DK_CLAIMED, DK_OTHER_DONE, DK_SUMS_LEFT
 };
 
 constexpr int kDkThreads = 384;
@@ -102,6 +104,9 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
     mbar_init(&s.g_free, 256);
     mbar_init(&s.acc_full, 1);
     mbar_init(&s.acc_free, 256);
+    mbar_init(&s.claimed, 1);
+    mbar_init(&s.other_done, 1);
+    mbar_init(&s.sums_left, 256);
     s.abort_flag = 0;
     mbar_fence_init();
   }
@@ -209,7 +214,7 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
       (void)leader;
       for (int it = 0; alive; ++it) {
         const int slot = it & 1;
-        if (!wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, DK_TK_FULL)) break;
+        if (!wait_barrier_warp(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, DK_TK_FULL)) break;
         const int ticket = s.tk_slot[slot];
         __syncwarp();
         mbar_arrive_w(&s.tk_empty[slot]);
@@ -219,15 +224,15 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
           const uint32_t gq = g + (q - q0);
           // G(gq-1) is in the registers of all 256 threads: the single G buffer is free again
           if (gq > 0 &&
-              !wait_barrier(&s.g_free, (gq - 1) & 1, cta_abort, ctl, limit, chain, i, DK_G_FREE)) { alive = false; break; }
+              !wait_barrier_warp(&s.g_free, (gq - 1) & 1, cta_abort, ctl, limit, chain, i, DK_G_FREE)) { alive = false; break; }
           if (leader) LUCID_TR(args.trace, 2, trc, 34, gq);
           // the A buffer changes from dV_i to V'_i at q == n_low; wait for the load that serves tile q
           if (dk_waits_a_at(q, q0, n_low)) {
-            if (!wait_barrier(&s.ai_full, swaps & 1, cta_abort, ctl, limit, chain, i, DK_AI_FULL)) { alive = false; break; }
+            if (!wait_barrier_warp(&s.ai_full, swaps & 1, cta_abort, ctl, limit, chain, i, DK_AI_FULL)) { alive = false; break; }
             ++swaps;
           }
           const uint32_t zs = gq & 1;
-          if (!wait_barrier(&s.z_full[zs], (gq >> 1) & 1, cta_abort, ctl, limit, chain, i, DK_Z_FULL)) { alive = false; break; }
+          if (!wait_barrier_warp(&s.z_full[zs], (gq >> 1) & 1, cta_abort, ctl, limit, chain, i, DK_Z_FULL)) { alive = false; break; }
           tc_fence_after_sync();
           if (leader) LUCID_TR(args.trace, 2, trc, 32, gq);
           const uint64_t db = d_zr0 + zs * (kTileBytes >> 4);
@@ -262,13 +267,13 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
       (void)leader;
       for (int it = 0; alive; ++it) {
         const int slot = it & 1;
-        if (!wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, DK_TK_FULL)) break;
+        if (!wait_barrier_warp(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, DK_TK_FULL)) break;
         const int ticket = s.tk_slot[slot];
         __syncwarp();
         mbar_arrive_w(&s.tk_empty[slot]);
         int chain, i, n_low, q0, q1;
         if (!item_geometry(ticket, chain, i, n_low, q0, q1)) break;
-        if (!wait_barrier(&s.ki_full, it & 1, cta_abort, ctl, limit, chain, i, DK_KI_FULL)) break;
+        if (!wait_barrier_warp(&s.ki_full, it & 1, cta_abort, ctl, limit, chain, i, DK_KI_FULL)) break;
         tc_fence_after_sync();
         if (leader) LUCID_TR(args.trace, 1, trc, 35, q1 - q0);
         for (int q = q0; q < q1; ++q) {
@@ -276,12 +281,12 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
           const uint32_t ks = gq % 3;
           const uint32_t buf = gq & 1;
           // W of two tiles ago lived in this buffer: its W*K_j product must have completed
-          if (!wait_barrier(&s.sbuf_free[buf], ((gq >> 1) & 1) ^ 1, cta_abort, ctl, limit, chain, i, DK_SBUF_FREE)) {
+          if (!wait_barrier_warp(&s.sbuf_free[buf], ((gq >> 1) & 1) ^ 1, cta_abort, ctl, limit, chain, i, DK_SBUF_FREE)) {
             alive = false;
             break;
           }
           if (leader) LUCID_TR(args.trace, 1, trc, 29, gq);
-          if (!wait_barrier(&s.k_full[ks], (gq / 3) & 1, cta_abort, ctl, limit, chain, i, DK_K_FULL)) { alive = false; break; }
+          if (!wait_barrier_warp(&s.k_full[ks], (gq / 3) & 1, cta_abort, ctl, limit, chain, i, DK_K_FULL)) { alive = false; break; }
           tc_fence_after_sync();
           if (leader) LUCID_TR(args.trace, 1, trc, 30, gq);
           const uint32_t dst = tmem + (buf ? kDkS1 : kDkS0);
@@ -315,7 +320,7 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
       (void)leader;
       for (int it = 0; alive; ++it) {
         const int slot = it & 1;
-        if (!wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, DK_TK_FULL)) break;
+        if (!wait_barrier_warp(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, DK_TK_FULL)) break;
         const int ticket = s.tk_slot[slot];
         __syncwarp();
         mbar_arrive_w(&s.tk_empty[slot]);
@@ -324,12 +329,12 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
         for (int q = q0; q < q1; ++q) {
           const uint32_t gq = g + (q - q0);
           // per-buffer barrier: the exp groups may be one tile ahead of this warp, never two on one buffer
-          if (!wait_barrier(&s.w_ready[gq & 1], (gq >> 1) & 1, cta_abort, ctl, limit, chain, i, DK_W_READY)) {
+          if (!wait_barrier_warp(&s.w_ready[gq & 1], (gq >> 1) & 1, cta_abort, ctl, limit, chain, i, DK_W_READY)) {
             alive = false;
             break;
           }
           if (q == q0 &&
-              !wait_barrier(&s.acc_free, (it & 1) ^ 1, cta_abort, ctl, limit, chain, i, DK_ACC_FREE)) {
+              !wait_barrier_warp(&s.acc_free, (it & 1) ^ 1, cta_abort, ctl, limit, chain, i, DK_ACC_FREE)) {
             alive = false;
             break;
           }
@@ -352,7 +357,7 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
         if (!alive) break;
         g += q1 - q0;
         // an item without tiles must not run ahead of the epilogue that still owns the previous phase
-        if (q1 == q0 && !wait_barrier(&s.acc_free, (it & 1) ^ 1, cta_abort, ctl, limit, chain, i, DK_ACC_FREE)) break;
+        if (q1 == q0 && !wait_barrier_warp(&s.acc_free, (it & 1) ^ 1, cta_abort, ctl, limit, chain, i, DK_ACC_FREE)) break;
         umma_commit_w(&s.acc_full);
       }
     }
@@ -363,6 +368,7 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
     const int row = ((warp & 3) << 5) + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     uint32_t g = 0;
+    uint32_t n_first = 0, n_second = 0;              // split items that finished first, second
     bool alive = true;
     int trc = 0;
     (void)trc;
@@ -370,7 +376,7 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
     (void)tr_lead;
     for (int it = 0; alive; ++it) {
       const int slot = it & 1;
-      if (!wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, DK_TK_FULL)) break;
+      if (!wait_barrier_warp(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, DK_TK_FULL)) break;
       const int ticket = s.tk_slot[slot];
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.tk_empty[slot]);
@@ -381,7 +387,7 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
         const uint32_t gq = g + (q - q0);
         const uint32_t s_tmem = lane_base + ((gq & 1) ? kDkS1 : kDkS0) + wg * 64;
         const uint32_t g_tmem = lane_base + kDkG + wg * 64;
-        if (!wait_barrier(&s.g_full, gq & 1, cta_abort, ctl, limit, chain, i, DK_G_FULL)) {
+        if (!wait_barrier_warp(&s.g_full, gq & 1, cta_abort, ctl, limit, chain, i, DK_G_FULL)) {
           alive = false;
           break;
         }
@@ -389,7 +395,7 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
         uint32_t gv0[32], gv1[32];
         tmem_ld32(g_tmem, gv0);
         tmem_ld32(g_tmem + 32, gv1);
-        if (!wait_barrier(&s.s_full[gq & 1], (gq >> 1) & 1, cta_abort, ctl, limit, chain, i, DK_S_FULL)) {
+        if (!wait_barrier_warp(&s.s_full[gq & 1], (gq >> 1) & 1, cta_abort, ctl, limit, chain, i, DK_S_FULL)) {
           alive = false;
           break;
         }
@@ -443,27 +449,34 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
       g += q1 - q0;
 
       // ---- epilogue: dK_i columns 64*wg .. +63 ----
-      if (!wait_barrier(&s.acc_full, it & 1, cta_abort, ctl, limit, chain, i, DK_ACC_FULL)) break;
+      if (!wait_barrier_warp(&s.acc_full, it & 1, cta_abort, ctl, limit, chain, i, DK_ACC_FULL)) break;
       tc_fence_after_sync();
       typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
       elem_t* out_row = reinterpret_cast<elem_t*>(args.dk) + (long long)b * args.dk_strides.b +
                         (long long)(i * kBlock + row) * args.dk_strides.n + (long long)h * args.dk_strides.h + wg * 64;
       // Split items: whichever half of the row-block finishes first leaves its fp32 sums in the workspace and
       // sets a flag; the other half waits for that flag (bounded; the first half is already in its epilogue
-      // when the second learns that it is second), adds the sums and writes dK_i.
+      // when the second learns that it is second), adds the sums and writes dK_i.  The eight warps meet on
+      // mbarriers, whose waits are bounded as well: a warp that has given up never comes to a named barrier.
       int order = -1;
       float* part_row = nullptr;
       const int rb = chain * T + i;
       if (args.split) {
         part_row = args.partial + ((long long)rb * kBlock + row) * kBlock + wg * 64;
-        if (tid == 128) s.claim = atomicAdd(args.sync + rb, 1);
-        named_bar_sync(1, 256);
+        if (tid == 128) {
+          s.claim = atomicAdd(args.sync + rb, 1);   // (every thread has read the claim of the item before: acc_free)
+          mbar_arrive(&s.claimed);
+        }
+        if (!wait_barrier_warp(&s.claimed, it & 1, cta_abort, ctl, limit, chain, i, DK_CLAIMED)) break;
         order = s.claim;
         if (order == 1) {
-          if (tid == 128 && !wait_flag(args.sync + P.C * T + rb, cta_abort, ctl, limit, chain, i, i, nullptr))
-            *cta_abort = 1;
-          named_bar_sync(1, 256);
-          if (*cta_abort) break;
+          bool there = true;
+          if (tid == 128) {
+            there = wait_flag(args.sync + P.C * T + rb, cta_abort, ctl, limit, chain, i, i, nullptr);
+            if (there) mbar_arrive(&s.other_done);
+          }
+          if (!__all_sync(0xffffffffu, there)) break;
+          if (!wait_barrier_warp(&s.other_done, n_second++ & 1, cta_abort, ctl, limit, chain, i, DK_OTHER_DONE)) break;
         }
       }
 #pragma unroll
@@ -515,10 +528,16 @@ __device__ __forceinline__ void dk_body(const CUtensorMap& tm_k,    // K,   box 
         }
       }
       if (order == 0) {
-        // every thread's sums are ordered before the flag: fence, meet, then one release store
+        // every thread's sums are ordered before the flag: fence, arrive, then one release store
         __threadfence();
-        named_bar_sync(1, 256);
-        if (tid == 128) st_release_gpu(args.sync + P.C * T + rb, kFlagComplete);
+        mbar_arrive(&s.sums_left);
+        bool left = true;
+        if (tid == 128) {
+          left = wait_barrier(&s.sums_left, n_first & 1, cta_abort, ctl, limit, chain, i, DK_SUMS_LEFT);
+          if (left) st_release_gpu(args.sync + P.C * T + rb, kFlagComplete);
+        }
+        ++n_first;
+        if (!__all_sync(0xffffffffu, left)) break;
       }
       tc_fence_before_sync();
       mbar_arrive(&s.acc_free);

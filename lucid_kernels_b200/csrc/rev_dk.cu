@@ -53,6 +53,7 @@ struct RevDkSmem {
   int tk_slot[2];
   uint32_t tmem_base;
   int abort_flag;
+  int leave_at;        // exp warps: the meeting after which one of them has left
 };
 
 enum RevDkBar : int {
@@ -116,6 +117,7 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
     mbar_init(&s.q_full, 1);
     mbar_init(&s.p_full, kRdExp);
     s.abort_flag = 0;
+    s.leave_at = 0x7fffffff;
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -255,9 +257,9 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRdRegsService));
     // =========================== the issuer of all products but S(1), S(2), ... ===========================
     // Program order per tile: G, then (as the exp groups deliver them) the products that read W and P; the next
-    // tile's G follows at once.  The tensor pipe runs one thread's products in order, so the G columns are never
+    // tile's G follows at once.  One thread has the role to itself, waits included.  The tensor pipe runs one thread's products in order, so the G columns are never
     // overwritten before the products that read W and P there have done so.
-    {
+    if (elect_one()) {
       constexpr int fmt = kBf16 ? 1 : 0;
       constexpr uint32_t idesc_kk = umma_idesc(fmt, 0, 0, 128, 128);    // both operands K-major
       constexpr uint32_t idesc_tb = umma_idesc(fmt, 0, 1, 128, 128);    // A from TMEM, B with rows = k
@@ -275,14 +277,11 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
       bool alive = true;
       int trc = 0;
       (void)trc;
-      const bool leader = lane == 0;
-      (void)leader;
       for (int it = 0; alive; ++it) {
         const int slot = it & 1;
         if (!wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, RD_TK_FULL)) break;
         const int ticket = s.tk_slot[slot];
-        __syncwarp();
-        mbar_arrive_w(&s.tk_empty[slot]);
+        mbar_arrive(&s.tk_empty[slot]);
         int chain, i, n;
         if (!item_geometry(ticket, chain, i, n)) break;
         if (!wait_barrier(&s.ki_full, it & 1, cta_abort, ctl, limit, chain, i, RD_KI_FULL)) break;
@@ -297,43 +296,43 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
           const uint32_t st = gt & 1;
           if (!wait_barrier(&s.kt_full[st], (gt >> 1) & 1, cta_abort, ctl, limit, chain, i, RD_KT_FULL)) return false;
           tc_fence_after_sync();
-          if (leader) LUCID_TR(args.trace, 2, trc, 18, gt);
+          LUCID_TR(args.trace, 2, trc, 18, gt);
           const uint64_t dbk = d_kr0 + st * (kTileBytes >> 4);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-            umma_ss_w(tmem + kRdS, d_ki + off, dbk + off, idesc_kk, k ? 1u : 0u);
+            umma_ss(tmem + kRdS, d_ki + off, dbk + off, idesc_kk, k ? 1u : 0u);
 #ifdef LUCID_TRACE_MMA
-            if (leader) LUCID_TR(args.trace, 2, trc, 50 + k, gt);
+            LUCID_TR(args.trace, 2, trc, 50 + k, gt);
 #endif
           }
-          umma_commit_w(&s.s_full);
-          if (leader) LUCID_TR(args.trace, 2, trc, 12, gt);
+          umma_commit(&s.s_full);
+          LUCID_TR(args.trace, 2, trc, 12, gt);
           return true;
         };
         if (n >= 1) {
           if (!issue_s(g)) break;
-          if (n == 1) umma_commit_w(&s.kt_empty[g & 1]);     // the newest predecessor's K_j has no other reader
+          if (n == 1) umma_commit(&s.kt_empty[g & 1]);     // the newest predecessor's K_j has no other reader
         }
         for (int q = 0; q + 1 < n; ++q, ++g) {
           const uint32_t st = g & 1;
           // ---- G(q) into region A (its previous readers, the products of the tile before, were issued above) ----
-          if (leader) LUCID_TR(args.trace, 2, trc, 9, g);
+          LUCID_TR(args.trace, 2, trc, 9, g);
           if (!wait_barrier(&s.vt_full[st], (g >> 1) & 1, cta_abort, ctl, limit, chain, i, RD_VT_FULL)) { alive = false; break; }
           tc_fence_after_sync();
-          if (leader) LUCID_TR(args.trace, 2, trc, 17, g);
+          LUCID_TR(args.trace, 2, trc, 17, g);
           const uint64_t dbv = d_vr0 + st * (kTileBytes >> 4);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-            umma_ss_w(tmem + kRdG, d_vpi + off, dbv + off, idesc_kk, k ? 1u : 0u);
+            umma_ss(tmem + kRdG, d_vpi + off, dbv + off, idesc_kk, k ? 1u : 0u);
 #ifdef LUCID_TRACE_MMA
-            if (leader) LUCID_TR(args.trace, 2, trc, 60 + k, g);
+            LUCID_TR(args.trace, 2, trc, 60 + k, g);
 #endif
           }
-          umma_commit_w(&s.g_full);
-          if (leader) LUCID_TR(args.trace, 2, trc, 10, g);
-          if (q == n - 2) umma_commit_w(&s.g_done);      // V'_i is no longer needed: X_i may take its buffer
+          umma_commit(&s.g_full);
+          LUCID_TR(args.trace, 2, trc, 10, g);
+          if (q == n - 2) umma_commit(&s.g_done);      // V'_i is no longer needed: X_i may take its buffer
           // (S(q+1) is issued by the other issuing warp as soon as every exp thread has S(q) in registers)
           // ---- ACC_dK += W K_j, then ACC_dV += P dV_j ----
           const uint64_t dbv_mn = d_vr0_mn + st * (kTileBytes >> 4);
@@ -351,20 +350,20 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
           // is made because this warp's products read the tile too
           if (!wait_barrier(&s.kt_full[st], (g >> 1) & 1, cta_abort, ctl, limit, chain, i, RD_KT_FULL)) { alive = false; break; }
           tc_fence_after_sync();
-          if (leader) LUCID_TR(args.trace, 2, trc, 13, g);
+          LUCID_TR(args.trace, 2, trc, 13, g);
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
-            umma_ts_w(tmem + kRdAccK, tmem + kRdW + 8 * ks, dbk_mn + ks * (2048 >> 4), idesc_tb, (q | ks) ? 1u : 0u);
-          umma_commit_w(&s.kt_empty[st]);
-          if (leader) LUCID_TR(args.trace, 2, trc, 14, g);
+            umma_ts(tmem + kRdAccK, tmem + kRdW + 8 * ks, dbk_mn + ks * (2048 >> 4), idesc_tb, (q | ks) ? 1u : 0u);
+          umma_commit(&s.kt_empty[st]);
+          LUCID_TR(args.trace, 2, trc, 14, g);
           if (!wait_barrier(&s.pw_full[1], gf & 1, cta_abort, ctl, limit, chain, i, RD_PW_FULL)) { alive = false; break; }
           tc_fence_after_sync();
-          if (leader) LUCID_TR(args.trace, 2, trc, 15, g);
+          LUCID_TR(args.trace, 2, trc, 15, g);
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
-            umma_ts_w(tmem + kRdAcc, tmem + kRdP + 8 * ks, dbv_mn + ks * (2048 >> 4), idesc_tb, (q | ks) ? 1u : 0u);
-          umma_commit_w(&s.vt_empty[st]);
-          if (leader) LUCID_TR(args.trace, 2, trc, 16, g);
+            umma_ts(tmem + kRdAcc, tmem + kRdP + 8 * ks, dbv_mn + ks * (2048 >> 4), idesc_tb, (q | ks) ? 1u : 0u);
+          umma_commit(&s.vt_empty[st]);
+          LUCID_TR(args.trace, 2, trc, 16, g);
           ++gf;
         }
         if (!alive) break;
@@ -375,8 +374,8 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
               !wait_barrier(&s.acck_free, (it & 1) ^ 1, cta_abort, ctl, limit, chain, i, RD_ACCK_FREE))
             break;
         }
-        umma_commit_w(&s.acc_full);
-        umma_commit_w(&s.acck_full);
+        umma_commit(&s.acc_full);
+        umma_commit(&s.acck_full);
         const uint32_t st_l = g & 1;               // ring stage of the newest predecessor (n >= 1)
         if (n >= 1) {
           // Q = X^T P_l into the S columns (every exp thread has read S_l and put P_l into shared memory)
@@ -385,11 +384,11 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
           tc_fence_after_sync();
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_ss_w(tmem + kRdS, desc_advance(d_x, k * 2048), desc_advance(d_pl, k * 2048), idesc_xt, k ? 1u : 0u);
-          umma_commit_w(&s.q_full);
-          umma_commit_w(&s.ki_free);
+            umma_ss(tmem + kRdS, desc_advance(d_x, k * 2048), desc_advance(d_pl, k * 2048), idesc_xt, k ? 1u : 0u);
+          umma_commit(&s.q_full);
+          umma_commit(&s.ki_free);
         } else {
-          mbar_arrive_w(&s.ki_free);
+          mbar_arrive(&s.ki_free);
         }
         // diagonal step: OUT = X^T rhs over ACC_dV
         if (!wait_barrier(&s.rhs_full, it & 1, cta_abort, ctl, limit, chain, i, RD_RHS_FULL)) break;
@@ -397,8 +396,8 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
         tc_fence_after_sync();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          umma_ss_w(tmem + kRdAcc, desc_advance(d_x, k * 2048), desc_advance(d_rhs, k * 2048), idesc_xt, k ? 1u : 0u);
-        umma_commit_w(&s.vx_free);
+          umma_ss(tmem + kRdAcc, desc_advance(d_x, k * 2048), desc_advance(d_rhs, k * 2048), idesc_xt, k ? 1u : 0u);
+        umma_commit(&s.vx_free);
         if (n >= 1) {
           // OUT += (-Q) dV_l: the only product that waits for the newest predecessor
           if (!wait_barrier(&s.p_full, nq & 1, cta_abort, ctl, limit, chain, i, RD_P_FULL)) break;
@@ -407,12 +406,12 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
           const uint64_t dbv_mn = d_vr0_mn + st_l * (kTileBytes >> 4);
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
-            umma_ts_w(tmem + kRdAcc, tmem + kRdS + 16 * ks, dbv_mn + ks * (2048 >> 4), idesc_tb, 1u);
-          umma_commit_w(&s.vt_empty[st_l]);
+            umma_ts(tmem + kRdAcc, tmem + kRdS + 16 * ks, dbv_mn + ks * (2048 >> 4), idesc_tb, 1u);
+          umma_commit(&s.vt_empty[st_l]);
           ++nq;
           ++g;
         }
-        umma_commit_w(&s.out_full);
+        umma_commit(&s.out_full);
       }
     }
   } else if (warp == 3) {
@@ -426,7 +425,7 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
     // this way no barrier has to say across warps that it is done.  This warp touches region B only between
     // s_loaded of a tile and s_full of the next, when the other warp has no product on it; it waits for every
     // s_loaded phase and for the ticket of every item, so no barrier it reads can run two phases ahead of it.
-    {
+    if (elect_one()) {
       constexpr int fmt = kBf16 ? 1 : 0;
       constexpr uint32_t idesc_kk = umma_idesc(fmt, 0, 0, 128, 128);
       const uint64_t d_ki = umma_smem_desc(smem_u32(s.ki), 16, 1024);
@@ -435,14 +434,11 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
       bool alive = true;
       int trc = 0;
       (void)trc;
-      const bool leader = lane == 0;
-      (void)leader;
       for (int it = 0; alive; ++it) {
         const int slot = it & 1;
         if (!wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, RD_TK_FULL)) break;
         const int ticket = s.tk_slot[slot];
-        __syncwarp();
-        mbar_arrive_w(&s.tk_empty[slot]);
+        mbar_arrive(&s.tk_empty[slot]);
         int chain, i, n;
         if (!item_geometry(ticket, chain, i, n)) break;
         for (int q = 1; q < n; ++q, ++gf) {
@@ -452,16 +448,16 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
           const uint32_t st = gt & 1;
           if (!wait_barrier(&s.kt_full[st], (gt >> 1) & 1, cta_abort, ctl, limit, chain, i, RD_KT_FULL)) { alive = false; break; }
           tc_fence_after_sync();
-          if (leader) LUCID_TR(args.trace, 5, trc, 18, gt);
+          LUCID_TR(args.trace, 5, trc, 18, gt);
           const uint64_t dbk = d_kr0 + st * (kTileBytes >> 4);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-            umma_ss_w(tmem + kRdS, d_ki + off, dbk + off, idesc_kk, k ? 1u : 0u);
+            umma_ss(tmem + kRdS, d_ki + off, dbk + off, idesc_kk, k ? 1u : 0u);
           }
-          umma_commit_w(&s.s_full);
-          if (q == n - 1) umma_commit_w(&s.kt_empty[st]);     // the newest predecessor: S_l is K_l's only reader
-          if (leader) LUCID_TR(args.trace, 5, trc, 12, gt);
+          umma_commit(&s.s_full);
+          if (q == n - 1) umma_commit(&s.kt_empty[st]);     // the newest predecessor: S_l is K_l's only reader
+          LUCID_TR(args.trace, 5, trc, 12, gt);
         }
         g0 += n;
       }
@@ -482,9 +478,15 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
     const bool tr_lead = tid == 128;
     (void)tr_lead;
     typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
+    // The groups meet on a named barrier in every full tile, and such a wait has no limit of its own.  So a warp that leaves,
+    // whyever, comes to one more meeting and says so before: the others find its number there and leave with it.  (A
+    // number, not a flag: what is said after a meeting is for the next one, however late somebody looks.)
+    volatile int* leave_at = &s.leave_at;
+    int meetings = 0;            // this warp has come to
+    bool told = false;
     for (int it = 0; alive; ++it) {
       const int slot = it & 1;
-      if (!wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, RD_TK_FULL)) break;
+      if (!wait_barrier_warp(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, RD_TK_FULL)) break;
       const int ticket = s.tk_slot[slot];
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.tk_empty[slot]);
@@ -496,7 +498,10 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
       // ---- full tiles: P = exp(S), W = -P o G for k-steps wg and 4 + wg (columns 16 wg .. and 64 + 16 wg ..) ----
       for (int q = 0; q + 1 < n; ++q, ++g, ++gf) {
         if (tr_lead) LUCID_TR(args.trace, 3, trc, 19, g);
-        if (!wait_barrier(&s.s_full, g & 1, cta_abort, ctl, limit, chain, i, RD_S_FULL)) { alive = false; break; }
+        // (a wait that runs out does not end the tile: the warp goes through it as one, on whatever stands there, and
+        // votes when it is done; votes at these two waits took 3 % longer)
+        bool ok = wait_barrier(&s.s_full, g & 1, cta_abort, ctl, limit, chain, i, RD_S_FULL);
+        __syncwarp();
         tc_fence_after_sync();
         if (tr_lead) LUCID_TR(args.trace, 3, trc, 20, g);
         uint32_t sv[32], gv[32];
@@ -510,7 +515,8 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
 #pragma unroll
         for (int e = 0; e < 32; ++e) ev[e] = ex2_approx(__uint_as_float(sv[e]) * xs);
         if (tr_lead) LUCID_TR(args.trace, 3, trc, 22, g);
-        if (!wait_barrier(&s.g_full, gf & 1, cta_abort, ctl, limit, chain, i, RD_G_FULL)) { alive = false; break; }
+        ok = wait_barrier(&s.g_full, gf & 1, cta_abort, ctl, limit, chain, i, RD_G_FULL) && ok;
+        __syncwarp();
         tc_fence_after_sync();
         if (tr_lead) LUCID_TR(args.trace, 3, trc, 23, g);
         tmem_ld16(lane_base + kRdG + 16 * wg, *reinterpret_cast<uint32_t(*)[16]>(&gv[0]));
@@ -519,6 +525,8 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
         // W and P are packed over G's columns, other threads' included: everybody holds its G values first
         if (tr_lead) LUCID_TR(args.trace, 3, trc, 24, g);
         named_bar_sync(2, kRdExp);
+        ++meetings;
+        const int leave = *leave_at;         // (read now, looked at when the tile is done: the answer is the same)
         if (tr_lead) LUCID_TR(args.trace, 3, trc, 25, g);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -544,12 +552,17 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
         tc_fence_before_sync();
         mbar_arrive(&s.pw_full[1]);
         if (tr_lead) LUCID_TR(args.trace, 3, trc, 27, g);
+        if (!__all_sync(0xffffffffu, ok && leave > meetings)) {
+          told = __any_sync(0xffffffffu, leave <= meetings);
+          alive = false;
+          break;
+        }
       }
       if (!alive) break;
 
       // ---- the newest predecessor: P_l to shared memory, Q back through the S columns ----
       if (n >= 1) {
-        if (!wait_barrier(&s.s_full, g & 1, cta_abort, ctl, limit, chain, i, RD_S_FULL)) break;
+        if (!wait_barrier_warp(&s.s_full, g & 1, cta_abort, ctl, limit, chain, i, RD_S_FULL)) break;
         tc_fence_after_sync();
         uint32_t v[32];
         tmem_ld16(lane_base + kRdS + 16 * wg, *reinterpret_cast<uint32_t(*)[16]>(&v[0]));
@@ -575,7 +588,7 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
         fence_proxy_async_smem();
         tc_fence_before_sync();
         mbar_arrive(&s.pq_full);
-        if (!wait_barrier(&s.q_full, nq & 1, cta_abort, ctl, limit, chain, i, RD_Q_FULL)) break;
+        if (!wait_barrier_warp(&s.q_full, nq & 1, cta_abort, ctl, limit, chain, i, RD_Q_FULL)) break;
         tc_fence_after_sync();
         tmem_ld16(lane_base + kRdS + 16 * wg, *reinterpret_cast<uint32_t(*)[16]>(&v[0]));
         tmem_ld16(lane_base + kRdS + 64 + 16 * wg, *reinterpret_cast<uint32_t(*)[16]>(&v[16]));
@@ -596,12 +609,12 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
       }
 
       // ---- epilogue, part 1: rhs = dV'_i - ACC_dV, this group's 32 output columns ----
-      if (!wait_barrier(&s.vi_full, it & 1, cta_abort, ctl, limit, chain, i, RD_VI_FULL)) break;
+      if (!wait_barrier_warp(&s.vi_full, it & 1, cta_abort, ctl, limit, chain, i, RD_VI_FULL)) break;
       uint4 vin[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) vin[c] = *reinterpret_cast<const uint4*>(my_rhs + sw128_off(row, vec0 + c));
       uint32_t acc[32];
-      if (!wait_barrier(&s.acc_full, it & 1, cta_abort, ctl, limit, chain, i, RD_ACC_FULL)) break;
+      if (!wait_barrier_warp(&s.acc_full, it & 1, cta_abort, ctl, limit, chain, i, RD_ACC_FULL)) break;
       if (n >= 2) {
         tc_fence_after_sync();
         tmem_ld32(lane_base + kRdAcc + wg * 32, acc);
@@ -626,7 +639,7 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
       mbar_arrive(&s.rhs_full);
 
       // ---- epilogue, part 2: dV_i = lam * (X^T rhs - Q dV_l), staged, stored, published ----
-      if (!wait_barrier(&s.out_full, it & 1, cta_abort, ctl, limit, chain, i, RD_OUT_FULL)) break;
+      if (!wait_barrier_warp(&s.out_full, it & 1, cta_abort, ctl, limit, chain, i, RD_OUT_FULL)) break;
       tc_fence_after_sync();
       tmem_ld32(lane_base + kRdAcc + wg * 32, acc);
       tmem_wait_ld();
@@ -676,6 +689,12 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
 #pragma unroll
       for (int c = 0; c < 8; ++c)
         *reinterpret_cast<uint4*>(up + c * 4) = make_uint4(acc[c * 4], acc[c * 4 + 1], acc[c * 4 + 2], acc[c * 4 + 3]);
+    }
+    __syncwarp();
+    if (!told) {
+      if (lane == 0) atomicMin(&s.leave_at, meetings + 1);
+      __syncwarp();
+      named_bar_sync(2, kRdExp);
     }
   }
 

@@ -387,15 +387,15 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
       (void)trc;
       for (int it = 0; alive; ++it) {
         const int slot = it & 1;
-        if (!wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, BAR_TK_FULL)) break;
+        if (!wait_barrier_warp(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, BAR_TK_FULL)) break;
         const int ticket = s.tk_slot[slot];
         __syncwarp();
         mbar_arrive_w(&s.tk_empty[slot]);
         int chain, i, n, jfirst;
         if (!item_geometry(ticket, chain, i, n, jfirst)) break;
         // K_i is in place: in shared memory, or (kKT) copied into tensor memory by the exp groups
-        if (kKT ? !wait_barrier(&s.kit_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_KIT_FULL)
-                : !wait_barrier(&s.ki_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_KI_FULL))
+        if (kKT ? !wait_barrier_warp(&s.kit_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_KIT_FULL)
+                : !wait_barrier_warp(&s.ki_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_KI_FULL))
           break;
         tc_fence_after_sync();
         if (leader) LUCID_TR(args.trace, 2, trc, 35, n);
@@ -403,7 +403,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
           const uint32_t gq = g + q;
           const uint32_t buf = gq % kNS;
           // the P*Y product of kNS tiles ago, which read P from this buffer, has completed
-          if (!wait_barrier(&s.sbuf_free[buf], ((gq / kNS) & 1) ^ 1, cta_abort, ctl, limit, chain, i, BAR_S_FREE)) {
+          if (!wait_barrier_warp(&s.sbuf_free[buf], ((gq / kNS) & 1) ^ 1, cta_abort, ctl, limit, chain, i, BAR_S_FREE)) {
             alive = false;
             break;
           }
@@ -413,7 +413,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
           for (int half = 0; half < 2; ++half) {
             const uint32_t u = gq * 2 + half;
             const uint32_t st = u & 3;
-            if (!wait_barrier(&s.k_full[st], (u >> 2) & 1, cta_abort, ctl, limit, chain, i, BAR_K_FULL)) {
+            if (!wait_barrier_warp(&s.k_full[st], (u >> 2) & 1, cta_abort, ctl, limit, chain, i, BAR_K_FULL)) {
               alive = false;
               break;
             }
@@ -463,7 +463,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
       (void)trc;
       for (int it = 0; alive; ++it) {
         const int slot = it & 1;
-        if (!wait_barrier(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, BAR_TK_FULL)) break;
+        if (!wait_barrier_warp(&s.tk_full[slot], (it >> 1) & 1, cta_abort, ctl, limit, -1, -1, BAR_TK_FULL)) break;
         const int ticket = s.tk_slot[slot];
         __syncwarp();
         mbar_arrive_w(&s.tk_empty[slot]);
@@ -474,16 +474,16 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
         // ACC (or OUT, with fold) += P[buf] * Y ring tile of tile gq
         auto issue_py = [&](uint32_t gq, bool first, bool fold) -> bool {
           const uint32_t buf = gq % kNS;
-          if (!wait_barrier(&s.p_full[buf], (gq / kNS) & 1, cta_abort, ctl, limit, chain, i, BAR_P_FULL)) return false;
+          if (!wait_barrier_warp(&s.p_full[buf], (gq / kNS) & 1, cta_abort, ctl, limit, chain, i, BAR_P_FULL)) return false;
           if (leader) LUCID_TR(args.trace, 5, trc, 32, gq);
-          if (first && !wait_barrier(&s.acc_free, (it & 1) ^ 1, cta_abort, ctl, limit, chain, i, BAR_ACC_FREE))
+          if (first && !wait_barrier_warp(&s.acc_free, (it & 1) ^ 1, cta_abort, ctl, limit, chain, i, BAR_ACC_FREE))
             return false;
           const uint32_t p_tmem = tmem + kTmemS + buf * 128;   // group g's P: columns g*kCols .. + kCols/2
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const uint32_t u = gq * 2 + half;
             const uint32_t st = u & 3;
-            if (!wait_barrier(&s.v_full[st], (u >> 2) & 1, cta_abort, ctl, limit, chain, i, BAR_V_FULL)) return false;
+            if (!wait_barrier_warp(&s.v_full[st], (u >> 2) & 1, cta_abort, ctl, limit, chain, i, BAR_V_FULL)) return false;
             // pair mode: the handed-over tile has arrived (second half), the peer may reuse its staging buffer
             if (kPair && fold && crank == 1 && half == 1 && elect_one())
               mbar_arrive_cluster(mapa_u32(smem_u32(&s.r_free), 0));
@@ -518,8 +518,8 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
         if (n_early == n_acc) umma_commit_w(&s.acc_full);
         if (via_q) {
           // Q = X(^T) P_l into the S buffer the last tile came from (its group has drained it)
-          if (!wait_barrier(&s.pq_full, nq & 1, cta_abort, ctl, limit, chain, i, BAR_PQ_FULL)) break;
-          if (!wait_barrier(&s.x_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_X_FULL)) break;
+          if (!wait_barrier_warp(&s.pq_full, nq & 1, cta_abort, ctl, limit, chain, i, BAR_PQ_FULL)) break;
+          if (!wait_barrier_warp(&s.x_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_X_FULL)) break;
           tc_fence_after_sync();
           const uint32_t q_tmem = tmem + kTmemS + ((g + n - 1) % kNS) * 128;
 #pragma unroll
@@ -536,11 +536,11 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
           umma_commit_w(&s.acc_full);
         }
         // diagonal step
-        if (!wait_barrier(&s.rhs_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_RHS_FULL)) break;
+        if (!wait_barrier_warp(&s.rhs_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_RHS_FULL)) break;
         tc_fence_after_sync();
         if (leader) LUCID_TR(args.trace, 5, trc, 36, 0);
         if (P.use_diag) {
-          if (!wait_barrier(&s.x_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_X_FULL)) break;
+          if (!wait_barrier_warp(&s.x_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_X_FULL)) break;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint64_t da = kReverse ? desc_advance(d_x, k * 2048)
@@ -606,7 +606,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
         // K_i, shared memory -> tensor memory: this thread's row, this group's kCols columns (kCols / 2 words of
         // 16-bit pairs).  The region's previous reader, the last S product of the item before, completed before
         // the load of this K_i was even issued.
-        if (!wait_barrier(&s.ki_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_KI_FULL)) break;
+        if (!wait_barrier_warp(&s.ki_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_KI_FULL)) break;
 #pragma unroll
         for (int c = 0; c < kCols / 32; ++c) {
           uint32_t w[16];
@@ -627,7 +627,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
         const uint32_t gq = g + q;
         const uint32_t buf = gq % kNS;
         const uint32_t ph = (gq / kNS) & 1;
-        if (!wait_barrier(&s.s_full[buf], ph, cta_abort, ctl, limit, chain, i, BAR_S_FULL)) {
+        if (!wait_barrier_warp(&s.s_full[buf], ph, cta_abort, ctl, limit, chain, i, BAR_S_FULL)) {
           alive = false;
           break;
         }
@@ -658,7 +658,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
           fence_proxy_async_smem();
           tc_fence_before_sync();
           mbar_arrive(&s.pq_full);          // all groups: S has been read, P_l is in shared memory
-          if (!wait_barrier(&s.q_full, nq & 1, cta_abort, ctl, limit, chain, i, BAR_Q_FULL)) {
+          if (!wait_barrier_warp(&s.q_full, nq & 1, cta_abort, ctl, limit, chain, i, BAR_Q_FULL)) {
             alive = false;
             break;
           }
@@ -711,7 +711,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
       // ---- epilogue: this group owns output columns kCols*wg .. + kCols-1 ----
       // Everything that does not depend on the accumulator is done before waiting for it: this
       // row-block's own right-hand side is read from shared memory now.
-      if (!wait_barrier(&s.vi_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_VI_FULL)) break;
+      if (!wait_barrier_warp(&s.vi_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_VI_FULL)) break;
       uint8_t* panel = my_rhs;
       uint4 vin[kVec];
 #pragma unroll
@@ -723,7 +723,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
                         (long long)(i * kBlock + row) * args.out_strides.n + (long long)h * args.out_strides.h +
                         wg * kCols;
       uint32_t acc[kCols];
-      if (!wait_barrier(&s.acc_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_ACC_FULL)) break;
+      if (!wait_barrier_warp(&s.acc_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_ACC_FULL)) break;
       if ((via_q ? n - 1 : n) > 0) {      // tiles accumulated before the diagonal product
         tc_fence_after_sync();
 #pragma unroll
@@ -764,7 +764,7 @@ __device__ __forceinline__ void solve_body(const CUtensorMap& tm_k,     // K, bo
       if (tr_lead) LUCID_TR(args.trace, 3 + wg, trc, 43, 0);
 
       if (P.use_diag) {
-        if (!wait_barrier(&s.out_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_OUT_FULL)) break;
+        if (!wait_barrier_warp(&s.out_full, it & 1, cta_abort, ctl, limit, chain, i, BAR_OUT_FULL)) break;
         tc_fence_after_sync();
         if (tr_lead) LUCID_TR(args.trace, 3 + wg, trc, 44, 0);
 #pragma unroll
