@@ -276,4 +276,20 @@ LUCID_HD QueryBlocks item_blocks(const AttnShape& a, const KvItem& it, int len) 
   return q;
 }
 
+// Single-token attention over a paged cache of `cap` positions: what the query at position len - 1 sees, positions 0 ..
+// first-1 and lo .. lo+near-1, counted through as 0 .. n-1.  A length beyond the cache (reported where the newest position is
+// looked up) moves the window like any other; the positions that do not exist are left out, not replaced by earlier ones.
+struct Visible {
+  int n, first, lo;
+  LUCID_HD int pos(int v) const { return v < first ? v : lo + v - first; }
+};
+LUCID_HD Visible cache_visible(int W, int S, int len, int cap) {
+  Visible v;
+  if (len < 0) len = 0;
+  v.lo = W < kNoWindow && W < len ? len - W : 0;
+  v.first = imin(imin(S, v.lo), cap);
+  v.n = v.first + imax(0, imin(len, cap) - v.lo);
+  return v;
+}
+
 }  // namespace lucid

@@ -35,21 +35,9 @@ struct PagedAttnSmem {
   float self[16];                                              // LUCID: row . k_n, unscaled
 };
 
-// What a sequence shows: positions 0 .. first-1 and lo .. lo+near-1, counted through as 0 .. n-1.
-struct Visible {
-  int n, first, lo;
-  __device__ __forceinline__ int pos(int v) const { return v < first ? v : lo + v - first; }
-};
+// What a sequence shows its newest query; LUCID: the rows before the newest one.
 __device__ __forceinline__ Visible visible(const PagedAttnArgs& a, bool lucid, int len) {
-  Visible v;
-  if (lucid) --len;                                            // the rows before the newest one
-  if (len < 0) len = 0;
-  // a length beyond the block table (reported where the newest position is looked up) does not make a longer loop
-  len = imin(len, a.c.table_width << a.c.page_shift);
-  v.lo = a.W < len ? len - a.W : 0;
-  v.first = a.S < v.lo ? a.S : v.lo;
-  v.n = v.first + len - v.lo;
-  return v;
+  return cache_visible(a.W, a.S, lucid ? len - 1 : len, a.c.table_width << a.c.page_shift);
 }
 __device__ __forceinline__ int chunk_keys(int n, int splits) {
   const int even = (n + splits - 1) / splits;

@@ -90,6 +90,20 @@ def make(B, Nq, Nk, Hq, Hkv, dt, seed=0):
 
 
 # ------------------------------------------------------------------------------------------------ host side
+def test_positions_a_single_token_query_sees(tmp_path):
+    import shutil
+
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no host compiler")
+    exe = str(tmp_path / "paged_visible")
+    subprocess.run([gxx, "-O2", "-std=c++17", "-I", os.path.join(ROOT, "lucid_kernels_b200", "csrc"), "-o", exe,
+                    os.path.join(ROOT, "tests", "host", "paged_visible.cpp")], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout
+    assert out.stdout.startswith("ok ")
+
+
 def test_tile_lists_cover_every_visible_pair_once(tmp_path):
     import shutil
 
@@ -971,6 +985,37 @@ def test_bad_pages_are_skipped_and_reported():
         paged_lucid_attention(q, x, kc, vc, table, n, check=True)
     n = torch.tensor([-5, 40], dtype=torch.int32, device="cuda")                  # and a negative one is none
     assert not paged_window_attention(q, kc, vc, table, n, check=True)[0].any()
+
+
+@gpu
+@pytest.mark.parametrize("width", [4, 600])                                       # a cluster's chunks, and more (two kernels)
+@pytest.mark.parametrize("window,sinks", [(40, 0), (40, 3), (5, 0), (0, 2), (1, 1), (8000, 5000)])
+def test_a_length_beyond_the_table_moves_the_window(window, sinks, width):
+    """Positions that do not exist are skipped: the query sees the rest of its window and the first keys, and no others."""
+    from lucid_kernels_b200 import _cabi, paged_window_attention
+
+    dt, page, Hq, Hkv = torch.bfloat16, 16, 4, 2
+    cap = width * page
+    over = [1, 20, window - 1, window, window + 1, 5 * cap, 2 ** 31 - 1 - cap]
+    lens = [cap] + [cap + max(0, n) for n in over]
+    B = len(lens)
+    kc, vc, table = pool_of(1, cap, page, Hkv, dt, seed=6)
+    table = table.expand(B, width)
+    q = torch.randn(B, Hq, D, device="cuda").to(dt)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = paged_window_attention(q, kc, vc, table, n, window=window, sinks=sinks, scale=0.1)
+    with pytest.raises(_cabi.LucidKernelError, match="block table"):
+        _cabi.raise_on_attention_error(torch.cuda.current_stream().cuda_stream, "step")
+    pos = torch.arange(cap, device="cuda")
+    pg = table[0].long()[pos // page]
+    kk, vv = kc[pg, pos % page].double(), vc[pg, pos % page].double()
+    for b, length in enumerate(lens):
+        seen = (pos >= length - window) | (pos < sinks)
+        for h in range(Hq):
+            s = q[b, h].double() @ kk[seen][:, h // 2].T * 0.1
+            v = vv[seen][:, h // 2]
+            ref, bound = (torch.softmax(s, -1) @ v, torch.softmax(s, -1) @ v.abs()) if int(seen.sum()) else (torch.zeros(D, device="cuda").double(),) * 2
+            close(got[b, h], ref, bound, dt, f"length {length}")
 
 
 def step_reference(q, kc, vc, table, lens, window, sinks, scale, v=None, k_scale=1.0):
