@@ -260,8 +260,8 @@ typedef struct {
   int64_t dout_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];  /* backward */
 } lucid_window_attn_desc;
 
-/* lse may be NULL (not wanted).  For a backward to come, `rest` (lucid_window_attn_rest_bytes(), 16-byte aligned, opaque;
- * NULL: not wanted) receives what the rounding of `out` to 16 bits took off; out, lse and rest then fit together so that
+/* lse may be NULL (not wanted).  For a backward to come, `rest` (lucid_window_attn_rest_bytes(): as many bytes as `out`, with
+ * Nq rounded up to whole blocks of 128 where it is longer than one; 16-byte aligned, opaque; NULL: not wanted) receives what the rounding of `out` to 16 bits took off; out, lse and rest then fit together so that
  * dO . out is accurate where one key has nearly all the weight. */
 size_t lucid_window_attn_rest_bytes(const lucid_window_attn_desc* desc);
 int lucid_window_attn_fwd(const lucid_window_attn_desc* desc, const void* q, const void* k, const void* v, void* out,

@@ -270,6 +270,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     hold; their outputs and gradients are 0.  So are a query's that sees nothing.  Values at positions inside a sequence
     must be finite.
 
+    For the backward a call keeps, besides its inputs and the result, a second tensor of the result's size (what the result's
+    rounding took off; Nq above 128 counts in whole blocks of 128) and 4 bytes per query and head.
+
     Differentiable in q, k and v (once, in reverse mode; forward-mode tangents are refused); gradients come out the same on every run.  In a training step recorded into a CUDA
     graph, record forward and backward together and, as torch asks for every operator, keep no eager graph of the same
     leaves alive while recording."""

@@ -20,7 +20,7 @@ struct AttnFwdArgs {
   const int* lengths;     // (B) valid positions, or null
   void* out;              // (B, Nq, Hq, 128)
   Strides out_strides;
-  void* rest;             // or null: (B, Hq, nqb, 16, 128, 8) 16-bit, what the rounding of `out` took off (needs lse)
+  void* rest;             // or null: (B, Hq, nqb, 16, rest_rows, 8) 16-bit, what the rounding of `out` took off (needs lse)
   float* lse;             // or null; (B, Hq, Nq) natural log of the row's sum of exponentials, -inf for an empty row
   float scale_log2;       // scale * log2(e)
   unsigned long long wait_ns;

@@ -143,7 +143,7 @@ int lucid_window_attn_fwd(const lucid_window_attn_desc* d, const void* q, const 
 size_t lucid_window_attn_rest_bytes(const lucid_window_attn_desc* d) {
   AttnShape a;
   if (make_shape(&a, d)) return 0;
-  return (size_t)a.B * a.Hq * a.nqb * kBlock * kBlock * 2;
+  return (size_t)a.B * a.Hq * a.nqb * rest_rows(a) * kBlock * 2;
 }
 
 size_t lucid_window_attn_bwd_workspace_bytes(const lucid_window_attn_desc* d) {

@@ -32,7 +32,8 @@ __global__ void __launch_bounds__(256) attn_stat_kernel(const AttnStatArgs args)
   const elem_t* o = reinterpret_cast<const elem_t*>(args.out) + b * args.out_strides.b + h * args.out_strides.h + ch * 8;
   const elem_t* g = reinterpret_cast<const elem_t*>(args.dout) + b * args.dout_strides.b + h * args.dout_strides.h + ch * 8;
   const long long tile = base >> 7;
-  const elem_t* rest = reinterpret_cast<const elem_t*>(args.rest) + tile * (16 * kBlock * 8) + ch * (kBlock * 8);
+  const int rest_step = rest_rows(A) * 8;
+  const elem_t* rest = reinterpret_cast<const elem_t*>(args.rest) + tile * 16 * rest_step + ch * rest_step;
 #pragma unroll
   for (int y = 0; y < kStatRows / 4; ++y) {
     const int r = 4 * y + (lane >> 3), i = i0 + r;
@@ -43,7 +44,7 @@ __global__ void __launch_bounds__(256) attn_stat_kernel(const AttnStatArgs args)
         const uint4 ov = *reinterpret_cast<const uint4*>(o + (long long)i * args.out_strides.n + 64 * c);
         const uint4 gv = *reinterpret_cast<const uint4*>(g + (long long)i * args.dout_strides.n + 64 * c);
         uint4 rv = make_uint4(0, 0, 0, 0);
-        if (args.rest) rv = *reinterpret_cast<const uint4*>(rest + 8 * c * (kBlock * 8) + (i & 127) * 8);
+        if (args.rest) rv = *reinterpret_cast<const uint4*>(rest + 8 * c * rest_step + (i & 127) * 8);
         const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w}, gw[4] = {gv.x, gv.y, gv.z, gv.w}, rw[4] = {rv.x, rv.y, rv.z, rv.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

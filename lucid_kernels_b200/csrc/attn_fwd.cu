@@ -427,7 +427,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         elem_t* out = reinterpret_cast<elem_t*>(args.out) + b * args.out_strides.b + h * args.out_strides.h + (lane & 7) * 8;
         const int r0 = block * kBlock + (warp & 3) * 32 + (lane >> 3);
         const uint32_t o_tmem = tmem + lanes + kFwO + 128 * t;
-        elem_t* rest = kTrain ? reinterpret_cast<elem_t*>(args.rest) + ((((long long)b * A.Hq + h) * A.nqb + block) * 16 * kBlock + row) * 8 : nullptr;
+        const int rest_step = rest_rows(A) * 8;
+        const bool keep = kTrain && args.rest && row < rest_rows(A);
+        elem_t* rest = keep ? reinterpret_cast<elem_t*>(args.rest) + (((long long)b * A.Hq + h) * A.nqb + block) * 16 * rest_step + row * 8 : nullptr;
         if (has) {
           uint32_t oa[16], ob[16];
           auto put = [&](const uint32_t (&o)[16], int c) {        // columns 16c .. 16c+15
@@ -447,7 +449,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 w.w = pack2<kBf16>(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
               }
               *reinterpret_cast<uint4*>(panel + (c >> 2) * 4096 + sw128_off(lane, 2 * (c & 3) + e)) = w;
-              if (kTrain && args.rest) {
+              if (kTrain && keep) {
                 const uint32_t hi[4] = {w.x, w.y, w.z, w.w};
                 uint32_t lo[4];
 #pragma unroll
@@ -455,7 +457,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                   const float2 h2 = unpack2<kBf16>(hi[y]);
                   lo[y] = some ? pack2<kBf16>(__uint_as_float(o[8 * e + 2 * y]) * inv - h2.x, __uint_as_float(o[8 * e + 2 * y + 1]) * inv - h2.y) : 0u;
                 }
-                *reinterpret_cast<uint4*>(rest + (2 * c + e) * (kBlock * 8)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                *reinterpret_cast<uint4*>(rest + (2 * c + e) * rest_step) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
               }
             }
           };
@@ -491,9 +493,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
           }
         }
-        if (kTrain && args.rest && !has) {
+        if (kTrain && keep && !has) {
 #pragma unroll 1
-          for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(rest + c * (kBlock * 8)) = make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(rest + c * rest_step) = make_uint4(0, 0, 0, 0);
         }
         if constexpr (kJoin) {
           reinterpret_cast<float2*>(s.ring[2])[row] = has ? make_float2(l, ref) : make_float2(0.f, -INFINITY);

@@ -21,6 +21,10 @@ struct AttnShape {
   int nqb, nkb;   // 128-row blocks of queries and keys
 };
 
+// Rows of a block in `rest` (what the rounding of the result took off): whole blocks, but no more rows than there are queries -
+// a few queries of many heads would otherwise keep up to 128 times what they need.
+LUCID_HD int rest_rows(const AttnShape& a) { return imin(a.Nq, 128); }
+
 // Key tiles of one block of 128 queries: an optional first tile 0 that holds only visible first keys, then lo .. hi.
 struct KeyTiles {
   int n;         // how many, 0 = no query of the block sees anything

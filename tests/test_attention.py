@@ -314,6 +314,44 @@ def test_window_attention_forward_and_backward(shape, dt):
         close(x, r, b, dt, name)
 
 
+def test_memory_kept_for_the_backward_is_of_the_size_of_the_result():
+    import ctypes
+
+    from lucid_kernels_b200 import _cabi
+
+    st = (ctypes.c_int64 * 3)(1 << 20, 1024, 128)
+    for Nq in (1, 2, 100, 127, 128, 129, 300, 4096):
+        d = _cabi.WindowAttnDesc(2, Nq, 5000, 6, 2, 128, 1, 300, 4, 0.1, *[st] * 8)
+        assert _cabi.load().lucid_window_attn_rest_bytes(ctypes.byref(d)) == 2 * 6 * (Nq if Nq < 128 else -(-Nq // 128) * 128) * 128 * 2
+
+
+@gpu
+@pytest.mark.parametrize("Nq", [1, 3, 8, 100, 127, 128, 129])
+def test_rest_stays_inside_its_memory(Nq):
+    """What the forward keeps for the backward: nothing is written behind it, whatever stood in it is not read, and gradients
+    of a few queries are as accurate as of many."""
+    import ctypes
+
+    from lucid_kernels_b200 import _cabi
+    from lucid_kernels_b200.attention import _window_attention_bwd
+
+    lib, dt, B, Nk, Hq, Hkv, window, sinks, scale = _cabi.load(), torch.bfloat16, 2, 400, 6, 2, 150, 3, 0.3
+    q, k, v, do = make(B, Nq, Nk, Hq, Hkv, dt, seed=Nq)
+    st = lambda t: (ctypes.c_int64 * 3)(*t.stride()[:3])
+    d = _cabi.WindowAttnDesc(B, Nq, Nk, Hq, Hkv, D, 1, window, sinks, scale, st(q), st(k), st(v), st(q), st(q), st(q), st(k), st(v))
+    n = lib.lucid_window_attn_rest_bytes(ctypes.byref(d))
+    out, lse = torch.empty_like(q), torch.empty(B, Hq, Nq, device="cuda")
+    memory = torch.full((n + 65536,), 255, dtype=torch.uint8, device="cuda")          # (16-bit NaNs)
+    assert lib.lucid_window_attn_fwd(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), memory.data_ptr(), lse.data_ptr(),
+                                     None, torch.cuda.current_stream().cuda_stream) == 0
+    assert bool((memory[n:] == 255).all())
+    ref, bound, _, grads, gb = reference(q, k, v, window, sinks, scale, None, do)
+    close(out, ref, bound, dt, "out")
+    got = _window_attention_bwd(q, k, v, out, lse, memory[:n], do, window, sinks, scale, check=True)
+    for name, x, r, b in zip(("dq", "dk", "dv"), got, grads, gb):
+        close(x, r, b, dt, name)
+
+
 @gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("Nq,Nk,Hq,Hkv,window,sinks,lens", [
