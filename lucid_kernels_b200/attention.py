@@ -53,7 +53,7 @@ def _refuse_tangents(name: str, *tensors) -> None:
 
 class _Plan:
     """What a call's shapes, strides, types and options determine."""
-    __slots__ = ("desc", "ref", "device", "copy", "empty", "workspace", "out_shape", "lse_shape", "hq")
+    __slots__ = ("desc", "ref", "device", "copy", "empty", "workspace", "rest", "out_shape", "lse_shape")
 
     def __init__(self, desc, device: int, copy: bool, empty: bool):
         self.desc, self.ref = desc, ctypes.byref(desc)
@@ -159,9 +159,11 @@ def _window_plan(key, q, k, v, out, dout, window, sinks, scale, lengths) -> _Pla
     desc.dq_strides, desc.dk_strides, desc.dv_strides = like_q, like_k, like_k
     plan = _Plan(desc, q.get_device(), copy, q.numel() == 0)
     plan.out_shape, plan.lse_shape = (B, Nq, Hq, D), (B, Hq, Nq)
-    plan.workspace = 0
-    if not plan.empty:       # backward: its scratch memory; forward: the size of `rest`
-        plan.workspace = getattr(_cabi.load(), "lucid_window_attn_rest_bytes" if dout is None else "lucid_window_attn_bwd_workspace_bytes")(plan.ref)
+    plan.workspace = plan.rest = 0
+    if not plan.empty:
+        plan.rest = _cabi.load().lucid_window_attn_rest_bytes(plan.ref)
+        if dout is not None:
+            plan.workspace = _cabi.load().lucid_window_attn_bwd_workspace_bytes(plan.ref)
     return _keep(key, plan)
 
 
@@ -187,7 +189,7 @@ def _window_attention_fwd(q, k, v, window: Optional[int] = None, sinks: int = 0,
     lse = rest = None
     if training:
         lse = _empty(plan.lse_shape, dtype=torch.float32, device=q.device)
-        rest = _empty(plan.workspace, dtype=_uint8, device=q.device)
+        rest = _empty(plan.rest, dtype=_uint8, device=q.device)
     if plan.empty:
         return out, lse, rest
     stream = _raw_stream(plan.device)
@@ -219,6 +221,8 @@ def _window_attention_bwd(q, k, v, out, lse, rest, dout, window: Optional[int] =
                                      None if lengths is None else lengths.contiguous(), need_dq=need_dq, need_dkv=need_dkv, check=check)
     assert lse.shape == plan.lse_shape and lse.dtype == torch.float32 and lse.device == q.device and lse.is_contiguous(), \
         "lse must be the forward's"
+    assert rest is None or (rest.numel() == plan.rest and rest.dtype == _uint8 and rest.device == q.device and rest.is_contiguous()), \
+        "rest must be the forward's"
     if _device_now() != plan.device:
         with torch.cuda.device(plan.device):
             return _window_attention_bwd(q, k, v, out, lse, rest, dout, window, sinks, scale, lengths, need_dq=need_dq, need_dkv=need_dkv,

@@ -314,6 +314,26 @@ def test_window_attention_forward_and_backward(shape, dt):
         close(x, r, b, dt, name)
 
 
+def test_backward_refuses_what_another_forward_kept(monkeypatch):
+    """(What the shapes determine is stubbed; the refusal comes before anything is launched.)"""
+    import lucid_kernels_b200.attention as A
+
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)
+    q, k = z(1, 8, 2, D), z(1, 8, 2, D)
+    plan = A._Plan(A._cabi.WindowAttnDesc(), q.get_device(), False, True)
+    plan.lse_shape, plan.rest, plan.workspace = (1, 2, 8), 8 * 2 * D * 2, 64
+    monkeypatch.setattr(A, "_window_plan", lambda *a: plan)
+    monkeypatch.setattr(A, "_plans", {})
+    monkeypatch.setattr(A, "_device_now", lambda: plan.device)
+    lse, rest = z(1, 2, 8, dt=torch.float32), z(plan.rest, dt=torch.uint8)
+    for bad_lse, bad_rest in [(z(1, 2, 9, dt=torch.float32), rest), (lse.double(), rest), (lse, rest[:-1]), (lse, z(2 * plan.rest, dt=torch.uint8)),
+                              (lse, z(2 * plan.rest, dt=torch.uint8)[::2]), (lse, z(plan.rest))]:
+        with pytest.raises(AssertionError, match="must be the forward's"):
+            A._window_attention_bwd(q, k, k, q, bad_lse, bad_rest, q)
+    A._window_attention_bwd(q, k, k, q, lse, rest, q)
+    A._window_attention_bwd(q, k, k, q, lse, None, q)
+
+
 def test_memory_kept_for_the_backward_is_of_the_size_of_the_result():
     import ctypes
 
