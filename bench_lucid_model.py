@@ -137,6 +137,8 @@ class Model:
 
         c = CFG
         B, N = ids.shape
+        assert B == cache.B and N <= cache.per * cache.page, f"the cache holds {cache.B} sequences of up to {cache.per * cache.page} positions"
+        assert not bool(cache.lens.any()), "the prompt's attention reads the prompt alone: the cache must be empty"
         D, Hq, Hkv = c["head_dim"], c["q_heads"], c["kv_heads"]
         x = self.embed[ids] * math.sqrt(c["hidden"])
         cu = torch.arange(B + 1, device=ids.device, dtype=torch.int32) * N

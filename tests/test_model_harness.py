@@ -19,6 +19,17 @@ def test_sliding_window_matches_dense_mask_cpu():
     assert float((out - ref).abs().max()) < 1e-5
 
 
+def test_prompt_needs_an_empty_cache_that_holds_it(monkeypatch):
+    m = importlib.import_module("bench_lucid_model")
+    monkeypatch.setitem(m.CFG, "layers", 2)
+    ids = torch.zeros(2, 48, dtype=torch.int64)
+    used, short, other = m.KVCache(2, 64, "cpu"), m.KVCache(2, 40, "cpu", page=8), m.KVCache(3, 64, "cpu")
+    used.lens[1] = 7
+    for cache, text in ((used, "empty"), (short, "up to 40 positions"), (other, "3 sequences")):
+        with pytest.raises(AssertionError, match=text):
+            m.Model.prefill_cached(None, ids, False, cache)
+
+
 @pytest.mark.gpu
 def test_reduced_model_runs_both_variants(monkeypatch):
     m = importlib.import_module("bench_lucid_model")
