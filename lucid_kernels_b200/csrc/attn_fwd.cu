@@ -33,15 +33,13 @@ struct FwdSlot {
   int n;                  // entries of the union, -1: no more items
   int b, hk, len, sink, lo;
   struct Tile {
-    int h, block, n;      // n: entries of its own
-    int first;            // entry 0 is its own, for the visible first keys
-    int from, to;         // and the entries from .. to-1
-    int sink, lo, p_lo, p_hi;
+    int h, block;
+    KeyTiles list;        // its own entries
+    OwnEntries own;       // which of the union's they are (not split)
   } t[2];
   __device__ __forceinline__ int tile(int u, bool split) const {
     if (!split) return u < sink ? 0 : lo + u - sink;
-    const Tile& y = t[u & 1];
-    return (u >> 1) < y.sink ? 0 : y.lo + (u >> 1) - y.sink;
+    return split_entry(t[0].list, t[1].list, u);
   }
 };
 struct AttnFwdSmem {
@@ -211,7 +209,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             return true;
           };
           for (int t = 0; t < 2; ++t) {
-            if (it->t[t].n == 0) continue;
+            if (it->t[t].list.n == 0) continue;
             if (!wait_lane(&s.q_free[t], (nq[t] & 1) ^ 1, cta_abort, limit, AF_Q_FREE)) {
               alive = false;
               break;
@@ -253,14 +251,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               FwdSlot::Tile& y = x.t[t];
               y.h = it.h(t);
               y.block = it.block(t);
-              y.n = kt.n;
-              y.first = kt.n > 0 && kt.sink;
-              y.from = kt.n > kt.sink ? kt.lo - pt.lo + pt.sink : 0;
-              y.to = y.from + (kt.n > kt.sink ? kt.n - kt.sink : 0);
-              y.sink = kt.sink;
-              y.lo = kt.lo;
-              y.p_lo = kt.p_lo;
-              y.p_hi = kt.p_hi;
+              y.list = kt;
+              y.own = own_entries(kt, pt.lo, pt.sink);
             }
           } else {
             x.n = -1;
@@ -356,13 +348,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         while (alive) {
           const FwdSlot* it = next(true);
           if (!it) break;
-          const int n = it->n, own = it->t[t].n, own_first = it->t[t].first, from = it->t[t].from, to = it->t[t].to;
+          const int n = it->n, count = it->t[t].list.n;
+          const OwnEntries own = it->t[t].own;
           done(true);
-          const bool narrow0 = own_first && A.S <= kNarrow;       // (tile_narrow)
+          const bool narrow0 = own.first && A.S <= kNarrow;       // (tile_narrow)
           int at = 0;
           for (int u = 0; u < n && alive; ++u) {
-            const bool act = split ? (u & 1) == t : (u == 0 && own_first) || (u >= from && u < to);
-            alive = step(true, act, at == 0, at == own - 1, narrow0 && u == 0);
+            const bool act = split ? (u & 1) == t : own.has(u);
+            alive = step(true, act, at == 0, at == count - 1, narrow0 && u == 0);
             if (act) ++at;
           }
         }
@@ -389,11 +382,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       for (int t = 0; t < 2; ++t) {
         const int block = it->t[t].block, h = it->t[t].h;
         if (block >= A.nqb || (split && t)) continue;
-        const bool has = it->t[t].n > 0;
+        const bool has = it->t[t].list.n > 0;
         const int i = block * kBlock + row;
         float l = 0.f, ref = 0.f;
         // split: the other half's sum and reference, and the factors that bring both halves to a common reference
-        const bool two = split && it->t[1].n > 0;
+        const bool two = split && it->t[1].list.n > 0;
         float f0 = 1.f, f1 = 0.f;
         if (two) {
           if (!wait_lean(&s.l_full[1], no1 & 1, cta_abort, limit, AF_L_FULL)) { alive = false; break; }
@@ -533,12 +526,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const FwdSlot* it = next();
       if (!it) break;
       const int len = it->len, u_sink = it->sink, u_lo = it->lo, u_n = it->n;
-      KeyTiles kt;
-      kt.n = it->t[t].n;
-      kt.sink = it->t[t].sink;
-      kt.lo = it->t[t].lo;
-      kt.p_lo = it->t[t].p_lo;
-      kt.p_hi = it->t[t].p_hi;
+      const KeyTiles kt = it->t[t].list;
       const int p = it->t[t].block * kBlock + row + A.off;
       done(false);
       float ref = -INFINITY, l16 = 0.f;                // l16: the sum of the weights as they are rounded

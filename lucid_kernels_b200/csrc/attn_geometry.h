@@ -173,18 +173,30 @@ LUCID_HD int longest_list(const AttnShape& a) {
   const int near = a.W >= kNoWindow ? a.nkb : imin(a.nkb, (a.W + 253) / 128 + 1);
   return near + (a.S > 0 ? 1 : 0);
 }
+// Entry u of such a run goes to tile u & 1, as the next of its half.
+LUCID_HD int split_entry(const KeyTiles& half0, const KeyTiles& half1, int u) { return (u & 1 ? half1 : half0).tile(u >> 1); }
+
+// The entries of a union of two lists that are one list's own: entry 0 for the visible first keys, and from .. to-1.
+struct OwnEntries {
+  int first, from, to;
+  LUCID_HD bool has(int u) const { return (u == 0 && first) || (u >= from && u < to); }
+};
+LUCID_HD OwnEntries own_entries(const KeyTiles& own, int union_lo, int union_sink) {
+  OwnEntries e;
+  const int near = own.n - own.sink;
+  e.first = own.n > 0 && own.sink;
+  e.from = near > 0 ? own.lo - union_lo + union_sink : 0;
+  e.to = e.from + (near > 0 ? near : 0);
+  return e;
+}
+
 // The union of the two tiles' lists, in increasing order; `active` says which of the two visits an entry.
 struct PairTiles {
   KeyTiles x, y;
   int n, sink, lo;
   LUCID_HD KeyTiles list(int k) const { return k ? y : x; }
   LUCID_HD int tile(int u) const { return u < sink ? 0 : lo + u - sink; }
-  LUCID_HD bool active(const KeyTiles& t, int u) const {
-    const int j = tile(u);
-    if (t.n == 0) return false;
-    if (j == 0 && t.sink) return true;
-    return u >= sink && j >= t.lo && j < t.lo + t.n - t.sink;
-  }
+  LUCID_HD bool active(const KeyTiles& t, int u) const { return own_entries(t, lo, sink).has(u); }
 };
 LUCID_HD PairTiles pair_tiles(const AttnShape& a, const FwdItem& it, int len) {
   PairTiles p;

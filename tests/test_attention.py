@@ -104,6 +104,20 @@ def test_positions_a_single_token_query_sees(tmp_path):
     assert out.stdout.startswith("ok ")
 
 
+def test_entries_of_split_lists_are_in_order(tmp_path):
+    import shutil
+
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no host compiler")
+    exe = str(tmp_path / "attn_entries")
+    subprocess.run([gxx, "-O2", "-std=c++17", "-I", os.path.join(ROOT, "lucid_kernels_b200", "csrc"), "-o", exe,
+                    os.path.join(ROOT, "tests", "host", "attn_entries.cpp")], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout
+    assert out.stdout.startswith("ok ")
+
+
 def test_tile_lists_cover_every_visible_pair_once(tmp_path):
     import shutil
 
