@@ -4,7 +4,7 @@
 //
 // One pass over the keys with a running maximum m and sum l per row; O is kept in tensor memory relative to a
 // reference maximum that is only moved when the running one has outgrown it by 2^8 (exact in the end: O and l share
-// the reference, and 2^8 is far from the limits of fp32 sums and 16-bit weights).
+// the reference, and 2^8, for fp16 2^15 (kTopWeight), is inside the limits of fp32 sums and 16-bit weights).
 //
 // A CTA works on two tiles of 128 queries that read the same keys (two heads of a key head, or two neighbouring
 // blocks), so a key/value tile brought into shared memory feeds four products.  Per tile of queries: S (fp32, 128
@@ -580,12 +580,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[c][e]));
           }
           const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-          const bool grow = m > ref + kFwSlack;
+          const float top = m - kTopWeight<kBf16>;
+          const bool grow = top > ref + kFwSlack;
           if (x == 0) {
-            ref = m;
+            ref = top;
           } else if (__any_sync(0xffffffffu, grow)) {
             // S(u) is complete, and with it every product issued before it: O holds all earlier tiles
-            const float next = fmaxf(ref, m);
+            const float next = fmaxf(ref, top);
             const float f = next == -INFINITY ? 1.f : ex2_approx(ref - next);
             ref = next;
             l16 *= f;

@@ -230,6 +230,12 @@ __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
+// log2 of the weight that a softmax's reference key gets.  fp16 loses bits below 2^-14 and ends at 2^-25: beside a key of
+// weight 1 the rest of a long row, each key at 2^-25 or less, would vanish, 0.1 % of the result at 65536 keys; 2^7 higher it
+// does not matter, and 2^16 is still out of reach.  bf16 has fp32's range.
+template <bool kBf16>
+constexpr float kTopWeight = kBf16 ? 0.f : 7.f;
+
 __device__ __forceinline__ uint64_t desc_advance(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 
 }  // namespace lucid

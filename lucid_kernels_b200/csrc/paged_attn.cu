@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, kPagedPerSm) paged_attn_kernel(
         acc[n][3] *= f1;
       }
     }
-    const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+    const float z0 = m0 == -INFINITY ? 0.f : m0 - kTopWeight<kBf16>, z1 = m1 == -INFINITY ? 0.f : m1 - kTopWeight<kBf16>;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       sa[e] = ex2_approx(sa[e] - z0);
@@ -299,9 +299,9 @@ __global__ void __launch_bounds__(kPaWarps * 32, kPagedPerSm) paged_attn_kernel(
     *reinterpret_cast<float2*>(mine + r1 * 128 + col) = make_float2(acc[n][2], acc[n][3]);
   }
   if ((lane & 3) == 0) {
-    s.ml[warp][r0][0] = m0;
+    s.ml[warp][r0][0] = m0 - kTopWeight<kBf16>;        // (what the sums are relative to)
     s.ml[warp][r0][1] = l0;
-    s.ml[warp][r1][0] = m1;
+    s.ml[warp][r1][0] = m1 - kTopWeight<kBf16>;
     s.ml[warp][r1][1] = l1;
   }
   __syncthreads();

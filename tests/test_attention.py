@@ -552,6 +552,35 @@ def test_extreme_scores_and_growing_maxima():
 
 
 @gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("N,drop", [(16384, 25.25), (65536, 20), (65536, 25.25), (65536, 28)])
+def test_many_small_weights_beside_a_large_one(N, drop, dt):
+    """One key outweighs each of the others by 2^drop, all of them together weigh up to 0.2 % of it: they count, although each
+    alone is below what 16 bits hold beside 1."""
+    from lucid_kernels_b200 import paged_window_attention
+    from lucid_kernels_b200.attention import _window_attention_fwd
+
+    Nq, Hq, scale, page = 128, 160, math.log(2.0), 64
+    g = torch.Generator(device="cuda")
+    g.manual_seed(7)
+    q, k = torch.zeros(1, Nq, Hq, D, device="cuda", dtype=dt), torch.zeros(1, N, 1, D, device="cuda", dtype=dt)
+    v = (torch.randn(1, N, 1, D, device="cuda", generator=g).abs() + 1).to(dt)
+    v[:, 0] = -1
+    q[..., 0], k[:, 0, 0, 0] = 1, drop
+    s = (q[0, :, 0].double() @ k[0, :, 0].double().T * scale).masked_fill(~visible(Nq, N, None, 0, N, "cuda"), -math.inf)
+    P, V = torch.softmax(s, -1), v[0, :, 0].double()
+    ref, bound = P @ V, P @ V.abs()
+    for heads in (1, 2, Hq):              # keys split or not, one tile of queries or two to a CTA
+        for training in (True, False):
+            out = _window_attention_fwd(q[:, :, :heads], k, v, scale=scale, training=training, check=True)[0]
+            for h in (0, heads - 1):
+                close(out[0, :, h], ref, bound, dt, f"{heads} heads, training {training}")
+    kc, vc = k.view(N // page, page, 1, D), v.view(N // page, page, 1, D)
+    table, n = torch.arange(N // page, device="cuda", dtype=torch.int32)[None], torch.tensor([N], device="cuda", dtype=torch.int32)
+    close(paged_window_attention(q[:, -1, :4].contiguous(), kc, vc, table, n, scale=scale, check=True)[0], ref[-1].expand(4, D), bound[-1].expand(4, D), dt, "paged")
+
+
+@gpu
 def test_runs_are_identical_and_graphs_replay():
     from lucid_kernels_b200 import window_attention
 
