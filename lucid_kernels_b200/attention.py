@@ -277,6 +277,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     For the backward a call keeps, besides its inputs and the result, a second tensor of the result's size (what the result's
     rounding took off; Nq above 128 counts in whole blocks of 128) and 4 bytes per query and head.
 
+    In fp16 the gradient of a score, weight * (dout.v - dout.out), is rounded where it stands: below 2^-14 it loses bits and above
+    65504 it overflows, as fp16 training does elsewhere - scale the loss accordingly.  bf16 has fp32's range.
+
     Differentiable in q, k and v (once, in reverse mode; forward-mode tangents are refused); gradients come out the same on every run.  In a training step recorded into a CUDA
     graph, record forward and backward together and, as torch asks for every operator, keep no eager graph of the same
     leaves alive while recording."""

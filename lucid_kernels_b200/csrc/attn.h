@@ -29,7 +29,7 @@ struct AttnFwdArgs {
 struct AttnBwdArgs {
   AttnShape a;
   const int* lengths;
-  const float* stat;      // (B, Hq, nqb, 2, 128): lse in base 2 (+inf: row without weight), delta
+  const float* stat;      // (B, Hq, nqb, 2, 128): lse in base 2 (+inf: row without weight), -delta, in the units of attn_stat_kernel
   void* dq;
   Strides dq_strides;
   void *dk, *dv;

@@ -14,9 +14,16 @@ namespace lucid {
 static __device__ Control g_attn_bwd_ctl;
 
 // ------------------------------------------------------------------------------------------------------------------
-// Row statistics {lse in base 2, delta}: delta = dO . (O + what its rounding took off).  Reads each once, bound by HBM.
-// Eight lanes per row, four rows per warp and round.
+// Row statistics {log2(sum of exponentials / unit), -delta / unit}, delta = dO . (O + what its rounding took off): as the dK/dV
+// kernel wants them, whose weights are `unit` times P (below).  Reads each once, bound by HBM.  Eight lanes per row, four rows
+// per warp and round.
 // ------------------------------------------------------------------------------------------------------------------
+// P^T enters its product times 2^kWeightBits, and dV leaves divided by that: fp16 loses bits of weights below 2^-14, which is
+// what a row of some ten thousand keys has; none is above 1.  dS, which has no such bound, is formed from them with its other
+// factor divided (part of an fma), and rounded as it is.  (Products with the unit in the dK/dV kernel took it 4 % longer.)
+template <bool kBf16>
+constexpr int kWeightBits = kBf16 ? 0 : 15;
+
 constexpr int kStatRows = 8;             // rows of a warp (4, 16 and 32: 3, 3 and 10 % slower at 64k)
 
 template <bool kBf16>
@@ -59,8 +66,8 @@ __global__ void __launch_bounds__(256) attn_stat_kernel(const AttnStatArgs args)
       const float lse = i < A.Nq ? args.lse[(long long)bh * A.Nq + i] : -INFINITY;
       const bool weight = lse != -INFINITY;                // (a row without weight: P = 0 from +infinity)
       float* st = args.stat + tile * (2 * kBlock) + (i & 127);
-      st[0] = weight ? lse * kLog2e : INFINITY;
-      st[kBlock] = weight ? d : 0.f;
+      st[0] = weight ? lse * kLog2e - kWeightBits<kBf16> : INFINITY;
+      st[kBlock] = weight ? -d / (1 << kWeightBits<kBf16>) : 0.f;
     }
   }
 }
@@ -177,7 +184,7 @@ struct AttnDqSmem {
   alignas(1024) uint8_t go[kTileBytes];            // dO
   alignas(1024) uint8_t kring[3][kTileBytes];
   alignas(1024) uint8_t vring[2][kTileBytes];
-  alignas(16) float stat[2][2 * kBlock];           // with the slot: lse in base 2, delta
+  alignas(16) float stat[2][2 * kBlock];           // with the slot: the rows' statistics
   alignas(8) uint64_t k_full[3];
   uint64_t k_empty[3], v_full[2], v_empty[2], slot_full[2], slot_free[2];
   uint64_t q_full, q_free, go_full, go_free, panel_done;
@@ -421,7 +428,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const int len = x->len, block = x->block, b = x->b, h = x->h;
       const int i = block * kBlock + row, p = i + A.off;
       // (a query that sees one key has dS = 0 exactly, not the difference of two nearly equal sums)
-      const float lse2 = sees_one(A, p) ? INFINITY : s.stat[slots & 1][row], delta = s.stat[slots & 1][kBlock + row];
+      const float lse2 = sees_one(A, p) ? INFINITY : s.stat[slots & 1][row] + kWeightBits<kBf16>;
+      const float delta = -s.stat[slots & 1][kBlock + row] * (1 << kWeightBits<kBf16>);
       done();
       const unsigned long long nlse2 = f32x2(-lse2, -lse2), ndelta = f32x2(-delta, -delta);
       for (int u = 0; u < kt.n; ++u, ++g) {
@@ -553,7 +561,7 @@ struct AttnDkvSmem {
   alignas(1024) uint8_t qring[2][kTileBytes];
   alignas(1024) uint8_t gring[2][kTileBytes];      // dO
   alignas(1024) uint8_t stage[kTileBytes];         // per warp a panel of 32 rows x 64 columns
-  alignas(16) float stat[2][2 * kBlock];           // with the Q stage: lse in base 2, delta
+  alignas(16) float stat[2][2 * kBlock];           // with the Q stage: the rows' statistics
   alignas(8) uint64_t q_full[2];
   uint64_t q_empty[2], go_full[2], go_empty[2], slot_full[2], slot_free[2];
   uint64_t k_full, k_free, v_full, v_free;
@@ -769,7 +777,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_tmem = lanes + kKvS + wg * 64, g_tmem = lanes + kKvG + wg * 64;
     const float sl2 = args.scale_log2;
-    const unsigned long long sl22 = f32x2(sl2, sl2), minus = f32x2(-1.f, -1.f);
+    constexpr float kUnit = 1 << kWeightBits<kBf16>;
+    const unsigned long long sl22 = f32x2(sl2, sl2), minus = f32x2(-1.f, -1.f), part = f32x2(1.f / kUnit, 1.f / kUnit);
     uint8_t* panel = s.stage + (warp - 4) * 4096;
     while (const DkvSlot* x = next()) {
       const int nb = x->nb, n = nb * A.G, len = x->len, tile = x->tile, chunk = x->chunk, b = x->b, hk = x->hk, first = x->first;
@@ -863,9 +872,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             for (int e = 0; e < 8; e += 2) {
               const float4 t = *reinterpret_cast<const float4*>(stat + kBlock + 16 * c + 2 * e);
               float2 a = f32x2_unpack(f32x2_mul(f32x2(__uint_as_float(pv[2 * e]), __uint_as_float(pv[2 * e + 1])),
-                                                f32x2_fma(f32x2(t.x, t.y), minus, f32x2(__uint_as_float(cur[2 * e]), __uint_as_float(cur[2 * e + 1])))));
+                                                f32x2_fma(f32x2(__uint_as_float(cur[2 * e]), __uint_as_float(cur[2 * e + 1])), part, f32x2(t.x, t.y))));
               float2 d = f32x2_unpack(f32x2_mul(f32x2(__uint_as_float(pv[2 * e + 2]), __uint_as_float(pv[2 * e + 3])),
-                                                f32x2_fma(f32x2(t.z, t.w), minus, f32x2(__uint_as_float(cur[2 * e + 2]), __uint_as_float(cur[2 * e + 3])))));
+                                                f32x2_fma(f32x2(__uint_as_float(cur[2 * e + 2]), __uint_as_float(cur[2 * e + 3])), part, f32x2(t.z, t.w))));
               if (kMasked && stale) {          // (elsewhere G is finite, and 0 * G is 0)
                 const uint32_t m = words[c >> 1] >> (16 * (c & 1) + 2 * e);
                 a.x = (m & 1u) ? a.x : 0.f;
@@ -902,7 +911,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll 1
       for (int which = 0; which < 2; ++which) {                  // 0: dV, 1: dK
         const uint32_t t_addr = lanes + (which ? kKvDk : kKvDv) + wg * 64;
-        const float f = which ? args.scale : 1.f;
+        const float f = which ? args.scale : 1.f / kUnit;
         if (has) {
           if (!wait_lean(which ? &s.dk_full : &s.dv_full, itn & 1, cta_abort, limit, AB_ACC_FULL)) { alive = false; break; }
           tc_fence_after_sync();

@@ -581,6 +581,28 @@ def test_many_small_weights_beside_a_large_one(N, drop, dt):
 
 
 @gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("N,window,sinks", [(20000, None, 0), (65536, None, 0), (40000, 30000, 100)])
+def test_gradient_of_values_of_small_weights(N, window, sinks, dt):
+    """Alike queries on many keys: each weight is some 2^-16, rounded the same way for every query, and its rounding must
+    stay relative to it."""
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+
+    Nq, scale = 256, 0.05
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    q = rnd(1, 1, 1, D).expand(1, Nq, 1, D).contiguous().to(dt)
+    k, v, do = rnd(1, N, 1, D).to(dt), rnd(1, N, 1, D).to(dt), rnd(1, 1, 1, D).expand(1, Nq, 1, D).contiguous().to(dt)
+    s = (q[0, :, 0].double() @ k[0, :, 0].double().T * scale).masked_fill(~visible(Nq, N, window, sinks, N, "cuda"), -math.inf)
+    P = torch.softmax(s, -1)
+    assert float(P.max()) < 2.0 ** -11 and float(P[P > 0].median()) < 2.0 ** -14
+    out, lse, rest = _window_attention_fwd(q, k, v, window, sinks, scale, check=True)
+    dv = _window_attention_bwd(q, k, v, out, lse, rest, do, window, sinks, scale, check=True)[2]
+    close(dv[0, :, 0], P.T @ do[0, :, 0].double(), P.T @ do[0, :, 0].double().abs(), dt, "dv")
+
+
+@gpu
 def test_runs_are_identical_and_graphs_replay():
     from lucid_kernels_b200 import window_attention
 
