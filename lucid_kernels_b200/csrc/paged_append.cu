@@ -4,7 +4,7 @@
 // Bound by HBM (each row is read once and written once) or, for a handful of tokens, by latency.  A warp owns one token
 // and some of its heads, four head rows at a time, 8 lanes a row, each lane the two 16-byte pieces that rotate into
 // one another.  The angle is a product in 64 bits reduced to a fraction of a turn there: at position 10^6 a product in 32
-// bits is off by up to 0.06 radians.  Tables of sines would be 512 bytes to read per token; computing them costs a lane
+// bits is off by up to 0.03 radians (half of its spacing there, 2^-4).  Tables of sines would be 512 bytes to read per token; computing them costs a lane
 // two angles per token.
 #include <type_traits>
 #include "attn.h"

@@ -20,8 +20,8 @@ namespace lucid {
 static __device__ Control g_paged_ctl;
 
 constexpr int kPaWarps = 4, kPaStages = 2, kPaKeys = 16;
-// (two blocks in flight per warp and three CTAs per SM; three blocks and two CTAs took 106 us where this takes 99 on 32
-// ragged sequences of up to 16384 keys, and 22 us against 16.5 on 12 of up to 3001)
+// (two stages - one block on its way while one is worked on - and three CTAs per SM; three stages and two CTAs took 106 us
+// where this takes 99 on 32 ragged sequences of up to 16384 keys, and 22 us against 16.5 on 12 of up to 3001)
 constexpr int kPaStageBytes = 2 * kPaKeys * 256;               // K block, V block
 constexpr int kPaRow = 132;                                    // floats of a partial sum: 128 sums, maximum, sum, 2 unused
 constexpr int kPaMinChunk = 64;                                // keys of a split: at least one block per warp
