@@ -167,7 +167,7 @@ struct PagedAttnArgs {
 // up to this many chunks of a sequence are one cluster's CTAs (and then a power of two)
 constexpr int kPagedCluster = 8, kPagedMaxSplits = 128, kPagedPerSm = 3;
 
-cudaError_t launch_paged_append(bool bf16, const AppendArgs& args, cudaStream_t stream);
+cudaError_t launch_paged_append(bool bf16, const AppendArgs& args, int sms, cudaStream_t stream);
 cudaError_t launch_paged_attn(bool bf16, bool lucid, const PagedAttnArgs& args, cudaStream_t stream);
 size_t paged_attn_partial_bytes(int B, int Hq, int Hkv, bool lucid, int splits);
 

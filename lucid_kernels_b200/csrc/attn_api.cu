@@ -235,7 +235,8 @@ int lucid_paged_append(const lucid_paged_append_desc* d, const void* k, const vo
   if (v && (rc = check_rows(v, d->v_strides, T, Hkv))) return rc;
   if (q && ((rc = check_rows(q, d->q_strides, T, Hq)) || reinterpret_cast<uintptr_t>(q_out) % 16))
     return rc ? rc : LUCID_E_BAD_ALIGNMENT;
-  if (sm_count() <= 0) return LUCID_E_NO_DEVICE;
+  const int sms = sm_count();
+  if (sms <= 0) return LUCID_E_NO_DEVICE;
   args.k = k;
   args.v = v;
   args.q = q;
@@ -259,7 +260,7 @@ int lucid_paged_append(const lucid_paged_append_desc* d, const void* k, const vo
   args.Hkv = Hkv;
   args.rot = inv_freq ? d->rotated : 0;
   args.interleaved = d->interleaved ? 1 : 0;
-  return (int)launch_paged_append(d->dtype == LUCID_DTYPE_BF16, args, static_cast<cudaStream_t>(cuda_stream));
+  return (int)launch_paged_append(d->dtype == LUCID_DTYPE_BF16, args, sms, static_cast<cudaStream_t>(cuda_stream));
 }
 
 size_t lucid_paged_attn_workspace_bytes(const lucid_paged_attn_desc* d, int lucid_step) {

@@ -130,10 +130,17 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Appen
   }
 }
 
-cudaError_t launch_paged_append(bool bf16, const AppendArgs& args, cudaStream_t stream) {
+// A warp takes four head rows of a token, or all of them.  Four, while the warps that makes fit the SMs at once (80 registers: six
+// CTAs an SM) as often as a warp with all rows has rounds of kAhead to do; beyond that its repeated lookups cost more than
+// its shorter chain saves.  Four against all, us, 8/4 query/key heads: 8 tokens 3.0 and 3.9, 768 4.1 and 4.7, 1024 5.6 and 4.7,
+// 3500 11.5 and 7.0, 9000 25.4 and 14.9; 32/8 heads: 640 7.8 and 8.2, 1024 10.4 and 8.2; 4/1 heads: 1536 4.1 and 4.3,
+// 2048 5.7 and 4.6.
+constexpr int kApPerSm = 6;
+
+cudaError_t launch_paged_append(bool bf16, const AppendArgs& args, int sms, cudaStream_t stream) {
   const int rows = args.Hkv + (args.v ? args.Hkv : 0) + (args.q ? args.Hq : 0);
   const int groups = (rows + 3) / 4;
-  const int parts = args.T < 4096 ? groups : 1;
+  const int parts = (long long)args.T * imin(groups, kAhead) <= (long long)kApPerSm * kApWarps * sms ? groups : 1;
   const long long units = (long long)args.T * parts;
   const unsigned grid = (unsigned)((units + kApWarps - 1) / kApWarps);
   if (bf16) paged_append_kernel<true><<<grid, kApWarps * 32, 0, stream>>>(args, parts);

@@ -1040,6 +1040,28 @@ def test_append_many_tokens(Hq, Hkv, B, most):
 
 
 @gpu
+@pytest.mark.parametrize("Hq,Hkv", [(8, 4), (4, 1), (33, 8), (1, 1)])
+def test_append_is_the_same_however_the_tokens_are_dealt_out(Hq, Hkv):
+    """One call, around the number of tokens at which a warp takes on a whole token, against many calls of a few tokens."""
+    from lucid_kernels_b200 import paged_append
+
+    dt, page = torch.float16, 32
+    groups = -(-(Hq + 2 * Hkv) // 4)
+    edge = torch.cuda.get_device_properties(0).multi_processor_count * 24 // min(groups, 4)
+    f = frequencies()
+    for T in (edge - 1, edge, edge + 1, 2 * edge + 5):
+        kc, vc, table = pool_of(1, T + 9, page, Hkv, dt, seed=T)
+        kd, vd = kc.clone(), vc.clone()
+        g = torch.Generator(device="cuda").manual_seed(T)
+        q, k, v = (torch.randn(T, n, D, device="cuda", generator=g).to(dt) for n in (Hq, Hkv, Hkv))
+        int32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+        got = paged_append(k, v, kc, vc, table, int32(9), cu_seqlens=int32(0, T), q=q, inv_freq=f, check=True)
+        parts = [paged_append(k[a:a + 100], v[a:a + 100], kd, vd, table, int32(9 + a), cu_seqlens=int32(0, min(100, T - a)), q=q[a:a + 100],
+                              inv_freq=f, check=True) for a in range(0, T, 100)]
+        assert torch.equal(got, torch.cat(parts)) and torch.equal(kc, kd) and torch.equal(vc, vd), T
+
+
+@gpu
 def test_offsets_beyond_32_bits():
     """Pools of more than 2^31 elements, the sequence's pages at their end; inputs whose rows lie that far apart."""
     from lucid_kernels_b200 import paged_append, paged_lucid_attention, paged_window_attention, window_attention
