@@ -480,7 +480,8 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
     typedef typename std::conditional<kBf16, __nv_bfloat16, __half>::type elem_t;
     // The groups meet on a named barrier in every full tile, and such a wait has no limit of its own.  So a warp that leaves,
     // whyever, comes to one more meeting and says so before: the others find its number there and leave with it.  (A
-    // number, not a flag: what is said after a meeting is for the next one, however late somebody looks.)
+    // number, not a flag: what is said after a meeting is for the next one, however late somebody looks.  The barrier's own
+    // reduction would do, but took the backward 1.5 % longer.)
     volatile int* leave_at = &s.leave_at;
     int meetings = 0;            // this warp has come to
     bool told = false;
