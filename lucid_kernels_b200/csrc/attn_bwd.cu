@@ -19,10 +19,11 @@ static __device__ Control g_attn_bwd_ctl;
 // per warp and round.
 // ------------------------------------------------------------------------------------------------------------------
 // P^T enters its product times 2^kWeightBits, and dV leaves divided by that: fp16 loses bits of weights below 2^-14, which is
-// what a row of some ten thousand keys has; none is above 1.  dS, which has no such bound, is formed from them with its other
+// what a row of some ten thousand keys has; none is above 1 but for the rounding of very large scores, for which there is room.
+// dS, which has no such bound, is formed from them with its other
 // factor divided (part of an fma), and rounded as it is.  (Products with the unit in the dK/dV kernel took it 4 % longer.)
 template <bool kBf16>
-constexpr int kWeightBits = kBf16 ? 0 : 15;
+constexpr int kWeightBits = kBf16 ? 0 : 12;
 
 constexpr int kStatRows = 8;             // rows of a warp (4, 16 and 32: 3, 3 and 10 % slower at 64k)
 

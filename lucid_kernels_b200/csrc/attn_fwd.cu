@@ -4,7 +4,7 @@
 //
 // One pass over the keys with a running maximum m and sum l per row; O is kept in tensor memory relative to a
 // reference maximum that is only moved when the running one has outgrown it by 2^8 (exact in the end: O and l share
-// the reference, and 2^8, for fp16 2^15 (kTopWeight), is inside the limits of fp32 sums and 16-bit weights).
+// the reference, and 2^8, for fp16 2^12 (kTopWeight), is inside the limits of fp32 sums and 16-bit weights).
 //
 // A CTA works on two tiles of 128 queries that read the same keys (two heads of a key head, or two neighbouring
 // blocks), so a key/value tile brought into shared memory feeds four products.  Per tile of queries: S (fp32, 128

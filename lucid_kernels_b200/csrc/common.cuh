@@ -231,10 +231,12 @@ __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
 }
 
 // log2 of the weight that a softmax's reference key gets.  fp16 loses bits below 2^-14 and ends at 2^-25: beside a key of
-// weight 1 the rest of a long row, each key at 2^-25 or less, would vanish, 0.1 % of the result at 65536 keys; 2^7 higher it
-// does not matter, and 2^16 is still out of reach.  bf16 has fp32's range.
+// weight 1 the rest of a long row, each key at 2^-25 or less, would vanish, 0.1 % of the result at 65536 keys.  2^4 higher that
+// is a quarter of a rounding of the result at most (a whole one at 262144 keys), and with the 2^8 by which a reference may
+// be outgrown, 2^16 is still far enough for scores so large (2^25) that fp32 holds them to within a few units only.  bf16 has
+// fp32's range.
 template <bool kBf16>
-constexpr float kTopWeight = kBf16 ? 0.f : 7.f;
+constexpr float kTopWeight = kBf16 ? 0.f : 4.f;
 
 __device__ __forceinline__ uint64_t desc_advance(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 

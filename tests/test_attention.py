@@ -603,6 +603,40 @@ def test_gradient_of_values_of_small_weights(N, window, sinks, dt):
 
 
 @gpu
+@pytest.mark.parametrize("size", [300.0, 700.0, 900.0])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (300, 4)])
+def test_scores_of_millions_in_fp16_stay_finite(window, sinks, size):
+    """Scores of up to 10^7, which fp32 holds to within one: weights are what they may be, but results are means of values, and
+    neither they nor gradients are infinite."""
+    from lucid_kernels_b200 import paged_window_attention
+    from lucid_kernels_b200.attention import _window_attention_bwd, _window_attention_fwd
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    B, N, Hq, Hkv, page = 2, 1024, 4, 2, 64
+    sign = lambda *s: torch.randint(0, 2, s, device="cuda", generator=g) * 2.0 - 1
+    line = sign(1, 1, 1, D)
+    jitter = lambda *s: 1 + 0.02 * torch.randn(*s, device="cuda", generator=g)
+    # every key lies along one line, growing along the sequence: maxima keep growing, in small and large steps
+    grow = torch.linspace(0.2, 1, N, device="cuda").reshape(1, N, 1, 1)
+    q, k = (size * line * jitter(B, N, Hq, 1)).half(), (size * line * grow * jitter(B, N, Hkv, D)).half()
+    v, do = (torch.randn(B, N, n, D, device="cuda", generator=g).half() for n in (Hkv, Hq))
+    out, lse, rest = _window_attention_fwd(q, k, v, window, sinks, check=True)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    assert float(lse.max()) > 0.9 * size ** 2 * D ** 0.5 * 0.9
+    top = v.float().abs().amax(dim=1).repeat_interleave(Hq // Hkv, dim=1)[:, None]
+    assert bool((out.float().abs() <= top * 1.01).all())
+    again = _window_attention_fwd(q, k, v, window, sinks, training=False, check=True)[0]
+    assert torch.isfinite(again).all() and bool((again.float().abs() <= top * 1.01).all())
+    dv = _window_attention_bwd(q, k, v, out, lse, rest, do, window, sinks, check=True)[2]
+    assert torch.isfinite(dv).all()
+    kc, vc = k.reshape(B * N // page, page, Hkv, D), v.reshape(B * N // page, page, Hkv, D)
+    table = torch.arange(B * N // page, device="cuda", dtype=torch.int32).reshape(B, -1)
+    step = paged_window_attention(q[:, -1].contiguous(), kc, vc, table, torch.full((B,), N, device="cuda", dtype=torch.int32), window, sinks, check=True)
+    assert torch.isfinite(step).all() and bool((step.float().abs() <= top[:, 0] * 1.01).all())
+
+
+@gpu
 def test_runs_are_identical_and_graphs_replay():
     from lucid_kernels_b200 import window_attention
 
