@@ -257,8 +257,8 @@ revdk_kernel(const __grid_constant__ CUtensorMap tm_k,     // K,   box 64 x 128
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRdRegsService));
     // =========================== the issuer of all products but S(1), S(2), ... ===========================
     // Program order per tile: G, then (as the exp groups deliver them) the products that read W and P; the next
-    // tile's G follows at once.  One thread has the role to itself, waits included.  The tensor pipe runs one thread's products in order, so the G columns are never
-    // overwritten before the products that read W and P there have done so.
+    // tile's G follows at once.  One thread has the role to itself, waits included.  The tensor pipe runs one thread's
+    // products in order, so the G columns are never overwritten before the products that read W and P there have done so.
     if (elect_one()) {
       constexpr int fmt = kBf16 ? 1 : 0;
       constexpr uint32_t idesc_kk = umma_idesc(fmt, 0, 0, 128, 128);    // both operands K-major
